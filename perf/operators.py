@@ -287,7 +287,7 @@ def _extend(s):
     s["table"].copy_(torch.where(mine, s["free"][(s["free_count"] - 1 - nth).clamp(0, s["free"].numel() - 1).long()], s["table"]))
     after = torch.where(granted, have + n, have)
     s["lengths"].copy_(after)
-    s["free_count"].sub_(torch.where(granted, taken, 0).amax(0, keepdim=True).to(torch.int32))
+    s["free_count"].sub_(torch.where(need > 0, taken, 0).amax(0, keepdim=True).to(torch.int32))
     t = torch.arange(T, device=dev)
     r = torch.searchsorted(end, t, right=True).clamp(max=R - 1)
     inside = t < end[-1]
