@@ -1,0 +1,456 @@
+// The paged 8-bit cache: block tables and slot maps from request lengths, and the writer of keys and values.
+#include <cuda_fp8.h>
+
+#include "fdma_internal.h"
+#include "fdma_rotary.cuh"
+
+namespace fdma {
+namespace {
+
+// ---- block tables -----------------------------------------------------------------------------------------------
+// Whole numbers and a few kilobytes: the time is that of a launch and of a chain of dependent loads. So extending is ONE launch.
+// Every CTA sums up the lengths of all requests itself (three scans over up to 1024 of them at a time, about 1 us) and then fills
+// its share of the tokens; what other CTAs still read (lengths, the free list's count) is updated by the CTA that arrives last.
+constexpr int kTableThreads = 1024;
+constexpr int kMaxRequests = 8192;
+
+// Inclusive scan over the CTA. s_warp: 33 words; ends with all threads past their reads of it.
+__device__ __forceinline__ long long scan(long long x, long long* s_warp, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    long long w = s_warp[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    s_warp[lane] = w;
+  }
+  __syncthreads();
+  if (warp > 0) x += s_warp[warp - 1];
+  *total = s_warp[31];
+  __syncthreads();
+  return x;
+}
+
+__device__ __forceinline__ int ceil_div(long long x, int shift) { return static_cast<int>((x + (1ll << shift) - 1) >> shift); }
+
+__global__ void __launch_bounds__(kTableThreads) extend_kernel(const fdma_tables_params p, const int shift) {
+  // per request: end of its tokens; tokens held before; place of its first new block among the step's (-1: refused)
+  extern __shared__ int32_t s_req[];
+  __shared__ long long s_warp[33];
+  __shared__ bool s_last;
+  int32_t *s_end = s_req, *s_have = s_req + p.requests, *s_first = s_req + 2 * p.requests;
+  const int tid = threadIdx.x;
+  const int R = p.requests;
+  const int n_free = max(0, min(*p.free_count, p.num_blocks));
+  const bool lead = blockIdx.x == 0;
+  long long tokens = 0, blocks = 0, units = 0;  // sums over the requests before; units: chunks << 32 | touched blocks
+  long long taken = 0;                          // blocks that leave the free list
+  for (int base = 0; base < R; base += kTableThreads) {
+    const int r = base + tid;
+    const bool in = r < R;
+    const int have = in ? max(0, p.lengths[r]) : 0, n = in ? max(0, p.new_lengths[r]) : 0;
+    long long sum;
+    const long long end = tokens + scan(n, s_warp, &sum);
+    tokens += sum;
+    const long long length = static_cast<long long>(have) + n;
+    const long long old = ceil_div(have, shift), want = (length + (1ll << shift) - 1) >> shift;
+    const bool may = n > 0 && want <= p.width && end <= p.tokens;
+    const int need = may ? static_cast<int>(want - old) : 0;
+    const long long upto = blocks + scan(need, s_warp, &sum);
+    blocks += sum;
+    const bool granted = n == 0 || (may && (need == 0 || upto <= n_free));
+    const bool active = granted && n > 0;
+    const int touched = active ? static_cast<int>(want - (have >> shift)) : 0;
+    const int chunks = active ? ceil_div(length, 6) : 0;
+    const long long both = units + scan((static_cast<long long>(chunks) << 32) | touched, s_warp, &sum);
+    units += sum;
+    long long most;  // (sums of the blocks that are granted are ascending, so the last of them is their total)
+    scan(active && need > 0 ? need : 0, s_warp, &most);
+    taken += most;
+    if (in) {
+      const int e = static_cast<int>(min(end, static_cast<long long>(p.tokens)));
+      s_end[r] = e;
+      s_have[r] = have;
+      s_first[r] = granted ? static_cast<int>(upto - need) : -1;
+      if (lead) {
+        p.cu_seqlens[r + 1] = e;
+        p.lengths_after[r] = granted ? static_cast<int>(length) : have;
+        p.granted[r] = granted ? 1 : 0;
+        p.cu_blocks[r + 1] = static_cast<int>(both & 0xFFFFFFFF);
+        p.cu_chunks[r + 1] = static_cast<int>(both >> 32);
+        if (r == 0) p.cu_seqlens[0] = p.cu_blocks[0] = p.cu_chunks[0] = 0;
+      }
+    }
+  }
+  __syncthreads();
+  const int mask = (1 << shift) - 1;
+  const int last_end = s_end[R - 1];
+  for (int t = blockIdx.x * kTableThreads + tid; t < p.tokens; t += gridDim.x * kTableThreads) {
+    int pos = 0;
+    int64_t slot = -1;
+    if (t < last_end) {
+      int lo = 0, hi = R - 1;  // first request whose tokens end behind t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_end[mid] > t) hi = mid;
+        else lo = mid + 1;
+      }
+      const int start = lo ? s_end[lo - 1] : 0, have = s_have[lo], first = s_first[lo];
+      pos = have + t - start;
+      if (first >= 0) {
+        const int page = pos >> shift, old = ceil_div(have, shift);
+        const int block = page < old ? p.table[static_cast<int64_t>(lo) * p.width + page] : p.free_list[n_free - 1 - (first + page - old)];
+        if (block >= 0) slot = (static_cast<int64_t>(block) << shift) + (pos & mask);
+      }
+    }
+    p.positions[t] = pos;
+    p.slots[t] = slot;
+  }
+  // the new blocks' entries, which nobody reads in this launch: a warp per request
+  const int warps = gridDim.x * (kTableThreads / 32);
+  for (int r = blockIdx.x * (kTableThreads / 32) + (tid >> 5); r < R; r += warps) {
+    const int first = s_first[r];
+    if (first < 0) continue;
+    const int have = s_have[r], n = s_end[r] - (r ? s_end[r - 1] : 0);
+    const int old = ceil_div(have, shift), want = ceil_div(static_cast<long long>(have) + n, shift);
+    for (int j = old + (tid & 31); j < want; j += 32)
+      p.table[static_cast<int64_t>(r) * p.width + j] = p.free_list[n_free - 1 - (first + j - old)];
+  }
+  // the last CTA: nobody reads lengths and free_count any more
+  if (gridDim.x > 1) {
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      s_last = atomicAdd(p.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
+  } else {
+    __syncthreads();
+  }
+  for (int r = tid; r < R; r += kTableThreads)
+    if (s_first[r] >= 0) p.lengths[r] = s_have[r] + s_end[r] - (r ? s_end[r - 1] : 0);
+  if (tid == 0) {
+    *p.free_count = n_free - static_cast<int>(taken);
+    *p.ticket = 0;
+  }
+}
+
+__global__ void __launch_bounds__(kTableThreads) truncate_kernel(const fdma_tables_params p, const int shift) {
+  extern __shared__ int32_t s_req[];  // per request: blocks kept, blocks held, place of its first freed block
+  __shared__ long long s_warp[33];
+  int32_t *s_keep = s_req, *s_held = s_req + p.requests, *s_first = s_req + 2 * p.requests;
+  const int tid = threadIdx.x, R = p.requests;
+  const int n_free = max(0, min(*p.free_count, p.num_blocks));
+  long long gone = 0;
+  for (int base = 0; base < R; base += kTableThreads) {
+    const int r = base + tid;
+    const int have = r < R ? max(0, p.lengths[r]) : 0, keep = r < R ? min(have, max(0, p.new_lengths[r])) : 0;
+    const int held = min(ceil_div(have, shift), p.width), left = min(ceil_div(keep, shift), p.width);
+    long long sum;
+    const long long upto = gone + scan(held - left, s_warp, &sum);
+    gone += sum;
+    if (r < R) {
+      s_keep[r] = left;
+      s_held[r] = held;
+      s_first[r] = static_cast<int>(upto - (held - left));
+      p.lengths[r] = keep;
+    }
+  }
+  __syncthreads();
+  const long long total = n_free + gone;
+  for (int r = tid >> 5; r < R; r += kTableThreads / 32) {
+    const int left = s_keep[r], held = s_held[r], first = s_first[r];
+    for (int j = left + (tid & 31); j < held; j += 32) {
+      int32_t* entry = p.table + static_cast<int64_t>(r) * p.width + j;
+      const long long at = total - 1 - (first + j - left);
+      if (at < p.num_blocks) p.free_list[at] = *entry;
+      *entry = -1;
+    }
+  }
+  if (tid == 0) *p.free_count = static_cast<int>(min(total, static_cast<long long>(p.num_blocks)));
+}
+
+int block_shift(int block_size) {
+  switch (block_size) {
+    case 16: return 4;
+    case 32: return 5;
+    case 64: return 6;
+    case 128: return 7;
+    default: return -1;
+  }
+}
+
+int check_tables(const fdma_tables_params* p) {
+  if (!p || !p->table || !p->lengths || !p->free_list || !p->free_count || !p->ticket || !p->new_lengths) return FDMA_ERR_BAD_ARG;
+  if (p->requests < 0 || p->width <= 0 || p->num_blocks <= 0 || p->tokens < 0) return FDMA_ERR_BAD_ARG;
+  const int shift = block_shift(p->block_size);
+  if (shift < 0 || p->requests > kMaxRequests) return FDMA_ERR_UNSUPPORTED;
+  if ((static_cast<int64_t>(p->width) << shift) > 0x7FFFFFFF || (static_cast<int64_t>(p->requests) * p->width << shift >> 6) > 0x7FFFFFFF)
+    return FDMA_ERR_UNSUPPORTED;
+  return 0;
+}
+
+template <typename K>
+int table_smem(K kernel, int requests, size_t* bytes) {
+  *bytes = static_cast<size_t>(requests) * 12;
+  if (*bytes <= 40 * 1024) return 0;
+  return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(*bytes)));
+}
+
+// ---- the writer ---------------------------------------------------------------------------------------------------
+// Memory-bound: keys and values are read twice (the second time from cache) and written once. A CTA takes one block and kv head
+// of K or of V: it looks for the largest magnitude, fixes the scale and writes. Queries are turned by CTAs behind those.
+struct AppendArgs {
+  fdma_cache_append_params p;
+  RotaryUnits key_units, value_units;
+  RotaryArgs query;  // tokens_per_cta = 0: none
+  int shift, most_units;
+  int64_t cache_ctas;
+};
+
+__device__ __forceinline__ uint8_t to_e4m3(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ float from_e4m3(uint8_t x) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(x, __NV_E4M3)));
+}
+
+// 2^e, e the smallest (from -100 on) with x <= 448 * 2^e: x and 448 = 1.75 * 2^8 by exponent and mantissa
+__device__ __forceinline__ float block_scale(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7FFFFF) > 0x600000 ? 1 : 0);
+  return __uint_as_float(static_cast<uint32_t>(max(e, -100) + 127) << 23);
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kRotaryThreads) append_kernel(const AppendArgs a) {
+  extern __shared__ float2 s_factors[];  // [new tokens of the block][half], or rotate_tokens' own
+  __shared__ float s_max[kRotaryThreads / 32];
+  __shared__ int s_request;
+  const fdma_cache_append_params& p = a.p;
+  const fdma_cache& c = p.c;
+  const int tid = threadIdx.x;
+  if (blockIdx.x >= a.cache_ctas) {
+    rotate_tokens<T, N>(a.query, blockIdx.x - a.cache_ctas, s_factors);
+    return;
+  }
+  const bool is_v = blockIdx.x & 1;
+  const int rest = blockIdx.x >> 1;
+  const int unit = rest / c.h_k, head = rest - unit * c.h_k;
+  if (tid == 0) s_request = -1;
+  __syncthreads();
+  for (int r = tid; r < c.requests; r += kRotaryThreads)
+    if (c.cu_blocks[r] <= unit && unit < c.cu_blocks[r + 1]) s_request = r;
+  __syncthreads();
+  const int r = s_request;
+  if (r < 0) return;
+  const int bs = 1 << a.shift;
+  const int token0 = c.cu_seqlens[r], n_new = c.cu_seqlens[r + 1] - token0, length = c.lengths[r], before = length - n_new;
+  const int page = (before >> a.shift) + unit - c.cu_blocks[r];
+  if (token0 < 0 || n_new < 0 || token0 + n_new > c.tokens || before < 0 || page >= c.width) return;
+  const int block = c.table[static_cast<int64_t>(r) * c.width + page];
+  if (block < 0 || block >= c.num_blocks) return;
+  const int begin = page << a.shift;
+  const int lo = max(before - begin, 0), hi = min(length - begin, bs);  // places of the new tokens in the block
+  const int n = hi - lo;
+  if (n <= 0) return;
+  const int first = token0 + begin + lo - before;  // the token at place lo
+
+  const RotaryUnits& ru = is_v ? a.value_units : a.key_units;
+  const T* src = static_cast<const T*>(is_v ? p.value : p.key) + first * (is_v ? p.value_row_stride : p.key_row_stride) +
+                 head * (is_v ? p.value_head_stride : p.key_head_stride);
+  const int64_t row_stride = is_v ? p.value_row_stride : p.key_row_stride;
+  const int64_t at_scale = static_cast<int64_t>(block) * c.h_k + head;
+  uint8_t* dst = static_cast<uint8_t*>(is_v ? c.v : c.k) + (at_scale * bs) * c.d;
+  float* scale = (is_v ? c.v_scale : c.k_scale) + at_scale;
+  const float old_scale = lo > 0 ? *scale : 0.f;
+  for (int i = tid; i < n * ru.half; i += kRotaryThreads) {
+    const int t = i / ru.half;
+    s_factors[i] = rotary_factors(before + (first - token0) + t, p.turns[i - t * ru.half], p.amplitude, false);
+  }
+  __syncthreads();
+  using V = Vec<T, N>;
+  auto load = [&](int i, float (&x)[N], float (&y)[N], int2& at, int& t, bool& pair) {
+    t = i / ru.units;
+    const int u = i - t * ru.units;
+    at = unit_offsets<N>(ru, u);
+    pair = u < ru.pair_units;
+    const V vx = *reinterpret_cast<const V*>(src + t * row_stride + at.x);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = to_f(vx.x[j]);
+    if (pair) {
+      const V vy = *reinterpret_cast<const V*>(src + t * row_stride + at.y);
+#pragma unroll
+      for (int j = 0; j < N; ++j) y[j] = to_f(vy.x[j]);
+      rotate_unit<N>(x, y, s_factors + t * ru.half + u * N, ru.interleaved);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) y[j] = 0.f;
+    }
+  };
+  float most = 0.f;
+  for (int i = tid; i < n * ru.units; i += kRotaryThreads) {
+    float x[N], y[N];
+    int2 at;
+    int t;
+    bool pair;
+    load(i, x, y, at, t, pair);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float fx = fabsf(x[j]), fy = fabsf(y[j]);
+      if (fx <= 3.402823466e38f) most = fmaxf(most, fx);
+      if (fy <= 3.402823466e38f) most = fmaxf(most, fy);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if ((tid & 31) == 0) s_max[tid >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kRotaryThreads / 32; ++w) most = fmaxf(most, s_max[w]);
+  const float now = fmaxf(block_scale(most), old_scale), inv = __frcp_rn(now);
+  if (tid == 0) *scale = now;
+  for (int i = tid; i < n * ru.units; i += kRotaryThreads) {
+    float x[N], y[N];
+    int2 at;
+    int t;
+    bool pair;
+    load(i, x, y, at, t, pair);
+    uint8_t* row = dst + (lo + t) * c.d;
+    Vec<uint8_t, N> out;
+#pragma unroll
+    for (int j = 0; j < N; ++j) out.x[j] = to_e4m3(x[j] * inv);
+    *reinterpret_cast<Vec<uint8_t, N>*>(row + at.x) = out;
+    if (pair) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) out.x[j] = to_e4m3(y[j] * inv);
+      *reinterpret_cast<Vec<uint8_t, N>*>(row + at.y) = out;
+    }
+  }
+  if (lo > 0 && now > old_scale) {  // the tokens that were there, at the new scale
+    const float f = old_scale * inv;
+    for (int i = tid; i < lo * c.d / 16; i += kRotaryThreads) {
+      Vec<uint8_t, 16>& v = *reinterpret_cast<Vec<uint8_t, 16>*>(dst + i * 16);
+      Vec<uint8_t, 16> x = v;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x.x[j] = to_e4m3(from_e4m3(x.x[j]) * f);
+      v = x;
+    }
+  }
+}
+
+template <typename T, int N>
+int launch_append(AppendArgs a, cudaStream_t stream) {
+  const fdma_cache_append_params& p = a.p;
+  const fdma_cache& c = p.c;
+  const bool turn = p.turns != nullptr;
+  a.key_units = rotary_units(c.d, turn ? p.rotary_dim : 0, p.interleaved != 0, N);
+  a.value_units = rotary_units(c.d, 0, false, N);
+  size_t smem = static_cast<size_t>(std::min(1 << a.shift, c.tokens)) * a.key_units.half * sizeof(float2);
+  int64_t query_ctas = 0;
+  a.query = RotaryArgs{};
+  if (turn && p.query) {
+    fdma_rotary_params q = {};
+    q.q = p.query; q.q_out = p.query_out;
+    q.turns = p.turns;
+    q.positions = c.positions; q.position_bits = 32; q.pos_row_stride = 1;
+    q.q_row_stride = p.query_row_stride; q.q_head_stride = p.query_head_stride;
+    q.qo_row_stride = p.out_row_stride; q.qo_head_stride = p.out_head_stride;
+    q.b = 1; q.seqlen = c.tokens; q.h = p.h; q.d = c.d; q.rotary_dim = p.rotary_dim;
+    q.interleaved = p.interleaved; q.dtype = p.dtype; q.amplitude = p.amplitude;
+    a.query = rotary_args(q, N);
+    query_ctas = (a.query.tokens + a.query.tokens_per_cta - 1) / a.query.tokens_per_cta;
+    smem = std::max(smem, static_cast<size_t>(a.query.tokens_per_cta) * a.query.ru.half * sizeof(float2));
+  }
+  auto kern = append_kernel<T, N>;
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  const int64_t ctas = a.cache_ctas + query_ctas;
+  if (ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
+  kern<<<static_cast<unsigned>(ctas), kRotaryThreads, smem, stream>>>(a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T>
+int launch_append_t(const AppendArgs& a, cudaStream_t stream) {
+  const fdma_cache_append_params& p = a.p;
+  uint64_t x = reinterpret_cast<uintptr_t>(p.key) | reinterpret_cast<uintptr_t>(p.value);
+  uint64_t strides = static_cast<uint64_t>(p.key_row_stride | p.key_head_stride | p.value_row_stride | p.value_head_stride);
+  if (p.turns && p.query) {
+    x |= reinterpret_cast<uintptr_t>(p.query) | reinterpret_cast<uintptr_t>(p.query_out);
+    strides |= static_cast<uint64_t>(p.query_row_stride | p.query_head_stride | p.out_row_stride | p.out_head_stride);
+  }
+  const bool vec = (x | strides * sizeof(T)) % 16 == 0 && rotary_units_fit(p.c.d, p.turns ? p.rotary_dim : 0, 8);
+  return vec ? launch_append<T, 8>(a, stream) : launch_append<T, 1>(a, stream);
+}
+
+}  // namespace
+
+int check_cache(const fdma_cache& c) {
+  if (!c.k || !c.v || !c.k_scale || !c.v_scale || !c.table || !c.cu_seqlens || !c.lengths || !c.cu_blocks || !c.cu_chunks) return FDMA_ERR_BAD_ARG;
+  if (c.requests < 0 || c.width <= 0 || c.num_blocks <= 0 || c.tokens < 0 || c.h_k <= 0 || c.d <= 0) return FDMA_ERR_BAD_ARG;
+  if (block_shift(c.block_size) < 0 || c.d % 16 || c.d > 256) return FDMA_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15) return FDMA_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(c.width) * c.block_size > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
+  return 0;
+}
+
+}  // namespace fdma
+
+using namespace fdma;
+
+extern "C" int fdma_tables_extend(const fdma_tables_params* p, void* stream) {
+  int st = check_tables(p);
+  if (st) return st;
+  if (!p->cu_seqlens || !p->cu_blocks || !p->cu_chunks || (p->tokens && (!p->positions || !p->slots))) return FDMA_ERR_BAD_ARG;
+  if (p->requests == 0 || !p->lengths_after || !p->granted) return FDMA_ERR_BAD_ARG;
+  size_t smem;
+  st = table_smem(extend_kernel, p->requests, &smem);
+  if (st) return st;
+  // a CTA for 2048 tokens: beyond that filling takes longer than another CTA's sums
+  const int ctas = std::max(1, std::min(sm_count(), p->tokens / 2048));
+  extend_kernel<<<ctas, kTableThreads, smem, static_cast<cudaStream_t>(stream)>>>(*p, block_shift(p->block_size));
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int fdma_tables_truncate(const fdma_tables_params* p, void* stream) {
+  int st = check_tables(p);
+  if (st) return st;
+  if (p->requests == 0) return FDMA_OK;
+  size_t smem;
+  st = table_smem(truncate_kernel, p->requests, &smem);
+  if (st) return st;
+  truncate_kernel<<<1, kTableThreads, smem, static_cast<cudaStream_t>(stream)>>>(*p, block_shift(p->block_size));
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int fdma_cache_append(const fdma_cache_append_params* p, void* stream_) {
+  if (!p) return FDMA_ERR_BAD_ARG;
+  const int st = check_cache(p->c);
+  if (st) return st;
+  if (p->c.tokens == 0 || p->c.requests == 0) return FDMA_OK;
+  if (!p->key || !p->value || !p->c.positions) return FDMA_ERR_BAD_ARG;
+  if (p->turns && (p->rotary_dim <= 0 || p->rotary_dim % 2 || p->rotary_dim > p->c.d)) return FDMA_ERR_BAD_ARG;
+  if (p->turns && p->query && (!p->query_out || p->h <= 0)) return FDMA_ERR_BAD_ARG;
+  AppendArgs a = {};
+  a.p = *p;
+  a.shift = block_shift(p->c.block_size);
+  a.most_units = static_cast<int>(std::min<int64_t>(p->c.tokens, (static_cast<int64_t>(p->c.tokens) >> a.shift) + 2 * static_cast<int64_t>(p->c.requests)));
+  a.cache_ctas = static_cast<int64_t>(a.most_units) * p->c.h_k * 2;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  switch (p->dtype) {
+    case FDMA_BF16: return launch_append_t<__nv_bfloat16>(a, stream);
+    case FDMA_FP16: return launch_append_t<__half>(a, stream);
+    default: return FDMA_ERR_UNSUPPORTED;
+  }
+}

@@ -1,0 +1,56 @@
+// Rotary positions on queries and keys, forward and backward (the same rotation by the negative angle).
+//
+//   y1 = a (x1 cos - x2 sin),  y2 = a (x2 cos + x1 sin),  angle = position * frequency
+//
+// Memory-bound: every element is read once and written once, three operations each. A CTA takes a few tokens, puts their cosines
+// and sines into shared memory (one evaluation per token and frequency, whatever the number of heads), then all its threads walk
+// the tokens' heads in 16-byte vectors.
+#include "fdma_rotary.cuh"
+
+namespace fdma {
+namespace {
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
+  extern __shared__ float2 s_factors[];
+  rotate_tokens<T, N>(a, blockIdx.x, s_factors);
+}
+
+template <typename T, int N>
+int launch(const fdma_rotary_params& p, cudaStream_t stream) {
+  const RotaryArgs a = rotary_args(p, N);
+  const int64_t ctas = (a.tokens + a.tokens_per_cta - 1) / a.tokens_per_cta;
+  if (ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
+  rotary_kernel<T, N><<<static_cast<unsigned>(ctas), kRotaryThreads, a.tokens_per_cta * a.ru.half * sizeof(float2), stream>>>(a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T>
+int launch_t(const fdma_rotary_params& p, cudaStream_t stream) {
+  constexpr int N = 16 / sizeof(T);
+  return rotary_units_fit(p.d, p.rotary_dim, N) && rotary_aligned16(p, sizeof(T)) ? launch<T, N>(p, stream) : launch<T, 1>(p, stream);
+}
+
+}  // namespace
+}  // namespace fdma
+
+using namespace fdma;
+
+extern "C" int fdma_rotary(const fdma_rotary_params* pp, void* stream_) {
+  if (!pp) return FDMA_ERR_BAD_ARG;
+  const fdma_rotary_params& p = *pp;
+  if (!p.q || !p.q_out || !p.turns || p.b < 0 || p.seqlen < 0 || p.h <= 0 || p.h_k < 0 || p.d <= 0) return FDMA_ERR_BAD_ARG;
+  if (p.h_k && (!p.k || !p.k_out)) return FDMA_ERR_BAD_ARG;
+  if (p.rotary_dim <= 0 || p.rotary_dim % 2 || p.rotary_dim > p.d) return FDMA_ERR_BAD_ARG;
+  if (p.positions && p.position_bits != 32 && p.position_bits != 64) return FDMA_ERR_BAD_ARG;
+  if (p.rotary_dim > 8192) return FDMA_ERR_UNSUPPORTED;  // a token's factors are held in 32 KB
+  if (static_cast<int64_t>(p.h + p.h_k) * p.d > (1 << 24)) return FDMA_ERR_UNSUPPORTED;
+  if (p.b == 0 || p.seqlen == 0) return FDMA_OK;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  switch (p.dtype) {
+    case FDMA_BF16: return launch_t<__nv_bfloat16>(p, stream);
+    case FDMA_FP16: return launch_t<__half>(p, stream);
+    case FDMA_FP32: return launch_t<float>(p, stream);
+    default: return FDMA_ERR_UNSUPPORTED;
+  }
+}

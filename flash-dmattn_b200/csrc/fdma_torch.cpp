@@ -33,6 +33,11 @@
 #include "../../include/fdma.h"
 
 namespace py = pybind11;
+
+// fdma_torch_cache.cpp: rotary positions, block tables, 8-bit cache
+void init_cache_ops(void* library);
+void bind_cache_ops(py::module& m);
+
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
 using torch::autograd::SavedVariable;
@@ -76,6 +81,7 @@ void init(const std::string& path) {
   get(api.strerror, "fdma_strerror");
   get(api.poll_kernel_status, "fdma_poll_kernel_status");
   get(api.last_kernel_status, "fdma_last_kernel_status");
+  init_cache_ops(h);
 }
 
 constexpr int64_t kTile = 128;
@@ -861,4 +867,5 @@ PYBIND11_MODULE(_fdma_torch, m) {
   m.def("attention", &py_attention);
   m.def("packed_attention", &py_packed_attention);
   m.def("topk_mask", &py_topk_mask);
+  bind_cache_ops(m);
 }

@@ -11,6 +11,10 @@ from .flash_sparse_attn_interface import (FlashDMAttnFunc, flash_sparse_attn_fun
                                           flash_sparse_attn_varlen_func)
 from .compaction import compact_keys, flash_sparse_attn_compact_func  # noqa: F401
 from .packed import PackedMask, pack_mask  # noqa: F401
+from .rotary import RotaryFrequencies, apply_rotary, rotary_frequencies  # noqa: F401
+from .cache import (BlockTables, CacheStep, QuantizedCache, block_tables, cache_append,  # noqa: F401
+                    flash_sparse_attn_cache_func, quantized_cache)
+from .utils.mask import KeptKeys  # noqa: F401
 
 CUDA_AVAILABLE = True
 TRITON_AVAILABLE = False

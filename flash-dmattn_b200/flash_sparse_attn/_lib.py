@@ -80,6 +80,12 @@ EXPORTED_SYMBOLS = (
     "fdma_gather_kept",
     "fdma_scatter_rows",
     "fdma_merge_partials",
+    "fdma_rotary",
+    "fdma_tables_extend",
+    "fdma_tables_truncate",
+    "fdma_cache_append",
+    "fdma_cache_attention_workspace_bytes",
+    "fdma_cache_attention",
 )
 
 

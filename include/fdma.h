@@ -380,6 +380,124 @@ typedef struct fdma_merge_params {
 int fdma_merge_partials(const fdma_merge_params* p, void* stream);
 
 /*
+ * Rotary positions: q_out = q and k_out = k with the first rotary_dim elements of every head turned in pairs,
+ *   y1 = amplitude (x1 cos - x2 sin),  y2 = amplitude (x2 cos + x1 sin),  angle = position * frequency of the pair;
+ * the rest is copied. Pairs are (i, i + rotary_dim / 2), or with `interleaved` (2 i, 2 i + 1). q (b, seqlen, h, d), k (b, seqlen,
+ * h_k, d), h_k = 0: queries alone; strides in elements, innermost 1. turns (rotary_dim / 2): the frequencies in turns per
+ * position as 64-bit fractions, frequency / (2 pi) * 2^64 (angles are then exact at any position). positions: int32 or int64
+ * (position_bits) with the strides given, NULL: 0 .. seqlen - 1. inverse: by the negative angle, which is the gradient.
+ * dtype BF16, FP16 or FP32; q_out and k_out do not overlap the inputs.
+ */
+typedef struct fdma_rotary_params {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const int64_t* turns;
+  const void* positions;
+  int64_t pos_batch_stride, pos_row_stride;
+  int64_t q_batch_stride, q_row_stride, q_head_stride;
+  int64_t k_batch_stride, k_row_stride, k_head_stride;
+  int64_t qo_batch_stride, qo_row_stride, qo_head_stride;
+  int64_t ko_batch_stride, ko_row_stride, ko_head_stride;
+  int32_t b, seqlen, h, h_k, d, rotary_dim;
+  int32_t interleaved, inverse, dtype, position_bits;
+  float amplitude;
+  int32_t reserved;
+} fdma_rotary_params;
+int fdma_rotary(const fdma_rotary_params* p, void* stream);
+
+/*
+ * Block tables of a paged cache, on the device. A request r holds lengths[r] tokens in the blocks table[r][0 ..
+ * ceil(lengths[r] / block_size)) (-1 behind them); free_list[0 .. *free_count) are the blocks nobody holds, taken from the end.
+ * *ticket is 0 between calls.
+ *
+ * fdma_tables_extend: requests get new_lengths[r] more tokens (negative counts as 0), in the order of the requests, and the
+ * blocks these need. A request gets all of its tokens or none: none when its table row is too short, its tokens would end
+ * beyond `tokens`, or blocks have run out. Brings table, lengths and free_count up to date and writes the plan of the step:
+ *   cu_seqlens (requests + 1)  first of each request's tokens among the step's tokens (at most `tokens`)
+ *   positions (tokens)         position of each token in its request, 0 behind the last one
+ *   slots (tokens)             block * block_size + place in the block; -1 for refused tokens and behind the last one
+ *   lengths_after, granted (requests)      tokens held now; 0 where the request was refused
+ *   cu_blocks (requests + 1)   blocks that the step's tokens go to, summed up over the requests before
+ *   cu_chunks (requests + 1)   64-token pieces of the requests with tokens in this step, summed up likewise
+ * fdma_tables_truncate: requests keep their first min(lengths[r], new_lengths[r]) tokens; blocks no longer needed return to the
+ * free list in the reverse of the order in which fdma_tables_extend takes them. The plan's fields are not used.
+ * Up to 8192 requests (FDMA_ERR_UNSUPPORTED beyond).
+ */
+typedef struct fdma_tables_params {
+  int32_t *table, *lengths, *free_list, *free_count, *ticket;
+  const int32_t* new_lengths;
+  int32_t *cu_seqlens, *positions;
+  int64_t* slots;
+  int32_t* lengths_after;
+  uint8_t* granted;
+  int32_t *cu_blocks, *cu_chunks;
+  int32_t requests, width, num_blocks, block_size, tokens, reserved;
+} fdma_tables_params;
+int fdma_tables_extend(const fdma_tables_params* p, void* stream);
+int fdma_tables_truncate(const fdma_tables_params* p, void* stream);
+
+/*
+ * A paged cache in 8 bits: k, v (num_blocks, h_k, block_size, d) e4m3, dense, and a scale for each block and head, k_scale and
+ * v_scale (num_blocks, h_k) fp32, powers of two: a value stands for its e4m3 number times its block's scale. table, cu_seqlens,
+ * lengths, cu_blocks, cu_chunks, positions: as fdma_tables_extend leaves them. block_size 16, 32, 64 or 128, d a multiple of 16,
+ * at most 256. Entries of the table outside [0, num_blocks) are skipped.
+ */
+typedef struct fdma_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  const int32_t *table, *cu_seqlens, *lengths, *cu_blocks, *cu_chunks, *positions;
+  int32_t requests, width, num_blocks, block_size, tokens, h_k, d, reserved;
+} fdma_cache;
+
+/*
+ * Writes the step's keys and values (tokens, h_k, d) into the cache. Scale of a block and head: the smallest power of two (at
+ * least 2^-100) whose 448-fold is no less than the magnitude of every finite value written to it, or the scale that it has if
+ * that is larger and the block held tokens of the request before; these are then rounded once to the new scale. Places of a
+ * block before the request's tokens and behind them stay as they are. Values beyond 448 scales (infinities) become +-448
+ * scales, NaN stays NaN. With turns given, keys are turned first (as by fdma_rotary, in 32 bits up to the 8), and queries
+ * (tokens, h, d) into query_out; query may be NULL then, and is not used without turns. Two requests must not write to one block.
+ */
+typedef struct fdma_cache_append_params {
+  fdma_cache c;
+  const void *key, *value, *query;
+  void* query_out;
+  const int64_t* turns;
+  int64_t key_row_stride, key_head_stride, value_row_stride, value_head_stride;
+  int64_t query_row_stride, query_head_stride, out_row_stride, out_head_stride;
+  int32_t h, rotary_dim, interleaved, dtype;
+  float amplitude;
+  int32_t reserved;
+} fdma_cache_append_params;
+int fdma_cache_append(const fdma_cache_append_params* p, void* stream);
+
+/*
+ * Attention of the step's queries (tokens, h, d) over the cache: query i of a request with n new tokens of L sees the keys at
+ * positions up to L - n + i (is_causal = 0: all L). bias, if given: dtype of query, ({requests|1}, {h|h_k|1}, 1, bias_keys), added
+ * to the scaled scores, 0 for keys at bias_keys and beyond. kept_pos, if given: ascending positions ({requests|1}, {h_k|1},
+ * kept_capacity) of the keys that are attended to, kept_count of them or as many as are below L. Rows of tokens that belong to
+ * no request, of refused requests and of queries that see no key are 0. max_seqlen_q, max_seqlen_k: no request has more new
+ * tokens, or more tokens; queries and keys beyond are not looked at.
+ */
+typedef struct fdma_cache_attention_params {
+  fdma_cache c;
+  const void* query;
+  void* out;
+  const void* bias;
+  int64_t query_row_stride, query_head_stride, out_row_stride, out_head_stride;
+  int64_t bias_batch_stride, bias_head_stride;
+  const int32_t* kept_pos;
+  const int32_t* kept_count;
+  int64_t kept_batch_stride, kept_head_stride, count_batch_stride, count_head_stride;
+  int32_t h, dtype, is_causal, h_bias, bias_keys, kept_capacity, max_seqlen_q, max_seqlen_k;
+  float softmax_scale;
+  int32_t reserved;
+  void* workspace;
+  size_t workspace_bytes;
+} fdma_cache_attention_params;
+size_t fdma_cache_attention_workspace_bytes(const fdma_cache_attention_params* p);
+int fdma_cache_attention(const fdma_cache_attention_params* p, void* stream);
+
+/*
  * Measurement hook (no counterpart in the reference, which is timed from Python with wall clocks,
  * benchmarks/forward_performance.py:388-399). The NEXT fdma_fwd or fdma_bwd call made by this host thread
  * records `start_event` immediately before and `stop_event` immediately after its main attention kernel
