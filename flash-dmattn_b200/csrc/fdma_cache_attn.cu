@@ -3,148 +3,883 @@
 //   x_j = scale * q . k_j + bias_j over the visible keys j,  out = sum_j e^(x_j - max) v_j / sum_j e^(x_j - max),
 //   k_j = k_scale[block, head] * e4m3, v_j likewise
 //
-// A warp per (token, query head): a lane forms the score of one of 32 keys, then all lanes share the sum over the values.
+// Few queries over many keys: HBM-bound, 2 d bytes per key and kv head. What follows from that:
+//  * The queries of a request that share a kv head -- new tokens x query heads -- are the M rows of mma.m16n8k16, so a key is
+//    read once for all of them. The products are in fp16 with 32-bit sums: e4m3 numbers are fp16 numbers (one conversion
+//    instruction for two), bf16 queries become fp16 after a power of two per row (exact up to 2^-29 of the row's largest), and
+//    scales, being powers of two or common to a product, go into the scores and the softmax's exponents.
+//  * The unit of work is a chunk of 64 keys of a (request, kv head). All chunks of a step form one row; every CTA takes an equal
+//    part of it, however long the requests are, and starts and ends in the middle of a unit where it must. Such partial results
+//    go through scratch and a second kernel; units that one CTA finishes are written directly.
+//  * A warp of the CTA copies chunks to shared memory by TMA, three ahead; four warps take 16 keys of each. The 128-byte swizzle
+//    and the order in which keys are assigned to the columns of the products (`key_row`) make all reads free of bank conflicts:
+//    K fragments are 16-byte reads of a key's row, V fragments 4-byte reads of four keys whose bytes are then paired.
+//  * With a list of kept keys the warps gather their 16 rows themselves with cp.async into the same layout.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <math_constants.h>
 
 #include <algorithm>
 
 #include "fdma_internal.h"
+#include "fdma_ptx.cuh"
 
 namespace fdma {
+
+int check_cache(const fdma_cache& c);  // fdma_cache.cu
+
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kChunk = 64;
+constexpr int kWarps = 4;  // that compute; each has 16 keys of a chunk
+constexpr int kSlice = kChunk / kWarps;
+constexpr int kSearch = 256;  // requests whose chunk sums are held in shared memory
+constexpr int kMinShare = 2;  // chunks per CTA
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPScale = 16384.f;  // probabilities in fp16: normal numbers down to 2^-28
 
 struct AttnArgs {
   fdma_cache_attention_params p;
-  int shift;
+  int shift, group;
+  int list_chunks;  // kept keys: chunks per unit; 0: from cu_chunks
+  int ctas;         // along the row of chunks
   float scale_log2;
+  bool q_vec;       // queries in 16-byte vectors
+  float* partial;   // [row tile][cta][2][ROWS][D + 4]: sums over the values, then maximum and sum
+  int* status;
 };
 
-__device__ __forceinline__ float e4m3_to_f(uint32_t byte) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+// Where the work of a launch lies: unit u = (request, kv head) has the chunks [start, start + n) of the row.
+struct Unit {
+  int r, hk, n;
+  int64_t start;
+};
+
+// lowest key row of a slice's eight keys for column n of the products: pairs of lanes that read K together, and lanes that read
+// V together, then fall into different banks
+__device__ __forceinline__ int key_row(int n) { return n & 1 ? (((n >> 1) ^ 2) << 1) | 1 : n; }
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
+  return r;
 }
-template <typename T>
-__device__ __forceinline__ float load_f(const void* p, int64_t i) {
-  return static_cast<float>(static_cast<const T*>(p)[i]);
+__device__ __forceinline__ uint32_t e4m3x2_hi_to_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(two));
+  return r;
 }
+__device__ __forceinline__ void mma_f16(float (&c)[2], float (&c8)[2], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c8[0]), "+f"(c8[1]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+template <int kOffset>
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(v) : "r"(addr), "n"(kOffset) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+template <bool kBf16>
+__device__ __forceinline__ float raw_to_f(uint16_t u) {
+  if (kBf16) return __uint_as_float(static_cast<uint32_t>(u) << 16);
+  return __half2float(__ushort_as_half(u));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (kBf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) { return pack2<false>(lo, hi); }
 // In units of log2. The lowest finite number of a type stays finite, so that a row of nothing else is an average and not empty.
 __device__ __forceinline__ float bias_log2(float b) {
   const float x = b * kLog2e;
   return fabsf(x) > 3.0e38f && fabsf(b) != CUDART_INF_F ? copysignf(3.0e38f, b) : x;
 }
+__device__ __forceinline__ float exponent_of(float x) { return static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) - 127); }
+__device__ __forceinline__ float exp2_or_zero(float x) { return x == -CUDART_INF_F ? 0.f : exp2f(x); }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const AttnArgs a) {
-  __shared__ float s_q[kThreads / 32][256];
-  const fdma_cache_attention_params& p = a.p;
-  const fdma_cache& c = p.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp;
-  if (w >= static_cast<int64_t>(c.tokens) * p.h) return;
-  const int t = static_cast<int>(w / p.h), h = static_cast<int>(w - static_cast<int64_t>(t) * p.h), hk = h / (p.h / c.h_k);
-  T* out = static_cast<T*>(p.out) + t * p.out_row_stride + h * p.out_head_stride;
-  int lo = 0, hi = c.requests;  // first request whose tokens end behind t
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (c.cu_seqlens[mid + 1] > t) hi = mid;
-    else lo = mid + 1;
+// The units in the order of their chunks; s_cu holds cu_chunks for up to kSearch requests.
+struct Units {
+  const AttnArgs& a;
+  const int32_t* cu;
+  __device__ int64_t total() const {
+    return (a.list_chunks ? static_cast<int64_t>(a.p.c.requests) * a.list_chunks : static_cast<int64_t>(cu[a.p.c.requests])) * a.p.c.h_k;
   }
-  float o[8], m = -CUDART_INF_F, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = 0.f;
-  if (lo < c.requests && c.cu_chunks[lo + 1] > c.cu_chunks[lo]) {
-    for (int i = lane; i < c.d; i += 32) s_q[warp][i] = load_f<T>(p.query, t * p.query_row_stride + h * p.query_head_stride + i) * a.scale_log2;
-    __syncwarp();
-    const int n = c.cu_seqlens[lo + 1] - c.cu_seqlens[lo], length = min(min(c.lengths[lo], p.max_seqlen_k), c.width << a.shift);
-    const int newest = p.is_causal ? c.lengths[lo] - n + t - c.cu_seqlens[lo] : length;
-    const int32_t* list = p.kept_pos ? p.kept_pos + lo * p.kept_batch_stride + hk * p.kept_head_stride : nullptr;
-    int slots = length;
-    if (list) slots = p.kept_count ? min(p.kept_count[lo * p.count_batch_stride + hk * p.count_head_stride], p.kept_capacity) : p.kept_capacity;
-    const int hb = p.h_bias == p.h ? h : p.h_bias == c.h_k ? hk : 0;
-    for (int base = 0; base < slots; base += 32) {
-      const int slot = base + lane;
-      int pos = slot < slots ? (list ? list[slot] : slot) : -1;
-      if (pos < 0 || pos >= length || pos > newest) pos = -1;
-      int block = pos < 0 ? -1 : c.table[static_cast<int64_t>(lo) * c.width + (pos >> a.shift)];
-      if (block < 0 || block >= c.num_blocks) block = -1;
-      float x = -CUDART_INF_F, vs = 0.f;
-      int64_t row = 0;
-      if (block >= 0) {
-        const int64_t at = static_cast<int64_t>(block) * c.h_k + hk;
-        row = ((at << a.shift) + (pos & ((1 << a.shift) - 1))) * c.d;
-        const uint4* k = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(c.k) + row);
-        float s = 0.f;
-        for (int i = 0; i < c.d / 16; ++i) {
-          const uint4 v = k[i];
-          const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int j = 0; j < 16; ++j) s = fmaf(s_q[warp][16 * i + j], e4m3_to_f((words[j / 4] >> (8 * (j % 4))) & 0xFF), s);
-        }
-        x = s * c.k_scale[at];
-        if (p.bias && pos < p.bias_keys) x += bias_log2(load_f<T>(p.bias, lo * p.bias_batch_stride + hb * p.bias_head_stride + pos));
-        vs = c.v_scale[at];
+  __device__ Unit of_request(int r, int hk) const {
+    Unit u;
+    u.r = r;
+    u.hk = hk;
+    u.n = a.list_chunks ? a.list_chunks : cu[r + 1] - cu[r];
+    u.start = (a.list_chunks ? static_cast<int64_t>(r) * a.list_chunks : static_cast<int64_t>(cu[r])) * a.p.c.h_k + static_cast<int64_t>(hk) * u.n;
+    return u;
+  }
+  // the unit of chunk w, w < total()
+  __device__ Unit at(int64_t w) const {
+    const int64_t per_head = w / a.p.c.h_k;  // cu[r] <= per_head < cu[r + 1]
+    int r;
+    if (a.list_chunks) {
+      r = static_cast<int>(per_head / a.list_chunks);
+    } else {
+      int lo = 0, hi = a.p.c.requests - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid + 1] > per_head) hi = mid;
+        else lo = mid + 1;
       }
-      float mx = x;
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      const float m_new = fmaxf(m, mx), m_use = m_new == -CUDART_INF_F ? 0.f : m_new;
-      const float corr = m == -CUDART_INF_F ? 0.f : exp2f(m - m_use);
-      m = m_new;
-      const float e = x == -CUDART_INF_F ? 0.f : exp2f(x - m_use);
-      l = l * corr + e;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] *= corr;
-      for (int j = 0; j < 32; ++j) {
-        const float pj = __shfl_sync(0xffffffffu, e, j), vj = __shfl_sync(0xffffffffu, vs, j);
-        const int bj = __shfl_sync(0xffffffffu, block, j);
-        const int64_t rj = __shfl_sync(0xffffffffu, row, j);
-        if (bj < 0) continue;
-        const uint8_t* v = static_cast<const uint8_t*>(c.v) + rj;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i * 32 + lane < c.d) o[i] = fmaf(pj, vj * e4m3_to_f(v[i * 32 + lane]), o[i]);
-      }
+      r = lo;
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    Unit u = of_request(r, 0);
+    u.hk = static_cast<int>((w - u.start) / u.n);
+    u.start += static_cast<int64_t>(u.hk) * u.n;
+    return u;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i * 32 + lane < c.d) out[i * 32 + lane] = static_cast<T>(l == 0.f ? 0.f : o[i] / l);
+};
+__device__ __forceinline__ int64_t share_of(int64_t total, int ctas) { return max(static_cast<int64_t>(kMinShare), (total + ctas - 1) / ctas); }
+
+// Queries and keys of a unit's request, made safe against plans that do not fit the call.
+struct Request {
+  int token0, n, length, rows;
+};
+__device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
+  const fdma_cache& c = a.p.c;
+  Request q;
+  q.token0 = max(0, c.cu_seqlens[r]);
+  q.n = max(0, min(c.cu_seqlens[r + 1], c.tokens) - q.token0);
+  q.length = c.lengths[r];
+  q.rows = min(q.n, a.p.max_seqlen_q) * a.group;
+  if (a.list_chunks && c.cu_chunks[r + 1] <= c.cu_chunks[r]) q.rows = 0;  // refused (not among the chunks of a call without a list)
+  return q;
 }
 
-}  // namespace
+template <int D, int ROWS, bool kGather>
+struct Layout {
+  static constexpr int kHalves = D > 128 ? 2 : 1;                   // 128-byte tiles side by side
+  static constexpr int kTileBytes = kChunk * 128 * kHalves;         // K or V of a chunk
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kStages = D > 128 ? 2 : 3;
+  static constexpr int kSteps = D / 16;                             // k steps of Q K^T
+  static constexpr int kQBytes = (ROWS + 15) / 16 * kSteps * 512;
+  static constexpr int kBufFloats = ROWS * D;                       // one warp's sums
+  static constexpr int kBufs = D > 128 ? 1 : 2;
+  static constexpr int kRing = 0;
+  static constexpr int kQ = kRing + kStages * kStageBytes;
+  static constexpr int kBuf = kQ + kQBytes;
+  static constexpr int kTotal = kBuf + kBufs * kBufFloats * 4 + 1024;
+  static constexpr int kThreads = kWarps * 32 + (kGather ? 0 : 32);
+  static constexpr int kCtas = D > 128 || ROWS > 16 ? 2 : 3;        // per SM
+};
 
-int check_cache(const fdma_cache& c);
+template <int D, int ROWS, bool kGather, bool kBf16>
+__global__ void __launch_bounds__(Layout<D, ROWS, kGather>::kThreads, Layout<D, ROWS, kGather>::kCtas)
+cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+  using L = Layout<D, ROWS, kGather>;
+  constexpr int kGroups = ROWS / 8;  // eight rows each
+  constexpr int kTiles = (ROWS + 15) / 16;
+  extern __shared__ unsigned char s_raw[];
+  __shared__ __align__(8) uint64_t s_full[L::kStages], s_empty[L::kStages];
+  // of a slice: 1 if its block is there, K scale, exponent of the V scale, its reciprocal; of a kept key: bias (-inf: not there),
+  // K scale, exponent of the V scale, position
+  __shared__ float4 s_meta[L::kStages][kGather ? kChunk : kWarps];
+  __shared__ int32_t s_cu[kSearch + 1];
+  __shared__ float s_row_scale[ROWS], s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+  __shared__ int s_abort;
+  unsigned char* smem = align_smem_1024(s_raw);
+  const fdma_cache_attention_params& p = a.p;
+  const fdma_cache& c = p.c;
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
+  const int row0 = blockIdx.y * ROWS;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-}  // namespace fdma
+  const bool in_smem = !kGather && c.requests <= kSearch;
+  if (in_smem)
+    for (int i = tid; i <= c.requests; i += L::kThreads) s_cu[i] = c.cu_chunks[i];
+  if (tid == 0) {
+    s_abort = 0;
+    if (!kGather) {
+      for (int i = 0; i < L::kStages; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&s_empty[i], kWarps);
+      }
+      fence_mbar_init();
+    }
+  }
+  if (kGather && c.d < D)  // columns beyond the head dim stay zero in every stage
+    for (int i = tid; i < L::kStages * L::kStageBytes / 16; i += L::kThreads) reinterpret_cast<uint4*>(smem + L::kRing)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  const Units units{a, in_smem ? s_cu : c.cu_chunks};
+  const int64_t total = units.total(), share = share_of(total, a.ctas);
+  const int64_t w0 = min(total, blockIdx.x * share), w1 = min(total, w0 + share);
+  if (w0 >= w1) return;
+  const WaitCtl ctl{&s_abort, a.status};
 
-using namespace fdma;
+  if (!kGather && warp == kWarps) {
+    // ---- the copying warp: lanes look up the blocks and scales of eight chunks at a time, four 16-key slices each ----
+    const int pages = max(1, kChunk >> a.shift), rows_per_copy = min(kChunk, 1 << a.shift);
+    auto look_up = [&](int64_t w, int& block, int& row, int& hk, float& ks, float& vs, bool& used) {
+      block = -1;
+      row = hk = 0;
+      ks = vs = 0.f;
+      used = false;
+      if (w < w1) {
+        const Unit u = units.at(w);
+        hk = u.hk;
+        const Request q = request_of(a, u.r);
+        used = q.rows > row0;
+        const int pos = static_cast<int>(w - u.start) * kChunk + (lane & 3) * kSlice;
+        if (used && pos < min(q.length, p.max_seqlen_k) && (pos >> a.shift) < c.width) {
+          block = c.table[static_cast<int64_t>(u.r) * c.width + (pos >> a.shift)];
+          row = pos & ((1 << a.shift) - 1);
+          if (block < 0 || block >= c.num_blocks) block = -1;
+        }
+        if (block >= 0) {
+          ks = __ldg(c.k_scale + static_cast<int64_t>(block) * c.h_k + hk);
+          vs = fmaxf(__ldg(c.v_scale + static_cast<int64_t>(block) * c.h_k + hk), 0x1p-100f);
+        }
+      }
+    };
+    int block, row, hk, n_block, n_row, n_hk;
+    float ks, vs, n_ks, n_vs;
+    bool used, n_used;
+    look_up(w0 + (lane >> 2), n_block, n_row, n_hk, n_ks, n_vs, n_used);
+    int st = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    for (int64_t w = w0; w < w1; w += 8) {
+      block = n_block; row = n_row; hk = n_hk; ks = n_ks; vs = n_vs; used = n_used;
+      look_up(w + 8 + (lane >> 2), n_block, n_row, n_hk, n_ks, n_vs, n_used);
+      for (int i = 0; i < 8 && w + i < w1; ++i) {
+        if (!__shfl_sync(0xffffffffu, used, i * 4)) continue;  // no rows of this unit in this row tile
+        mbar_wait(&s_empty[st], phase ^ 1, ctl, 701);
+        if ((lane >> 2) == i)
+          s_meta[st][lane & 3] = make_float4(block >= 0 ? 1.f : 0.f, ks, exponent_of(vs), block >= 0 ? __frcp_rn(vs) : 0.f);
+        __syncwarp();
+        const int hk_i = __shfl_sync(0xffffffffu, hk, i * 4);
+        unsigned char* dst = smem + L::kRing + st * L::kStageBytes;
+        uint32_t bytes = 0;
+        int blocks[4], rows[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int first = g * (4 / pages);  // the page's first slice
+          blocks[g] = g < pages ? __shfl_sync(0xffffffffu, block, (i * 4 + first) & 31) : -1;
+          rows[g] = __shfl_sync(0xffffffffu, row, (i * 4 + first) & 31);
+          if (blocks[g] >= 0) bytes += 2u * rows_per_copy * 128 * L::kHalves;
+        }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&s_full[st], bytes);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            if (blocks[g] < 0) continue;
+            const int at = blocks[g] * c.h_k + hk_i;
+#pragma unroll
+            for (int x = 0; x < L::kHalves; ++x) {
+              unsigned char* to = dst + x * kChunk * 128 + g * rows_per_copy * 128;
+              tma_load_4d(to, &map_k, &s_full[st], x * 128, rows[g], at, 0);
+              tma_load_4d(to + L::kTileBytes, &map_v, &s_full[st], x * 128, rows[g], at, 0);
+            }
+          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++st == L::kStages) {
+          st = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    // after a wait that gave up: the copies in flight land before the CTA ends
+    if (s_abort) {
+      for (int i = 0; i < min(issued, L::kStages); ++i) {
+        if (st == 0) phase ^= 1;
+        st = st == 0 ? L::kStages - 1 : st - 1;
+        mbar_wait_limit(&s_full[st], phase, WaitCtl{&s_abort, a.status}, 703, 1000000ull);
+      }
+    }
+    return;
+  }
 
-extern "C" size_t fdma_cache_attention_workspace_bytes(const fdma_cache_attention_params*) { return 0; }
+  // ---- the computing warps ----
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(smem) + L::kRing + warp * kSlice * 128;
+  // K: row key_row(g), 16-byte piece t (^ 4 for the second four); V: rows key_row(2 t), key_row(2 t + 1), word g of 32 columns
+  const uint32_t k_at = key_row(g) * 128 + ((t ^ (key_row(g) & 7)) << 4);
+  const int r0 = key_row(2 * t), r1 = key_row(2 * t + 1);
+  const uint32_t v_at0 = L::kTileBytes + r0 * 128 + (((g >> 2) ^ (r0 & 7)) << 4) + (g & 3) * 4;
+  const uint32_t v_at1 = L::kTileBytes + r1 * 128 + (((g >> 2) ^ (r1 & 7)) << 4) + (g & 3) * 4;
+  const uint32_t q_at = smem_u32(smem) + L::kQ + lane * 16;
+  float* const s_buf = reinterpret_cast<float*>(smem + L::kBuf);
+  int st = 0;
+  uint32_t phase = 0;
+  int64_t w = w0;
+  while (w < w1) {
+    const Unit u = units.at(w);
+    const int64_t unit_end = max(u.start + u.n, w + 1);
+    const int first = static_cast<int>(w - u.start), last = static_cast<int>(min(unit_end, w1) - u.start);
+    const Request q = request_of(a, u.r);
+    w = min(unit_end, w1);
+    const int nrows = min(ROWS, q.rows - row0);
+    if (nrows <= 0) continue;
+    const int length = min(q.length, p.max_seqlen_k);
+    // oldest key that not every row sees
+    const int sure = p.is_causal ? min(length, q.length - q.n + row0 / a.group + 1) : length;
 
-extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void* stream) {
+    // queries: eight threads a row, to fp16 in the order of the fragments
+    consumers_sync();
+    for (int rr = tid >> 3; rr < kTiles * 16; rr += 16) {
+      constexpr int E = D / 8;  // elements per thread, in 16-byte vectors vec * 8 + part
+      const int part = tid & 7, row = row0 + rr;
+      uint32_t x[E / 2];
+      float most = 0.f;
+      const bool there = rr < nrows;
+      const uint16_t* src = static_cast<const uint16_t*>(p.query);
+      if (there) src += static_cast<int64_t>(q.token0 + row / a.group) * p.query_row_stride + (u.hk * a.group + row % a.group) * p.query_head_stride;
+#pragma unroll
+      for (int e = 0; e < E / 8; ++e) {
+        const int at = (e * 8 + part) * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (there && at < c.d) {
+          if (a.q_vec) {
+            v = *reinterpret_cast<const uint4*>(src + at);
+          } else {
+            uint32_t y[4];
+            for (int j = 0; j < 4; ++j) y[j] = src[at + 2 * j] | static_cast<uint32_t>(src[at + 2 * j + 1]) << 16;
+            v = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+        x[4 * e] = v.x; x[4 * e + 1] = v.y; x[4 * e + 2] = v.z; x[4 * e + 3] = v.w;
+      }
+      float scale = 1.f;
+      if (kBf16) {
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e)
+#pragma unroll
+          for (int hw = 0; hw < 2; ++hw) {
+            const float f = fabsf(raw_to_f<true>(static_cast<uint16_t>(x[e] >> (16 * hw))));
+            if (f < CUDART_INF_F) most = fmaxf(most, f);
+          }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // the largest becomes 2^13 ... 2^14
+        const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100), 127) - 13;
+        scale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        if (part == 0 && rr < ROWS) s_row_scale[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      } else if (part == 0 && rr < ROWS) {
+        s_row_scale[rr] = a.scale_log2;
+      }
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        uint32_t y = x[e];
+        if (kBf16) y = pack_f16(raw_to_f<true>(static_cast<uint16_t>(y)) * scale, raw_to_f<true>(static_cast<uint16_t>(y >> 16)) * scale);
+        const int dd = ((e >> 2) * 8 + part) * 8 + (e & 3) * 2;  // element of the row
+        const int step = (dd >> 6) * 4 + ((dd >> 2) & 3), to_lane = (rr & 7) * 4 + ((dd >> 4) & 3);
+        const int reg = ((rr >> 3) & 1) + ((dd >> 1) & 1) * 2;
+        reinterpret_cast<uint32_t*>(smem + L::kQ)[(((rr >> 4) * L::kSteps + step) * 32 + to_lane) * 4 + reg] = y;
+      }
+    }
+    consumers_sync();
+
+    float o[kGroups][D / 32][4][2], m[kGroups], l[kGroups], row_scale[kGroups];
+    int newest[kGroups];
+    const uint16_t* bias_row[kGroups];
+#pragma unroll
+    for (int rs = 0; rs < kGroups; ++rs) {
+      m[rs] = -CUDART_INF_F;
+      l[rs] = 0.f;
+      const int row = row0 + min(g + 8 * rs, nrows - 1);
+      row_scale[rs] = s_row_scale[min(g + 8 * rs, nrows - 1)];
+      newest[rs] = p.is_causal ? min(length - 1, q.length - q.n + row / a.group) : length - 1;
+      const int head = u.hk * a.group + row % a.group;
+      bias_row[rs] = p.bias ? static_cast<const uint16_t*>(p.bias) + u.r * p.bias_batch_stride +
+                                  (p.h_bias == p.h ? head : p.h_bias == c.h_k ? u.hk : 0) * p.bias_head_stride
+                            : nullptr;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[rs][j][i][0] = o[rs][j][i][1] = 0.f;
+    }
+    float zero[2] = {0.f, 0.f};  // rows 8-15 where there are none: always zero
+
+    // Kept keys: at chunk i the rows of chunk i + kAhead are asked for, the block numbers of the one behind it and the positions
+    // of the next, so that nothing here waits for a load of its own. Lanes 0 - 15 stand for the slice's keys.
+    constexpr int kAhead = L::kStages - 1;
+    const int32_t* list = nullptr;
+    int slots = 0, pos2 = -1, pos3 = -1, block2 = -1;
+    float g_scale_k = 0.f, g_scale_v = 1.f, g_add = 0.f;
+    int g_pos = -1;
+    const bool head_bias = p.bias && p.h_bias == p.h && a.group > 1;
+    auto load_pos = [&](int chunk) {
+      const int slot = chunk * kChunk + warp * kSlice + (lane & 15);
+      return chunk < last && slot < slots ? __ldg(list + slot) : -1;
+    };
+    auto load_block = [&](int& pos) {
+      if (pos < 0 || pos >= length || (pos >> a.shift) >= c.width) pos = -1;
+      return pos < 0 ? -1 : __ldg(c.table + static_cast<int64_t>(u.r) * c.width + (pos >> a.shift));
+    };
+    if (kGather) {
+      list = p.kept_pos + u.r * p.kept_batch_stride + u.hk * p.kept_head_stride;
+      slots = p.kept_count ? min(p.kept_count[u.r * p.count_batch_stride + u.hk * p.count_head_stride], p.kept_capacity) : p.kept_capacity;
+      pos2 = load_pos(first);
+      pos3 = load_pos(first + 1);
+      block2 = load_block(pos2);
+    }
+    auto gather = [&](int i) {       // st: the stage of chunk i
+      if (i + kAhead - 1 >= first) {  // what the iteration before has loaded about chunk i + kAhead - 1
+        const int at = (st + kAhead - 1) % L::kStages;
+        if (lane < kSlice)
+          s_meta[at][warp * kSlice + lane] = make_float4(g_pos < 0 ? -CUDART_INF_F : g_add, g_scale_k, exponent_of(g_scale_v), __int_as_float(g_pos));
+      }
+      if (block2 < 0 || block2 >= c.num_blocks) pos2 = block2 = -1;
+      g_pos = pos2;
+      if (pos2 >= 0) {
+        const int64_t at = static_cast<int64_t>(block2) * c.h_k + u.hk;
+        g_scale_k = __ldg(c.k_scale + at);
+        g_scale_v = fmaxf(__ldg(c.v_scale + at), 0x1p-100f);
+        g_add = p.bias && !head_bias && pos2 < p.bias_keys ? bias_log2(raw_to_f<kBf16>(__ldg(bias_row[0] + pos2))) : 0.f;
+      }
+      if (i + kAhead < last) {
+        constexpr int kLanes = D / 16;  // 16-byte pieces of a row
+        const int piece = lane % kLanes;
+        const uint32_t dst = ring + (st == 0 ? L::kStages - 1 : st - 1) * L::kStageBytes + (piece >> 3) * kChunk * 128;
+#pragma unroll
+        for (int r = lane / kLanes; r < kSlice; r += 32 / kLanes) {
+          const int pos = __shfl_sync(0xffffffffu, pos2, r), block = __shfl_sync(0xffffffffu, block2, r);
+          const uint32_t to = dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+          if (piece * 16 < c.d) {
+            if (pos >= 0) {
+              const int64_t row = ((static_cast<int64_t>(block) * c.h_k + u.hk) << a.shift) + (pos & ((1 << a.shift) - 1));
+              cp_async16(to, static_cast<const uint8_t*>(c.k) + row * c.d + piece * 16);
+              cp_async16(to + L::kTileBytes, static_cast<const uint8_t*>(c.v) + row * c.d + piece * 16);
+            } else {
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to), "r"(0) : "memory");
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to + L::kTileBytes), "r"(0) : "memory");
+            }
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      pos2 = pos3;
+      block2 = load_block(pos2);
+      pos3 = load_pos(i + kAhead + 2);
+    };
+    if (kGather) {
+      st = L::kStages - kAhead;
+      for (int i = first - kAhead; i < first; ++i) {
+        gather(i);
+        if (++st == L::kStages) st = 0;
+      }
+    }
+
+    for (int chunk = first; chunk < last; ++chunk) {
+      const int pos0 = chunk * kChunk + warp * kSlice;
+      if (kGather) gather(chunk);
+      uint16_t raw_bias[kGroups][4];
+      const bool with_bias = !kGather && p.bias;
+      if (with_bias) {
+#pragma unroll
+        for (int rs = 0; rs < kGroups; ++rs)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int pos = pos0 + (k >> 1) * 8 + (k & 1 ? r1 : r0);
+            raw_bias[rs][k] = pos < min(length, p.bias_keys) ? __ldg(bias_row[rs] + pos) : static_cast<uint16_t>(0);
+          }
+      }
+      float4 meta;
+      float4 key_meta[4];
+      if (kGather) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) key_meta[k] = s_meta[st][warp * kSlice + (k >> 1) * 8 + (k & 1 ? r1 : r0)];
+      } else {
+        mbar_wait(&s_full[st], phase, ctl, 702);
+        meta = s_meta[st][warp];
+      }
+      const uint32_t tile = ring + st * L::kStageBytes;
+      // scores: s[row group][keys 0-7 | 8-15][column pair]
+      float s[kGroups][2][2];
+#pragma unroll
+      for (int rs = 0; rs < kGroups; ++rs) s[rs][0][0] = s[rs][0][1] = s[rs][1][0] = s[rs][1][1] = 0.f;
+#pragma unroll
+      for (int jj = 0; jj < D / 64; ++jj) {
+        const uint32_t at = tile + (jj >> 1) * kChunk * 128 + (k_at ^ ((jj & 1) << 6));
+        const uint4 ka = lds128(at), kb = lds128(at + 1024);
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t a0 = e4m3x2_to_f16x2(wa[x]), a1 = e4m3x2_hi_to_f16x2(wa[x]);
+          const uint32_t b0 = e4m3x2_to_f16x2(wb[x]), b1 = e4m3x2_hi_to_f16x2(wb[x]);
+#pragma unroll
+          for (int mt = 0; mt < kTiles; ++mt) {
+            const uint4 f = lds128(q_at + (mt * L::kSteps + jj * 4 + x) * 512);
+            mma_f16(s[2 * mt][0], ROWS > 8 ? s[(2 * mt + 1) % kGroups][0] : zero, f.x, f.y, f.z, f.w, a0, a1);
+            mma_f16(s[2 * mt][1], ROWS > 8 ? s[(2 * mt + 1) % kGroups][1] : zero, f.x, f.y, f.z, f.w, b0, b1);
+          }
+        }
+      }
+      // all 16 keys are there and seen by every row
+      const bool clean = !kGather && pos0 + kSlice <= sure && meta.x != 0.f;
+      uint32_t pa[kGroups][2];
+      float inv_v[4];
+      if (kGather) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) inv_v[k] = exp2f(-key_meta[k].z);
+      }
+#pragma unroll
+      for (int rs = 0; rs < kGroups; ++rs) {
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (kGather) {
+            const int pos = __float_as_int(key_meta[k].w);
+            float add = key_meta[k].x;
+            if (head_bias && pos >= 0 && pos < p.bias_keys) add = bias_log2(raw_to_f<kBf16>(__ldg(bias_row[rs] + pos)));
+            x[k] = fmaf(s[rs][k >> 1][k & 1], row_scale[rs] * key_meta[k].y, add) + key_meta[k].z;
+            if (pos < 0 || pos > newest[rs]) x[k] = -CUDART_INF_F;
+          } else {
+            x[k] = s[rs][k >> 1][k & 1] * (row_scale[rs] * meta.y);
+            if (with_bias) x[k] += bias_log2(raw_to_f<kBf16>(raw_bias[rs][k]));
+            x[k] += meta.z;
+            if (!clean && (pos0 + (k >> 1) * 8 + (k & 1 ? r1 : r0) > newest[rs] || meta.x == 0.f)) x[k] = -CUDART_INF_F;
+          }
+        }
+        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (__any_sync(0xffffffffu, mx > m[rs])) {
+          const float m_new = fmaxf(m[rs], mx);
+          const float corr = exp2_or_zero(m[rs] - (m_new == -CUDART_INF_F ? 0.f : m_new));
+          m[rs] = m_new;
+          l[rs] *= corr;
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[rs][j][i][0] *= corr;
+              o[rs][j][i][1] *= corr;
+            }
+        }
+        const float base = m[rs] == -CUDART_INF_F ? 0.f : m[rs];
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = exp2f(x[k] - base);
+        if (kGather) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) l[rs] = fmaf(e[k], inv_v[k], l[rs]);
+        } else {
+          l[rs] = fmaf((e[0] + e[1]) + (e[2] + e[3]), meta.w, l[rs]);
+        }
+        pa[rs][0] = pack_f16(e[0] * kPScale, e[1] * kPScale);
+        pa[rs][1] = pack_f16(e[2] * kPScale, e[3] * kPScale);
+      }
+      const bool whole = kGather || (pos0 + kSlice <= length && meta.x != 0.f);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const uint32_t half = tile + (j >> 2) * kChunk * 128;
+        const uint32_t at0 = half + (v_at0 ^ ((j & 3) << 5)), at1 = half + (v_at1 ^ ((j & 3) << 5));
+        uint32_t y0 = lds32<0>(at0), y1 = lds32<0>(at1), y2 = lds32<1024>(at0), y3 = lds32<1024>(at1);
+        if (!whole) {  // what lies behind the last key may be anything
+          if (meta.x == 0.f || pos0 + r0 >= length) y0 = 0;
+          if (meta.x == 0.f || pos0 + r1 >= length) y1 = 0;
+          if (meta.x == 0.f || pos0 + 8 + r0 >= length) y2 = 0;
+          if (meta.x == 0.f || pos0 + 8 + r1 >= length) y3 = 0;
+        }
+        const uint32_t lo01 = __byte_perm(y0, y1, 0x5140), hi01 = __byte_perm(y0, y1, 0x7362);
+        const uint32_t lo23 = __byte_perm(y2, y3, 0x5140), hi23 = __byte_perm(y2, y3, 0x7362);
+        const uint32_t b0[4] = {e4m3x2_to_f16x2(lo01), e4m3x2_hi_to_f16x2(lo01), e4m3x2_to_f16x2(hi01), e4m3x2_hi_to_f16x2(hi01)};
+        const uint32_t b1[4] = {e4m3x2_to_f16x2(lo23), e4m3x2_hi_to_f16x2(lo23), e4m3x2_to_f16x2(hi23), e4m3x2_hi_to_f16x2(hi23)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int mt = 0; mt < kTiles; ++mt)
+            mma_f16(o[2 * mt][j][i], ROWS > 8 ? o[(2 * mt + 1) % kGroups][j][i] : zero, pa[2 * mt][0], ROWS > 8 ? pa[(2 * mt + 1) % kGroups][0] : 0u,
+                    pa[2 * mt][1], ROWS > 8 ? pa[(2 * mt + 1) % kGroups][1] : 0u, b0[i], b1[i]);
+      }
+      __syncwarp();  // every lane has read the stage before it is overwritten
+      if (!kGather && lane == 0) mbar_arrive(&s_empty[st]);
+      if (++st == L::kStages) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
+
+    // ---- the four warps' sums: to a common maximum, then added up through shared memory ----
+#pragma unroll
+    for (int rs = 0; rs < kGroups; ++rs) {
+      l[rs] += __shfl_xor_sync(0xffffffffu, l[rs], 1);
+      l[rs] += __shfl_xor_sync(0xffffffffu, l[rs], 2);
+      if (t == 0) {
+        s_m[warp][g + 8 * rs] = m[rs];
+        s_l[warp][g + 8 * rs] = l[rs];
+      }
+    }
+    consumers_sync();
+#pragma unroll
+    for (int rs = 0; rs < kGroups; ++rs) {
+      float cm = -CUDART_INF_F, cl = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) cm = fmaxf(cm, s_m[x][g + 8 * rs]);
+      const float base = cm == -CUDART_INF_F ? 0.f : cm;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) cl = fmaf(s_l[x][g + 8 * rs], exp2_or_zero(s_m[x][g + 8 * rs] - base), cl);
+      const float f = exp2_or_zero(m[rs] - base) * (1.f / kPScale);
+      m[rs] = cm;
+      l[rs] = cl;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[rs][j][i][0] *= f;
+          o[rs][j][i][1] *= f;
+        }
+    }
+    auto put = [&](float* buf) {
+#pragma unroll
+      for (int rs = 0; rs < kGroups; ++rs)
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            *reinterpret_cast<float4*>(buf + ((rs * (D / 32) + j) * 2 + x) * 128 + lane * 4) =
+                make_float4(o[rs][j][0][x], o[rs][j][1][x], o[rs][j][2][x], o[rs][j][3][x]);
+    };
+    auto add = [&](const float* buf) {
+#pragma unroll
+      for (int rs = 0; rs < kGroups; ++rs)
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float4 y = *reinterpret_cast<const float4*>(buf + ((rs * (D / 32) + j) * 2 + x) * 128 + lane * 4);
+            o[rs][j][0][x] += y.x; o[rs][j][1][x] += y.y; o[rs][j][2][x] += y.z; o[rs][j][3][x] += y.w;
+          }
+    };
+    if constexpr (L::kBufs == 2) {
+      if (warp >= 2) put(s_buf + (warp - 2) * L::kBufFloats);
+      consumers_sync();
+      if (warp < 2) add(s_buf + warp * L::kBufFloats);
+      consumers_sync();
+      if (warp == 1) put(s_buf);
+      consumers_sync();
+      if (warp == 0) add(s_buf);
+    } else {
+      for (int x = kWarps - 1; x > 0; --x) {
+        if (warp == x) put(s_buf);
+        consumers_sync();
+        if (warp == 0) add(s_buf);
+        consumers_sync();
+      }
+    }
+    if (warp != 0) continue;
+    const bool complete = first == 0 && last == u.n;
+    float* part = a.partial + ((static_cast<int64_t>(blockIdx.y) * a.ctas + blockIdx.x) * 2 + (first > 0 ? 0 : 1)) * ROWS * (D + 4);
+#pragma unroll
+    for (int rs = 0; rs < kGroups; ++rs) {
+      const int rr = g + 8 * rs, row = row0 + rr;
+      if (rr >= nrows) continue;
+      if (complete) {
+        const float inv = l[rs] == 0.f ? 0.f : 1.f / l[rs];
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(q.token0 + row / a.group) * p.out_row_stride +
+                        (u.hk * a.group + row % a.group) * p.out_head_stride;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const int dd = 32 * j + 8 * t;
+          if (dd < c.d) {
+            const float(&y)[4][2] = o[rs][j];
+            *reinterpret_cast<uint4*>(dst + dd) =
+                make_uint4(pack2<kBf16>(y[0][0] * inv, y[1][0] * inv), pack2<kBf16>(y[2][0] * inv, y[3][0] * inv),
+                           pack2<kBf16>(y[0][1] * inv, y[1][1] * inv), pack2<kBf16>(y[2][1] * inv, y[3][1] * inv));
+          }
+        }
+      } else {
+        float* dst = part + rr * (D + 4);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const float(&y)[4][2] = o[rs][j];
+          *reinterpret_cast<float4*>(dst + 32 * j + 8 * t) = make_float4(y[0][0], y[1][0], y[2][0], y[3][0]);
+          *reinterpret_cast<float4*>(dst + 32 * j + 8 * t + 4) = make_float4(y[0][1], y[1][1], y[2][1], y[3][1]);
+        }
+        if (t == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[rs], l[rs]);
+      }
+    }
+  }
+}
+
+// Joins the sums of units that several CTAs share, and writes the zeros of rows that nobody computes: a warp per (token, head).
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant__ AttnArgs a, const int rows_per_tile) {
+  const fdma_cache_attention_params& p = a.p;
+  const fdma_cache& c = p.c;
+  const int lane = threadIdx.x & 31;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (id >= static_cast<int64_t>(c.tokens) * p.h) return;
+  const int token = static_cast<int>(id / p.h), head = static_cast<int>(id - static_cast<int64_t>(token) * p.h);
+  int lo = 0, hi = c.requests;  // first request whose tokens end behind this one
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (c.cu_seqlens[mid + 1] > token) hi = mid;
+    else lo = mid + 1;
+  }
+  constexpr int E = D / 32;  // elements per lane
+  float acc[E], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) acc[i] = 0.f;
+  const Units units{a, c.cu_chunks};
+  const int64_t total = units.total(), share = share_of(total, a.ctas);
+  if (lo < c.requests) {
+    const Request q = request_of(a, lo);
+    const int row = (token - q.token0) * a.group + head % a.group;
+    const Unit u = units.of_request(lo, head / a.group);
+    if (row >= 0 && row < q.rows && u.n > 0) {
+      const int c0 = static_cast<int>(u.start / share), c1 = static_cast<int>((u.start + u.n - 1) / share);
+      if (c0 == c1) return;  // written by that CTA
+      const int tile = row / rows_per_tile;
+      const float* base = a.partial + ((static_cast<int64_t>(tile) * a.ctas * 2) * rows_per_tile + row - tile * rows_per_tile) * (D + 4);
+      const int64_t step = static_cast<int64_t>(rows_per_tile) * (D + 4);
+      float top = -CUDART_INF_F;
+      for (int x = c0 + lane; x <= c1; x += 32) top = fmaxf(top, base[(2 * static_cast<int64_t>(x) + (x == c0)) * step + D]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float from = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll 4
+      for (int x = c0; x <= c1; ++x) {
+        const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
+        const float2 ml = *reinterpret_cast<const float2*>(src + D);
+        const float f = exp2_or_zero(ml.x - from);
+        sum = fmaf(ml.y, f, sum);
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+          const float2 y = *reinterpret_cast<const float2*>(src + lane * E + i);
+          acc[i] = fmaf(y.x, f, acc[i]);
+          acc[i + 1] = fmaf(y.y, f, acc[i + 1]);
+        }
+      }
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + token * p.out_row_stride + head * p.out_head_stride;
+#pragma unroll
+  for (int i = 0; i < E; i += 2)
+    if (lane * E + i < c.d) *reinterpret_cast<uint32_t*>(dst + lane * E + i) = pack2<kBf16>(acc[i] * inv, acc[i + 1] * inv);
+}
+
+int tile_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+struct Plan {
+  int D, rows, tiles, ctas, list_chunks;
+  size_t bytes;
+};
+Plan plan_of(const fdma_cache_attention_params& p) {
+  Plan pl;
+  const int64_t most = static_cast<int64_t>(std::min(p.max_seqlen_q, p.c.tokens)) * (p.h / p.c.h_k);
+  pl.D = tile_dim(p.c.d);
+  // rows of a tile: as few as hold the queries of a request, up to what the accumulators leave registers for
+  pl.rows = most <= 8 ? 8 : most <= 16 || pl.D == 256 ? 16 : 32;
+  pl.tiles = static_cast<int>(std::max<int64_t>(1, (most + pl.rows - 1) / pl.rows));
+  const int resident = (pl.D == 256 || pl.rows == 32 ? 2 : 3) * sm_count();
+  pl.ctas = std::max(1, resident / pl.tiles);
+  pl.list_chunks = p.kept_pos ? (p.kept_capacity + kChunk - 1) / kChunk : 0;
+  pl.bytes = align256(static_cast<size_t>(pl.tiles) * pl.ctas * 2 * pl.rows * (pl.D + 4) * sizeof(float));
+  return pl;
+}
+
+template <int D, int ROWS, bool kGather, bool kBf16>
+int launch(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
+  using L = Layout<D, ROWS, kGather>;
+  const fdma_cache& c = a.p.c;
+  CUtensorMap map_k{}, map_v{};
+  if (!kGather) {
+    const uint64_t d = c.d, bs = c.block_size, heads = static_cast<uint64_t>(c.num_blocks) * c.h_k;
+    const uint64_t dims[4] = {d, bs, heads, 1}, strides[3] = {d, bs * d, heads * bs * d};
+    const uint32_t box[4] = {128, std::min<uint32_t>(bs, kChunk), 1, 1};
+    int st = encode_tmap_4d(&map_k, c.k, 1, dims, strides, box);
+    if (!st) st = encode_tmap_4d(&map_v, c.v, 1, dims, strides, box);
+    if (st) return st;
+  }
+  auto kern = cache_attend_kernel<D, ROWS, kGather, kBf16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  kern<<<dim3(pl.ctas, pl.tiles), L::kThreads, L::kTotal, stream>>>(a, map_k, map_v);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  // the second kernel's CTAs start while the first one's finish, and wait for them only where they need their sums
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(c.tokens) * a.p.h + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, cache_merge_kernel<D, kBf16>, a, ROWS));
+}
+template <int D, int ROWS>
+int launch_t(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
+  const bool bf16 = a.p.dtype == FDMA_BF16;
+  if (a.list_chunks) return bf16 ? launch<D, ROWS, true, true>(a, pl, stream) : launch<D, ROWS, true, false>(a, pl, stream);
+  return bf16 ? launch<D, ROWS, false, true>(a, pl, stream) : launch<D, ROWS, false, false>(a, pl, stream);
+}
+
+int check_attention(const fdma_cache_attention_params* pp) {
   if (!pp) return FDMA_ERR_BAD_ARG;
   const fdma_cache_attention_params& p = *pp;
   const int st = check_cache(p.c);
   if (st) return st;
-  if (p.c.tokens == 0) return FDMA_OK;
-  if (!p.query || !p.out || p.h <= 0 || p.h % p.c.h_k || p.max_seqlen_q < 0 || p.max_seqlen_k < 0) return FDMA_ERR_BAD_ARG;
+  if (p.h <= 0 || p.h % p.c.h_k || p.max_seqlen_q < 0 || p.max_seqlen_k < 0) return FDMA_ERR_BAD_ARG;
   if (p.bias && ((p.h_bias != 1 && p.h_bias != p.c.h_k && p.h_bias != p.h) || p.bias_keys <= 0)) return FDMA_ERR_BAD_ARG;
   if (p.kept_pos && p.kept_capacity <= 0) return FDMA_ERR_BAD_ARG;
   if (p.dtype != FDMA_BF16 && p.dtype != FDMA_FP16) return FDMA_ERR_UNSUPPORTED;
-  AttnArgs a;
+  if (static_cast<int64_t>(p.c.num_blocks) * p.c.h_k > 0x7FFFFFFF || static_cast<int64_t>(p.c.tokens) * p.h > (1ll << 32)) return FDMA_ERR_UNSUPPORTED;
+  return 0;
+}
+
+}  // namespace
+}  // namespace fdma
+
+using namespace fdma;
+
+extern "C" size_t fdma_cache_attention_workspace_bytes(const fdma_cache_attention_params* p) {
+  if (check_attention(p) || p->c.tokens == 0) return 0;
+  return plan_of(*p).bytes;
+}
+
+extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void* stream_) {
+  const int st = check_attention(pp);
+  if (st) return st;
+  const fdma_cache_attention_params& p = *pp;
+  if (p.c.tokens == 0) return FDMA_OK;
+  if (!p.query || !p.out) return FDMA_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uint64_t>(p.out_row_stride | p.out_head_stride) * 2) % 16) return FDMA_ERR_UNSUPPORTED;
+  const Plan pl = plan_of(p);
+  if (!p.workspace || p.workspace_bytes < pl.bytes) return FDMA_ERR_WORKSPACE;
+  if (pl.tiles > 65535) return FDMA_ERR_UNSUPPORTED;
+  AttnArgs a = {};
   a.p = p;
   a.shift = p.c.block_size == 16 ? 4 : p.c.block_size == 32 ? 5 : p.c.block_size == 64 ? 6 : 7;
+  a.group = p.h / p.c.h_k;
+  a.list_chunks = pl.list_chunks;
+  a.ctas = pl.ctas;
   a.scale_log2 = p.softmax_scale * kLog2e;
-  const int64_t ctas = (static_cast<int64_t>(p.c.tokens) * p.h + 3) / 4;
-  if (ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
-  if (p.dtype == FDMA_BF16) attend_kernel<__nv_bfloat16><<<static_cast<unsigned>(ctas), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  else attend_kernel<__half><<<static_cast<unsigned>(ctas), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  return static_cast<int>(cudaGetLastError());
+  a.q_vec = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uint64_t>(p.query_row_stride | p.query_head_stride) * 2) % 16 == 0;
+  a.partial = static_cast<float*>(p.workspace);
+  a.status = kernel_status_ptr();
+  if (!a.status) return FDMA_ERR_DRIVER;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (pl.D == 256) return pl.rows == 8 ? launch_t<256, 8>(a, pl, stream) : launch_t<256, 16>(a, pl, stream);
+  if (pl.D == 128) return pl.rows == 8 ? launch_t<128, 8>(a, pl, stream) : pl.rows == 16 ? launch_t<128, 16>(a, pl, stream) : launch_t<128, 32>(a, pl, stream);
+  return pl.rows == 8 ? launch_t<64, 8>(a, pl, stream) : pl.rows == 16 ? launch_t<64, 16>(a, pl, stream) : launch_t<64, 32>(a, pl, stream);
 }
