@@ -109,6 +109,10 @@ __device__ __forceinline__ float bias_log2(float b) {
   const float x = b * kLog2e;
   return fabsf(x) > 3.0e38f && fabsf(b) != CUDART_INF_F ? copysignf(3.0e38f, b) : x;
 }
+// Scales below 2^-100 stand for zeros: the keys count in the softmax's sum (which a smaller scale could carry out of range: it is
+// held in units of the probabilities times the V scales), and their values do not count.
+__device__ __forceinline__ float value_scale(float x) { return x < 0x1p-100f ? 0x1p-101f : x; }
+__device__ __forceinline__ float p_scale(float exponent) { return exponent < -100.f ? 0.f : kPScale; }
 __device__ __forceinline__ float exponent_of(float x) { return static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) - 127); }
 __device__ __forceinline__ float exp2_or_zero(float x) { return x == -CUDART_INF_F ? 0.f : exp2f(x); }
 
@@ -247,7 +251,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
         if (block >= 0) {
           ks = __ldg(c.k_scale + static_cast<int64_t>(block) * c.h_k + hk);
-          vs = fmaxf(__ldg(c.v_scale + static_cast<int64_t>(block) * c.h_k + hk), 0x1p-100f);
+          vs = value_scale(__ldg(c.v_scale + static_cast<int64_t>(block) * c.h_k + hk));
         }
       }
     };
@@ -446,7 +450,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       if (pos2 >= 0) {
         const int64_t at = static_cast<int64_t>(block2) * c.h_k + u.hk;
         g_scale_k = __ldg(c.k_scale + at);
-        g_scale_v = fmaxf(__ldg(c.v_scale + at), 0x1p-100f);
+        g_scale_v = value_scale(__ldg(c.v_scale + at));
         g_add = p.bias && !head_bias && pos2 < p.bias_keys ? bias_log2(raw_to_f<kBf16>(__ldg(bias_row[0] + pos2))) : 0.f;
       }
       if (i + kAhead < last) {
@@ -581,8 +585,10 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         } else {
           l[rs] = fmaf((e[0] + e[1]) + (e[2] + e[3]), meta.w, l[rs]);
         }
-        pa[rs][0] = pack_f16(e[0] * kPScale, e[1] * kPScale);
-        pa[rs][1] = pack_f16(e[2] * kPScale, e[3] * kPScale);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] *= p_scale(kGather ? key_meta[k].z : meta.z);
+        pa[rs][0] = pack_f16(e[0], e[1]);
+        pa[rs][1] = pack_f16(e[2], e[3]);
       }
       const bool whole = kGather || (pos0 + kSlice <= length && meta.x != 0.f);
 #pragma unroll

@@ -71,6 +71,9 @@ int dtype_code(const Tensor& t) {
 // 0 along dimensions of one element, whose stride says nothing
 int64_t stride_of(const Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
 
+Tensor given(const OptTensor& t) { return t ? *t : Tensor(); }
+OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
 // ---- rotary positions -----------------------------------------------------------------------------------------------
 struct Rotation {
   Tensor turns;
@@ -130,13 +133,13 @@ variable_list rotate_differentiable(const Tensor& q, const Tensor& k, const Tens
 
 // The gradient of a rotation is the rotation by the negative angle, itself differentiable.
 struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
-  static variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& positions,
+  static variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& positions,
                                const Tensor& turns, bool interleaved, bool inverse, double amplitude) {
-    ctx->save_for_backward({positions, turns});
+    ctx->save_for_backward({given(positions), turns});
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["inverse"] = inverse;
     ctx->saved_data["amplitude"] = amplitude;
-    return rotate(q, k, positions, Rotation{turns, interleaved, inverse, amplitude});
+    return rotate(q, given(k), given(positions), Rotation{turns, interleaved, inverse, amplitude});
   }
   static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
@@ -158,7 +161,7 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 
 variable_list rotate_differentiable(const Tensor& q, const Tensor& k, const Tensor& positions, const Rotation& r) {
   if (at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad())))
-    return RotaryFunction::apply(q, k, positions, r.turns, r.interleaved, r.inverse, r.amplitude);
+    return RotaryFunction::apply(q, optional(k), optional(positions), r.turns, r.interleaved, r.inverse, r.amplitude);
   return rotate(q, k, positions, r);
 }
 

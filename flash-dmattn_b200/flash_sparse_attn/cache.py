@@ -13,7 +13,7 @@ None of these synchronises; a whole step can be captured into a CUDA graph and r
 activations. The reference's packed-sequence call has a `block_table` argument for 16-bit caches
 (flash_sparse_attn/flash_sparse_attn_interface.py:687-790); it has no 8-bit cache.
 """
-from typing import List, NamedTuple, Optional, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -51,7 +51,8 @@ class BlockTables(NamedTuple):
         """Gives request r new_lengths[r] more tokens (int32 on the GPU; 0: none in this step) and the blocks these need.
         total_tokens: tokens of the step's activations, at least the sum of new_lengths (more: a padded step). A request that
         would outgrow its table row or total_tokens, or for which no blocks are left, is refused: it keeps what it has,
-        `step.granted` is False, its tokens are written nowhere and their attention is 0. Requests are served in order."""
+        `step.granted` is False, its tokens are written nowhere and their attention is 0. Requests are served in order, and behind
+        one for which no blocks were left none gets any, however few it asks for."""
         native = _native.load()
         args = (self.table, self.lengths, self.free, self.free_count, self.ticket, new_lengths)
         out = None
@@ -206,10 +207,11 @@ def _plain(result, what):
 @torch.library.custom_op("flash_sparse_attn::_tables_extend", mutates_args=("table", "lengths", "free_count", "ticket"),
                          device_types="cuda")
 def _tables_extend(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, ticket: torch.Tensor,
-                   new_lengths: torch.Tensor, block_size: int, total_tokens: int) -> List[torch.Tensor]:
+                   new_lengths: torch.Tensor, block_size: int, total_tokens: int) -> Tuple[
+                       torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     out = _plain(_native.load().tables_extend((table, lengths, free, free_count, ticket, new_lengths), block_size, total_tokens),
                  "extend")
-    return [t.clone() for t in out]  # (parts of one buffer, which an operator must not return)
+    return tuple(t.clone() for t in out)  # (parts of one buffer, which an operator must not return)
 
 
 @torch.library.register_fake("flash_sparse_attn::_tables_extend")
@@ -218,7 +220,7 @@ def _tables_extend_fake(table, lengths, free, free_count, ticket, new_lengths, b
         return torch.empty((n,), dtype=dtype, device=table.device)
 
     R = table.shape[0]
-    return [new(R + 1), new(total_tokens), new(total_tokens, torch.int64), new(R), new(R, torch.bool), new(R + 1), new(R + 1)]
+    return new(R + 1), new(total_tokens), new(total_tokens, torch.int64), new(R), new(R, torch.bool), new(R + 1), new(R + 1)
 
 
 @torch.library.custom_op("flash_sparse_attn::_tables_truncate",

@@ -412,7 +412,7 @@ int fdma_rotary(const fdma_rotary_params* p, void* stream);
  *
  * fdma_tables_extend: requests get new_lengths[r] more tokens (negative counts as 0), in the order of the requests, and the
  * blocks these need. A request gets all of its tokens or none: none when its table row is too short, its tokens would end
- * beyond `tokens`, or blocks have run out. Brings table, lengths and free_count up to date and writes the plan of the step:
+ * beyond `tokens`, or the blocks asked for up to it, refused ones included, are more than there are. Brings table, lengths and free_count up to date and writes the plan of the step:
  *   cu_seqlens (requests + 1)  first of each request's tokens among the step's tokens (at most `tokens`)
  *   positions (tokens)         position of each token in its request, 0 behind the last one
  *   slots (tokens)             block * block_size + place in the block; -1 for refused tokens and behind the last one
