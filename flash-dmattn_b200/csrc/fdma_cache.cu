@@ -9,35 +9,43 @@ namespace {
 
 // ---- block tables -----------------------------------------------------------------------------------------------
 // Whole numbers and a few kilobytes: the time is that of a launch and of a chain of dependent loads. So extending is ONE launch.
-// Every CTA sums up the lengths of all requests itself (three scans over up to 1024 of them at a time, about 1 us) and then fills
+// Every CTA sums up the lengths of all requests itself (one scan over up to 1024 of them at a time) and then fills
 // its share of the tokens; what other CTAs still read (lengths, the free list's count) is updated by the CTA that arrives last.
 constexpr int kTableThreads = 1024;
 constexpr int kMaxRequests = 8192;
 
-// Inclusive scan over the CTA. s_warp: 33 words; ends with all threads past their reads of it.
-__device__ __forceinline__ long long scan(long long x, long long* s_warp, long long* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Inclusive scan of K numbers per thread over the CTA, and their totals. s_warp: K * 33 words; ends with all threads past their
+// reads of it.
+template <int K>
+__device__ __forceinline__ void scan(long long (&x)[K], long long (&total)[K], long long* s_warp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) s_warp[warp] = x;
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const long long y = __shfl_up_sync(0xffffffffu, x[k], o);
+      if (lane >= o) x[k] += y;
+    }
+  if (lane == 31)
+#pragma unroll
+    for (int k = 0; k < K; ++k) s_warp[k * 33 + warp] = x[k];
   __syncthreads();
-  if (warp == 0) {
-    long long w = s_warp[lane];
+  if (warp < K) {  // a warp each
+    long long w = lane < warps ? s_warp[warp * 33 + lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long y = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += y;
     }
-    s_warp[lane] = w;
+    s_warp[warp * 33 + lane] = w;
   }
   __syncthreads();
-  if (warp > 0) x += s_warp[warp - 1];
-  *total = s_warp[31];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (warp > 0) x[k] += s_warp[k * 33 + warp - 1];
+    total[k] = s_warp[k * 33 + 31];
+  }
   __syncthreads();
-  return x;
 }
 
 __device__ __forceinline__ int ceil_div(long long x, int shift) { return static_cast<int>((x + (1ll << shift) - 1) >> shift); }
@@ -45,37 +53,48 @@ __device__ __forceinline__ int ceil_div(long long x, int shift) { return static_
 __global__ void __launch_bounds__(kTableThreads) extend_kernel(const fdma_tables_params p, const int shift) {
   // per request: end of its tokens; tokens held before; place of its first new block among the step's (-1: refused)
   extern __shared__ int32_t s_req[];
-  __shared__ long long s_warp[33];
+  __shared__ long long s_warp[3 * 33];
   __shared__ bool s_last;
   int32_t *s_end = s_req, *s_have = s_req + p.requests, *s_first = s_req + 2 * p.requests;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x;
   const int R = p.requests;
   const int n_free = max(0, min(*p.free_count, p.num_blocks));
   const bool lead = blockIdx.x == 0;
   long long tokens = 0, blocks = 0, units = 0;  // sums over the requests before; units: chunks << 32 | touched blocks
   long long taken = 0;                          // blocks that leave the free list
-  for (int base = 0; base < R; base += kTableThreads) {
+  for (int base = 0; base < R; base += threads) {
     const int r = base + tid;
     const bool in = r < R;
     const int have = in ? max(0, p.lengths[r]) : 0, n = in ? max(0, p.new_lengths[r]) : 0;
-    long long sum;
-    const long long end = tokens + scan(n, s_warp, &sum);
-    tokens += sum;
     const long long length = static_cast<long long>(have) + n;
     const long long old = ceil_div(have, shift), want = (length + (1ll << shift) - 1) >> shift;
-    const bool may = n > 0 && want <= p.width && end <= p.tokens;
-    const int need = may ? static_cast<int>(want - old) : 0;
-    const long long upto = blocks + scan(need, s_warp, &sum);
-    blocks += sum;
-    const bool granted = n == 0 || (may && (need == 0 || upto <= n_free));
-    const bool active = granted && n > 0;
-    const int touched = active ? static_cast<int>(want - (have >> shift)) : 0;
-    const int chunks = active ? ceil_div(length, 6) : 0;
-    const long long both = units + scan((static_cast<long long>(chunks) << 32) | touched, s_warp, &sum);
-    units += sum;
-    long long most;  // (sums of the blocks that are granted are ascending, so the last of them is their total)
-    scan(active && need > 0 ? need : 0, s_warp, &most);
-    taken += most;
+    const bool fits = n > 0 && want <= p.width;
+    int need = fits ? static_cast<int>(want - old) : 0;
+    const long long work = (static_cast<long long>(ceil_div(length, 6)) << 32) | static_cast<int>(want - (have >> shift));
+    // all sums at once, as if tokens and blocks were enough; where they are not, one after the other
+    long long x[3] = {n, need, fits ? work : 0}, sum[3];
+    scan(x, sum, s_warp);
+    long long end = tokens + x[0], upto = blocks + x[1], both = units + x[2];
+    bool granted = n == 0 || fits;
+    if (tokens + sum[0] > p.tokens || blocks + sum[1] > n_free) {
+      const bool may = fits && end <= p.tokens;
+      need = may ? need : 0;
+      long long y[1] = {need}, t[1];
+      scan(y, t, s_warp);
+      upto = blocks + y[0];
+      sum[1] = t[0];
+      granted = n == 0 || (may && (need == 0 || upto <= n_free));
+      long long z[2] = {granted && n > 0 ? work : 0, granted ? need : 0}, u[2];
+      scan(z, u, s_warp);
+      both = units + z[0];
+      sum[2] = u[0];
+      taken += u[1];
+    } else {
+      taken += sum[1];
+    }
+    tokens += sum[0];
+    blocks += sum[1];
+    units += sum[2];
     if (in) {
       const int e = static_cast<int>(min(end, static_cast<long long>(p.tokens)));
       s_end[r] = e;
@@ -94,7 +113,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(const fdma_tables
   __syncthreads();
   const int mask = (1 << shift) - 1;
   const int last_end = s_end[R - 1];
-  for (int t = blockIdx.x * kTableThreads + tid; t < p.tokens; t += gridDim.x * kTableThreads) {
+  for (int t = blockIdx.x * threads + tid; t < p.tokens; t += gridDim.x * threads) {
     int pos = 0;
     int64_t slot = -1;
     if (t < last_end) {
@@ -108,22 +127,15 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(const fdma_tables
       pos = have + t - start;
       if (first >= 0) {
         const int page = pos >> shift, old = ceil_div(have, shift);
-        const int block = page < old ? p.table[static_cast<int64_t>(lo) * p.width + page] : p.free_list[n_free - 1 - (first + page - old)];
+        int32_t* entry = p.table + static_cast<int64_t>(lo) * p.width + page;
+        const int block = page < old ? *entry : p.free_list[n_free - 1 - (first + page - old)];
+        // a new block's first token enters it (nobody reads that entry in this launch)
+        if (page >= old && (t == start || (pos & mask) == 0)) *entry = block;
         if (block >= 0) slot = (static_cast<int64_t>(block) << shift) + (pos & mask);
       }
     }
     p.positions[t] = pos;
     p.slots[t] = slot;
-  }
-  // the new blocks' entries, which nobody reads in this launch: a warp per request
-  const int warps = gridDim.x * (kTableThreads / 32);
-  for (int r = blockIdx.x * (kTableThreads / 32) + (tid >> 5); r < R; r += warps) {
-    const int first = s_first[r];
-    if (first < 0) continue;
-    const int have = s_have[r], n = s_end[r] - (r ? s_end[r - 1] : 0);
-    const int old = ceil_div(have, shift), want = ceil_div(static_cast<long long>(have) + n, shift);
-    for (int j = old + (tid & 31); j < want; j += 32)
-      p.table[static_cast<int64_t>(r) * p.width + j] = p.free_list[n_free - 1 - (first + j - old)];
   }
   // the last CTA: nobody reads lengths and free_count any more
   if (gridDim.x > 1) {
@@ -137,7 +149,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(const fdma_tables
   } else {
     __syncthreads();
   }
-  for (int r = tid; r < R; r += kTableThreads)
+  for (int r = tid; r < R; r += threads)
     if (s_first[r] >= 0) p.lengths[r] = s_have[r] + s_end[r] - (r ? s_end[r - 1] : 0);
   if (tid == 0) {
     *p.free_count = n_free - static_cast<int>(taken);
@@ -146,36 +158,40 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(const fdma_tables
 }
 
 __global__ void __launch_bounds__(kTableThreads) truncate_kernel(const fdma_tables_params p, const int shift) {
-  extern __shared__ int32_t s_req[];  // per request: blocks kept, blocks held, place of its first freed block
+  extern __shared__ int32_t s_req[];  // per request: blocks kept, place of its first freed block
   __shared__ long long s_warp[33];
-  int32_t *s_keep = s_req, *s_held = s_req + p.requests, *s_first = s_req + 2 * p.requests;
+  const int threads = blockDim.x;
+  int32_t *s_keep = s_req, *s_first = s_req + p.requests;
   const int tid = threadIdx.x, R = p.requests;
   const int n_free = max(0, min(*p.free_count, p.num_blocks));
   long long gone = 0;
-  for (int base = 0; base < R; base += kTableThreads) {
+  for (int base = 0; base < R; base += threads) {
     const int r = base + tid;
     const int have = r < R ? max(0, p.lengths[r]) : 0, keep = r < R ? min(have, max(0, p.new_lengths[r])) : 0;
     const int held = min(ceil_div(have, shift), p.width), left = min(ceil_div(keep, shift), p.width);
-    long long sum;
-    const long long upto = gone + scan(held - left, s_warp, &sum);
-    gone += sum;
+    long long x[1] = {held - left}, sum[1];
+    scan(x, sum, s_warp);
+    const long long upto = gone + x[0];
+    gone += sum[0];
     if (r < R) {
       s_keep[r] = left;
-      s_held[r] = held;
       s_first[r] = static_cast<int>(upto - (held - left));
       p.lengths[r] = keep;
     }
   }
   __syncthreads();
   const long long total = n_free + gone;
-  for (int r = tid >> 5; r < R; r += kTableThreads / 32) {
-    const int left = s_keep[r], held = s_held[r], first = s_first[r];
-    for (int j = left + (tid & 31); j < held; j += 32) {
-      int32_t* entry = p.table + static_cast<int64_t>(r) * p.width + j;
-      const long long at = total - 1 - (first + j - left);
-      if (at < p.num_blocks) p.free_list[at] = *entry;
-      *entry = -1;
+  for (int i = tid; i < gone; i += threads) {
+    int below = 0, above = R - 1;  // last request whose first freed block is no later: it has freed this one
+    while (below < above) {
+      const int mid = (below + above + 1) >> 1;
+      if (s_first[mid] <= i) below = mid;
+      else above = mid - 1;
     }
+    int32_t* entry = p.table + static_cast<int64_t>(below) * p.width + s_keep[below] + i - s_first[below];
+    const long long at = total - 1 - i;
+    if (at < p.num_blocks) p.free_list[at] = *entry;
+    *entry = -1;
   }
   if (tid == 0) *p.free_count = static_cast<int>(min(total, static_cast<long long>(p.num_blocks)));
 }
@@ -200,6 +216,9 @@ int check_tables(const fdma_tables_params* p) {
   return 0;
 }
 
+// a thread per request in whole warps, at least as many warps as there are sums
+int table_threads(int64_t n) { return static_cast<int>(std::min<int64_t>(kTableThreads, std::max<int64_t>(128, (n + 31) / 32 * 32))); }
+
 template <typename K>
 int table_smem(K kernel, int requests, size_t* bytes) {
   *bytes = static_cast<size_t>(requests) * 12;
@@ -210,14 +229,30 @@ int table_smem(K kernel, int requests, size_t* bytes) {
 // ---- the writer ---------------------------------------------------------------------------------------------------
 // Memory-bound: keys and values are read twice (the second time from cache) and written once. A CTA takes one block and kv head
 // of K or of V: it looks for the largest magnitude, fixes the scale and writes. Queries are turned by CTAs behind those.
+constexpr int kAppendThreads = kRotaryWarps * 32;
 struct AppendArgs {
   fdma_cache_append_params p;
-  RotaryUnits key_units, value_units;
-  RotaryArgs query;  // tokens_per_cta = 0: none
+  RotaryUnits key_units;    // of keys that are turned
+  RotaryUnits plain_units;  // of values, and keys that are not: two vectors, half a row apart
+  RotaryArgs query;
   int shift, most_units;
+  int key_heads;  // of a CTA: they share the factors of its tokens
   int64_t cache_ctas;
 };
 
+// N numbers times f, rounded; beyond 448 they become 448
+template <int N>
+__device__ __forceinline__ Vec<uint8_t, N> to_e4m3(const float (&x)[N], float f) {
+  Vec<uint8_t, N> v;
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int j = 0; j < N; j += 2)
+      *reinterpret_cast<uint16_t*>(&v.x[j]) = __nv_cvt_float2_to_fp8x2(make_float2(x[j] * f, x[j + 1] * f), __NV_SATFINITE, __NV_E4M3);
+  } else {
+    v.x[0] = __nv_cvt_float_to_fp8(x[0] * f, __NV_SATFINITE, __NV_E4M3);
+  }
+  return v;
+}
 __device__ __forceinline__ uint8_t to_e4m3(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ float from_e4m3(uint8_t x) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(x, __NV_E4M3)));
@@ -230,24 +265,28 @@ __device__ __forceinline__ float block_scale(float x) {
   return __uint_as_float(static_cast<uint32_t>(max(e, -100) + 127) << 23);
 }
 
-template <typename T, int N>
-__global__ void __launch_bounds__(kRotaryThreads) append_kernel(const AppendArgs a) {
+template <typename T, int N, bool kInterleaved>
+__global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_constant__ AppendArgs a) {
   extern __shared__ float2 s_factors[];  // [new tokens of the block][half], or rotate_tokens' own
-  __shared__ float s_max[kRotaryThreads / 32];
+  __shared__ float s_max[2][kAppendThreads / 32];
   __shared__ int s_request;
   const fdma_cache_append_params& p = a.p;
   const fdma_cache& c = p.c;
   const int tid = threadIdx.x;
   if (blockIdx.x >= a.cache_ctas) {
-    rotate_tokens<T, N>(a.query, blockIdx.x - a.cache_ctas, s_factors);
+    const int warp = tid >> 5;
+    rotate_tokens<T, N, kInterleaved>(a.query, (blockIdx.x - a.cache_ctas) * kRotaryWarps + warp, s_factors + warp * a.query.abreast * a.query.ru.half);
     return;
   }
-  const bool is_v = blockIdx.x & 1;
-  const int rest = blockIdx.x >> 1;
-  const int unit = rest / c.h_k, head = rest - unit * c.h_k;
+  // first the CTAs of K, a few heads of a block each, then those of V, a head each
+  const int key_groups = (c.h_k + a.key_heads - 1) / a.key_heads, key_ctas = a.most_units * key_groups;
+  const bool is_v = blockIdx.x >= key_ctas;
+  const int rest = is_v ? blockIdx.x - key_ctas : blockIdx.x, per_unit = is_v ? c.h_k : key_groups;
+  const int unit = rest / per_unit, head0 = (rest - unit * per_unit) * (is_v ? 1 : a.key_heads);
+  const int heads = is_v ? 1 : min(a.key_heads, c.h_k - head0);
   if (tid == 0) s_request = -1;
   __syncthreads();
-  for (int r = tid; r < c.requests; r += kRotaryThreads)
+  for (int r = tid; r < c.requests; r += kAppendThreads)
     if (c.cu_blocks[r] <= unit && unit < c.cu_blocks[r + 1]) s_request = r;
   __syncthreads();
   const int r = s_request;
@@ -264,97 +303,129 @@ __global__ void __launch_bounds__(kRotaryThreads) append_kernel(const AppendArgs
   if (n <= 0) return;
   const int first = token0 + begin + lo - before;  // the token at place lo
 
-  const RotaryUnits& ru = is_v ? a.value_units : a.key_units;
-  const T* src = static_cast<const T*>(is_v ? p.value : p.key) + first * (is_v ? p.value_row_stride : p.key_row_stride) +
-                 head * (is_v ? p.value_head_stride : p.key_head_stride);
-  const int64_t row_stride = is_v ? p.value_row_stride : p.key_row_stride;
-  const int64_t at_scale = static_cast<int64_t>(block) * c.h_k + head;
-  uint8_t* dst = static_cast<uint8_t*>(is_v ? c.v : c.k) + (at_scale * bs) * c.d;
-  float* scale = (is_v ? c.v_scale : c.k_scale) + at_scale;
-  const float old_scale = lo > 0 ? *scale : 0.f;
-  for (int i = tid; i < n * ru.half; i += kRotaryThreads) {
-    const int t = i / ru.half;
-    s_factors[i] = rotary_factors(before + (first - token0) + t, p.turns[i - t * ru.half], p.amplitude, false);
+  const bool turn = !is_v && p.turns;
+  const RotaryUnits& ru = turn ? a.key_units : a.plain_units;
+  const int half = turn ? ru.half : 0;
+  const int64_t row_stride = is_v ? p.value_row_stride : p.key_row_stride, head_stride = is_v ? p.value_head_stride : p.key_head_stride;
+  for (int i = tid; i < n * half; i += kAppendThreads) {
+    const int t = i / half, f = i - t * half;
+    s_factors[i] = rotary_factors(before + (first - token0) + t, p.turns[f], p.amplitude, false);
   }
-  __syncthreads();
+  // A thread keeps its unit and walks the tokens. The first kHold of its vectors stay in registers between the two passes.
   using V = Vec<T, N>;
-  auto load = [&](int i, float (&x)[N], float (&y)[N], int2& at, int& t, bool& pair) {
-    t = i / ru.units;
-    const int u = i - t * ru.units;
-    at = unit_offsets<N>(ru, u);
-    pair = u < ru.pair_units;
-    const V vx = *reinterpret_cast<const V*>(src + t * row_stride + at.x);
+  constexpr int kHold = 2;
+  const int abreast = kAppendThreads / ru.units;  // units <= 256
+  const int t_first = tid / ru.units, u = tid - t_first * ru.units;
+  const int t_begin = t_first < abreast ? t_first : n;
+  const bool pair = u < ru.pair_units;
+  const int2 at = unit_offsets<N, kInterleaved>(ru, u);
+  V hx[kHold], hy[kHold];
+  auto hold = [&](const T* from) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = to_f(vx.x[j]);
-    if (pair) {
-      const V vy = *reinterpret_cast<const V*>(src + t * row_stride + at.y);
-#pragma unroll
-      for (int j = 0; j < N; ++j) y[j] = to_f(vy.x[j]);
-      rotate_unit<N>(x, y, s_factors + t * ru.half + u * N, ru.interleaved);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) y[j] = 0.f;
+    for (int k = 0; k < kHold; ++k) {
+      const int t = t_begin + k * abreast;
+      if (t < n) {
+        hx[k] = *reinterpret_cast<const V*>(from + t * row_stride + at.x);
+        if (pair) hy[k] = *reinterpret_cast<const V*>(from + t * row_stride + at.y);
+      }
     }
   };
-  float most = 0.f;
-  for (int i = tid; i < n * ru.units; i += kRotaryThreads) {
-    float x[N], y[N];
-    int2 at;
-    int t;
-    bool pair;
-    load(i, x, y, at, t, pair);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float fx = fabsf(x[j]), fy = fabsf(y[j]);
-      if (fx <= 3.402823466e38f) most = fmaxf(most, fx);
-      if (fy <= 3.402823466e38f) most = fmaxf(most, fy);
+  for (int head = head0; head < head0 + heads; ++head) {
+    const T* src = static_cast<const T*>(is_v ? p.value : p.key) + first * row_stride + head * head_stride;
+    const int64_t at_scale = static_cast<int64_t>(block) * c.h_k + head;
+    uint8_t* dst = static_cast<uint8_t*>(is_v ? c.v : c.k) + (at_scale * bs) * c.d;
+    float* scale = (is_v ? c.v_scale : c.k_scale) + at_scale;
+    const float old_scale = lo > 0 ? *scale : 0.f;
+    if (head == head0) {
+      hold(src);
+      __syncthreads();  // the factors
     }
-  }
+    auto values = [&](const V& vx, const V& vy, int t, float (&x)[N], float (&y)[N]) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if ((tid & 31) == 0) s_max[tid >> 5] = most;
-  __syncthreads();
+      for (int j = 0; j < N; ++j) {
+        x[j] = to_f(vx.x[j]);
+        y[j] = pair ? to_f(vy.x[j]) : 0.f;
+      }
+      if (turn && pair) rotate_unit<N, kInterleaved>(x, y, s_factors + t * half + u * N);
+    };
+    float most = 0.f;
+    auto look = [&](const float (&x)[N], const float (&y)[N]) {
 #pragma unroll
-  for (int w = 0; w < kRotaryThreads / 32; ++w) most = fmaxf(most, s_max[w]);
-  const float now = fmaxf(block_scale(most), old_scale), inv = __frcp_rn(now);
-  if (tid == 0) *scale = now;
-  for (int i = tid; i < n * ru.units; i += kRotaryThreads) {
-    float x[N], y[N];
-    int2 at;
-    int t;
-    bool pair;
-    load(i, x, y, at, t, pair);
-    uint8_t* row = dst + (lo + t) * c.d;
-    Vec<uint8_t, N> out;
+      for (int j = 0; j < N; ++j) {
+        const float fx = fabsf(x[j]), fy = fabsf(y[j]);
+        if (fx <= 3.402823466e38f) most = fmaxf(most, fx);
+        if (fy <= 3.402823466e38f) most = fmaxf(most, fy);
+      }
+    };
 #pragma unroll
-    for (int j = 0; j < N; ++j) out.x[j] = to_e4m3(x[j] * inv);
-    *reinterpret_cast<Vec<uint8_t, N>*>(row + at.x) = out;
-    if (pair) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) out.x[j] = to_e4m3(y[j] * inv);
-      *reinterpret_cast<Vec<uint8_t, N>*>(row + at.y) = out;
+    for (int k = 0; k < kHold; ++k) {
+      const int t = t_begin + k * abreast;
+      if (t < n) {
+        float x[N], y[N];
+        values(hx[k], hy[k], t, x, y);
+        look(x, y);
+      }
     }
-  }
-  if (lo > 0 && now > old_scale) {  // the tokens that were there, at the new scale
-    const float f = old_scale * inv;
-    for (int i = tid; i < lo * c.d / 16; i += kRotaryThreads) {
-      Vec<uint8_t, 16>& v = *reinterpret_cast<Vec<uint8_t, 16>*>(dst + i * 16);
-      Vec<uint8_t, 16> x = v;
+    for (int t = t_begin + kHold * abreast; t < n; t += abreast) {
+      float x[N], y[N];
+      const V vx = *reinterpret_cast<const V*>(src + t * row_stride + at.x);
+      V vy = vx;
+      if (pair) vy = *reinterpret_cast<const V*>(src + t * row_stride + at.y);
+      values(vx, vy, t, x, y);
+      look(x, y);
+    }
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x.x[j] = to_e4m3(from_e4m3(x.x[j]) * f);
-      v = x;
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if ((tid & 31) == 0) s_max[head & 1][tid >> 5] = most;  // (two rows: the next head's maxima must not overtake readers of these)
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) most = fmaxf(most, s_max[head & 1][w]);
+    const float now = fmaxf(block_scale(most), old_scale), inv = __frcp_rn(now);
+    if (tid == 0) *scale = now;
+    auto write = [&](const float (&x)[N], const float (&y)[N], int t) {
+      uint8_t* row = dst + (lo + t) * c.d;
+      *reinterpret_cast<Vec<uint8_t, N>*>(row + at.x) = to_e4m3<N>(x, inv);
+      if (pair) *reinterpret_cast<Vec<uint8_t, N>*>(row + at.y) = to_e4m3<N>(y, inv);
+    };
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      const int t = t_begin + k * abreast;
+      if (t < n) {
+        float x[N], y[N];
+        values(hx[k], hy[k], t, x, y);
+        write(x, y, t);
+      }
+    }
+    if (head + 1 < head0 + heads) hold(src + head_stride);  // on their way while the rest is done
+    for (int t = t_begin + kHold * abreast; t < n; t += abreast) {
+      float x[N], y[N];
+      const V vx = *reinterpret_cast<const V*>(src + t * row_stride + at.x);
+      V vy = vx;
+      if (pair) vy = *reinterpret_cast<const V*>(src + t * row_stride + at.y);
+      values(vx, vy, t, x, y);
+      write(x, y, t);
+    }
+    if (lo > 0 && now > old_scale) {  // the tokens that were there, at the new scale
+      const float f = old_scale * inv;
+      for (int i = tid; i < lo * c.d / 16; i += kAppendThreads) {
+        Vec<uint8_t, 16>& v = *reinterpret_cast<Vec<uint8_t, 16>*>(dst + i * 16);
+        Vec<uint8_t, 16> x = v;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x.x[j] = to_e4m3(from_e4m3(x.x[j]) * f);
+        v = x;
+      }
     }
   }
 }
 
-template <typename T, int N>
+template <typename T, int N, bool kInterleaved>
 int launch_append(AppendArgs a, cudaStream_t stream) {
   const fdma_cache_append_params& p = a.p;
   const fdma_cache& c = p.c;
   const bool turn = p.turns != nullptr;
-  a.key_units = rotary_units(c.d, turn ? p.rotary_dim : 0, p.interleaved != 0, N);
-  a.value_units = rotary_units(c.d, 0, false, N);
-  size_t smem = static_cast<size_t>(std::min(1 << a.shift, c.tokens)) * a.key_units.half * sizeof(float2);
+  a.key_units = rotary_units(c.d, turn ? p.rotary_dim : c.d, N);
+  a.plain_units = rotary_units(c.d, c.d, N);
+  size_t smem = turn ? static_cast<size_t>(std::min(1 << a.shift, c.tokens)) * a.key_units.half * sizeof(float2) : 0;
   int64_t query_ctas = 0;
   a.query = RotaryArgs{};
   if (turn && p.query) {
@@ -367,17 +438,17 @@ int launch_append(AppendArgs a, cudaStream_t stream) {
     q.b = 1; q.seqlen = c.tokens; q.h = p.h; q.d = c.d; q.rotary_dim = p.rotary_dim;
     q.interleaved = p.interleaved; q.dtype = p.dtype; q.amplitude = p.amplitude;
     a.query = rotary_args(q, N);
-    query_ctas = (a.query.tokens + a.query.tokens_per_cta - 1) / a.query.tokens_per_cta;
-    smem = std::max(smem, static_cast<size_t>(a.query.tokens_per_cta) * a.query.ru.half * sizeof(float2));
+    query_ctas = (a.query.groups + kRotaryWarps - 1) / kRotaryWarps;
+    smem = std::max(smem, rotary_smem(a.query));
   }
-  auto kern = append_kernel<T, N>;
+  auto kern = append_kernel<T, N, kInterleaved>;
   if (smem > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   const int64_t ctas = a.cache_ctas + query_ctas;
   if (ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
-  kern<<<static_cast<unsigned>(ctas), kRotaryThreads, smem, stream>>>(a);
+  kern<<<static_cast<unsigned>(ctas), kAppendThreads, smem, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -390,8 +461,9 @@ int launch_append_t(const AppendArgs& a, cudaStream_t stream) {
     x |= reinterpret_cast<uintptr_t>(p.query) | reinterpret_cast<uintptr_t>(p.query_out);
     strides |= static_cast<uint64_t>(p.query_row_stride | p.query_head_stride | p.out_row_stride | p.out_head_stride);
   }
-  const bool vec = (x | strides * sizeof(T)) % 16 == 0 && rotary_units_fit(p.c.d, p.turns ? p.rotary_dim : 0, 8);
-  return vec ? launch_append<T, 8>(a, stream) : launch_append<T, 1>(a, stream);
+  const bool vec = (x | strides * sizeof(T)) % 16 == 0 && rotary_units_fit(p.c.d, p.turns ? p.rotary_dim : p.c.d, 8);
+  if (vec) return p.interleaved ? launch_append<T, 8, true>(a, stream) : launch_append<T, 8, false>(a, stream);
+  return p.interleaved ? launch_append<T, 1, true>(a, stream) : launch_append<T, 1, false>(a, stream);
 }
 
 }  // namespace
@@ -419,7 +491,7 @@ extern "C" int fdma_tables_extend(const fdma_tables_params* p, void* stream) {
   if (st) return st;
   // a CTA for 2048 tokens: beyond that filling takes longer than another CTA's sums
   const int ctas = std::max(1, std::min(sm_count(), p->tokens / 2048));
-  extend_kernel<<<ctas, kTableThreads, smem, static_cast<cudaStream_t>(stream)>>>(*p, block_shift(p->block_size));
+  extend_kernel<<<ctas, table_threads(std::max(p->requests, p->tokens)), smem, static_cast<cudaStream_t>(stream)>>>(*p, block_shift(p->block_size));
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -446,7 +518,10 @@ extern "C" int fdma_cache_append(const fdma_cache_append_params* p, void* stream
   a.p = *p;
   a.shift = block_shift(p->c.block_size);
   a.most_units = static_cast<int>(std::min<int64_t>(p->c.tokens, (static_cast<int64_t>(p->c.tokens) >> a.shift) + 2 * static_cast<int64_t>(p->c.requests)));
-  a.cache_ctas = static_cast<int64_t>(a.most_units) * p->c.h_k * 2;
+  // Heads of a CTA: the factors (as much work as all the rest of a head) are shared by as many as leave two CTAs per SM.
+  a.key_heads = p->turns ? std::max(1, std::min(p->c.h_k, a.most_units * p->c.h_k / (2 * sm_count()))) : 1;
+  a.cache_ctas = static_cast<int64_t>(a.most_units) * ((p->c.h_k + a.key_heads - 1) / a.key_heads + p->c.h_k);
+  if (a.cache_ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   switch (p->dtype) {
     case FDMA_BF16: return launch_append_t<__nv_bfloat16>(a, stream);

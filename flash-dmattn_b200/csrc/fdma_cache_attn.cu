@@ -215,7 +215,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     s_abort = 0;
     if (!kGather) {
       for (int i = 0; i < L::kStages; ++i) {
-        mbar_init(&s_full[i], 1);
+        mbar_init(&s_full[i], 2);  // the copies, and the scales
         mbar_init(&s_empty[i], kWarps);
       }
       fence_mbar_init();
@@ -251,7 +251,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
         if (block >= 0) {
           ks = __ldg(c.k_scale + static_cast<int64_t>(block) * c.h_k + hk);
-          vs = value_scale(__ldg(c.v_scale + static_cast<int64_t>(block) * c.h_k + hk));
+          vs = __ldg(c.v_scale + static_cast<int64_t>(block) * c.h_k + hk);
         }
       }
     };
@@ -264,13 +264,11 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     int issued = 0;
     for (int64_t w = w0; w < w1; w += 8) {
       block = n_block; row = n_row; hk = n_hk; ks = n_ks; vs = n_vs; used = n_used;
-      look_up(w + 8 + (lane >> 2), n_block, n_row, n_hk, n_ks, n_vs, n_used);
       for (int i = 0; i < 8 && w + i < w1; ++i) {
+        // the next eight are looked up, three dependent loads, when the ring has been filled from these
+        if (i == L::kStages - 1) look_up(w + 8 + (lane >> 2), n_block, n_row, n_hk, n_ks, n_vs, n_used);
         if (!__shfl_sync(0xffffffffu, used, i * 4)) continue;  // no rows of this unit in this row tile
         mbar_wait(&s_empty[st], phase ^ 1, ctl, 701);
-        if ((lane >> 2) == i)
-          s_meta[st][lane & 3] = make_float4(block >= 0 ? 1.f : 0.f, ks, exponent_of(vs), block >= 0 ? __frcp_rn(vs) : 0.f);
-        __syncwarp();
         const int hk_i = __shfl_sync(0xffffffffu, hk, i * 4);
         unsigned char* dst = smem + L::kRing + st * L::kStageBytes;
         uint32_t bytes = 0;
@@ -296,7 +294,12 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             }
           }
         }
+        if ((lane >> 2) == i) {
+          const float v = value_scale(vs);
+          s_meta[st][lane & 3] = make_float4(block >= 0 ? 1.f : 0.f, ks, exponent_of(v), block >= 0 ? __frcp_rn(v) : 0.f);
+        }
         __syncwarp();
+        if (lane == 0) mbar_arrive(&s_full[st]);
         ++issued;
         if (++st == L::kStages) {
           st = 0;
@@ -421,7 +424,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     constexpr int kAhead = L::kStages - 1;
     const int32_t* list = nullptr;
     int slots = 0, pos2 = -1, pos3 = -1, block2 = -1;
-    float g_scale_k = 0.f, g_scale_v = 1.f, g_add = 0.f;
+    float g_scale_k = 0.f, g_scale_v = 1.f;  // as loaded: a conversion beside a load would wait for it
+    uint16_t g_bias = 0;
     int g_pos = -1;
     const bool head_bias = p.bias && p.h_bias == p.h && a.group > 1;
     auto load_pos = [&](int chunk) {
@@ -443,15 +447,16 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       if (i + kAhead - 1 >= first) {  // what the iteration before has loaded about chunk i + kAhead - 1
         const int at = (st + kAhead - 1) % L::kStages;
         if (lane < kSlice)
-          s_meta[at][warp * kSlice + lane] = make_float4(g_pos < 0 ? -CUDART_INF_F : g_add, g_scale_k, exponent_of(g_scale_v), __int_as_float(g_pos));
+          s_meta[at][warp * kSlice + lane] = make_float4(g_pos < 0 ? -CUDART_INF_F : bias_log2(raw_to_f<kBf16>(g_bias)), g_scale_k,
+                                                         exponent_of(value_scale(g_scale_v)), __int_as_float(g_pos));
       }
       if (block2 < 0 || block2 >= c.num_blocks) pos2 = block2 = -1;
       g_pos = pos2;
       if (pos2 >= 0) {
         const int64_t at = static_cast<int64_t>(block2) * c.h_k + u.hk;
         g_scale_k = __ldg(c.k_scale + at);
-        g_scale_v = value_scale(__ldg(c.v_scale + at));
-        g_add = p.bias && !head_bias && pos2 < p.bias_keys ? bias_log2(raw_to_f<kBf16>(__ldg(bias_row[0] + pos2))) : 0.f;
+        g_scale_v = __ldg(c.v_scale + at);
+        g_bias = p.bias && !head_bias && pos2 < p.bias_keys ? __ldg(bias_row[0] + pos2) : static_cast<uint16_t>(0);
       }
       if (i + kAhead < last) {
         constexpr int kLanes = D / 16;  // 16-byte pieces of a row
@@ -723,63 +728,80 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   }
 }
 
-// Joins the sums of units that several CTAs share, and writes the zeros of rows that nobody computes: a warp per (token, head).
+// Joins the sums of units that several CTAs share, and writes the zeros of rows that nobody computes: a CTA per (token, head),
+// whose warps take a quarter of the sums each.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant__ AttnArgs a, const int rows_per_tile) {
   const fdma_cache_attention_params& p = a.p;
   const fdma_cache& c = p.c;
-  const int lane = threadIdx.x & 31;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (id >= static_cast<int64_t>(c.tokens) * p.h) return;
-  const int token = static_cast<int>(id / p.h), head = static_cast<int>(id - static_cast<int64_t>(token) * p.h);
-  int lo = 0, hi = c.requests;  // first request whose tokens end behind this one
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (c.cu_seqlens[mid + 1] > token) hi = mid;
-    else lo = mid + 1;
+  __shared__ int s_request;
+  __shared__ float s_top[4], s_sum[4], s_acc[4][D];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int token = static_cast<int>(blockIdx.x / p.h), head = static_cast<int>(blockIdx.x - static_cast<unsigned>(token) * p.h);
+  if (tid == 0) s_request = -1;
+  __syncthreads();
+  for (int r = tid; r < c.requests; r += 128)
+    if (c.cu_seqlens[r] <= token && token < c.cu_seqlens[r + 1]) s_request = r;
+  const Units units{a, c.cu_chunks};
+  const int64_t total = units.total(), share = share_of(total, a.ctas);
+  __syncthreads();
+  const int r = s_request;
+  int c0 = 0, c1 = -1;
+  const float* base = nullptr;
+  const int64_t step = static_cast<int64_t>(rows_per_tile) * (D + 4);
+  bool written = false;
+  if (r >= 0) {
+    const Request q = request_of(a, r);
+    const int row = (token - q.token0) * a.group + head % a.group;
+    const Unit u = units.of_request(r, head / a.group);
+    if (row >= 0 && row < q.rows && u.n > 0) {
+      c0 = static_cast<int>(u.start / share);
+      c1 = static_cast<int>((u.start + u.n - 1) / share);
+      written = c0 == c1;  // by that CTA
+      const int tile = row / rows_per_tile;
+      base = a.partial + (static_cast<int64_t>(tile) * a.ctas * 2 * rows_per_tile + row - tile * rows_per_tile) * (D + 4);
+    }
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (written) return;
+  float top = -CUDART_INF_F;
+  for (int x = c0 + tid; x <= c1; x += 128) top = fmaxf(top, base[(2 * static_cast<int64_t>(x) + (x == c0)) * step + D]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  const float from = top == -CUDART_INF_F ? 0.f : top;
   constexpr int E = D / 32;  // elements per lane
   float acc[E], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
-  const Units units{a, c.cu_chunks};
-  const int64_t total = units.total(), share = share_of(total, a.ctas);
-  if (lo < c.requests) {
-    const Request q = request_of(a, lo);
-    const int row = (token - q.token0) * a.group + head % a.group;
-    const Unit u = units.of_request(lo, head / a.group);
-    if (row >= 0 && row < q.rows && u.n > 0) {
-      const int c0 = static_cast<int>(u.start / share), c1 = static_cast<int>((u.start + u.n - 1) / share);
-      if (c0 == c1) return;  // written by that CTA
-      const int tile = row / rows_per_tile;
-      const float* base = a.partial + ((static_cast<int64_t>(tile) * a.ctas * 2) * rows_per_tile + row - tile * rows_per_tile) * (D + 4);
-      const int64_t step = static_cast<int64_t>(rows_per_tile) * (D + 4);
-      float top = -CUDART_INF_F;
-      for (int x = c0 + lane; x <= c1; x += 32) top = fmaxf(top, base[(2 * static_cast<int64_t>(x) + (x == c0)) * step + D]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float from = top == -CUDART_INF_F ? 0.f : top;
 #pragma unroll 4
-      for (int x = c0; x <= c1; ++x) {
-        const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
-        const float2 ml = *reinterpret_cast<const float2*>(src + D);
-        const float f = exp2_or_zero(ml.x - from);
-        sum = fmaf(ml.y, f, sum);
+  for (int x = c0 + warp; x <= c1; x += 4) {
+    const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
+    const float2 ml = *reinterpret_cast<const float2*>(src + D);
+    const float f = exp2_or_zero(ml.x - from);
+    sum = fmaf(ml.y, f, sum);
 #pragma unroll
-        for (int i = 0; i < E; i += 2) {
-          const float2 y = *reinterpret_cast<const float2*>(src + lane * E + i);
-          acc[i] = fmaf(y.x, f, acc[i]);
-          acc[i + 1] = fmaf(y.y, f, acc[i + 1]);
-        }
-      }
+    for (int i = 0; i < E; i += 2) {
+      const float2 y = *reinterpret_cast<const float2*>(src + lane * E + i);
+      acc[i] = fmaf(y.x, f, acc[i]);
+      acc[i + 1] = fmaf(y.y, f, acc[i + 1]);
     }
   }
+  if (lane == 0) s_sum[warp] = sum;
+#pragma unroll
+  for (int i = 0; i < E; ++i) s_acc[warp][lane * E + i] = acc[i];
+  __syncthreads();
+  sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* dst = static_cast<uint16_t*>(p.out) + token * p.out_row_stride + head * p.out_head_stride;
+  for (int i = 2 * tid; i < c.d; i += 256) {
+    float y[2];
 #pragma unroll
-  for (int i = 0; i < E; i += 2)
-    if (lane * E + i < c.d) *reinterpret_cast<uint32_t*>(dst + lane * E + i) = pack2<kBf16>(acc[i] * inv, acc[i + 1] * inv);
+    for (int k = 0; k < 2; ++k) y[k] = (s_acc[0][i + k] + s_acc[1][i + k]) + (s_acc[2][i + k] + s_acc[3][i + k]);
+    *reinterpret_cast<uint32_t*>(dst + i) = pack2<kBf16>(y[0] * inv, y[1] * inv);
+  }
 }
 
 int tile_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -816,14 +838,15 @@ int launch(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
     if (st) return st;
   }
   auto kern = cache_attend_kernel<D, ROWS, kGather, kBf16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
-  if (e != cudaSuccess) return static_cast<int>(e);
+  static std::atomic<uint64_t> prepared{0};
+  const int st_smem = allow_smem_once(reinterpret_cast<const void*>(kern), L::kTotal, prepared);
+  if (st_smem) return st_smem;
   kern<<<dim3(pl.ctas, pl.tiles), L::kThreads, L::kTotal, stream>>>(a, map_k, map_v);
-  e = cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
   // the second kernel's CTAs start while the first one's finish, and wait for them only where they need their sums
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(c.tokens) * a.p.h + 3) / 4));
+  cfg.gridDim = dim3(static_cast<unsigned>(c.tokens) * a.p.h);
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -849,7 +872,7 @@ int check_attention(const fdma_cache_attention_params* pp) {
   if (p.bias && ((p.h_bias != 1 && p.h_bias != p.c.h_k && p.h_bias != p.h) || p.bias_keys <= 0)) return FDMA_ERR_BAD_ARG;
   if (p.kept_pos && p.kept_capacity <= 0) return FDMA_ERR_BAD_ARG;
   if (p.dtype != FDMA_BF16 && p.dtype != FDMA_FP16) return FDMA_ERR_UNSUPPORTED;
-  if (static_cast<int64_t>(p.c.num_blocks) * p.c.h_k > 0x7FFFFFFF || static_cast<int64_t>(p.c.tokens) * p.h > (1ll << 32)) return FDMA_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(p.c.num_blocks) * p.c.h_k > 0x7FFFFFFF || static_cast<int64_t>(p.c.tokens) * p.h > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
   return 0;
 }
 

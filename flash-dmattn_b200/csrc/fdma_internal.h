@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/fdma.h"
 
 namespace fdma {
@@ -116,6 +118,19 @@ int export_softmax_d(const fdma_bwd_params& bp, const float* dsum, int sq_r, cud
 
 // Number of SMs of the current device (cudaDevAttrMultiProcessorCount, cached per device).
 int sm_count();
+
+// Allows a kernel `bytes` of dynamic shared memory on the current device, once per device (`prepared`: a bit each).
+inline int allow_smem_once(const void* kernel, int bytes, std::atomic<uint64_t>& prepared) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (prepared.load(std::memory_order_acquire) & bit)) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 64) prepared.fetch_or(bit, std::memory_order_release);
+  return 0;
+}
 
 // Events registered by fdma_time_next_kernel for this host thread (both null when none); take_* clears them.
 void take_timing_events(cudaEvent_t* start, cudaEvent_t* stop);

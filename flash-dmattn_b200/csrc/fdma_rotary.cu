@@ -2,33 +2,40 @@
 //
 //   y1 = a (x1 cos - x2 sin),  y2 = a (x2 cos + x1 sin),  angle = position * frequency
 //
-// Memory-bound: every element is read once and written once, three operations each. A CTA takes a few tokens, puts their cosines
-// and sines into shared memory (one evaluation per token and frequency, whatever the number of heads), then all its threads walk
-// the tokens' heads in 16-byte vectors.
+// Memory-bound: every element is read once and written once, three operations each. A warp takes a token: one evaluation of sine
+// and cosine per frequency, whatever the number of heads, then the heads in 16-byte vectors (rotate_tokens in fdma_rotary.cuh).
 #include "fdma_rotary.cuh"
 
 namespace fdma {
 namespace {
 
-template <typename T, int N>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
+template <typename T, int N, bool kInterleaved>
+__global__ void __launch_bounds__(kRotaryWarps * 32, 4) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   extern __shared__ float2 s_factors[];
-  rotate_tokens<T, N>(a, blockIdx.x, s_factors);
+  const int warp = threadIdx.x >> 5;
+  rotate_tokens<T, N, kInterleaved>(a, static_cast<int64_t>(blockIdx.x) * kRotaryWarps + warp, s_factors + warp * a.abreast * a.ru.half);
 }
 
-template <typename T, int N>
+template <typename T, int N, bool kInterleaved>
 int launch(const fdma_rotary_params& p, cudaStream_t stream) {
   const RotaryArgs a = rotary_args(p, N);
-  const int64_t ctas = (a.tokens + a.tokens_per_cta - 1) / a.tokens_per_cta;
+  const int64_t ctas = (a.groups + kRotaryWarps - 1) / kRotaryWarps;
   if (ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
-  rotary_kernel<T, N><<<static_cast<unsigned>(ctas), kRotaryThreads, a.tokens_per_cta * a.ru.half * sizeof(float2), stream>>>(a);
+  const size_t smem = rotary_smem(a);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(rotary_kernel<T, N, kInterleaved>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  rotary_kernel<T, N, kInterleaved><<<static_cast<unsigned>(ctas), kRotaryWarps * 32, smem, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T>
 int launch_t(const fdma_rotary_params& p, cudaStream_t stream) {
   constexpr int N = 16 / sizeof(T);
-  return rotary_units_fit(p.d, p.rotary_dim, N) && rotary_aligned16(p, sizeof(T)) ? launch<T, N>(p, stream) : launch<T, 1>(p, stream);
+  if (rotary_units_fit(p.d, p.rotary_dim, N) && rotary_aligned16(p, sizeof(T)))
+    return p.interleaved ? launch<T, N, true>(p, stream) : launch<T, N, false>(p, stream);
+  return p.interleaved ? launch<T, 1, true>(p, stream) : launch<T, 1, false>(p, stream);
 }
 
 }  // namespace
@@ -43,7 +50,7 @@ extern "C" int fdma_rotary(const fdma_rotary_params* pp, void* stream_) {
   if (p.h_k && (!p.k || !p.k_out)) return FDMA_ERR_BAD_ARG;
   if (p.rotary_dim <= 0 || p.rotary_dim % 2 || p.rotary_dim > p.d) return FDMA_ERR_BAD_ARG;
   if (p.positions && p.position_bits != 32 && p.position_bits != 64) return FDMA_ERR_BAD_ARG;
-  if (p.rotary_dim > 8192) return FDMA_ERR_UNSUPPORTED;  // a token's factors are held in 32 KB
+  if (p.rotary_dim > 4096) return FDMA_ERR_UNSUPPORTED;  // a CTA's factors are held in 128 KB
   if (static_cast<int64_t>(p.h + p.h_k) * p.d > (1 << 24)) return FDMA_ERR_UNSUPPORTED;
   if (p.b == 0 || p.seqlen == 0) return FDMA_OK;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fdma_internal.h"
 
@@ -14,10 +15,19 @@ namespace fdma {
 // the product modulo 2^64 IS the angle modulo a turn, without rounding: an angle at position 10^6 is as exact as one at 1, and no
 // 64-bit floating-point arithmetic or table over positions is needed. (fp32 angles are off by 0.06 at 10^6.)
 __device__ __forceinline__ float2 rotary_factors(int64_t position, int64_t turns, float amplitude, bool inverse) {
-  const int64_t phase = static_cast<int64_t>(static_cast<uint64_t>(position) * static_cast<uint64_t>(turns));
+  const uint64_t phase = static_cast<uint64_t>(position) * static_cast<uint64_t>(turns);
+  // the nearest quarter turn, and what is left of it as half turns in [-1/4, 1/4], rounded to 24 bits of ITS size
+  const uint64_t quarter = phase + (1ull << 61);
+  const int64_t left = static_cast<int64_t>(phase - (quarter & (3ull << 62)));
   float s, c;
-  sincospif(__ll2float_rn(phase) * 0x1p-63f, &s, &c);  // half turns in [-1, 1]
-  return make_float2(c * amplitude, inverse ? -s * amplitude : s * amplitude);
+  sincospif(__ll2float_rn(left) * 0x1p-63f, &s, &c);
+  const uint32_t n = static_cast<uint32_t>(quarter >> 62);
+  float cn = n & 1 ? -s : c, sn = n & 1 ? c : s;
+  if (n & 2) {
+    cn = -cn;
+    sn = -sn;
+  }
+  return make_float2(cn * amplitude, inverse ? -sn * amplitude : sn * amplitude);
 }
 
 template <typename T>
@@ -35,42 +45,55 @@ template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec {
   T x[N];
 };
+// N numbers rounded to T, two at a time where the type has an instruction for that
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> round_to(const float (&f)[N]) {
+  Vec<T, N> v;
+  if constexpr (N % 2 == 0 && sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) *reinterpret_cast<__nv_bfloat162*>(&v.x[j]) = __floats2bfloat162_rn(f[j], f[j + 1]);
+      else *reinterpret_cast<__half2*>(&v.x[j]) = __floats2half2_rn(f[j], f[j + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v.x[j] = from_f<T>(f[j]);
+  }
+  return v;
+}
 
 // A row is handled in units: N pairs each (2 N elements) for the rotated part, then N elements each for the rest. In the half
 // layout the two elements of a pair are rotary_dim / 2 apart, in the interleaved one they are neighbours.
 struct RotaryUnits {
-  int d, half, pair_units, units;  // half = rotary_dim / 2 (0: nothing rotated)
-  bool interleaved;
+  int half, pair_units, units;  // half = rotary_dim / 2 (0: nothing rotated)
 };
-inline RotaryUnits rotary_units(int d, int rotary_dim, bool interleaved, int n) {
+inline RotaryUnits rotary_units(int d, int rotary_dim, int n) {
   RotaryUnits u;
-  u.d = d;
   u.half = rotary_dim / 2;
   u.pair_units = u.half / n;
   u.units = u.pair_units + (d - rotary_dim) / n;
-  u.interleaved = interleaved;
   return u;
 }
 // whether units of n elements fit: otherwise n = 1
 inline bool rotary_units_fit(int d, int rotary_dim, int n) { return rotary_dim / 2 % n == 0 && (d - rotary_dim) % n == 0; }
 
 // The two vectors of unit u of a row in memory (the second is the first for a unit of the rest).
-template <int N>
+template <int N, bool kInterleaved>
 __device__ __forceinline__ int2 unit_offsets(const RotaryUnits& ru, int u) {
   if (u >= ru.pair_units) {
     const int at = 2 * ru.half + (u - ru.pair_units) * N;
     return make_int2(at, at);
   }
-  return ru.interleaved ? make_int2(2 * u * N, 2 * u * N + N) : make_int2(u * N, ru.half + u * N);
+  return kInterleaved ? make_int2(2 * u * N, 2 * u * N + N) : make_int2(u * N, ru.half + u * N);
 }
 
-// Rotates the 2 N values of unit u in place, given the N factors of its pairs.
-template <int N>
-__device__ __forceinline__ void rotate_unit(float (&a)[N], float (&b)[N], const float2* factors, bool interleaved) {
+// Rotates the 2 N values of a unit in place, given the factors of its pairs.
+template <int N, bool kInterleaved>
+__device__ __forceinline__ void rotate_unit(float (&a)[N], float (&b)[N], const float2* factors) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float2 f = factors[i];
-    if (interleaved) {  // pair i: elements 2 i, 2 i + 1 of a followed by b
+    if (kInterleaved) {  // pair i: elements 2 i, 2 i + 1 of a followed by b
       float& x1 = 2 * i < N ? a[(2 * i) % N] : b[(2 * i) % N];
       float& x2 = 2 * i + 1 < N ? a[(2 * i + 1) % N] : b[(2 * i + 1) % N];
       const float y1 = x1 * f.x - x2 * f.y;
@@ -84,70 +107,97 @@ __device__ __forceinline__ void rotate_unit(float (&a)[N], float (&b)[N], const 
   }
 }
 
-constexpr int kRotaryThreads = 256;
-
+// A warp takes one token (`abreast` of them where they are small), computes its factors, and goes over the heads of q and k: a lane
+// keeps its unit, and with it the factors in registers, and takes every so many heads. Nothing is shared between warps.
+// 2 x 4096 tokens of 32 + 8 heads, d = 128 (168 MB): 35 us (4.8 TB/s; a plain copy between the same buffers takes 33). Asking for
+// two or four heads at a time instead needs the registers of half the warps and took 42 and 44 us; going over the units of all
+// heads as one row, with the factors read for each vector, 42 us.
+constexpr int kRotaryWarps = 8;  // per CTA
 struct RotaryArgs {
   fdma_rotary_params p;
   RotaryUnits ru;
-  int tokens_per_cta;
-  int64_t tokens;
+  int abreast;
+  int64_t tokens, groups;  // groups: a warp each
 };
-// What CTA `cta` of a rotation does; s_factors holds tokens_per_cta * half pairs.
-template <typename T, int N>
-__device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int64_t cta, float2* s_factors) {
-  const fdma_rotary_params& p = a.p;
-  const RotaryUnits& ru = a.ru;
-  const int64_t token0 = cta * a.tokens_per_cta;
-  const int n = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_cta), a.tokens - token0));
-  for (int i = threadIdx.x; i < n * ru.half; i += kRotaryThreads) {
-    const int64_t token = token0 + i / ru.half;
-    const int64_t b = token / p.seqlen, s = token - b * p.seqlen;
-    int64_t pos = s;
-    if (p.positions) {
-      const int64_t at = b * p.pos_batch_stride + s * p.pos_row_stride;
-      pos = p.position_bits == 64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
-    }
-    s_factors[i] = rotary_factors(pos, p.turns[i % ru.half], p.amplitude, p.inverse != 0);
-  }
-  __syncthreads();
-  const int per_token = (p.h + p.h_k) * ru.units;
-  for (int i = threadIdx.x; i < n * per_token; i += kRotaryThreads) {
-    const int t = i / per_token, rest = i - t * per_token;
-    const int head = rest / ru.units, u = rest - head * ru.units;
-    const int64_t token = token0 + t;
-    const int64_t b = token / p.seqlen, s = token - b * p.seqlen;
-    const T* src;
-    T* dst;
-    if (head < p.h) {
-      src = static_cast<const T*>(p.q) + b * p.q_batch_stride + s * p.q_row_stride + head * p.q_head_stride;
-      dst = static_cast<T*>(p.q_out) + b * p.qo_batch_stride + s * p.qo_row_stride + head * p.qo_head_stride;
-    } else {
-      src = static_cast<const T*>(p.k) + b * p.k_batch_stride + s * p.k_row_stride + (head - p.h) * p.k_head_stride;
-      dst = static_cast<T*>(p.k_out) + b * p.ko_batch_stride + s * p.ko_row_stride + (head - p.h) * p.ko_head_stride;
-    }
-    const int2 at = unit_offsets<N>(ru, u);
-    using V = Vec<T, N>;
-    V x = *reinterpret_cast<const V*>(src + at.x);
-    if (u < ru.pair_units) {
-      V y = *reinterpret_cast<const V*>(src + at.y);
-      float fa[N], fb[N];
+
+// Units [first, first + units) of `heads` heads of n tokens.
+template <typename T, int N, bool kInterleaved, bool kPair>
+__device__ __forceinline__ void rotate_heads(const T* src, T* dst, int64_t src_row, int64_t dst_row, int64_t src_head, int64_t dst_head, int heads,
+                                             int n, const RotaryUnits& ru, const float2* s_factors) {
+  using V = Vec<T, N>;
+  const int lane = threadIdx.x & 31;
+  const int units = kPair ? ru.pair_units : ru.units - ru.pair_units;
+  for (int u0 = 0; u0 < units; u0 += 32) {
+    const int across = min(units - u0, 32);           // lanes of a head
+    const int place = lane / across, u = u0 + lane - place * across;
+    const int hs = min(32 / across, heads), ts = 32 / (across * hs);  // heads and tokens side by side
+    const int tsub = place / hs, hsub = place - tsub * hs;
+    if (tsub >= ts) continue;
+    const int2 at = unit_offsets<N, kInterleaved>(ru, kPair ? u : ru.pair_units + u);
+    const int64_t src_step = hs * src_head, dst_step = hs * dst_head;
+    for (int t = tsub; t < n; t += ts) {
+      float2 f[N];
+      if (kPair) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        fa[j] = to_f(x.x[j]);
-        fb[j] = to_f(y.x[j]);
+        for (int j = 0; j < N; ++j) f[j] = s_factors[t * ru.half + u * N + j];
       }
-      rotate_unit<N>(fa, fb, s_factors + t * ru.half + u * N, ru.interleaved);
+      const T* from = src + t * src_row + hsub * src_head + at.x;
+      T* to = dst + t * dst_row + hsub * dst_head + at.x;
+      const int apart = at.y - at.x;
+      for (int h = hsub; h < heads; h += hs) {
+        V x = *reinterpret_cast<const V*>(from);
+        if (kPair) {
+          const V y = *reinterpret_cast<const V*>(from + apart);
+          float fa[N], fb[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        x.x[j] = from_f<T>(fa[j]);
-        y.x[j] = from_f<T>(fb[j]);
+          for (int j = 0; j < N; ++j) {
+            fa[j] = to_f(x.x[j]);
+            fb[j] = to_f(y.x[j]);
+          }
+          rotate_unit<N, kInterleaved>(fa, fb, f);
+          x = round_to<T, N>(fa);
+          *reinterpret_cast<V*>(to + apart) = round_to<T, N>(fb);
+        }
+        *reinterpret_cast<V*>(to) = x;
+        from += src_step;
+        to += dst_step;
       }
-      *reinterpret_cast<V*>(dst + at.y) = y;
     }
-    *reinterpret_cast<V*>(dst + at.x) = x;
   }
 }
 
+// What warp `group` of a rotation does; s_factors: abreast * half pairs of the warp's own.
+template <typename T, int N, bool kInterleaved>
+__device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int64_t group, float2* s_factors) {
+  if (group >= a.groups) return;
+  const fdma_rotary_params& p = a.p;
+  const RotaryUnits& ru = a.ru;
+  const int lane = threadIdx.x & 31;
+  // groups do not cross batch rows
+  const int per_row = (p.seqlen + a.abreast - 1) / a.abreast;
+  const int64_t b = a.groups <= 0x7FFFFFFF ? static_cast<uint32_t>(group) / static_cast<uint32_t>(per_row) : group / per_row;
+  const int s = static_cast<int>(group - b * per_row) * a.abreast, n = min(a.abreast, p.seqlen - s);
+  for (int i = lane; i < n * ru.half; i += 32) {
+    const int t = a.abreast > 1 ? i / ru.half : 0, f = i - t * ru.half;
+    int64_t pos = s + t;
+    if (p.positions) {
+      const int64_t at = b * p.pos_batch_stride + pos * p.pos_row_stride;
+      pos = p.position_bits == 64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
+    }
+    s_factors[i] = rotary_factors(pos, p.turns[f], p.amplitude, p.inverse != 0);
+  }
+  __syncwarp();
+  const T* q = static_cast<const T*>(p.q) + b * p.q_batch_stride + s * p.q_row_stride;
+  T* qo = static_cast<T*>(p.q_out) + b * p.qo_batch_stride + s * p.qo_row_stride;
+  const T* k = static_cast<const T*>(p.k) + b * p.k_batch_stride + s * p.k_row_stride;
+  T* ko = static_cast<T*>(p.k_out) + b * p.ko_batch_stride + s * p.ko_row_stride;
+  rotate_heads<T, N, kInterleaved, true>(q, qo, p.q_row_stride, p.qo_row_stride, p.q_head_stride, p.qo_head_stride, p.h, n, ru, s_factors);
+  if (p.h_k) rotate_heads<T, N, kInterleaved, true>(k, ko, p.k_row_stride, p.ko_row_stride, p.k_head_stride, p.ko_head_stride, p.h_k, n, ru, s_factors);
+  if (ru.units > ru.pair_units) {
+    rotate_heads<T, N, kInterleaved, false>(q, qo, p.q_row_stride, p.qo_row_stride, p.q_head_stride, p.qo_head_stride, p.h, n, ru, s_factors);
+    if (p.h_k) rotate_heads<T, N, kInterleaved, false>(k, ko, p.k_row_stride, p.ko_row_stride, p.k_head_stride, p.ko_head_stride, p.h_k, n, ru, s_factors);
+  }
+}
 
 // Whether every row of the given tensors can be accessed in 16-byte vectors.
 inline bool rotary_aligned16(const fdma_rotary_params& p, int bytes) {
@@ -162,13 +212,12 @@ inline bool rotary_aligned16(const fdma_rotary_params& p, int bytes) {
 inline RotaryArgs rotary_args(const fdma_rotary_params& p, int n) {
   RotaryArgs a;
   a.p = p;
-  a.ru = rotary_units(p.d, p.rotary_dim, p.interleaved != 0, n);
+  a.ru = rotary_units(p.d, p.rotary_dim, n);
+  a.abreast = std::max(1, std::min(p.seqlen, 32 / (p.h * std::max(1, a.ru.pair_units))));
   a.tokens = static_cast<int64_t>(p.b) * p.seqlen;
-  const int64_t per_token = static_cast<int64_t>(p.h + p.h_k) * a.ru.units;
-  int64_t t = std::max<int64_t>(1, 4 * kRotaryThreads / per_token);
-  t = std::min<int64_t>(t, std::max(1, 4096 / a.ru.half));  // 32 KB of factors
-  a.tokens_per_cta = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(t, a.tokens / (4 * sm_count()))));
+  a.groups = static_cast<int64_t>(p.b) * ((p.seqlen + a.abreast - 1) / a.abreast);
   return a;
 }
+inline size_t rotary_smem(const RotaryArgs& a) { return static_cast<size_t>(kRotaryWarps) * a.abreast * a.ru.half * sizeof(float2); }
 
 }  // namespace fdma

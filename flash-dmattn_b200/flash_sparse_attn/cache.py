@@ -172,8 +172,6 @@ def flash_sparse_attn_cache_func(
     Returns (tokens, H, d). Rows of tokens behind the last request, of refused requests and of queries that see no key are 0.
     Scores, probabilities' sums and outputs are accumulated in 32 bits; probabilities enter the second product in 16 bits.
     There are no gradients: a call that would need them raises."""
-    from .compaction import index_kept_keys
-
     args = _cache_args(cache, tables, step)
     key_pos = count = None
     if isinstance(attn_mask, KeptKeys):
@@ -185,6 +183,8 @@ def flash_sparse_attn_cache_func(
         else:
             if attn_mask.dtype != torch.bool or attn_mask.dim() != 4 or attn_mask.shape[2] != 1:
                 raise RuntimeError("attn_mask must be a KeptKeys or a bool tensor ({1|requests}, {1|num_heads_k}, 1, keys)")
+            from .compaction import index_kept_keys
+
             m = attn_mask[:, :, 0]
             key_pos, count, _ = index_kept_keys(m if m.stride(-1) == 1 else m.contiguous(), m.shape[-1], False)
     max_q = query.shape[0] if max_seqlen_q is None else max_seqlen_q
