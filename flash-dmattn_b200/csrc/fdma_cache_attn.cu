@@ -8,9 +8,9 @@
 //    read once for all of them. The products are in fp16 with 32-bit sums: e4m3 numbers are fp16 numbers (one conversion
 //    instruction for two), bf16 queries become fp16 after a power of two per row (exact up to 2^-29 of the row's largest), and
 //    scales, being powers of two or common to a product, go into the scores and the softmax's exponents.
-//  * The unit of work is a chunk of 64 keys of a (request, kv head). All chunks of a step form one row; every CTA takes an equal
-//    part of it, however long the requests are, and starts and ends in the middle of a unit where it must. Such partial results
-//    go through scratch and a second kernel; units that one CTA finishes are written directly.
+//  * A unit of work is a (request, kv head, tile of 8 or 16 rows), made of chunks of 64 keys. The chunks of all units form one row;
+//    every CTA takes an equal part of it, however long the requests are, and starts and ends in the middle of a unit where it
+//    must. Such partial results go through scratch and a second kernel; units that one CTA finishes are written directly.
 //  * A warp of the CTA copies chunks to shared memory by TMA, three ahead; four warps take 16 keys of each. The 128-byte swizzle
 //    and the order in which keys are assigned to the columns of the products (`key_row`) make all reads free of bank conflicts:
 //    K fragments are 16-byte reads of a key's row, V fragments 4-byte reads of four keys whose bytes are then paired.
@@ -33,26 +33,31 @@ namespace {
 constexpr int kChunk = 64;
 constexpr int kWarps = 4;  // that compute; each has 16 keys of a chunk
 constexpr int kSlice = kChunk / kWarps;
-constexpr int kSearch = 256;  // requests whose chunk sums are held in shared memory
+constexpr int kHeld = 128;  // requests whose work a CTA holds in shared memory
 constexpr int kMinShare = 2;  // chunks per CTA
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPScale = 16384.f;  // probabilities in fp16: normal numbers down to 2^-28
 
 struct AttnArgs {
   fdma_cache_attention_params p;
-  int shift, group;
-  int list_chunks;  // kept keys: chunks per unit; 0: from cu_chunks
-  int ctas;         // along the row of chunks
+  int shift, group, rows;  // rows: of a tile
+  int list_chunks;         // kept keys: chunks per unit; 0: from cu_chunks
+  int tiles;               // row tiles of the request with the most queries
+  int ctas;                // along the row of chunks
   float scale_log2;
-  bool q_vec;       // queries in 16-byte vectors
-  float* partial;   // [row tile][cta][2][ROWS][D + 4]: sums over the values, then maximum and sum
+  bool q_vec;              // queries in 16-byte vectors
+  float* partial;          // [cta][2][rows][D + 4]: sums over the values, then maximum and sum
   int* status;
 };
 
-// Where the work of a launch lies: unit u = (request, kv head) has the chunks [start, start + n) of the row.
+// Where the work lies: unit (request, kv head, tile) has the chunks [start, start + n) of the row.
 struct Unit {
-  int r, hk, n;
+  int r, hk, tile, n;
   int64_t start;
+};
+// Queries and keys of a request, made safe against plans that do not fit the call.
+struct Request {
+  int token0, n, length, rows, chunks;
 };
 
 // lowest key row of a slice's eight keys for column n of the products: pairs of lanes that read K together, and lanes that read
@@ -116,58 +121,110 @@ __device__ __forceinline__ float p_scale(float exponent) { return exponent < -10
 __device__ __forceinline__ float exponent_of(float x) { return static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) - 127); }
 __device__ __forceinline__ float exp2_or_zero(float x) { return x == -CUDART_INF_F ? 0.f : exp2f(x); }
 
-// The units in the order of their chunks; s_cu holds cu_chunks for up to kSearch requests.
+__device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
+  const fdma_cache& c = a.p.c;
+  Request q;
+  const int first = c.cu_seqlens[r], end = c.cu_seqlens[r + 1], chunk0 = c.cu_chunks[r], chunk1 = c.cu_chunks[r + 1];
+  q.length = c.lengths[r];
+  q.token0 = max(0, first);
+  q.n = max(0, min(end, c.tokens) - q.token0);
+  q.chunks = max(0, chunk1 - chunk0);
+  q.rows = q.chunks ? min(q.n, a.p.max_seqlen_q) * a.group : 0;  // no chunks: refused
+  if (a.list_chunks) q.chunks = a.list_chunks;
+  return q;
+}
+
+// The units in the order of their chunks. Up to kHeld requests: their data and the sums of their chunks x tiles are held in shared
+// memory. More: every request counts with the tiles of the largest, and what is needed is read where it is needed.
+struct Held {
+  int pre[kHeld + 1], token0[kHeld], n[kHeld], length[kHeld], rows[kHeld], chunks[kHeld], warp[4];
+};
 struct Units {
   const AttnArgs& a;
-  const int32_t* cu;
+  const Held* held;  // null: too many requests
   __device__ int64_t total() const {
-    return (a.list_chunks ? static_cast<int64_t>(a.p.c.requests) * a.list_chunks : static_cast<int64_t>(cu[a.p.c.requests])) * a.p.c.h_k;
+    const fdma_cache& c = a.p.c;
+    if (held) return static_cast<int64_t>(held->pre[c.requests]) * c.h_k;
+    return (a.list_chunks ? static_cast<int64_t>(c.requests) * a.list_chunks : static_cast<int64_t>(c.cu_chunks[c.requests])) * a.tiles * c.h_k;
   }
-  __device__ Unit of_request(int r, int hk) const {
+  __device__ Request request(int r) const {
+    if (!held) return load_request(a, r);
+    return Request{held->token0[r], held->n[r], held->length[r], held->rows[r], held->chunks[r]};
+  }
+  __device__ Unit of(int r, int hk, int tile) const {
+    const fdma_cache& c = a.p.c;
     Unit u;
-    u.r = r;
-    u.hk = hk;
-    u.n = a.list_chunks ? a.list_chunks : cu[r + 1] - cu[r];
-    u.start = (a.list_chunks ? static_cast<int64_t>(r) * a.list_chunks : static_cast<int64_t>(cu[r])) * a.p.c.h_k + static_cast<int64_t>(hk) * u.n;
+    u.r = r; u.hk = hk; u.tile = tile;
+    int tiles = a.tiles;
+    if (held) {
+      u.n = held->chunks[r];
+      tiles = (held->rows[r] + a.rows - 1) / a.rows;
+      u.start = static_cast<int64_t>(held->pre[r]) * c.h_k;
+    } else if (a.list_chunks) {
+      u.n = a.list_chunks;
+      u.start = static_cast<int64_t>(r) * u.n * tiles * c.h_k;
+    } else {
+      const int first = c.cu_chunks[r];
+      u.n = c.cu_chunks[r + 1] - first;
+      u.start = static_cast<int64_t>(first) * tiles * c.h_k;
+    }
+    u.start += (static_cast<int64_t>(hk) * tiles + tile) * u.n;
     return u;
   }
   // the unit of chunk w, w < total()
   __device__ Unit at(int64_t w) const {
-    const int64_t per_head = w / a.p.c.h_k;  // cu[r] <= per_head < cu[r + 1]
+    const fdma_cache& c = a.p.c;
+    const int64_t per_head = w / c.h_k;  // of the request: start / h_k <= per_head < end / h_k
     int r;
-    if (a.list_chunks) {
-      r = static_cast<int>(per_head / a.list_chunks);
+    if (!held && a.list_chunks) {
+      r = static_cast<int>(per_head / (static_cast<int64_t>(a.list_chunks) * a.tiles));
     } else {
-      int lo = 0, hi = a.p.c.requests - 1;
+      const int64_t scale = held ? 1 : a.tiles;
+      const int32_t* ends = held ? held->pre + 1 : c.cu_chunks + 1;
+      int lo = 0, hi = c.requests - 1;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (cu[mid + 1] > per_head) hi = mid;
+        if (ends[mid] * scale > per_head) hi = mid;
         else lo = mid + 1;
       }
       r = lo;
     }
-    Unit u = of_request(r, 0);
-    u.hk = static_cast<int>((w - u.start) / u.n);
-    u.start += static_cast<int64_t>(u.hk) * u.n;
+    Unit u = of(r, 0, 0);
+    const int tiles = held ? (held->rows[r] + a.rows - 1) / a.rows : a.tiles;
+    const int i = static_cast<int>((w - u.start) / max(u.n, 1));
+    u.hk = i / tiles;
+    u.tile = i - u.hk * tiles;
+    u.start += static_cast<int64_t>(i) * u.n;
     return u;
   }
 };
-__device__ __forceinline__ int64_t share_of(int64_t total, int ctas) { return max(static_cast<int64_t>(kMinShare), (total + ctas - 1) / ctas); }
-
-// Queries and keys of a unit's request, made safe against plans that do not fit the call.
-struct Request {
-  int token0, n, length, rows;
-};
-__device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
-  const fdma_cache& c = a.p.c;
-  Request q;
-  q.token0 = max(0, c.cu_seqlens[r]);
-  q.n = max(0, min(c.cu_seqlens[r + 1], c.tokens) - q.token0);
-  q.length = c.lengths[r];
-  q.rows = min(q.n, a.p.max_seqlen_q) * a.group;
-  if (a.list_chunks && c.cu_chunks[r + 1] <= c.cu_chunks[r]) q.rows = 0;  // refused (not among the chunks of a call without a list)
-  return q;
+// All threads of a CTA of at least 128.
+__device__ __forceinline__ Units make_units(const AttnArgs& a, Held& h) {
+  const int R = a.p.c.requests;
+  if (R > kHeld) return Units{a, nullptr};
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int w = 0;
+  if (tid < R) {
+    const Request q = load_request(a, tid);
+    h.token0[tid] = q.token0; h.n[tid] = q.n; h.length[tid] = q.length; h.rows[tid] = q.rows; h.chunks[tid] = q.chunks;
+    w = q.chunks * ((q.rows + a.rows - 1) / a.rows);
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  if (lane == 31 && warp < 4) h.warp[warp] = w;
+  __syncthreads();
+  if (tid < kHeld) {
+    for (int i = 0; i < warp; ++i) w += h.warp[i];
+    h.pre[tid + 1] = w;
+    if (tid == 0) h.pre[0] = 0;
+  }
+  __syncthreads();
+  return Units{a, &h};
 }
+__device__ __forceinline__ int64_t share_of(int64_t total, int ctas) { return max(static_cast<int64_t>(kMinShare), (total + ctas - 1) / ctas); }
 
 template <int D, int ROWS, bool kGather>
 struct Layout {
@@ -184,7 +241,7 @@ struct Layout {
   static constexpr int kBuf = kQ + kQBytes;
   static constexpr int kTotal = kBuf + kBufs * kBufFloats * 4 + 1024;
   static constexpr int kThreads = kWarps * 32 + (kGather ? 0 : 32);
-  static constexpr int kCtas = D > 128 || ROWS > 16 ? 2 : 3;        // per SM
+  static constexpr int kCtas = D > 128 ? 2 : 3;                     // per SM
 };
 
 template <int D, int ROWS, bool kGather, bool kBf16>
@@ -198,19 +255,14 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   // of a slice: 1 if its block is there, K scale, exponent of the V scale, its reciprocal; of a kept key: bias (-inf: not there),
   // K scale, exponent of the V scale, position
   __shared__ float4 s_meta[L::kStages][kGather ? kChunk : kWarps];
-  __shared__ int32_t s_cu[kSearch + 1];
+  __shared__ Held s_held;
   __shared__ float s_row_scale[ROWS], s_m[kWarps][ROWS], s_l[kWarps][ROWS];
   __shared__ int s_abort;
   unsigned char* smem = align_smem_1024(s_raw);
   const fdma_cache_attention_params& p = a.p;
   const fdma_cache& c = p.c;
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
-  const int row0 = blockIdx.y * ROWS;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  const bool in_smem = !kGather && c.requests <= kSearch;
-  if (in_smem)
-    for (int i = tid; i <= c.requests; i += L::kThreads) s_cu[i] = c.cu_chunks[i];
   if (tid == 0) {
     s_abort = 0;
     if (!kGather) {
@@ -223,8 +275,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   }
   if (kGather && c.d < D)  // columns beyond the head dim stay zero in every stage
     for (int i = tid; i < L::kStages * L::kStageBytes / 16; i += L::kThreads) reinterpret_cast<uint4*>(smem + L::kRing)[i] = make_uint4(0, 0, 0, 0);
+  const Units units = make_units(a, s_held);
   __syncthreads();
-  const Units units{a, in_smem ? s_cu : c.cu_chunks};
   const int64_t total = units.total(), share = share_of(total, a.ctas);
   const int64_t w0 = min(total, blockIdx.x * share), w1 = min(total, w0 + share);
   if (w0 >= w1) return;
@@ -241,8 +293,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       if (w < w1) {
         const Unit u = units.at(w);
         hk = u.hk;
-        const Request q = request_of(a, u.r);
-        used = q.rows > row0;
+        const Request q = units.request(u.r);
+        used = q.rows > u.tile * ROWS;
         const int pos = static_cast<int>(w - u.start) * kChunk + (lane & 3) * kSlice;
         if (used && pos < min(q.length, p.max_seqlen_k) && (pos >> a.shift) < c.width) {
           block = c.table[static_cast<int64_t>(u.r) * c.width + (pos >> a.shift)];
@@ -335,7 +387,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const Unit u = units.at(w);
     const int64_t unit_end = max(u.start + u.n, w + 1);
     const int first = static_cast<int>(w - u.start), last = static_cast<int>(min(unit_end, w1) - u.start);
-    const Request q = request_of(a, u.r);
+    const Request q = units.request(u.r);
+    const int row0 = u.tile * ROWS;
     w = min(unit_end, w1);
     const int nrows = min(ROWS, q.rows - row0);
     if (nrows <= 0) continue;
@@ -695,7 +748,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
     if (warp != 0) continue;
     const bool complete = first == 0 && last == u.n;
-    float* part = a.partial + ((static_cast<int64_t>(blockIdx.y) * a.ctas + blockIdx.x) * 2 + (first > 0 ? 0 : 1)) * ROWS * (D + 4);
+    float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (first > 0 ? 0 : 1)) * ROWS * (D + 4);
 #pragma unroll
     for (int rs = 0; rs < kGroups; ++rs) {
       const int rr = g + 8 * rs, row = row0 + rr;
@@ -731,9 +784,10 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 // Joins the sums of units that several CTAs share, and writes the zeros of rows that nobody computes: a CTA per (token, head),
 // whose warps take a quarter of the sums each.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant__ AttnArgs a, const int rows_per_tile) {
+__global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant__ AttnArgs a) {
   const fdma_cache_attention_params& p = a.p;
   const fdma_cache& c = p.c;
+  __shared__ Held s_held;
   __shared__ int s_request;
   __shared__ float s_top[4], s_sum[4], s_acc[4][D];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -742,64 +796,89 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant_
   __syncthreads();
   for (int r = tid; r < c.requests; r += 128)
     if (c.cu_seqlens[r] <= token && token < c.cu_seqlens[r + 1]) s_request = r;
-  const Units units{a, c.cu_chunks};
-  const int64_t total = units.total(), share = share_of(total, a.ctas);
+  const Units units = make_units(a, s_held);
   __syncthreads();
+  const int64_t total = units.total(), share = share_of(total, a.ctas);
   const int r = s_request;
   int c0 = 0, c1 = -1;
   const float* base = nullptr;
-  const int64_t step = static_cast<int64_t>(rows_per_tile) * (D + 4);
+  const int64_t step = static_cast<int64_t>(a.rows) * (D + 4);
   bool written = false;
   if (r >= 0) {
-    const Request q = request_of(a, r);
-    const int row = (token - q.token0) * a.group + head % a.group;
-    const Unit u = units.of_request(r, head / a.group);
-    if (row >= 0 && row < q.rows && u.n > 0) {
+    const Request q = units.request(r);
+    const int row = (token - q.token0) * a.group + head % a.group, tile = row / a.rows;
+    if (row >= 0 && row < q.rows) {
+      const Unit u = units.of(r, head / a.group, tile);
       c0 = static_cast<int>(u.start / share);
       c1 = static_cast<int>((u.start + u.n - 1) / share);
       written = c0 == c1;  // by that CTA
-      const int tile = row / rows_per_tile;
-      base = a.partial + (static_cast<int64_t>(tile) * a.ctas * 2 * rows_per_tile + row - tile * rows_per_tile) * (D + 4);
+      base = a.partial + static_cast<int64_t>(row - tile * a.rows) * (D + 4);
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (written) return;
-  float top = -CUDART_INF_F;
-  for (int x = c0 + tid; x <= c1; x += 128) top = fmaxf(top, base[(2 * static_cast<int64_t>(x) + (x == c0)) * step + D]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) s_top[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  const float from = top == -CUDART_INF_F ? 0.f : top;
-  constexpr int E = D / 32;  // elements per lane
-  float acc[E], sum = 0.f;
+  // each warp takes every fourth sum, eight at a time, and scales to its own maximum
+  constexpr int E = D / 32, kAhead = D > 128 ? 4 : 8;  // elements per lane
+  float acc[E], sum = 0.f, top = -CUDART_INF_F;
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int x = c0 + warp; x <= c1; x += 4) {
-    const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
-    const float2 ml = *reinterpret_cast<const float2*>(src + D);
-    const float f = exp2_or_zero(ml.x - from);
-    sum = fmaf(ml.y, f, sum);
+  for (int x0 = c0 + warp; x0 <= c1; x0 += 4 * kAhead) {
+    float2 ml[kAhead], y[kAhead][E / 2];
 #pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const float2 y = *reinterpret_cast<const float2*>(src + lane * E + i);
-      acc[i] = fmaf(y.x, f, acc[i]);
-      acc[i + 1] = fmaf(y.y, f, acc[i + 1]);
+    for (int k = 0; k < kAhead; ++k) {
+      const int x = x0 + 4 * k;
+      ml[k] = make_float2(-CUDART_INF_F, 0.f);
+      if (x <= c1) {
+        const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
+        ml[k] = *reinterpret_cast<const float2*>(src + D);
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) y[k][i] = *reinterpret_cast<const float2*>(src + lane * E + 2 * i);
+      }
     }
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) now = fmaxf(now, ml[k].x);
+    const float from = now == -CUDART_INF_F ? 0.f : now, f0 = exp2_or_zero(top - from);
+    top = now;
+    sum *= f0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] *= f0;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (x0 + 4 * k <= c1) {
+        const float f = exp2_or_zero(ml[k].x - from);
+        sum = fmaf(ml[k].y, f, sum);
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+          acc[2 * i] = fmaf(y[k][i].x, f, acc[2 * i]);
+          acc[2 * i + 1] = fmaf(y[k][i].y, f, acc[2 * i + 1]);
+        }
+      }
   }
-  if (lane == 0) s_sum[warp] = sum;
+  if (lane == 0) {
+    s_top[warp] = top;
+    s_sum[warp] = sum;
+  }
 #pragma unroll
   for (int i = 0; i < E; ++i) s_acc[warp][lane * E + i] = acc[i];
   __syncthreads();
-  sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  const float from = top == -CUDART_INF_F ? 0.f : top;
+  float f[4];
+  sum = 0.f;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    f[x] = exp2_or_zero(s_top[x] - from);
+    sum = fmaf(s_sum[x], f[x], sum);
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* dst = static_cast<uint16_t*>(p.out) + token * p.out_row_stride + head * p.out_head_stride;
   for (int i = 2 * tid; i < c.d; i += 256) {
-    float y[2];
+    float y[2] = {0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) y[k] = (s_acc[0][i + k] + s_acc[1][i + k]) + (s_acc[2][i + k] + s_acc[3][i + k]);
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) y[k] = fmaf(s_acc[x][i + k], f[x], y[k]);
     *reinterpret_cast<uint32_t*>(dst + i) = pack2<kBf16>(y[0] * inv, y[1] * inv);
   }
 }
@@ -814,13 +893,11 @@ Plan plan_of(const fdma_cache_attention_params& p) {
   Plan pl;
   const int64_t most = static_cast<int64_t>(std::min(p.max_seqlen_q, p.c.tokens)) * (p.h / p.c.h_k);
   pl.D = tile_dim(p.c.d);
-  // rows of a tile: as few as hold the queries of a request, up to what the accumulators leave registers for
-  pl.rows = most <= 8 ? 8 : most <= 16 || pl.D == 256 ? 16 : 32;
+  pl.rows = most <= 8 ? 8 : 16;
   pl.tiles = static_cast<int>(std::max<int64_t>(1, (most + pl.rows - 1) / pl.rows));
-  const int resident = (pl.D == 256 || pl.rows == 32 ? 2 : 3) * sm_count();
-  pl.ctas = std::max(1, resident / pl.tiles);
+  pl.ctas = (pl.D == 256 ? 2 : 3) * sm_count();
   pl.list_chunks = p.kept_pos ? (p.kept_capacity + kChunk - 1) / kChunk : 0;
-  pl.bytes = align256(static_cast<size_t>(pl.tiles) * pl.ctas * 2 * pl.rows * (pl.D + 4) * sizeof(float));
+  pl.bytes = align256(static_cast<size_t>(pl.ctas) * 2 * pl.rows * (pl.D + 4) * sizeof(float));
   return pl;
 }
 
@@ -841,7 +918,7 @@ int launch(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
   static std::atomic<uint64_t> prepared{0};
   const int st_smem = allow_smem_once(reinterpret_cast<const void*>(kern), L::kTotal, prepared);
   if (st_smem) return st_smem;
-  kern<<<dim3(pl.ctas, pl.tiles), L::kThreads, L::kTotal, stream>>>(a, map_k, map_v);
+  kern<<<pl.ctas, L::kThreads, L::kTotal, stream>>>(a, map_k, map_v);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
   // the second kernel's CTAs start while the first one's finish, and wait for them only where they need their sums
@@ -854,7 +931,7 @@ int launch(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, cache_merge_kernel<D, kBf16>, a, ROWS));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, cache_merge_kernel<D, kBf16>, a));
 }
 template <int D, int ROWS>
 int launch_t(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
@@ -895,11 +972,12 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   if ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uint64_t>(p.out_row_stride | p.out_head_stride) * 2) % 16) return FDMA_ERR_UNSUPPORTED;
   const Plan pl = plan_of(p);
   if (!p.workspace || p.workspace_bytes < pl.bytes) return FDMA_ERR_WORKSPACE;
-  if (pl.tiles > 65535) return FDMA_ERR_UNSUPPORTED;
   AttnArgs a = {};
   a.p = p;
   a.shift = p.c.block_size == 16 ? 4 : p.c.block_size == 32 ? 5 : p.c.block_size == 64 ? 6 : 7;
   a.group = p.h / p.c.h_k;
+  a.rows = pl.rows;
+  a.tiles = pl.tiles;
   a.list_chunks = pl.list_chunks;
   a.ctas = pl.ctas;
   a.scale_log2 = p.softmax_scale * kLog2e;
@@ -909,6 +987,6 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   if (!a.status) return FDMA_ERR_DRIVER;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (pl.D == 256) return pl.rows == 8 ? launch_t<256, 8>(a, pl, stream) : launch_t<256, 16>(a, pl, stream);
-  if (pl.D == 128) return pl.rows == 8 ? launch_t<128, 8>(a, pl, stream) : pl.rows == 16 ? launch_t<128, 16>(a, pl, stream) : launch_t<128, 32>(a, pl, stream);
-  return pl.rows == 8 ? launch_t<64, 8>(a, pl, stream) : pl.rows == 16 ? launch_t<64, 16>(a, pl, stream) : launch_t<64, 32>(a, pl, stream);
+  if (pl.D == 128) return pl.rows == 8 ? launch_t<128, 8>(a, pl, stream) : launch_t<128, 16>(a, pl, stream);
+  return pl.rows == 8 ? launch_t<64, 8>(a, pl, stream) : launch_t<64, 16>(a, pl, stream);
 }

@@ -233,6 +233,15 @@ void bump(std::initializer_list<Tensor> written) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// `n` elements of a buffer from a byte offset on, as a tensor of its own that shares the storage
+Tensor part_of(const Tensor& buf, int64_t bytes, int64_t n, at::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), c10::scalarTypeToTypeMeta(type));
+  c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+  impl->set_sizes_contiguous({n});
+  impl->set_storage_offset(bytes / static_cast<int64_t>(c10::elementSize(type)));
+  return t;
+}
+
 std::vector<Tensor> extend(const Tables& t, const Tensor& new_lengths, int64_t tokens) {
   fdma_tables_params p = tables_params(t, new_lengths);
   need(tokens >= 0 && tokens <= (1 << 30), "the number of tokens must be between 0 and 2^30");
@@ -240,28 +249,24 @@ std::vector<Tensor> extend(const Tables& t, const Tensor& new_lengths, int64_t t
   const c10::cuda::CUDAGuard device(t.table.device());
   const int64_t R = p.requests;
   p.tokens = static_cast<int32_t>(tokens);
-  // one allocation for the int32 parts of the plan
-  const int64_t parts[] = {R + 1, tokens, R, R + 1, R + 1};
-  int64_t total = 0;
-  for (int64_t n : parts) total += (n + 31) / 32 * 32;
-  const Tensor buf = empty({total}, at::kInt, t.table);
-  Tensor part[5];
-  int64_t at_ = 0;
-  for (int i = 0; i < 5; ++i) {
-    part[i] = buf.narrow(0, at_, parts[i]);
-    at_ += (parts[i] + 31) / 32 * 32;
-  }
-  Tensor slots = empty({tokens}, at::kLong, t.table), granted = empty({R}, at::kBool, t.table);
+  // the plan in one allocation
+  const int64_t parts[] = {R + 1, tokens, tokens, R, R, R + 1, R + 1};
+  const at::ScalarType types[] = {at::kInt, at::kInt, at::kLong, at::kInt, at::kBool, at::kInt, at::kInt};
+  int64_t offsets[8] = {0};
+  for (int i = 0; i < 7; ++i) offsets[i + 1] = offsets[i] + (parts[i] * static_cast<int64_t>(c10::elementSize(types[i])) + 127) / 128 * 128;
+  const Tensor buf = empty({offsets[7]}, at::kByte, t.table);
+  Tensor part[7];
+  for (int i = 0; i < 7; ++i) part[i] = part_of(buf, offsets[i], parts[i], types[i]);
   p.cu_seqlens = part[0].data_ptr<int32_t>();
   p.positions = tokens ? part[1].data_ptr<int32_t>() : nullptr;
-  p.slots = tokens ? slots.data_ptr<int64_t>() : nullptr;
-  p.lengths_after = part[2].data_ptr<int32_t>();
-  p.granted = static_cast<uint8_t*>(granted.data_ptr());
-  p.cu_blocks = part[3].data_ptr<int32_t>();
-  p.cu_chunks = part[4].data_ptr<int32_t>();
+  p.slots = tokens ? part[2].data_ptr<int64_t>() : nullptr;
+  p.lengths_after = part[3].data_ptr<int32_t>();
+  p.granted = static_cast<uint8_t*>(part[4].data_ptr());
+  p.cu_blocks = part[5].data_ptr<int32_t>();
+  p.cu_chunks = part[6].data_ptr<int32_t>();
   check(api.tables_extend(&p, stream_of(t.table)), "fdma_tables_extend");
   bump({t.table, t.lengths, t.free_count});
-  return {part[0], part[1], slots, part[2], granted, part[3], part[4]};
+  return std::vector<Tensor>(part, part + 7);
 }
 
 void truncate(const Tables& t, const Tensor& lengths) {
