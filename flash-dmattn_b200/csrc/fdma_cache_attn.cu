@@ -26,8 +26,6 @@
 
 namespace fdma {
 
-int check_cache(const fdma_cache& c);  // fdma_cache.cu
-
 namespace {
 
 constexpr int kChunk = 64;
@@ -42,10 +40,13 @@ struct AttnArgs {
   fdma_cache_attention_params p;
   int shift, group, rows;  // rows: of a tile
   int list_chunks;         // kept keys: chunks per unit; 0: from cu_chunks
-  int tiles;               // row tiles of the request with the most queries
+  const int32_t* pre;      // more than kHeld requests: sums of their chunks x tiles, requests + 1
   int ctas;                // along the row of chunks
   float scale_log2;
   bool q_vec;              // queries in 16-byte vectors
+  const int32_t* prompts;  // not null: rows of no request are written already, and if it points to a number above 0, those of
+                           // requests with kPromptTokens or more as well
+  bool merge_requests;     // CTAs of the second kernel: kPromptTokens - 1 for each request, not one for every token
   float* partial;          // [cta][2][rows][D + 4]: sums over the values, then maximum and sum
   int* status;
 };
@@ -57,7 +58,7 @@ struct Unit {
 };
 // Queries and keys of a request, made safe against plans that do not fit the call.
 struct Request {
-  int token0, n, length, rows, chunks;
+  int token0, n, length, rows, chunks;  // rows = -1: done already
 };
 
 // lowest key row of a slice's eight keys for column n of the products: pairs of lanes that read K together, and lanes that read
@@ -130,72 +131,49 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
   q.n = max(0, min(end, c.tokens) - q.token0);
   q.chunks = max(0, chunk1 - chunk0);
   q.rows = q.chunks ? min(q.n, a.p.max_seqlen_q) * a.group : 0;  // no chunks: refused
+  if (a.prompts && q.n >= kPromptTokens && *a.prompts > 0) q.rows = -1;
   if (a.list_chunks) q.chunks = a.list_chunks;
   return q;
 }
 
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, int rows) { return rows > 0 ? (rows + a.rows - 1) / a.rows : 0; }
+
 // The units in the order of their chunks. Up to kHeld requests: their data and the sums of their chunks x tiles are held in shared
-// memory. More: every request counts with the tiles of the largest, and what is needed is read where it is needed.
+// memory. More: the sums are in global memory, and the data is read where it is needed.
 struct Held {
   int pre[kHeld + 1], token0[kHeld], n[kHeld], length[kHeld], rows[kHeld], chunks[kHeld], warp[4];
 };
 struct Units {
   const AttnArgs& a;
   const Held* held;  // null: too many requests
-  __device__ int64_t total() const {
-    const fdma_cache& c = a.p.c;
-    if (held) return static_cast<int64_t>(held->pre[c.requests]) * c.h_k;
-    return (a.list_chunks ? static_cast<int64_t>(c.requests) * a.list_chunks : static_cast<int64_t>(c.cu_chunks[c.requests])) * a.tiles * c.h_k;
-  }
+  __device__ const int32_t* pre() const { return held ? held->pre : a.pre; }
+  __device__ int64_t total() const { return static_cast<int64_t>(pre()[a.p.c.requests]) * a.p.c.h_k; }
   __device__ Request request(int r) const {
     if (!held) return load_request(a, r);
     return Request{held->token0[r], held->n[r], held->length[r], held->rows[r], held->chunks[r]};
   }
-  __device__ Unit of(int r, int hk, int tile) const {
-    const fdma_cache& c = a.p.c;
+  // `tile` and `hk` may be past the end of the request's: the start then is, too
+  __device__ Unit of(int r, const Request& q, int hk, int tile) const {
     Unit u;
     u.r = r; u.hk = hk; u.tile = tile;
-    int tiles = a.tiles;
-    if (held) {
-      u.n = held->chunks[r];
-      tiles = (held->rows[r] + a.rows - 1) / a.rows;
-      u.start = static_cast<int64_t>(held->pre[r]) * c.h_k;
-    } else if (a.list_chunks) {
-      u.n = a.list_chunks;
-      u.start = static_cast<int64_t>(r) * u.n * tiles * c.h_k;
-    } else {
-      const int first = c.cu_chunks[r];
-      u.n = c.cu_chunks[r + 1] - first;
-      u.start = static_cast<int64_t>(first) * tiles * c.h_k;
-    }
-    u.start += (static_cast<int64_t>(hk) * tiles + tile) * u.n;
+    u.n = q.chunks;
+    u.start = static_cast<int64_t>(pre()[r]) * a.p.c.h_k + (static_cast<int64_t>(hk) * tiles_of(a, q.rows) + tile) * q.chunks;
     return u;
   }
-  // the unit of chunk w, w < total()
-  __device__ Unit at(int64_t w) const {
-    const fdma_cache& c = a.p.c;
-    const int64_t per_head = w / c.h_k;  // of the request: start / h_k <= per_head < end / h_k
-    int r;
-    if (!held && a.list_chunks) {
-      r = static_cast<int>(per_head / (static_cast<int64_t>(a.list_chunks) * a.tiles));
-    } else {
-      const int64_t scale = held ? 1 : a.tiles;
-      const int32_t* ends = held ? held->pre + 1 : c.cu_chunks + 1;
-      int lo = 0, hi = c.requests - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (ends[mid] * scale > per_head) hi = mid;
-        else lo = mid + 1;
-      }
-      r = lo;
+  // the unit of chunk w, w < total(), and its request
+  __device__ Unit at(int64_t w, Request& q) const {
+    const int64_t per_head = w / a.p.c.h_k;
+    const int32_t* ends = pre() + 1;
+    int lo = 0, hi = a.p.c.requests - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (ends[mid] > per_head) hi = mid;
+      else lo = mid + 1;
     }
-    Unit u = of(r, 0, 0);
-    const int tiles = held ? (held->rows[r] + a.rows - 1) / a.rows : a.tiles;
-    const int i = static_cast<int>((w - u.start) / max(u.n, 1));
-    u.hk = i / tiles;
-    u.tile = i - u.hk * tiles;
-    u.start += static_cast<int64_t>(i) * u.n;
-    return u;
+    q = request(lo);
+    const int tiles = max(tiles_of(a, q.rows), 1);
+    const int i = static_cast<int>((w - static_cast<int64_t>(pre()[lo]) * a.p.c.h_k) / max(q.chunks, 1));
+    return of(lo, q, i / tiles, i % tiles);
   }
 };
 // All threads of a CTA of at least 128.
@@ -207,7 +185,7 @@ __device__ __forceinline__ Units make_units(const AttnArgs& a, Held& h) {
   if (tid < R) {
     const Request q = load_request(a, tid);
     h.token0[tid] = q.token0; h.n[tid] = q.n; h.length[tid] = q.length; h.rows[tid] = q.rows; h.chunks[tid] = q.chunks;
-    w = q.chunks * ((q.rows + a.rows - 1) / a.rows);
+    w = q.chunks * tiles_of(a, q.rows);
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -291,9 +269,9 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       ks = vs = 0.f;
       used = false;
       if (w < w1) {
-        const Unit u = units.at(w);
+        Request q;
+        const Unit u = units.at(w, q);
         hk = u.hk;
-        const Request q = units.request(u.r);
         used = q.rows > u.tile * ROWS;
         const int pos = static_cast<int>(w - u.start) * kChunk + (lane & 3) * kSlice;
         if (used && pos < min(q.length, p.max_seqlen_k) && (pos >> a.shift) < c.width) {
@@ -384,10 +362,10 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   uint32_t phase = 0;
   int64_t w = w0;
   while (w < w1) {
-    const Unit u = units.at(w);
+    Request q;
+    const Unit u = units.at(w, q);
     const int64_t unit_end = max(u.start + u.n, w + 1);
     const int first = static_cast<int>(w - u.start), last = static_cast<int>(min(unit_end, w1) - u.start);
-    const Request q = units.request(u.r);
     const int row0 = u.tile * ROWS;
     w = min(unit_end, w1);
     const int nrows = min(ROWS, q.rows - row0);
@@ -781,6 +759,35 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   }
 }
 
+// AttnArgs::pre for many requests, by one CTA.
+__global__ void __launch_bounds__(1024) cache_sums_kernel(const __grid_constant__ AttnArgs a, int32_t* pre) {
+  __shared__ int s_warp[32];
+  const int R = a.p.c.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int carry = 0;
+  for (int base = 0; base < R; base += 1024) {
+    int x = 0;
+    if (base + tid < R) {
+      const Request q = load_request(a, base + tid);
+      x = q.chunks * tiles_of(a, q.rows);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    x += carry;
+    for (int i = 0; i < 32; ++i) {
+      if (i < warp) x += s_warp[i];
+      carry += s_warp[i];
+    }
+    if (base + tid < R) pre[base + tid + 1] = x;
+    __syncthreads();
+  }
+  if (tid == 0) pre[0] = 0;
+}
+
 // Joins the sums of units that several CTAs share, and writes the zeros of rows that nobody computes: a CTA per (token, head),
 // whose warps take a quarter of the sums each.
 template <int D, bool kBf16>
@@ -791,118 +798,134 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant_
   __shared__ int s_request;
   __shared__ float s_top[4], s_sum[4], s_acc[4][D];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int token = static_cast<int>(blockIdx.x / p.h), head = static_cast<int>(blockIdx.x - static_cast<unsigned>(token) * p.h);
-  if (tid == 0) s_request = -1;
-  __syncthreads();
-  for (int r = tid; r < c.requests; r += 128)
-    if (c.cu_seqlens[r] <= token && token < c.cu_seqlens[r + 1]) s_request = r;
+  const int slot = static_cast<int>(blockIdx.x / p.h), head = static_cast<int>(blockIdx.x - static_cast<unsigned>(slot) * p.h);
+  int r, token = slot, end = slot + 1;
+  if (a.merge_requests) {  // tokens i, i + 31 ... of request r
+    r = slot / (kPromptTokens - 1);
+    token = max(0, c.cu_seqlens[r]) + slot - r * (kPromptTokens - 1);
+    end = min(c.cu_seqlens[r + 1], c.tokens);
+  } else {
+    if (tid == 0) s_request = -1;
+    __syncthreads();
+    for (int x = tid; x < c.requests; x += 128)
+      if (c.cu_seqlens[x] <= token && token < c.cu_seqlens[x + 1]) s_request = x;
+    __syncthreads();
+    r = s_request;
+  }
   const Units units = make_units(a, s_held);
-  __syncthreads();
   const int64_t total = units.total(), share = share_of(total, a.ctas);
-  const int r = s_request;
-  int c0 = 0, c1 = -1;
-  const float* base = nullptr;
   const int64_t step = static_cast<int64_t>(a.rows) * (D + 4);
-  bool written = false;
-  if (r >= 0) {
-    const Request q = units.request(r);
+  Request q{};
+  if (r >= 0) q = units.request(r);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (q.rows < 0) return;  // done already
+  for (; token < end; token += kPromptTokens - 1) {
+    int c0 = 0, c1 = -1;
+    const float* base = nullptr;
     const int row = (token - q.token0) * a.group + head % a.group, tile = row / a.rows;
-    if (row >= 0 && row < q.rows) {
-      const Unit u = units.of(r, head / a.group, tile);
+    if (r >= 0 && row >= 0 && row < q.rows) {
+      const Unit u = units.of(r, q, head / a.group, tile);
       c0 = static_cast<int>(u.start / share);
       c1 = static_cast<int>((u.start + u.n - 1) / share);
-      written = c0 == c1;  // by that CTA
       base = a.partial + static_cast<int64_t>(row - tile * a.rows) * (D + 4);
+      if (c0 == c1) continue;  // written by that CTA
     }
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (written) return;
-  // each warp takes every fourth sum, eight at a time, and scales to its own maximum
-  constexpr int E = D / 32, kAhead = D > 128 ? 4 : 8;  // elements per lane
-  float acc[E], sum = 0.f, top = -CUDART_INF_F;
+    // each warp takes every fourth sum, eight at a time, and scales to its own maximum
+    constexpr int E = D / 32, kAhead = D > 128 ? 4 : 8;  // elements per lane
+    float acc[E], sum = 0.f, top = -CUDART_INF_F;
 #pragma unroll
-  for (int i = 0; i < E; ++i) acc[i] = 0.f;
-  for (int x0 = c0 + warp; x0 <= c1; x0 += 4 * kAhead) {
-    float2 ml[kAhead], y[kAhead][E / 2];
+    for (int i = 0; i < E; ++i) acc[i] = 0.f;
+    for (int x0 = c0 + warp; x0 <= c1; x0 += 4 * kAhead) {
+      float2 ml[kAhead], y[kAhead][E / 2];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int x = x0 + 4 * k;
-      ml[k] = make_float2(-CUDART_INF_F, 0.f);
-      if (x <= c1) {
-        const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
-        ml[k] = *reinterpret_cast<const float2*>(src + D);
+      for (int k = 0; k < kAhead; ++k) {
+        const int x = x0 + 4 * k;
+        ml[k] = make_float2(-CUDART_INF_F, 0.f);
+        if (x <= c1) {
+          const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
+          ml[k] = *reinterpret_cast<const float2*>(src + D);
 #pragma unroll
-        for (int i = 0; i < E / 2; ++i) y[k][i] = *reinterpret_cast<const float2*>(src + lane * E + 2 * i);
-      }
-    }
-    float now = top;
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) now = fmaxf(now, ml[k].x);
-    const float from = now == -CUDART_INF_F ? 0.f : now, f0 = exp2_or_zero(top - from);
-    top = now;
-    sum *= f0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] *= f0;
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (x0 + 4 * k <= c1) {
-        const float f = exp2_or_zero(ml[k].x - from);
-        sum = fmaf(ml[k].y, f, sum);
-#pragma unroll
-        for (int i = 0; i < E / 2; ++i) {
-          acc[2 * i] = fmaf(y[k][i].x, f, acc[2 * i]);
-          acc[2 * i + 1] = fmaf(y[k][i].y, f, acc[2 * i + 1]);
+          for (int i = 0; i < E / 2; ++i) y[k][i] = *reinterpret_cast<const float2*>(src + lane * E + 2 * i);
         }
       }
-  }
-  if (lane == 0) {
-    s_top[warp] = top;
-    s_sum[warp] = sum;
-  }
+      float now = top;
 #pragma unroll
-  for (int i = 0; i < E; ++i) s_acc[warp][lane * E + i] = acc[i];
-  __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  const float from = top == -CUDART_INF_F ? 0.f : top;
-  float f[4];
-  sum = 0.f;
+      for (int k = 0; k < kAhead; ++k) now = fmaxf(now, ml[k].x);
+      const float from = now == -CUDART_INF_F ? 0.f : now, f0 = exp2_or_zero(top - from);
+      top = now;
+      sum *= f0;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    f[x] = exp2_or_zero(s_top[x] - from);
-    sum = fmaf(s_sum[x], f[x], sum);
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t* dst = static_cast<uint16_t*>(p.out) + token * p.out_row_stride + head * p.out_head_stride;
-  for (int i = 2 * tid; i < c.d; i += 256) {
-    float y[2] = {0.f, 0.f};
+      for (int i = 0; i < E; ++i) acc[i] *= f0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+      for (int k = 0; k < kAhead; ++k)
+        if (x0 + 4 * k <= c1) {
+          const float f = exp2_or_zero(ml[k].x - from);
+          sum = fmaf(ml[k].y, f, sum);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) y[k] = fmaf(s_acc[x][i + k], f[x], y[k]);
-    *reinterpret_cast<uint32_t*>(dst + i) = pack2<kBf16>(y[0] * inv, y[1] * inv);
+          for (int i = 0; i < E / 2; ++i) {
+            acc[2 * i] = fmaf(y[k][i].x, f, acc[2 * i]);
+            acc[2 * i + 1] = fmaf(y[k][i].y, f, acc[2 * i + 1]);
+          }
+        }
+    }
+    if (lane == 0) {
+      s_top[warp] = top;
+      s_sum[warp] = sum;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) s_acc[warp][lane * E + i] = acc[i];
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    const float from = top == -CUDART_INF_F ? 0.f : top;
+    float f[4];
+    sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      f[x] = exp2_or_zero(s_top[x] - from);
+      sum = fmaf(s_sum[x], f[x], sum);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint16_t* dst = static_cast<uint16_t*>(p.out) + token * p.out_row_stride + head * p.out_head_stride;
+    for (int i = 2 * tid; i < c.d; i += 256) {
+      float y[2] = {0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) y[k] = fmaf(s_acc[x][i + k], f[x], y[k]);
+      *reinterpret_cast<uint32_t*>(dst + i) = pack2<kBf16>(y[0] * inv, y[1] * inv);
+    }
+    __syncthreads();  // (the next token uses the same shared memory)
   }
 }
 
 int tile_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 struct Plan {
-  int D, rows, tiles, ctas, list_chunks;
-  size_t bytes;
+  int D, rows, ctas, list_chunks;
+  bool sums;  // by a kernel of their own: many requests, and not one tile of cu_chunks' chunks for each
+  int64_t most_chunks;
+  bool prompts;
+  size_t sums_off, prompt_off, bytes;
 };
 Plan plan_of(const fdma_cache_attention_params& p) {
   Plan pl;
+  pl.prompts = cache_prompt_taken(p);
   const int64_t most = static_cast<int64_t>(std::min(p.max_seqlen_q, p.c.tokens)) * (p.h / p.c.h_k);
   pl.D = tile_dim(p.c.d);
   pl.rows = most <= 8 ? 8 : 16;
-  pl.tiles = static_cast<int>(std::max<int64_t>(1, (most + pl.rows - 1) / pl.rows));
   pl.ctas = (pl.D == 256 ? 2 : 3) * sm_count();
   pl.list_chunks = p.kept_pos ? (p.kept_capacity + kChunk - 1) / kChunk : 0;
-  pl.bytes = align256(static_cast<size_t>(pl.ctas) * 2 * pl.rows * (pl.D + 4) * sizeof(float));
+  pl.sums = p.c.requests > kHeld && (pl.list_chunks || most > pl.rows);
+  const int64_t tiles = static_cast<int64_t>(p.c.tokens) * (p.h / p.c.h_k) / pl.rows + p.c.requests;
+  pl.most_chunks = tiles * (pl.list_chunks ? pl.list_chunks : (static_cast<int64_t>(p.c.width) * p.c.block_size + kChunk - 1) / kChunk);
+  pl.sums_off = align256(static_cast<size_t>(pl.ctas) * 2 * pl.rows * (pl.D + 4) * sizeof(float));
+  pl.prompt_off = pl.sums_off + (pl.sums ? align256((static_cast<size_t>(p.c.requests) + 1) * sizeof(int32_t)) : 0);
+  pl.bytes = pl.prompt_off + (pl.prompts ? cache_prompt_workspace_bytes(p) : 0);
   return pl;
 }
 
 template <int D, int ROWS, bool kGather, bool kBf16>
-int launch(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
+int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
   using L = Layout<D, ROWS, kGather>;
   const fdma_cache& c = a.p.c;
   CUtensorMap map_k{}, map_v{};
@@ -923,7 +946,9 @@ int launch(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
   if (e != cudaSuccess) return static_cast<int>(e);
   // the second kernel's CTAs start while the first one's finish, and wait for them only where they need their sums
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(c.tokens) * a.p.h);
+  const int64_t few = static_cast<int64_t>(c.requests) * (kPromptTokens - 1);
+  a.merge_requests = a.prompts && few < c.tokens;
+  cfg.gridDim = dim3(static_cast<unsigned>(a.merge_requests ? few : c.tokens) * a.p.h);
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -971,13 +996,13 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   if (!p.query || !p.out) return FDMA_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uint64_t>(p.out_row_stride | p.out_head_stride) * 2) % 16) return FDMA_ERR_UNSUPPORTED;
   const Plan pl = plan_of(p);
-  if (!p.workspace || p.workspace_bytes < pl.bytes) return FDMA_ERR_WORKSPACE;
+  if (pl.most_chunks > 0x7FFFFFFF) return FDMA_ERR_TOO_LARGE;
+  if (!p.workspace || p.workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(p.workspace) & 255)) return FDMA_ERR_WORKSPACE;
   AttnArgs a = {};
   a.p = p;
   a.shift = p.c.block_size == 16 ? 4 : p.c.block_size == 32 ? 5 : p.c.block_size == 64 ? 6 : 7;
   a.group = p.h / p.c.h_k;
   a.rows = pl.rows;
-  a.tiles = pl.tiles;
   a.list_chunks = pl.list_chunks;
   a.ctas = pl.ctas;
   a.scale_log2 = p.softmax_scale * kLog2e;
@@ -986,6 +1011,19 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   a.status = kernel_status_ptr();
   if (!a.status) return FDMA_ERR_DRIVER;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (pl.prompts) {
+    const int status = cache_prompt(p, a.shift, static_cast<char*>(p.workspace) + pl.prompt_off, stream);
+    if (status) return status;
+    a.prompts = reinterpret_cast<const int32_t*>(static_cast<char*>(p.workspace) + pl.prompt_off + cache_prompt_keys(p));
+  }
+  a.pre = p.c.cu_chunks;
+  if (pl.sums) {
+    int32_t* pre = reinterpret_cast<int32_t*>(static_cast<char*>(p.workspace) + pl.sums_off);
+    cache_sums_kernel<<<1, 1024, 0, stream>>>(a, pre);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return static_cast<int>(e);
+    a.pre = pre;
+  }
   if (pl.D == 256) return pl.rows == 8 ? launch_t<256, 8>(a, pl, stream) : launch_t<256, 16>(a, pl, stream);
   if (pl.D == 128) return pl.rows == 8 ? launch_t<128, 8>(a, pl, stream) : launch_t<128, 16>(a, pl, stream);
   return pl.rows == 8 ? launch_t<64, 8>(a, pl, stream) : launch_t<64, 16>(a, pl, stream);

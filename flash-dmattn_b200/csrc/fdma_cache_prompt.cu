@@ -1,0 +1,213 @@
+// Attention of prompt parts over the paged 8-bit cache: requests with many new tokens at once.
+//
+// Tensor-bound: with n queries per key the keys are worth converting once. One kernel turns the requests' blocks into 16-bit keys and
+// values, packed request after request (8-bit numbers times a power of two: exact in bf16, and in fp16 as far as it reaches: what
+// is larger becomes its largest number); the packed-sequence forward kernel does the rest with tcgen05. The conversion is
+// memory-bound, 6 d bytes per key and kv head (read 2 d, write 4 d).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "fdma_internal.h"
+
+namespace fdma {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 64;
+constexpr int64_t kMostRows = 1 << 20;               // keys of all requests, what the forward kernel's tables hold
+constexpr int64_t kMostBytes = int64_t{1} << 32;     // of scratch
+
+struct UnpackArgs {
+  fdma_cache c;
+  int32_t* cu_k;
+  void *k, *v;  // (rows, h_k, d)
+  int shift, max_keys, rows, heads;
+};
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack_scaled(uint16_t two, float scale) {
+  const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3));
+  float2 f = __half22float2(h);
+  f.x *= scale;
+  f.y *= scale;
+  if (kBf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  if (fabsf(f.x) > 65504.f) f.x = copysignf(65504.f, f.x);
+  if (fabsf(f.y) > 65504.f) f.y = copysignf(65504.f, f.y);
+  const __half2 v = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A CTA converts a 64-key chunk of a request, all heads of K and V, at a time.
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant__ UnpackArgs a) {
+  extern __shared__ int s_pre[];  // chunks, then rows, of the requests before
+  __shared__ long long s_warp[kThreads / 32];
+  __shared__ int s_block[4], s_tokens[kThreads / 32];
+  const fdma_cache& c = a.c;
+  const int R = c.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int *pre_chunks = s_pre, *pre_rows = s_pre + R + 1;
+  long long carry = 0, tokens = 0;  // carry: rows << 32 | chunks
+  for (int base = 0; base < R; base += kThreads) {
+    const int r = base + tid;
+    long long x = 0;
+    int mine = 0;
+    if (r < R && c.cu_chunks[r + 1] > c.cu_chunks[r] && c.cu_seqlens[r + 1] - c.cu_seqlens[r] >= kPromptTokens) {
+      const int n = max(0, min(min(c.lengths[r], a.max_keys), c.width << a.shift));
+      x = (static_cast<long long>(n) << 32) | ((n + kChunk - 1) / kChunk);
+      mine = c.cu_seqlens[r + 1] - c.cu_seqlens[r];
+    }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) s_tokens[warp] = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    long long before = carry;
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < warp) before += s_warp[i];
+      carry += s_warp[i];
+      tokens += s_tokens[i];
+    }
+    x += before;
+    if (r < R) {
+      pre_chunks[r + 1] = static_cast<int>(x & 0xFFFFFFFF);
+      pre_rows[r + 1] = static_cast<int>(min(x >> 32, static_cast<long long>(a.rows)));
+    }
+    __syncthreads();
+  }
+  if (tid == 0) pre_chunks[0] = pre_rows[0] = 0;
+  __syncthreads();
+  const bool taken = tokens * a.heads >= prompt_work(c.d);
+  if (blockIdx.x == 0)
+    for (int r = tid; r <= R; r += kThreads) a.cu_k[r] = taken ? pre_rows[r] : 0;
+  const int total = taken ? pre_chunks[R] : 0;
+  const int pieces = c.d / 16, per_head = kChunk * pieces, per_tensor = per_head * c.h_k;
+  for (int w = blockIdx.x; w < total; w += gridDim.x) {
+    int lo = 0, hi = R - 1;  // first request whose chunks end behind w
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (pre_chunks[mid + 1] > w) hi = mid;
+      else lo = mid + 1;
+    }
+    const int pos0 = (w - pre_chunks[lo]) * kChunk, row0 = pre_rows[lo] + pos0, n = min(kChunk, pre_rows[lo + 1] - row0);
+    if (tid < 4) {
+      const int pos = pos0 + tid * 16;
+      int block = tid * 16 < n ? c.table[static_cast<int64_t>(lo) * c.width + (pos >> a.shift)] : -1;
+      s_block[tid] = block >= c.num_blocks ? -1 : block;
+    }
+    __syncthreads();
+    for (int i = tid; i < 2 * per_tensor; i += kThreads) {
+      const bool is_v = i >= per_tensor;
+      const int j = is_v ? i - per_tensor : i, head = j / per_head, rest = j - head * per_head, row = rest / pieces, piece = rest - row * pieces;
+      if (row >= n) continue;
+      const int block = s_block[row >> 4];
+      uint32_t y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (block >= 0) {
+        const int64_t at = static_cast<int64_t>(block) * c.h_k + head;
+        const int place = (pos0 + row) & ((1 << a.shift) - 1);
+        const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(is_v ? c.v : c.k) + ((at << a.shift) + place) * c.d + piece * 16);
+        const float scale = (is_v ? c.v_scale : c.k_scale)[at];
+        const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          y[2 * k] = pack_scaled<kBf16>(static_cast<uint16_t>(words[k]), scale);
+          y[2 * k + 1] = pack_scaled<kBf16>(static_cast<uint16_t>(words[k] >> 16), scale);
+        }
+      }
+      uint16_t* dst = static_cast<uint16_t*>(is_v ? a.v : a.k) + (static_cast<int64_t>(row0 + row) * c.h_k + head) * c.d + piece * 16;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(dst + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+    __syncthreads();
+  }
+}
+
+// At most so many keys: requests that have kPromptTokens new ones each, of the longest length.
+int64_t most_rows(const fdma_cache_attention_params& p) {
+  const int64_t requests = std::min<int64_t>(p.c.requests, p.c.tokens / kPromptTokens);
+  return requests * std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size);
+}
+struct Scratch {
+  size_t v, lse, cu_k, total;
+};
+Scratch scratch(const fdma_cache_attention_params& p) {
+  Scratch s;
+  const size_t kv = align256(static_cast<size_t>(most_rows(p)) * p.c.h_k * p.c.d * 2);
+  s.v = kv;
+  s.lse = 2 * kv;
+  s.cu_k = s.lse + align256(static_cast<size_t>(p.h) * p.c.tokens * sizeof(float));
+  s.total = s.cu_k + align256((static_cast<size_t>(p.c.requests) + 1) * sizeof(int32_t));
+  return s;
+}
+fdma_fwd_params forward_params(const fdma_cache_attention_params& p, char* ws) {
+  const Scratch s = scratch(p);
+  fdma_fwd_params f = {};
+  f.q = p.query;
+  f.k = ws;
+  f.v = ws + s.v;
+  f.out = p.out;
+  f.lse = reinterpret_cast<float*>(ws + s.lse);
+  f.q_row_stride = p.query_row_stride; f.q_head_stride = p.query_head_stride;
+  f.k_row_stride = f.v_row_stride = static_cast<int64_t>(p.c.h_k) * p.c.d;
+  f.k_head_stride = f.v_head_stride = p.c.d;
+  f.o_row_stride = p.out_row_stride; f.o_head_stride = p.out_head_stride;
+  f.b = 1;
+  f.seqlen_q = p.c.tokens;
+  f.seqlen_k = static_cast<int32_t>(most_rows(p));
+  f.h = p.h; f.h_k = p.c.h_k; f.h_mask = f.h_bias = 1; f.d = p.c.d;
+  f.dtype = p.dtype;
+  f.is_causal = p.is_causal;
+  f.softmax_scale = p.softmax_scale;
+  return f;
+}
+
+}  // namespace
+
+bool cache_prompt_taken(const fdma_cache_attention_params& p) {
+  if (std::min(p.max_seqlen_q, p.c.tokens) < kPromptTokens || static_cast<int64_t>(p.c.tokens) * p.h < prompt_work(p.c.d) || p.bias || p.kept_pos || p.c.requests > 8192) return false;
+  const int64_t rows = most_rows(p);
+  if (rows <= 0 || rows > kMostRows || scratch(p).total > static_cast<size_t>(kMostBytes)) return false;
+  if (p.c.tokens > (1 << 19)) return false;
+  // the workspace is 256-byte aligned wherever it lies
+  return tc_fwd_supported(forward_params(p, reinterpret_cast<char*>(uintptr_t{256})));
+}
+size_t cache_prompt_workspace_bytes(const fdma_cache_attention_params& p) { return scratch(p).total; }
+size_t cache_prompt_keys(const fdma_cache_attention_params& p) { return scratch(p).cu_k + static_cast<size_t>(p.c.requests) * sizeof(int32_t); }
+
+int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspace, cudaStream_t stream) {
+  char* ws = static_cast<char*>(workspace);
+  const Scratch s = scratch(p);
+  UnpackArgs a;
+  a.c = p.c;
+  a.cu_k = reinterpret_cast<int32_t*>(ws + s.cu_k);
+  a.k = ws;
+  a.v = ws + s.v;
+  a.shift = shift;
+  a.max_keys = p.max_seqlen_k;
+  a.rows = static_cast<int>(most_rows(p));
+  a.heads = p.h;
+  const size_t smem = (static_cast<size_t>(p.c.requests) + 1) * 8;
+  const bool bf16 = p.dtype == FDMA_BF16;
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(bf16 ? unpack_kernel<true> : unpack_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  const int64_t most_chunks = a.rows / kChunk + std::min<int64_t>(p.c.requests, p.c.tokens / kPromptTokens);
+  const int ctas = static_cast<int>(std::min<int64_t>(most_chunks, 8 * sm_count()));
+  if (bf16) unpack_kernel<true><<<ctas, kThreads, smem, stream>>>(a);
+  else unpack_kernel<false><<<ctas, kThreads, smem, stream>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  return tc_fwd(forward_params(p, ws), stream, PackedSeqs{p.c.cu_seqlens, a.cu_k, p.c.requests});
+}
+
+}  // namespace fdma

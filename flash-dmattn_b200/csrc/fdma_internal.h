@@ -108,6 +108,23 @@ int single_query_fwd_in(const fdma_fwd_params& p, cudaStream_t stream);
 // ---- create_mask -------------------------------------------------------------------------------
 int create_mask(const fdma_mask_params& p, cudaStream_t stream);
 
+// ---- attention over the 8-bit cache ---------------------------------------------------------------
+// Requests with kPromptTokens or more new tokens have their keys converted to 16 bits once, for the tensor-core forward kernel
+// (fdma_cache_prompt.cu), if these are prompt_work() tokens x query heads in all; otherwise keys are read for 16 rows of queries at a
+// time (fdma_cache_attn.cu). The former needs 17 us per 1000 keys however few its CTAs are, the latter's time grows with the rows;
+// 32 heads over 8, d = 128, 32000 keys: 4 x 32 tokens 672 against 411 us, 4 x 64 672 against 803, 4 x 128 676 against 1650;
+// 16 heads over 1, d = 256: 4 x 64 tokens 715 against 750.
+constexpr int kPromptTokens = 32;
+__host__ __device__ inline int prompt_work(int d) { return d > 128 ? 4096 : 6144; }
+int check_cache(const fdma_cache& c);
+// Whether the call may have such requests, and scratch and layouts for them. Then cache_prompt writes all rows, those of other
+// requests 0; what the device has found is at cache_prompt_keys in the scratch: the number of converted keys, 0 if the requests have
+// too few tokens together and none are converted.
+bool cache_prompt_taken(const fdma_cache_attention_params& p);
+size_t cache_prompt_workspace_bytes(const fdma_cache_attention_params& p);
+size_t cache_prompt_keys(const fdma_cache_attention_params& p);
+int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspace, cudaStream_t stream);
+
 // ---- helpers -----------------------------------------------------------------------------------
 // Device address of the current device's kernel status word (written by bounded waits that give up).
 int* kernel_status_ptr();

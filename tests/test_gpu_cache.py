@@ -291,7 +291,8 @@ def attend(query, cache, tables, step, kept=None, bias=None, scale=None, causal=
 
     Scores are sums of d exact products in 32 bits, at worst 2^-23 of their magnitudes per addition, times two factors and plus a bias
     (2^-22 of what they are added to): that makes an error of the score, and so of a probability relative to itself, twice (numerator
-    and sum). Probabilities are rounded to 11 bits, 2^-12 of themselves, or 2^-38 of the largest times a value. One rounding to the type."""
+    and sum). Probabilities are rounded to fp16, 2^-11 of themselves, or 2^-38 of the largest times a value; for requests with 32 or more
+    new tokens to the type of the queries, eps / 2. One rounding to the type."""
     T, H, d = query.shape
     Hk, bs = cache.k.shape[1], tables.block_size
     scale = d ** -0.5 if scale is None else scale
@@ -335,7 +336,8 @@ def attend(query, cache, tables, step, kept=None, bias=None, scale=None, causal=
             worst = (2 * err + 2.0 ** -22 * (x - top).abs().nan_to_num(0, 0, 0).clamp(max=1e4)).amax(-1, keepdim=True) if x.shape[1] else 0.0
             worst = torch.as_tensor(worst)
             out[cu[r]:cu[r + 1], h] = y
-            tol[cu[r]:cu[r + 1], h] = ((2.0 ** -11 + 2 * worst.expm1()) * (p @ vv.abs()) + torch.finfo(query.dtype).eps / 2 * y.abs() +
+            rounding = 2.0 ** -11 if n < 32 else torch.finfo(query.dtype).eps / 2
+            tol[cu[r]:cu[r + 1], h] = ((rounding + 2 * worst.expm1()) * (p @ vv.abs()) + torch.finfo(query.dtype).eps / 2 * y.abs() +
                                        2.0 ** -30 * vv.abs().amax().item() if v.numel() else 0.0)
     return out, tol + torch.finfo(query.dtype).tiny
 
@@ -350,7 +352,8 @@ ATTEND = [  # cached, new, heads, kv heads, head dim, block size
     ([0], [1], 1, 1, 64, 16), ([4096], [1], 8, 2, 128, 64), ([1000, 0, 63, 64, 4099], [1] * 5, 8, 8, 128, 16),
     ([130, 3], [1, 1], 32, 2, 96, 32), ([500, 777], [1, 1], 20, 1, 256, 128), ([127, 129, 90], [1, 5, 3], 8, 2, 64, 64),
     ([700, 0, 12], [5, 9, 1], 12, 4, 128, 16), ([300], [40], 6, 2, 128, 64), ([65, 40], [33, 0], 2, 1, 256, 32), ([0, 10], [130, 70], 4, 4, 64, 128),
-    ([40] * 300, [1] * 300, 2, 1, 16, 16), ([2000, 100], [2, 1], 9, 3, 80, 64), ([513, 60], [1, 7], 4, 2, 192, 64), ([5000], [1], 4, 4, 48, 128)]
+    ([40] * 300, [1] * 300, 2, 1, 16, 16), ([0, 500, 31, 7, 900], [31, 32, 1, 300, 65], 8, 2, 128, 16), ([1000, 64], [257, 2], 4, 1, 64, 32),
+    ([20] * 140, [1, 40] * 70, 4, 2, 64, 16), ([33] * 200, [2, 30, 1, 5] * 50, 4, 4, 32, 16), ([100, 0], [33, 31], 32, 4, 64, 16), ([300, 64], [128, 129], 3, 1, 96, 64), ([2000, 100], [2, 1], 9, 3, 80, 64), ([513, 60], [1, 7], 4, 2, 192, 64), ([5000], [1], 4, 4, 48, 128)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
