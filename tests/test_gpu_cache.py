@@ -353,7 +353,8 @@ ATTEND = [  # cached, new, heads, kv heads, head dim, block size
     ([130, 3], [1, 1], 32, 2, 96, 32), ([500, 777], [1, 1], 20, 1, 256, 128), ([127, 129, 90], [1, 5, 3], 8, 2, 64, 64),
     ([700, 0, 12], [5, 9, 1], 12, 4, 128, 16), ([300], [40], 6, 2, 128, 64), ([65, 40], [33, 0], 2, 1, 256, 32), ([0, 10], [130, 70], 4, 4, 64, 128),
     ([40] * 300, [1] * 300, 2, 1, 16, 16), ([0, 500, 31, 7, 900], [31, 32, 1, 300, 65], 8, 2, 128, 16), ([1000, 64], [257, 2], 4, 1, 64, 32),
-    ([20] * 140, [1, 40] * 70, 4, 2, 64, 16), ([33] * 200, [2, 30, 1, 5] * 50, 4, 4, 32, 16), ([100, 0], [33, 31], 32, 4, 64, 16), ([300, 64], [128, 129], 3, 1, 96, 64), ([2000, 100], [2, 1], 9, 3, 80, 64), ([513, 60], [1, 7], 4, 2, 192, 64), ([5000], [1], 4, 4, 48, 128)]
+    ([20] * 140, [1, 40] * 70, 4, 2, 64, 16), ([33] * 200, [2, 30, 1, 5] * 50, 4, 4, 32, 16), ([100, 0], [33, 31], 32, 4, 64, 16),
+    ([50] * 100, [31] * 99 + [45], 2, 1, 16, 32), ([9] * 150, [31] * 149 + [40], 4, 4, 16, 16), ([300, 64], [128, 129], 3, 1, 96, 64), ([2000, 100], [2, 1], 9, 3, 80, 64), ([513, 60], [1, 7], 4, 2, 192, 64), ([5000], [1], 4, 4, 48, 128)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
