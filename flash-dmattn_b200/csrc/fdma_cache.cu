@@ -236,7 +236,7 @@ struct AppendArgs {
   RotaryUnits plain_units;  // of values, and keys that are not: two vectors, half a row apart
   RotaryArgs query;
   int shift, most_units;
-  int key_heads;  // of a CTA: they share the factors of its tokens
+  int heads;  // of K or V that a CTA writes, one after the other
   int64_t cache_ctas;
 };
 
@@ -267,59 +267,64 @@ __device__ __forceinline__ float block_scale(float x) {
 
 template <typename T, int N, bool kInterleaved>
 __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_constant__ AppendArgs a) {
-  extern __shared__ float2 s_factors[];  // [new tokens of the block][half], or rotate_tokens' own
+  extern __shared__ __align__(16) float2 s_factors[];  // of the block's new tokens, or rotate_tokens' own
   __shared__ float s_max[2][kAppendThreads / 32];
-  __shared__ int s_request;
+  __shared__ int s_found[5];
   const fdma_cache_append_params& p = a.p;
   const fdma_cache& c = p.c;
   const int tid = threadIdx.x;
-  if (blockIdx.x >= a.cache_ctas) {
+  // the CTAs that write and those that turn queries are spread over the launch evenly: the former wait for loads most of the time
+  const int64_t before_me = blockIdx.x * a.cache_ctas / gridDim.x;
+  if ((blockIdx.x + int64_t{1}) * a.cache_ctas / gridDim.x == before_me) {
     const int warp = tid >> 5;
-    rotate_tokens<T, N, kInterleaved>(a.query, (blockIdx.x - a.cache_ctas) * kRotaryWarps + warp, s_factors + warp * a.query.abreast * a.query.ru.half);
+    rotate_tokens<T, N, kInterleaved>(a.query, (blockIdx.x - before_me) * kRotaryWarps + warp, s_factors + warp * rotary_warp_pairs<N>(a.query));
     return;
   }
-  // first the CTAs of K, a few heads of a block each, then those of V, a head each
-  const int key_groups = (c.h_k + a.key_heads - 1) / a.key_heads, key_ctas = a.most_units * key_groups;
-  const bool is_v = blockIdx.x >= key_ctas;
-  const int rest = is_v ? blockIdx.x - key_ctas : blockIdx.x, per_unit = is_v ? c.h_k : key_groups;
-  const int unit = rest / per_unit, head0 = (rest - unit * per_unit) * (is_v ? 1 : a.key_heads);
-  const int heads = is_v ? 1 : min(a.key_heads, c.h_k - head0);
-  if (tid == 0) s_request = -1;
+  // K of a block's next few heads, or V
+  const int id = static_cast<int>(before_me), groups = (c.h_k + a.heads - 1) / a.heads;
+  const bool is_v = id & 1;
+  const int unit = (id >> 1) / groups, head0 = ((id >> 1) - unit * groups) * a.heads, head_end = min(head0 + a.heads, c.h_k);
+  if (tid == 0) s_found[0] = -1;
   __syncthreads();
-  for (int r = tid; r < c.requests; r += kAppendThreads)
-    if (c.cu_blocks[r] <= unit && unit < c.cu_blocks[r + 1]) s_request = r;
+  for (int r = tid; r < c.requests; r += kAppendThreads) {
+    const int first = c.cu_blocks[r], end = c.cu_blocks[r + 1], token = c.cu_seqlens[r], token_end = c.cu_seqlens[r + 1], length = c.lengths[r];
+    if (first <= unit && unit < end) {
+      s_found[0] = r;
+      s_found[1] = token;
+      s_found[2] = token_end - token;
+      s_found[3] = length;
+      s_found[4] = unit - first;
+    }
+  }
   __syncthreads();
-  const int r = s_request;
+  const int r = s_found[0];
   if (r < 0) return;
   const int bs = 1 << a.shift;
-  const int token0 = c.cu_seqlens[r], n_new = c.cu_seqlens[r + 1] - token0, length = c.lengths[r], before = length - n_new;
-  const int page = (before >> a.shift) + unit - c.cu_blocks[r];
+  const int token0 = s_found[1], n_new = s_found[2], length = s_found[3], before = length - n_new;
+  const int page = (before >> a.shift) + s_found[4];
   if (token0 < 0 || n_new < 0 || token0 + n_new > c.tokens || before < 0 || page >= c.width) return;
-  const int block = c.table[static_cast<int64_t>(r) * c.width + page];
-  if (block < 0 || block >= c.num_blocks) return;
   const int begin = page << a.shift;
   const int lo = max(before - begin, 0), hi = min(length - begin, bs);  // places of the new tokens in the block
   const int n = hi - lo;
   if (n <= 0) return;
   const int first = token0 + begin + lo - before;  // the token at place lo
+  const int block = c.table[static_cast<int64_t>(r) * c.width + page];
 
   const bool turn = !is_v && p.turns;
   const RotaryUnits& ru = turn ? a.key_units : a.plain_units;
   const int half = turn ? ru.half : 0;
   const int64_t row_stride = is_v ? p.value_row_stride : p.key_row_stride, head_stride = is_v ? p.value_head_stride : p.key_head_stride;
-  for (int i = tid; i < n * half; i += kAppendThreads) {
-    const int t = i / half, f = i - t * half;
-    s_factors[i] = rotary_factors(before + (first - token0) + t, p.turns[f], p.amplitude, false);
-  }
-  // A thread keeps its unit and walks the tokens. The first kHold of its vectors stay in registers between the two passes.
+  // A thread keeps its unit and walks the tokens. The first kHold of its vectors are asked for a head ahead, and stay in registers
+  // between the two passes.
   using V = Vec<T, N>;
-  constexpr int kHold = 2;
+  constexpr int kHold = 1;
   const int abreast = kAppendThreads / ru.units;  // units <= 256
   const int t_first = tid / ru.units, u = tid - t_first * ru.units;
   const int t_begin = t_first < abreast ? t_first : n;
   const bool pair = u < ru.pair_units;
   const int2 at = unit_offsets<N, kInterleaved>(ru, u);
   V hx[kHold], hy[kHold];
+  const T* src = static_cast<const T*>(is_v ? p.value : p.key) + first * row_stride + head0 * head_stride;
   auto hold = [&](const T* from) {
 #pragma unroll
     for (int k = 0; k < kHold; ++k) {
@@ -330,26 +335,30 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
       }
     }
   };
-  for (int head = head0; head < head0 + heads; ++head) {
-    const T* src = static_cast<const T*>(is_v ? p.value : p.key) + first * row_stride + head * head_stride;
+  hold(src);
+  for (int i = tid; i < n * half; i += kAppendThreads) {
+    const int t = i / half, f = i - t * half;
+    s_factors[t * factor_pitch<N>(half) + factor_at<N>(f)] = rotary_factors(before + (first - token0) + t, p.turns[f], p.amplitude, false);
+  }
+  if (block < 0 || block >= c.num_blocks) return;
+  __syncthreads();  // the factors
+  auto values = [&](const V& vx, const V& vy, int t, float (&x)[N], float (&y)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      x[j] = to_f(vx.x[j]);
+      y[j] = pair ? to_f(vy.x[j]) : 0.f;
+    }
+    if (turn && pair) rotate_unit<N, kInterleaved>(x, y, s_factors + t * factor_pitch<N>(half) + u * kFactorUnit<N>);
+  };
+  for (int head = head0; head < head_end; ++head, src += head_stride) {
     const int64_t at_scale = static_cast<int64_t>(block) * c.h_k + head;
     uint8_t* dst = static_cast<uint8_t*>(is_v ? c.v : c.k) + (at_scale * bs) * c.d;
     float* scale = (is_v ? c.v_scale : c.k_scale) + at_scale;
     const float old_scale = lo > 0 ? *scale : 0.f;
-    if (head == head0) {
-      hold(src);
-      __syncthreads();  // the factors
-    }
-    auto values = [&](const V& vx, const V& vy, int t, float (&x)[N], float (&y)[N]) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        x[j] = to_f(vx.x[j]);
-        y[j] = pair ? to_f(vy.x[j]) : 0.f;
-      }
-      if (turn && pair) rotate_unit<N, kInterleaved>(x, y, s_factors + t * half + u * N);
-    };
     float most = 0.f;
-    auto look = [&](const float (&x)[N], const float (&y)[N]) {
+    auto look = [&](const V& vx, const V& vy, int t) {
+      float x[N], y[N];
+      values(vx, vy, t, x, y);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float fx = fabsf(x[j]), fy = fabsf(y[j]);
@@ -357,23 +366,20 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
         if (fy <= 3.402823466e38f) most = fmaxf(most, fy);
       }
     };
+    auto rest = [&](auto&& use) {  // the vectors that are not held
+      for (int t = t_begin + kHold * abreast; t < n; t += abreast) {
+        const V vx = *reinterpret_cast<const V*>(src + t * row_stride + at.x);
+        V vy = vx;
+        if (pair) vy = *reinterpret_cast<const V*>(src + t * row_stride + at.y);
+        use(vx, vy, t);
+      }
+    };
 #pragma unroll
     for (int k = 0; k < kHold; ++k) {
       const int t = t_begin + k * abreast;
-      if (t < n) {
-        float x[N], y[N];
-        values(hx[k], hy[k], t, x, y);
-        look(x, y);
-      }
+      if (t < n) look(hx[k], hy[k], t);
     }
-    for (int t = t_begin + kHold * abreast; t < n; t += abreast) {
-      float x[N], y[N];
-      const V vx = *reinterpret_cast<const V*>(src + t * row_stride + at.x);
-      V vy = vx;
-      if (pair) vy = *reinterpret_cast<const V*>(src + t * row_stride + at.y);
-      values(vx, vy, t, x, y);
-      look(x, y);
-    }
+    rest(look);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     if ((tid & 31) == 0) s_max[head & 1][tid >> 5] = most;  // (two rows: the next head's maxima must not overtake readers of these)
@@ -382,7 +388,9 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
     for (int w = 0; w < kAppendThreads / 32; ++w) most = fmaxf(most, s_max[head & 1][w]);
     const float now = fmaxf(block_scale(most), old_scale), inv = __frcp_rn(now);
     if (tid == 0) *scale = now;
-    auto write = [&](const float (&x)[N], const float (&y)[N], int t) {
+    auto write = [&](const V& vx, const V& vy, int t) {
+      float x[N], y[N];
+      values(vx, vy, t, x, y);
       uint8_t* row = dst + (lo + t) * c.d;
       *reinterpret_cast<Vec<uint8_t, N>*>(row + at.x) = to_e4m3<N>(x, inv);
       if (pair) *reinterpret_cast<Vec<uint8_t, N>*>(row + at.y) = to_e4m3<N>(y, inv);
@@ -390,21 +398,10 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
 #pragma unroll
     for (int k = 0; k < kHold; ++k) {
       const int t = t_begin + k * abreast;
-      if (t < n) {
-        float x[N], y[N];
-        values(hx[k], hy[k], t, x, y);
-        write(x, y, t);
-      }
+      if (t < n) write(hx[k], hy[k], t);
     }
-    if (head + 1 < head0 + heads) hold(src + head_stride);  // on their way while the rest is done
-    for (int t = t_begin + kHold * abreast; t < n; t += abreast) {
-      float x[N], y[N];
-      const V vx = *reinterpret_cast<const V*>(src + t * row_stride + at.x);
-      V vy = vx;
-      if (pair) vy = *reinterpret_cast<const V*>(src + t * row_stride + at.y);
-      values(vx, vy, t, x, y);
-      write(x, y, t);
-    }
+    rest(write);
+    if (head + 1 < head_end) hold(src + head_stride);
     if (lo > 0 && now > old_scale) {  // the tokens that were there, at the new scale
       const float f = old_scale * inv;
       for (int i = tid; i < lo * c.d / 16; i += kAppendThreads) {
@@ -425,7 +422,7 @@ int launch_append(AppendArgs a, cudaStream_t stream) {
   const bool turn = p.turns != nullptr;
   a.key_units = rotary_units(c.d, turn ? p.rotary_dim : c.d, N);
   a.plain_units = rotary_units(c.d, c.d, N);
-  size_t smem = turn ? static_cast<size_t>(std::min(1 << a.shift, c.tokens)) * a.key_units.half * sizeof(float2) : 0;
+  size_t smem = turn ? static_cast<size_t>(std::min(1 << a.shift, c.tokens)) * factor_pitch<N>(a.key_units.half) * sizeof(float2) : 0;
   int64_t query_ctas = 0;
   a.query = RotaryArgs{};
   if (turn && p.query) {
@@ -439,7 +436,7 @@ int launch_append(AppendArgs a, cudaStream_t stream) {
     q.interleaved = p.interleaved; q.dtype = p.dtype; q.amplitude = p.amplitude;
     a.query = rotary_args(q, N);
     query_ctas = (a.query.groups + kRotaryWarps - 1) / kRotaryWarps;
-    smem = std::max(smem, rotary_smem(a.query));
+    smem = std::max(smem, rotary_smem<N>(a.query));
   }
   auto kern = append_kernel<T, N, kInterleaved>;
   if (smem > 40 * 1024) {
@@ -518,9 +515,9 @@ extern "C" int fdma_cache_append(const fdma_cache_append_params* p, void* stream
   a.p = *p;
   a.shift = block_shift(p->c.block_size);
   a.most_units = static_cast<int>(std::min<int64_t>(p->c.tokens, (static_cast<int64_t>(p->c.tokens) >> a.shift) + 2 * static_cast<int64_t>(p->c.requests)));
-  // Heads of a CTA: the factors (as much work as all the rest of a head) are shared by as many as leave two CTAs per SM.
-  a.key_heads = p->turns ? std::max(1, std::min(p->c.h_k, a.most_units * p->c.h_k / (2 * sm_count()))) : 1;
-  a.cache_ctas = static_cast<int64_t>(a.most_units) * ((p->c.h_k + a.key_heads - 1) / a.key_heads + p->c.h_k);
+  // Heads of a CTA: as many as leave a CTA for each place on the GPU. They share the look-ups and the factors.
+  a.heads = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p->c.h_k, 2 * static_cast<int64_t>(a.most_units) * p->c.h_k / (4 * sm_count()))));
+  a.cache_ctas = 2 * static_cast<int64_t>(a.most_units) * ((p->c.h_k + a.heads - 1) / a.heads);
   if (a.cache_ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   switch (p->dtype) {

@@ -11,9 +11,9 @@ namespace {
 
 template <typename T, int N, bool kInterleaved>
 __global__ void __launch_bounds__(kRotaryWarps * 32, 4) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  extern __shared__ float2 s_factors[];
+  extern __shared__ __align__(16) float2 s_factors[];
   const int warp = threadIdx.x >> 5;
-  rotate_tokens<T, N, kInterleaved>(a, static_cast<int64_t>(blockIdx.x) * kRotaryWarps + warp, s_factors + warp * a.abreast * a.ru.half);
+  rotate_tokens<T, N, kInterleaved>(a, static_cast<int64_t>(blockIdx.x) * kRotaryWarps + warp, s_factors + warp * rotary_warp_pairs<N>(a));
 }
 
 template <typename T, int N, bool kInterleaved>
@@ -21,7 +21,7 @@ int launch(const fdma_rotary_params& p, cudaStream_t stream) {
   const RotaryArgs a = rotary_args(p, N);
   const int64_t ctas = (a.groups + kRotaryWarps - 1) / kRotaryWarps;
   if (ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
-  const size_t smem = rotary_smem(a);
+  const size_t smem = rotary_smem<N>(a);
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(rotary_kernel<T, N, kInterleaved>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -50,7 +50,7 @@ extern "C" int fdma_rotary(const fdma_rotary_params* pp, void* stream_) {
   if (p.h_k && (!p.k || !p.k_out)) return FDMA_ERR_BAD_ARG;
   if (p.rotary_dim <= 0 || p.rotary_dim % 2 || p.rotary_dim > p.d) return FDMA_ERR_BAD_ARG;
   if (p.positions && p.position_bits != 32 && p.position_bits != 64) return FDMA_ERR_BAD_ARG;
-  if (p.rotary_dim > 4096) return FDMA_ERR_UNSUPPORTED;  // a CTA's factors are held in 128 KB
+  if (p.rotary_dim > 4096) return FDMA_ERR_UNSUPPORTED;  // a CTA's factors are held in 160 KB
   if (static_cast<int64_t>(p.h + p.h_k) * p.d > (1 << 24)) return FDMA_ERR_UNSUPPORTED;
   if (p.b == 0 || p.seqlen == 0) return FDMA_OK;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);

@@ -11,17 +11,35 @@
 
 namespace fdma {
 
+// sin and cos of pi x for |x| <= 1/4, by their Taylor series (remainders 1.7e-9 and 4.6e-10 at the ends); pi in two parts, so that
+// its rounding does not count.
+__device__ __forceinline__ void sincos_quarter(float x, float* s, float* c) {
+  const float z = x * x;
+  float p = 0.08214588661112823f;           // pi^9 / 9!
+  p = fmaf(p, z, -0.5992645293207921f);     // -pi^7 / 7!
+  p = fmaf(p, z, 2.550164039877345f);       // pi^5 / 5!
+  p = fmaf(p, z, -5.16771278004997f);       // -pi^3 / 3!
+  p = fmaf(p, z, -8.742277657347586e-8f);   // pi - (its first part)
+  *s = fmaf(p, x, 3.1415927410125732f * x);
+  float q = -0.02580689139001406f;          // -pi^10 / 10!
+  q = fmaf(q, z, 0.23533063035889312f);     // pi^8 / 8!
+  q = fmaf(q, z, -1.3352627688545893f);     // -pi^6 / 6!
+  q = fmaf(q, z, 4.058712126416768f);       // pi^4 / 4!
+  q = fmaf(q, z, -4.934802200544679f);      // -pi^2 / 2!
+  *c = fmaf(q, z, 1.f);
+}
+
 // cos and sin of position * frequency, times the amplitude. The frequency is in turns per position as a 64-bit fraction, so that
 // the product modulo 2^64 IS the angle modulo a turn, without rounding: an angle at position 10^6 is as exact as one at 1, and no
 // 64-bit floating-point arithmetic or table over positions is needed. (fp32 angles are off by 0.06 at 10^6.)
 __device__ __forceinline__ float2 rotary_factors(int64_t position, int64_t turns, float amplitude, bool inverse) {
   const uint64_t phase = static_cast<uint64_t>(position) * static_cast<uint64_t>(turns);
-  // the nearest quarter turn, and what is left of it as half turns in [-1/4, 1/4], rounded to 24 bits of ITS size
-  const uint64_t quarter = phase + (1ull << 61);
-  const int64_t left = static_cast<int64_t>(phase - (quarter & (3ull << 62)));
+  // the nearest quarter turn, and what is left of it in units of 2^-32 turn: 2^-33 turn is lost, which is 7e-10 of a result
+  const uint32_t top = static_cast<uint32_t>(phase >> 32), quarter = top + (1u << 29);
+  const int32_t left = static_cast<int32_t>(top - (quarter & (3u << 30)));
   float s, c;
-  sincospif(__ll2float_rn(left) * 0x1p-63f, &s, &c);
-  const uint32_t n = static_cast<uint32_t>(quarter >> 62);
+  sincos_quarter(static_cast<float>(left) * 0x1p-31f, &s, &c);
+  const uint32_t n = quarter >> 30;
   float cn = n & 1 ? -s : c, sn = n & 1 ? c : s;
   if (n & 2) {
     cn = -cn;
@@ -107,6 +125,15 @@ __device__ __forceinline__ void rotate_unit(float (&a)[N], float (&b)[N], const 
   }
 }
 
+// Factors in shared memory: those of a unit side by side, units 16 bytes apart from one another, so that eight lanes on neighbouring
+// units read different banks. factor_pitch: of a token.
+template <int N>
+constexpr int kFactorUnit = N > 1 ? N + 2 : 1;
+template <int N>
+__host__ __device__ __forceinline__ int factor_pitch(int half) { return half / N * kFactorUnit<N>; }
+template <int N>
+__device__ __forceinline__ int factor_at(int f) { return f / N * kFactorUnit<N> + f % N; }
+
 // A warp takes one token (`abreast` of them where they are small), computes its factors, and goes over the heads of q and k: a lane
 // keeps its unit, and with it the factors in registers, and takes every so many heads. Nothing is shared between warps.
 // 2 x 4096 tokens of 32 + 8 heads, d = 128 (168 MB): 35 us (4.8 TB/s; a plain copy between the same buffers takes 33). Asking for
@@ -139,7 +166,7 @@ __device__ __forceinline__ void rotate_heads(const T* src, T* dst, int64_t src_r
       float2 f[N];
       if (kPair) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = s_factors[t * ru.half + u * N + j];
+        for (int j = 0; j < N; ++j) f[j] = s_factors[t * factor_pitch<N>(ru.half) + u * kFactorUnit<N> + j];
       }
       const T* from = src + t * src_row + hsub * src_head + at.x;
       T* to = dst + t * dst_row + hsub * dst_head + at.x;
@@ -166,7 +193,7 @@ __device__ __forceinline__ void rotate_heads(const T* src, T* dst, int64_t src_r
   }
 }
 
-// What warp `group` of a rotation does; s_factors: abreast * half pairs of the warp's own.
+// What warp `group` of a rotation does; s_factors: abreast * factor_pitch pairs of the warp's own.
 template <typename T, int N, bool kInterleaved>
 __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int64_t group, float2* s_factors) {
   if (group >= a.groups) return;
@@ -184,7 +211,7 @@ __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int64_t group
       const int64_t at = b * p.pos_batch_stride + pos * p.pos_row_stride;
       pos = p.position_bits == 64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
     }
-    s_factors[i] = rotary_factors(pos, p.turns[f], p.amplitude, p.inverse != 0);
+    s_factors[t * factor_pitch<N>(ru.half) + factor_at<N>(f)] = rotary_factors(pos, p.turns[f], p.amplitude, p.inverse != 0);
   }
   __syncwarp();
   const T* q = static_cast<const T*>(p.q) + b * p.q_batch_stride + s * p.q_row_stride;
@@ -218,6 +245,9 @@ inline RotaryArgs rotary_args(const fdma_rotary_params& p, int n) {
   a.groups = static_cast<int64_t>(p.b) * ((p.seqlen + a.abreast - 1) / a.abreast);
   return a;
 }
-inline size_t rotary_smem(const RotaryArgs& a) { return static_cast<size_t>(kRotaryWarps) * a.abreast * a.ru.half * sizeof(float2); }
+template <int N>
+__host__ __device__ __forceinline__ int rotary_warp_pairs(const RotaryArgs& a) { return a.abreast * factor_pitch<N>(a.ru.half); }
+template <int N>
+inline size_t rotary_smem(const RotaryArgs& a) { return static_cast<size_t>(kRotaryWarps) * rotary_warp_pairs<N>(a) * sizeof(float2); }
 
 }  // namespace fdma
