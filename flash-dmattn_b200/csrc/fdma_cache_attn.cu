@@ -4,10 +4,12 @@
 //   k_j = k_scale[block, head] * e4m3, v_j likewise
 //
 // Few queries over many keys: HBM-bound, 2 d bytes per key and kv head. What follows from that:
-//  * The queries of a request that share a kv head -- new tokens x query heads -- are the M rows of mma.m16n8k16, so a key is
-//    read once for all of them. The products are in fp16 with 32-bit sums: e4m3 numbers are fp16 numbers (one conversion
-//    instruction for two), bf16 queries become fp16 after a power of two per row (exact up to 2^-29 of the row's largest), and
-//    scales, being powers of two or common to a product, go into the scores and the softmax's exponents.
+//  * The queries of a request that share a kv head -- new tokens x query heads -- are the eight columns of mma.m16n8k16 (of two, when
+//    there are more), so a key is read once for all of them, and the rows are full: 16 keys of K Q^T, 16 elements of V^T P^T.
+//    (With the queries as the 16 rows half of each product, of its accumulators and of their moves was for nothing: 461 instructions
+//    for 16 keys, %NOW% so.) The products are in fp16 with 32-bit sums: e4m3 numbers are fp16 numbers (one conversion instruction for
+//    two), bf16 queries become fp16 after a power of two per row (exact up to 2^-29 of the row's largest), and scales, being powers
+//    of two or common to a product, go into the scores and the softmax's exponents.
 //  * A unit of work is a (request, kv head, tile of 8 or 16 rows), made of chunks of 64 keys. The chunks of all units form one row;
 //    every CTA takes an equal part of it, however long the requests are, and starts and ends in the middle of a unit where it
 //    must. Such partial results go through scratch and a second kernel; units that one CTA finishes are written directly.
@@ -75,9 +77,20 @@ __device__ __forceinline__ uint32_t e4m3x2_hi_to_f16x2(uint32_t two) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(two));
   return r;
 }
-__device__ __forceinline__ void mma_f16(float (&c)[2], float (&c8)[2], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c8[0]), "+f"(c8[1]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// An 8 x 8 matrix of 16-bit numbers, a row per four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
@@ -211,7 +224,7 @@ struct Layout {
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kStages = D > 128 ? 2 : 3;
   static constexpr int kSteps = D / 16;                             // k steps of Q K^T
-  static constexpr int kQBytes = (ROWS + 15) / 16 * kSteps * 512;
+  static constexpr int kQBytes = ROWS / 8 * kSteps * 256;
   static constexpr int kBufFloats = ROWS * D;                       // one warp's sums
   static constexpr int kBufs = D > 128 ? 1 : 2;
   static constexpr int kRing = 0;
@@ -226,8 +239,8 @@ template <int D, int ROWS, bool kGather, bool kBf16>
 __global__ void __launch_bounds__(Layout<D, ROWS, kGather>::kThreads, Layout<D, ROWS, kGather>::kCtas)
 cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using L = Layout<D, ROWS, kGather>;
-  constexpr int kGroups = ROWS / 8;  // eight rows each
-  constexpr int kTiles = (ROWS + 15) / 16;
+  constexpr int kTiles = ROWS / 8;                     // of eight queries
+  constexpr bool kQHeld = ROWS == 8 && D <= 128;       // queries in registers
   extern __shared__ unsigned char s_raw[];
   __shared__ __align__(8) uint64_t s_full[L::kStages], s_empty[L::kStages];
   // of a slice: 1 if its block is there, K scale, exponent of the V scale, its reciprocal; of a kept key: bias (-inf: not there),
@@ -356,7 +369,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   const int r0 = key_row(2 * t), r1 = key_row(2 * t + 1);
   const uint32_t v_at0 = L::kTileBytes + r0 * 128 + (((g >> 2) ^ (r0 & 7)) << 4) + (g & 3) * 4;
   const uint32_t v_at1 = L::kTileBytes + r1 * 128 + (((g >> 2) ^ (r1 & 7)) << 4) + (g & 3) * 4;
-  const uint32_t q_at = smem_u32(smem) + L::kQ + lane * 16;
+  const uint32_t q_at = smem_u32(smem) + L::kQ + lane * 8;
   float* const s_buf = reinterpret_cast<float*>(smem + L::kBuf);
   int st = 0;
   uint32_t phase = 0;
@@ -376,7 +389,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 
     // queries: eight threads a row, to fp16 in the order of the fragments
     consumers_sync();
-    for (int rr = tid >> 3; rr < kTiles * 16; rr += 16) {
+    for (int rr = tid >> 3; rr < ROWS; rr += 16) {
       constexpr int E = D / 8;  // elements per thread, in 16-byte vectors vec * 8 + part
       const int part = tid & 7, row = row0 + rr;
       uint32_t x[E / 2];
@@ -413,8 +426,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         // the largest becomes 2^13 ... 2^14
         const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100), 127) - 13;
         scale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        if (part == 0 && rr < ROWS) s_row_scale[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      } else if (part == 0 && rr < ROWS) {
+        if (part == 0) s_row_scale[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      } else if (part == 0) {
         s_row_scale[rr] = a.scale_log2;
       }
 #pragma unroll
@@ -423,32 +436,40 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         if (kBf16) y = pack_f16(raw_to_f<true>(static_cast<uint16_t>(y)) * scale, raw_to_f<true>(static_cast<uint16_t>(y >> 16)) * scale);
         const int dd = ((e >> 2) * 8 + part) * 8 + (e & 3) * 2;  // element of the row
         const int step = (dd >> 6) * 4 + ((dd >> 2) & 3), to_lane = (rr & 7) * 4 + ((dd >> 4) & 3);
-        const int reg = ((rr >> 3) & 1) + ((dd >> 1) & 1) * 2;
-        reinterpret_cast<uint32_t*>(smem + L::kQ)[(((rr >> 4) * L::kSteps + step) * 32 + to_lane) * 4 + reg] = y;
+        reinterpret_cast<uint32_t*>(smem + L::kQ)[(((rr >> 3) * L::kSteps + step) * 32 + to_lane) * 2 + ((dd >> 1) & 1)] = y;
       }
     }
     consumers_sync();
-
-    float o[kGroups][D / 32][4][2], m[kGroups], l[kGroups], row_scale[kGroups];
-    int newest[kGroups];
-    const uint16_t* bias_row[kGroups];
+    uint2 q_held[kQHeld ? L::kSteps : 1];
+    if (kQHeld) {
 #pragma unroll
-    for (int rs = 0; rs < kGroups; ++rs) {
-      m[rs] = -CUDART_INF_F;
-      l[rs] = 0.f;
-      const int row = row0 + min(g + 8 * rs, nrows - 1);
-      row_scale[rs] = s_row_scale[min(g + 8 * rs, nrows - 1)];
-      newest[rs] = p.is_causal ? min(length - 1, q.length - q.n + row / a.group) : length - 1;
-      const int head = u.hk * a.group + row % a.group;
-      bias_row[rs] = p.bias ? static_cast<const uint16_t*>(p.bias) + u.r * p.bias_batch_stride +
-                                  (p.h_bias == p.h ? head : p.h_bias == c.h_k ? u.hk : 0) * p.bias_head_stride
-                            : nullptr;
+      for (int x = 0; x < (kQHeld ? L::kSteps : 1); ++x) q_held[x] = lds64(q_at + x * 256);
+    }
+
+    // of queries 8 tile + 2 t, + 1: sums over the values (elements 32 j + 4 g + 2 half + {0: [0, 1], 1: [2, 3]}), maximum, this lane's
+    // share of the softmax's sum, factor of the scores, newest position seen
+    float o[kTiles][D / 32][2][4], m[kTiles][2], l[kTiles][2], row_scale[kTiles][2];
+    int newest[kTiles][2];
+    const uint16_t* bias_row[kTiles][2];
+#pragma unroll
+    for (int nt = 0; nt < kTiles; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[nt][e] = -CUDART_INF_F;
+        l[nt][e] = 0.f;
+        const int rr = min(8 * nt + 2 * t + e, nrows - 1), row = row0 + rr;
+        row_scale[nt][e] = s_row_scale[rr];
+        newest[nt][e] = p.is_causal ? min(length - 1, q.length - q.n + row / a.group) : length - 1;
+        const int head = u.hk * a.group + row % a.group;
+        bias_row[nt][e] = p.bias ? static_cast<const uint16_t*>(p.bias) + u.r * p.bias_batch_stride +
+                                       (p.h_bias == p.h ? head : p.h_bias == c.h_k ? u.hk : 0) * p.bias_head_stride
+                                 : nullptr;
+      }
 #pragma unroll
       for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[rs][j][i][0] = o[rs][j][i][1] = 0.f;
+        for (int i = 0; i < 8; ++i) o[nt][j][i >> 2][i & 3] = 0.f;
     }
-    float zero[2] = {0.f, 0.f};  // rows 8-15 where there are none: always zero
 
     // Kept keys: at chunk i the rows of chunk i + kAhead are asked for, the block numbers of the one behind it and the positions
     // of the next, so that nothing here waits for a load of its own. Lanes 0 - 15 stand for the slice's keys.
@@ -487,7 +508,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const int64_t at = static_cast<int64_t>(block2) * c.h_k + u.hk;
         g_scale_k = __ldg(c.k_scale + at);
         g_scale_v = __ldg(c.v_scale + at);
-        g_bias = p.bias && !head_bias && pos2 < p.bias_keys ? __ldg(bias_row[0] + pos2) : static_cast<uint16_t>(0);
+        g_bias = p.bias && !head_bias && pos2 < p.bias_keys ? __ldg(bias_row[0][0] + pos2) : static_cast<uint16_t>(0);
       }
       if (i + kAhead < last) {
         constexpr int kLanes = D / 16;  // 16-byte pieces of a row
@@ -525,33 +546,35 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     for (int chunk = first; chunk < last; ++chunk) {
       const int pos0 = chunk * kChunk + warp * kSlice;
       if (kGather) gather(chunk);
-      uint16_t raw_bias[kGroups][4];
-      const bool with_bias = !kGather && p.bias;
+      const int key = key_row(g);  // this lane's scores: keys pos0 + key, + 8
+      uint16_t raw_bias[kTiles][2][2];
+      const bool with_bias = !kGather && p.bias, head_bias_dense = with_bias && head_bias;
       if (with_bias) {
 #pragma unroll
-        for (int rs = 0; rs < kGroups; ++rs)
+        for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int pos = pos0 + (k >> 1) * 8 + (k & 1 ? r1 : r0);
-            raw_bias[rs][k] = pos < min(length, p.bias_keys) ? __ldg(bias_row[rs] + pos) : static_cast<uint16_t>(0);
+            const int pos = pos0 + (k >> 1) * 8 + key;
+            if ((k & 1) == 0 || head_bias_dense) raw_bias[nt][k >> 1][k & 1] = pos < min(length, p.bias_keys) ? __ldg(bias_row[nt][k & 1] + pos) : static_cast<uint16_t>(0);
+            else raw_bias[nt][k >> 1][1] = raw_bias[nt][k >> 1][0];
           }
       }
       float4 meta;
-      float4 key_meta[4];
+      float4 key_meta[2];
       if (kGather) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) key_meta[k] = s_meta[st][warp * kSlice + (k >> 1) * 8 + (k & 1 ? r1 : r0)];
+        for (int k = 0; k < 2; ++k) key_meta[k] = s_meta[st][warp * kSlice + k * 8 + key];
       } else {
         mbar_wait(&s_full[st], phase, ctl, 702);
         meta = s_meta[st][warp];
       }
       const uint32_t tile = ring + st * L::kStageBytes;
-      // scores: s[row group][keys 0-7 | 8-15][column pair]
-      float s[kGroups][2][2];
+      // scores: s[tile][2 * (second eight keys) + (second query)]
+      float s[kTiles][4];
 #pragma unroll
-      for (int rs = 0; rs < kGroups; ++rs) s[rs][0][0] = s[rs][0][1] = s[rs][1][0] = s[rs][1][1] = 0.f;
+      for (int nt = 0; nt < kTiles; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
       for (int jj = 0; jj < D / 64; ++jj) {
         const uint32_t at = tile + (jj >> 1) * kChunk * 128 + (k_at ^ ((jj & 1) << 6));
@@ -559,72 +582,77 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const uint32_t a0 = e4m3x2_to_f16x2(wa[x]), a1 = e4m3x2_hi_to_f16x2(wa[x]);
-          const uint32_t b0 = e4m3x2_to_f16x2(wb[x]), b1 = e4m3x2_hi_to_f16x2(wb[x]);
+          const uint32_t a0 = e4m3x2_to_f16x2(wa[x]), a1 = e4m3x2_to_f16x2(wb[x]), a2 = e4m3x2_hi_to_f16x2(wa[x]), a3 = e4m3x2_hi_to_f16x2(wb[x]);
 #pragma unroll
-          for (int mt = 0; mt < kTiles; ++mt) {
-            const uint4 f = lds128(q_at + (mt * L::kSteps + jj * 4 + x) * 512);
-            mma_f16(s[2 * mt][0], ROWS > 8 ? s[(2 * mt + 1) % kGroups][0] : zero, f.x, f.y, f.z, f.w, a0, a1);
-            mma_f16(s[2 * mt][1], ROWS > 8 ? s[(2 * mt + 1) % kGroups][1] : zero, f.x, f.y, f.z, f.w, b0, b1);
+          for (int nt = 0; nt < kTiles; ++nt) {
+            const uint2 f = kQHeld ? q_held[kQHeld ? jj * 4 + x : 0] : lds64(q_at + (nt * L::kSteps + jj * 4 + x) * 256);
+            mma_f16(s[nt], a0, a1, a2, a3, f.x, f.y);
           }
         }
       }
       // all 16 keys are there and seen by every row
       const bool clean = !kGather && pos0 + kSlice <= sure && meta.x != 0.f;
-      uint32_t pa[kGroups][2];
-      float inv_v[4];
-      if (kGather) {
+      float x[kTiles][4];
+      bool grows = false;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) inv_v[k] = exp2f(-key_meta[k].z);
-      }
-#pragma unroll
-      for (int rs = 0; rs < kGroups; ++rs) {
-        float x[4];
+      for (int nt = 0; nt < kTiles; ++nt) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+          float& v = x[nt][k];
           if (kGather) {
-            const int pos = __float_as_int(key_meta[k].w);
-            float add = key_meta[k].x;
-            if (head_bias && pos >= 0 && pos < p.bias_keys) add = bias_log2(raw_to_f<kBf16>(__ldg(bias_row[rs] + pos)));
-            x[k] = fmaf(s[rs][k >> 1][k & 1], row_scale[rs] * key_meta[k].y, add) + key_meta[k].z;
-            if (pos < 0 || pos > newest[rs]) x[k] = -CUDART_INF_F;
+            const float4& km = key_meta[k >> 1];
+            const int pos = __float_as_int(km.w);
+            float add = km.x;
+            if (head_bias && pos >= 0 && pos < p.bias_keys) add = bias_log2(raw_to_f<kBf16>(__ldg(bias_row[nt][k & 1] + pos)));
+            v = fmaf(s[nt][k], row_scale[nt][k & 1] * km.y, add) + km.z;
+            if (pos < 0 || pos > newest[nt][k & 1]) v = -CUDART_INF_F;
           } else {
-            x[k] = s[rs][k >> 1][k & 1] * (row_scale[rs] * meta.y);
-            if (with_bias) x[k] += bias_log2(raw_to_f<kBf16>(raw_bias[rs][k]));
-            x[k] += meta.z;
-            if (!clean && (pos0 + (k >> 1) * 8 + (k & 1 ? r1 : r0) > newest[rs] || meta.x == 0.f)) x[k] = -CUDART_INF_F;
+            v = s[nt][k] * (row_scale[nt][k & 1] * meta.y);
+            if (with_bias) v += bias_log2(raw_to_f<kBf16>(raw_bias[nt][k >> 1][k & 1]));
+            v += meta.z;
+            if (!clean && (pos0 + (k >> 1) * 8 + key > newest[nt][k & 1] || meta.x == 0.f)) v = -CUDART_INF_F;
           }
+          grows |= v > m[nt][k & 1];
         }
-        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        if (__any_sync(0xffffffffu, mx > m[rs])) {
-          const float m_new = fmaxf(m[rs], mx);
-          const float corr = exp2_or_zero(m[rs] - (m_new == -CUDART_INF_F ? 0.f : m_new));
-          m[rs] = m_new;
-          l[rs] *= corr;
+      }
+      if (__any_sync(0xffffffffu, grows)) {  // a query's maxima are compared over its keys only when one of them grows
+#pragma unroll
+        for (int nt = 0; nt < kTiles; ++nt) {
+          float corr[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(x[nt][e], x[nt][2 + e]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            const float m_new = fmaxf(m[nt][e], mx);
+            corr[e] = exp2_or_zero(m[nt][e] - (m_new == -CUDART_INF_F ? 0.f : m_new));
+            m[nt][e] = m_new;
+            l[nt][e] *= corr[e];
+          }
 #pragma unroll
           for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              o[rs][j][i][0] *= corr;
-              o[rs][j][i][1] *= corr;
-            }
+            for (int i = 0; i < 8; ++i) o[nt][j][i >> 2][i & 3] *= corr[i & 1];
         }
-        const float base = m[rs] == -CUDART_INF_F ? 0.f : m[rs];
+      }
+      uint32_t pb[kTiles][2];  // P^T: queries' probabilities, keys 0-7 | 8-15
+#pragma unroll
+      for (int nt = 0; nt < kTiles; ++nt) {
         float e[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = exp2f(x[k] - base);
+        for (int k = 0; k < 4; ++k) e[k] = exp2f(x[nt][k] - (m[nt][k & 1] == -CUDART_INF_F ? 0.f : m[nt][k & 1]));
         if (kGather) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) l[rs] = fmaf(e[k], inv_v[k], l[rs]);
+          for (int k = 0; k < 4; ++k) l[nt][k & 1] = fmaf(e[k], exp2f(-key_meta[k >> 1].z), l[nt][k & 1]);
         } else {
-          l[rs] = fmaf((e[0] + e[1]) + (e[2] + e[3]), meta.w, l[rs]);
+          l[nt][0] = fmaf(e[0] + e[2], meta.w, l[nt][0]);
+          l[nt][1] = fmaf(e[1] + e[3], meta.w, l[nt][1]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] *= p_scale(kGather ? key_meta[k].z : meta.z);
-        pa[rs][0] = pack_f16(e[0], e[1]);
-        pa[rs][1] = pack_f16(e[2], e[3]);
+        for (int k = 0; k < 2; ++k) {
+          const float f = p_scale(kGather ? key_meta[k].z : meta.z);
+          pb[nt][k] = transpose8(pack_f16(e[2 * k] * f, e[2 * k + 1] * f));
+        }
       }
       const bool whole = kGather || (pos0 + kSlice <= length && meta.x != 0.f);
 #pragma unroll
@@ -638,16 +666,13 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           if (meta.x == 0.f || pos0 + 8 + r0 >= length) y2 = 0;
           if (meta.x == 0.f || pos0 + 8 + r1 >= length) y3 = 0;
         }
-        const uint32_t lo01 = __byte_perm(y0, y1, 0x5140), hi01 = __byte_perm(y0, y1, 0x7362);
-        const uint32_t lo23 = __byte_perm(y2, y3, 0x5140), hi23 = __byte_perm(y2, y3, 0x7362);
-        const uint32_t b0[4] = {e4m3x2_to_f16x2(lo01), e4m3x2_hi_to_f16x2(lo01), e4m3x2_to_f16x2(hi01), e4m3x2_hi_to_f16x2(hi01)};
-        const uint32_t b1[4] = {e4m3x2_to_f16x2(lo23), e4m3x2_hi_to_f16x2(lo23), e4m3x2_to_f16x2(hi23), e4m3x2_hi_to_f16x2(hi23)};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int h = 0; h < 2; ++h) {  // bytes 0, 1 | 2, 3 of the words: rows g | g + 8 of the product
+          const uint32_t first = __byte_perm(y0, y1, h ? 0x7362 : 0x5140), second = __byte_perm(y2, y3, h ? 0x7362 : 0x5140);
+          const uint32_t a0 = e4m3x2_to_f16x2(first), a1 = e4m3x2_hi_to_f16x2(first), a2 = e4m3x2_to_f16x2(second), a3 = e4m3x2_hi_to_f16x2(second);
 #pragma unroll
-          for (int mt = 0; mt < kTiles; ++mt)
-            mma_f16(o[2 * mt][j][i], ROWS > 8 ? o[(2 * mt + 1) % kGroups][j][i] : zero, pa[2 * mt][0], ROWS > 8 ? pa[(2 * mt + 1) % kGroups][0] : 0u,
-                    pa[2 * mt][1], ROWS > 8 ? pa[(2 * mt + 1) % kGroups][1] : 0u, b0[i], b1[i]);
+          for (int nt = 0; nt < kTiles; ++nt) mma_f16(o[nt][j][h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+        }
       }
       __syncwarp();  // every lane has read the stage before it is overwritten
       if (!kGather && lane == 0) mbar_arrive(&s_empty[st]);
@@ -659,54 +684,56 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 
     // ---- the four warps' sums: to a common maximum, then added up through shared memory ----
 #pragma unroll
-    for (int rs = 0; rs < kGroups; ++rs) {
-      l[rs] += __shfl_xor_sync(0xffffffffu, l[rs], 1);
-      l[rs] += __shfl_xor_sync(0xffffffffu, l[rs], 2);
-      if (t == 0) {
-        s_m[warp][g + 8 * rs] = m[rs];
-        s_l[warp][g + 8 * rs] = l[rs];
+    for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+        if (g == 0) {
+          s_m[warp][8 * nt + 2 * t + e] = m[nt][e];
+          s_l[warp][8 * nt + 2 * t + e] = l[nt][e];
+        }
       }
-    }
     consumers_sync();
 #pragma unroll
-    for (int rs = 0; rs < kGroups; ++rs) {
-      float cm = -CUDART_INF_F, cl = 0.f;
+    for (int nt = 0; nt < kTiles; ++nt) {
+      float f[2];
 #pragma unroll
-      for (int x = 0; x < kWarps; ++x) cm = fmaxf(cm, s_m[x][g + 8 * rs]);
-      const float base = cm == -CUDART_INF_F ? 0.f : cm;
+      for (int e = 0; e < 2; ++e) {
+        const int rr = 8 * nt + 2 * t + e;
+        float cm = -CUDART_INF_F, cl = 0.f;
 #pragma unroll
-      for (int x = 0; x < kWarps; ++x) cl = fmaf(s_l[x][g + 8 * rs], exp2_or_zero(s_m[x][g + 8 * rs] - base), cl);
-      const float f = exp2_or_zero(m[rs] - base) * (1.f / kPScale);
-      m[rs] = cm;
-      l[rs] = cl;
+        for (int x = 0; x < kWarps; ++x) cm = fmaxf(cm, s_m[x][rr]);
+        const float base = cm == -CUDART_INF_F ? 0.f : cm;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) cl = fmaf(s_l[x][rr], exp2_or_zero(s_m[x][rr] - base), cl);
+        f[e] = exp2_or_zero(m[nt][e] - base) * (1.f / kPScale);
+        m[nt][e] = cm;
+        l[nt][e] = cl;
+      }
 #pragma unroll
       for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[rs][j][i][0] *= f;
-          o[rs][j][i][1] *= f;
-        }
+        for (int i = 0; i < 8; ++i) o[nt][j][i >> 2][i & 3] *= f[i & 1];
     }
     auto put = [&](float* buf) {
 #pragma unroll
-      for (int rs = 0; rs < kGroups; ++rs)
+      for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            *reinterpret_cast<float4*>(buf + ((rs * (D / 32) + j) * 2 + x) * 128 + lane * 4) =
-                make_float4(o[rs][j][0][x], o[rs][j][1][x], o[rs][j][2][x], o[rs][j][3][x]);
+        for (int i = 0; i < D / 16; ++i) {
+          const float(&y)[4] = o[nt][i >> 1][i & 1];
+          *reinterpret_cast<float4*>(buf + (nt * (D / 16) + i) * 128 + lane * 4) = make_float4(y[0], y[1], y[2], y[3]);
+        }
     };
     auto add = [&](const float* buf) {
 #pragma unroll
-      for (int rs = 0; rs < kGroups; ++rs)
+      for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float4 y = *reinterpret_cast<const float4*>(buf + ((rs * (D / 32) + j) * 2 + x) * 128 + lane * 4);
-            o[rs][j][0][x] += y.x; o[rs][j][1][x] += y.y; o[rs][j][2][x] += y.z; o[rs][j][3][x] += y.w;
-          }
+        for (int i = 0; i < D / 16; ++i) {
+          float(&y)[4] = o[nt][i >> 1][i & 1];
+          const float4 x = *reinterpret_cast<const float4*>(buf + (nt * (D / 16) + i) * 128 + lane * 4);
+          y[0] += x.x; y[1] += x.y; y[2] += x.z; y[3] += x.w;
+        }
     };
     if constexpr (L::kBufs == 2) {
       if (warp >= 2) put(s_buf + (warp - 2) * L::kBufFloats);
@@ -728,34 +755,32 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const bool complete = first == 0 && last == u.n;
     float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (first > 0 ? 0 : 1)) * ROWS * (D + 4);
 #pragma unroll
-    for (int rs = 0; rs < kGroups; ++rs) {
-      const int rr = g + 8 * rs, row = row0 + rr;
-      if (rr >= nrows) continue;
-      if (complete) {
-        const float inv = l[rs] == 0.f ? 0.f : 1.f / l[rs];
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(q.token0 + row / a.group) * p.out_row_stride +
-                        (u.hk * a.group + row % a.group) * p.out_head_stride;
+    for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const int dd = 32 * j + 8 * t;
-          if (dd < c.d) {
-            const float(&y)[4][2] = o[rs][j];
-            *reinterpret_cast<uint4*>(dst + dd) =
-                make_uint4(pack2<kBf16>(y[0][0] * inv, y[1][0] * inv), pack2<kBf16>(y[2][0] * inv, y[3][0] * inv),
-                           pack2<kBf16>(y[0][1] * inv, y[1][1] * inv), pack2<kBf16>(y[2][1] * inv, y[3][1] * inv));
+      for (int e = 0; e < 2; ++e) {
+        const int rr = 8 * nt + 2 * t + e, row = row0 + rr;
+        if (rr >= nrows) continue;
+        if (complete) {
+          const float inv = l[nt][e] == 0.f ? 0.f : 1.f / l[nt][e];
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(q.token0 + row / a.group) * p.out_row_stride +
+                          (u.hk * a.group + row % a.group) * p.out_head_stride;
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const int dd = 32 * j + 4 * g;
+            const float(&y)[2][4] = o[nt][j];
+            if (dd < c.d)
+              *reinterpret_cast<uint2*>(dst + dd) = make_uint2(pack2<kBf16>(y[0][e] * inv, y[0][2 + e] * inv), pack2<kBf16>(y[1][e] * inv, y[1][2 + e] * inv));
           }
-        }
-      } else {
-        float* dst = part + rr * (D + 4);
+        } else {
+          float* dst = part + rr * (D + 4);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const float(&y)[4][2] = o[rs][j];
-          *reinterpret_cast<float4*>(dst + 32 * j + 8 * t) = make_float4(y[0][0], y[1][0], y[2][0], y[3][0]);
-          *reinterpret_cast<float4*>(dst + 32 * j + 8 * t + 4) = make_float4(y[0][1], y[1][1], y[2][1], y[3][1]);
+          for (int j = 0; j < D / 32; ++j) {
+            const float(&y)[2][4] = o[nt][j];
+            *reinterpret_cast<float4*>(dst + 32 * j + 4 * g) = make_float4(y[0][e], y[0][2 + e], y[1][e], y[1][2 + e]);
+          }
+          if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[nt][e], l[nt][e]);
         }
-        if (t == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[rs], l[rs]);
       }
-    }
   }
 }
 
