@@ -7,7 +7,7 @@
 //  * The queries of a request that share a kv head -- new tokens x query heads -- are the eight columns of mma.m16n8k16 (of two, when
 //    there are more), so a key is read once for all of them, and the rows are full: 16 keys of K Q^T, 16 elements of V^T P^T.
 //    (With the queries as the 16 rows half of each product, of its accumulators and of their moves was for nothing: 461 instructions
-//    for 16 keys, %NOW% so.) The products are in fp16 with 32-bit sums: e4m3 numbers are fp16 numbers (one conversion instruction for
+//    for 16 keys, 349 so.) The products are in fp16 with 32-bit sums: e4m3 numbers are fp16 numbers (one conversion instruction for
 //    two), bf16 queries become fp16 after a power of two per row (exact up to 2^-29 of the row's largest), and scales, being powers
 //    of two or common to a product, go into the scores and the softmax's exponents.
 //  * A unit of work is a (request, kv head, tile of 8 or 16 rows), made of chunks of 64 keys. The chunks of all units form one row;
@@ -40,9 +40,11 @@ constexpr float kPScale = 16384.f;  // probabilities in fp16: normal numbers dow
 
 struct AttnArgs {
   fdma_cache_attention_params p;
-  int shift, group, rows;  // rows: of a tile
+  int shift, group, row_shift;  // log2 of the block size, and of the rows of a tile
+  uint32_t group_inverse, h_k_inverse;  // floor(2^32 / x), at most 2^32 - 1
   int list_chunks;         // kept keys: chunks per unit; 0: from cu_chunks
-  const int32_t* pre;      // more than kHeld requests: sums of their chunks x tiles, requests + 1
+  int32_t* pre;            // sums of the requests' chunks x tiles, requests + 1: for more than kHeld requests made before, for fewer
+                           // by the first CTA, for the second kernel
   int ctas;                // along the row of chunks
   float scale_log2;
   bool q_vec;              // queries in 16-byte vectors
@@ -149,12 +151,30 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
   return q;
 }
 
-__device__ __forceinline__ int tiles_of(const AttnArgs& a, int rows) { return rows > 0 ? (rows + a.rows - 1) / a.rows : 0; }
+// x / y and the remainder, given floor(2^32 / y): the product is at most one too small.
+__device__ __forceinline__ uint2 divide(uint32_t x, uint32_t y, uint32_t inverse) {
+  uint32_t quot = __umulhi(x, inverse), rem = x - quot * y;
+  if (rem >= y) {
+    ++quot;
+    rem -= y;
+  }
+  return make_uint2(quot, rem);
+}
+// Both positive. (A 64-bit division is a few hundred cycles.)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, int rows) { return rows > 0 ? (rows + (1 << a.row_shift) - 1) >> a.row_shift : 0; }
+// (token, head) of a request's row
+__device__ __forceinline__ uint2 token_head(const AttnArgs& a, int row) { return divide(row, a.group, a.group_inverse); }
 
 // The units in the order of their chunks. Up to kHeld requests: their data and the sums of their chunks x tiles are held in shared
 // memory. More: the sums are in global memory, and the data is read where it is needed.
 struct Held {
   int pre[kHeld + 1], token0[kHeld], n[kHeld], length[kHeld], rows[kHeld], chunks[kHeld], warp[4];
+};
+struct Cursor {
+  int r, hk, tile;
 };
 struct Units {
   const AttnArgs& a;
@@ -165,28 +185,48 @@ struct Units {
     if (!held) return load_request(a, r);
     return Request{held->token0[r], held->n[r], held->length[r], held->rows[r], held->chunks[r]};
   }
-  // `tile` and `hk` may be past the end of the request's: the start then is, too
-  __device__ Unit of(int r, const Request& q, int hk, int tile) const {
+  __device__ Unit of(const Cursor& x, const Request& q) const {
     Unit u;
-    u.r = r; u.hk = hk; u.tile = tile;
+    u.r = x.r; u.hk = x.hk; u.tile = x.tile;
     u.n = q.chunks;
-    u.start = static_cast<int64_t>(pre()[r]) * a.p.c.h_k + (static_cast<int64_t>(hk) * tiles_of(a, q.rows) + tile) * q.chunks;
+    u.start = static_cast<int64_t>(pre()[x.r]) * a.p.c.h_k + (static_cast<int64_t>(x.hk) * tiles_of(a, q.rows) + x.tile) * q.chunks;
     return u;
   }
-  // the unit of chunk w, w < total(), and its request
-  __device__ Unit at(int64_t w, Request& q) const {
-    const int64_t per_head = w / a.p.c.h_k;
-    const int32_t* ends = pre() + 1;
-    int lo = 0, hi = a.p.c.requests - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (ends[mid] > per_head) hi = mid;
-      else lo = mid + 1;
+  // the unit of chunk w, w < total(), and its request; the same w in all lanes of a warp
+  __device__ Cursor at(int64_t w, Request& q) const {
+    const fdma_cache& c = a.p.c;
+    const int64_t per_head = w >> 32 ? w / c.h_k : divide(static_cast<uint32_t>(w), c.h_k, a.h_k_inverse).x;
+    int r = 0;  // requests that end at or before it
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < kHeld; i += 32) {
+        const int at = i + (threadIdx.x & 31);
+        r += __popc(__ballot_sync(0xffffffffu, at < c.requests && held->pre[at + 1] <= per_head));
+      }
+    } else {
+      int hi = c.requests - 1;
+      while (r < hi) {
+        const int mid = (r + hi) >> 1;
+        if (a.pre[mid + 1] > per_head) hi = mid;
+        else r = mid + 1;
+      }
     }
-    q = request(lo);
+    r = min(r, c.requests - 1);
+    q = request(r);
     const int tiles = max(tiles_of(a, q.rows), 1);
-    const int i = static_cast<int>((w - static_cast<int64_t>(pre()[lo]) * a.p.c.h_k) / max(q.chunks, 1));
-    return of(lo, q, i / tiles, i % tiles);
+    const int i = static_cast<int>(quotient(max(w - static_cast<int64_t>(pre()[r]) * c.h_k, int64_t{0}), max(q.chunks, 1)));
+    return tiles == 1 ? Cursor{r, i, 0} : Cursor{r, i / tiles, i % tiles};
+  }
+  // the unit behind, whose request is q then; past the last one x.r == requests
+  __device__ void advance(Cursor& x, Request& q) const {
+    if (++x.tile < tiles_of(a, q.rows)) return;
+    x.tile = 0;
+    if (++x.hk < a.p.c.h_k) return;
+    x.hk = 0;
+    while (++x.r < a.p.c.requests) {
+      q = request(x.r);
+      if (q.chunks > 0 && q.rows > 0) return;
+    }
   }
 };
 // All threads of a CTA of at least 128.
@@ -215,7 +255,7 @@ __device__ __forceinline__ Units make_units(const AttnArgs& a, Held& h) {
   __syncthreads();
   return Units{a, &h};
 }
-__device__ __forceinline__ int64_t share_of(int64_t total, int ctas) { return max(static_cast<int64_t>(kMinShare), (total + ctas - 1) / ctas); }
+__device__ __forceinline__ int64_t share_of(int64_t total, int ctas) { return max(static_cast<int64_t>(kMinShare), quotient(total + ctas - 1, ctas)); }
 
 template <int D, int ROWS, bool kGather>
 struct Layout {
@@ -240,7 +280,7 @@ __global__ void __launch_bounds__(Layout<D, ROWS, kGather>::kThreads, Layout<D, 
 cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using L = Layout<D, ROWS, kGather>;
   constexpr int kTiles = ROWS / 8;                     // of eight queries
-  constexpr bool kQHeld = ROWS == 8 && D <= 128;       // queries in registers
+  constexpr bool kQHeld = kTiles * L::kSteps <= 8;     // queries in registers
   extern __shared__ unsigned char s_raw[];
   __shared__ __align__(8) uint64_t s_full[L::kStages], s_empty[L::kStages];
   // of a slice: 1 if its block is there, K scale, exponent of the V scale, its reciprocal; of a kept key: bias (-inf: not there),
@@ -268,6 +308,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     for (int i = tid; i < L::kStages * L::kStageBytes / 16; i += L::kThreads) reinterpret_cast<uint4*>(smem + L::kRing)[i] = make_uint4(0, 0, 0, 0);
   const Units units = make_units(a, s_held);
   __syncthreads();
+  if (blockIdx.x == 0 && units.held)
+    for (int i = tid; i <= c.requests; i += L::kThreads) a.pre[i] = s_held.pre[i];
   const int64_t total = units.total(), share = share_of(total, a.ctas);
   const int64_t w0 = min(total, blockIdx.x * share), w1 = min(total, w0 + share);
   if (w0 >= w1) return;
@@ -276,18 +318,24 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   if (!kGather && warp == kWarps) {
     // ---- the copying warp: lanes look up the blocks and scales of eight chunks at a time, four 16-key slices each ----
     const int pages = max(1, kChunk >> a.shift), rows_per_copy = min(kChunk, 1 << a.shift);
+    Request lane_q;
+    Cursor at = units.at(w0, lane_q);  // of this lane's chunk, from here on
     auto look_up = [&](int64_t w, int& block, int& row, int& hk, float& ks, float& vs, bool& used) {
       block = -1;
       row = hk = 0;
       ks = vs = 0.f;
       used = false;
       if (w < w1) {
-        Request q;
-        const Unit u = units.at(w, q);
+        Unit u = units.of(at, lane_q);
+        while (w >= u.start + u.n) {
+          units.advance(at, lane_q);
+          if (at.r >= c.requests) return;
+          u = units.of(at, lane_q);
+        }
         hk = u.hk;
-        used = q.rows > u.tile * ROWS;
+        used = lane_q.rows > u.tile * ROWS;
         const int pos = static_cast<int>(w - u.start) * kChunk + (lane & 3) * kSlice;
-        if (used && pos < min(q.length, p.max_seqlen_k) && (pos >> a.shift) < c.width) {
+        if (used && pos < min(lane_q.length, p.max_seqlen_k) && (pos >> a.shift) < c.width) {
           block = c.table[static_cast<int64_t>(u.r) * c.width + (pos >> a.shift)];
           row = pos & ((1 << a.shift) - 1);
           if (block < 0 || block >= c.num_blocks) block = -1;
@@ -328,12 +376,12 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             if (blocks[g] < 0) continue;
-            const int at = blocks[g] * c.h_k + hk_i;
+            const int at_block = blocks[g] * c.h_k + hk_i;
 #pragma unroll
             for (int x = 0; x < L::kHalves; ++x) {
               unsigned char* to = dst + x * kChunk * 128 + g * rows_per_copy * 128;
-              tma_load_4d(to, &map_k, &s_full[st], x * 128, rows[g], at, 0);
-              tma_load_4d(to + L::kTileBytes, &map_v, &s_full[st], x * 128, rows[g], at, 0);
+              tma_load_4d(to, &map_k, &s_full[st], x * 128, rows[g], at_block, 0);
+              tma_load_4d(to + L::kTileBytes, &map_v, &s_full[st], x * 128, rows[g], at_block, 0);
             }
           }
         }
@@ -374,9 +422,9 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   int st = 0;
   uint32_t phase = 0;
   int64_t w = w0;
-  while (w < w1) {
-    Request q;
-    const Unit u = units.at(w, q);
+  Request q;
+  for (Cursor at = units.at(w0, q); w < w1 && at.r < c.requests; units.advance(at, q)) {
+    const Unit u = units.of(at, q);
     const int64_t unit_end = max(u.start + u.n, w + 1);
     const int first = static_cast<int>(w - u.start), last = static_cast<int>(min(unit_end, w1) - u.start);
     const int row0 = u.tile * ROWS;
@@ -385,7 +433,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     if (nrows <= 0) continue;
     const int length = min(q.length, p.max_seqlen_k);
     // oldest key that not every row sees
-    const int sure = p.is_causal ? min(length, q.length - q.n + row0 / a.group + 1) : length;
+    const int sure = p.is_causal ? min(length, q.length - q.n + static_cast<int>(token_head(a, row0).x) + 1) : length;
 
     // queries: eight threads a row, to fp16 in the order of the fragments
     consumers_sync();
@@ -396,7 +444,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       float most = 0.f;
       const bool there = rr < nrows;
       const uint16_t* src = static_cast<const uint16_t*>(p.query);
-      if (there) src += static_cast<int64_t>(q.token0 + row / a.group) * p.query_row_stride + (u.hk * a.group + row % a.group) * p.query_head_stride;
+      const uint2 th = token_head(a, row);
+      if (there) src += static_cast<int64_t>(q.token0 + th.x) * p.query_row_stride + (u.hk * a.group + th.y) * p.query_head_stride;
 #pragma unroll
       for (int e = 0; e < E / 8; ++e) {
         const int at = (e * 8 + part) * 8;
@@ -440,10 +489,11 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
     }
     consumers_sync();
-    uint2 q_held[kQHeld ? L::kSteps : 1];
+    constexpr int kHeldSteps = kQHeld ? kTiles * L::kSteps : 1;
+    uint2 q_held[kHeldSteps];
     if (kQHeld) {
 #pragma unroll
-      for (int x = 0; x < (kQHeld ? L::kSteps : 1); ++x) q_held[x] = lds64(q_at + x * 256);
+      for (int x = 0; x < kHeldSteps; ++x) q_held[x] = lds64(q_at + x * 256);
     }
 
     // of queries 8 tile + 2 t, + 1: sums over the values (elements 32 j + 4 g + 2 half + {0: [0, 1], 1: [2, 3]}), maximum, this lane's
@@ -459,8 +509,9 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         l[nt][e] = 0.f;
         const int rr = min(8 * nt + 2 * t + e, nrows - 1), row = row0 + rr;
         row_scale[nt][e] = s_row_scale[rr];
-        newest[nt][e] = p.is_causal ? min(length - 1, q.length - q.n + row / a.group) : length - 1;
-        const int head = u.hk * a.group + row % a.group;
+        const uint2 th = token_head(a, row);
+        newest[nt][e] = p.is_causal ? min(length - 1, q.length - q.n + static_cast<int>(th.x)) : length - 1;
+        const int head = u.hk * a.group + th.y;
         bias_row[nt][e] = p.bias ? static_cast<const uint16_t*>(p.bias) + u.r * p.bias_batch_stride +
                                        (p.h_bias == p.h ? head : p.h_bias == c.h_k ? u.hk : 0) * p.bias_head_stride
                                  : nullptr;
@@ -585,7 +636,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           const uint32_t a0 = e4m3x2_to_f16x2(wa[x]), a1 = e4m3x2_to_f16x2(wb[x]), a2 = e4m3x2_hi_to_f16x2(wa[x]), a3 = e4m3x2_hi_to_f16x2(wb[x]);
 #pragma unroll
           for (int nt = 0; nt < kTiles; ++nt) {
-            const uint2 f = kQHeld ? q_held[kQHeld ? jj * 4 + x : 0] : lds64(q_at + (nt * L::kSteps + jj * 4 + x) * 256);
+            const int step = nt * L::kSteps + jj * 4 + x;
+            const uint2 f = kQHeld ? q_held[kQHeld ? step : 0] : lds64(q_at + step * 256);
             mma_f16(s[nt], a0, a1, a2, a3, f.x, f.y);
           }
         }
@@ -762,8 +814,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         if (rr >= nrows) continue;
         if (complete) {
           const float inv = l[nt][e] == 0.f ? 0.f : 1.f / l[nt][e];
-          uint16_t* dst = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(q.token0 + row / a.group) * p.out_row_stride +
-                          (u.hk * a.group + row % a.group) * p.out_head_stride;
+          const uint2 th = token_head(a, row);
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(q.token0 + th.x) * p.out_row_stride + (u.hk * a.group + th.y) * p.out_head_stride;
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const int dd = 32 * j + 4 * g;
@@ -816,10 +868,9 @@ __global__ void __launch_bounds__(1024) cache_sums_kernel(const __grid_constant_
 // Joins the sums of units that several CTAs share, and writes the zeros of rows that nobody computes: a CTA per (token, head),
 // whose warps take a quarter of the sums each.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(128, D > 128 ? 6 : 10) cache_merge_kernel(const __grid_constant__ AttnArgs a) {
   const fdma_cache_attention_params& p = a.p;
   const fdma_cache& c = p.c;
-  __shared__ Held s_held;
   __shared__ int s_request;
   __shared__ float s_top[4], s_sum[4], s_acc[4][D];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -829,6 +880,8 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant_
     r = slot / (kPromptTokens - 1);
     token = max(0, c.cu_seqlens[r]) + slot - r * (kPromptTokens - 1);
     end = min(c.cu_seqlens[r + 1], c.tokens);
+  } else if (token < c.requests && c.cu_seqlens[token] == token && c.cu_seqlens[token + 1] == token + 1) {
+    r = token;  // one token each
   } else {
     if (tid == 0) s_request = -1;
     __syncthreads();
@@ -837,26 +890,27 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const __grid_constant_
     __syncthreads();
     r = s_request;
   }
-  const Units units = make_units(a, s_held);
-  const int64_t total = units.total(), share = share_of(total, a.ctas);
-  const int64_t step = static_cast<int64_t>(a.rows) * (D + 4);
+  const Units units{a, nullptr};
+  const int64_t step = (static_cast<int64_t>(D) + 4) << a.row_shift;
   Request q{};
   if (r >= 0) q = units.request(r);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (q.rows < 0) return;  // done already
+  const int64_t share = share_of(units.total(), a.ctas);
   for (; token < end; token += kPromptTokens - 1) {
     int c0 = 0, c1 = -1;
     const float* base = nullptr;
-    const int row = (token - q.token0) * a.group + head % a.group, tile = row / a.rows;
+    const uint2 kv = token_head(a, head);  // kv head, and the head among those that share it
+    const int row = (token - q.token0) * a.group + kv.y, tile = row >> a.row_shift;
     if (r >= 0 && row >= 0 && row < q.rows) {
-      const Unit u = units.of(r, q, head / a.group, tile);
-      c0 = static_cast<int>(u.start / share);
-      c1 = static_cast<int>((u.start + u.n - 1) / share);
-      base = a.partial + static_cast<int64_t>(row - tile * a.rows) * (D + 4);
+      const Unit u = units.of(Cursor{r, static_cast<int>(kv.x), tile}, q);
+      c0 = static_cast<int>(quotient(u.start, share));
+      c1 = static_cast<int>(quotient(u.start + u.n - 1, share));
+      base = a.partial + static_cast<int64_t>(row - (tile << a.row_shift)) * (D + 4);
       if (c0 == c1) continue;  // written by that CTA
     }
-    // each warp takes every fourth sum, eight at a time, and scales to its own maximum
-    constexpr int E = D / 32, kAhead = D > 128 ? 4 : 8;  // elements per lane
+    // each warp takes every fourth sum, four at a time, and scales to its own maximum
+    constexpr int E = D / 32, kAhead = 4;  // elements per lane
     float acc[E], sum = 0.f, top = -CUDART_INF_F;
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = 0.f;
@@ -944,7 +998,7 @@ Plan plan_of(const fdma_cache_attention_params& p) {
   const int64_t tiles = static_cast<int64_t>(p.c.tokens) * (p.h / p.c.h_k) / pl.rows + p.c.requests;
   pl.most_chunks = tiles * (pl.list_chunks ? pl.list_chunks : (static_cast<int64_t>(p.c.width) * p.c.block_size + kChunk - 1) / kChunk);
   pl.sums_off = align256(static_cast<size_t>(pl.ctas) * 2 * pl.rows * (pl.D + 4) * sizeof(float));
-  pl.prompt_off = pl.sums_off + (pl.sums ? align256((static_cast<size_t>(p.c.requests) + 1) * sizeof(int32_t)) : 0);
+  pl.prompt_off = pl.sums_off + align256((static_cast<size_t>(p.c.requests) + 1) * sizeof(int32_t));
   pl.bytes = pl.prompt_off + (pl.prompts ? cache_prompt_workspace_bytes(p) : 0);
   return pl;
 }
@@ -1027,7 +1081,11 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   a.p = p;
   a.shift = p.c.block_size == 16 ? 4 : p.c.block_size == 32 ? 5 : p.c.block_size == 64 ? 6 : 7;
   a.group = p.h / p.c.h_k;
-  a.rows = pl.rows;
+  a.row_shift = pl.rows == 8 ? 3 : 4;
+  auto inverse = [](int x) { return static_cast<uint32_t>(std::min<uint64_t>((uint64_t{1} << 32) / x, 0xFFFFFFFFu)); };
+  a.group_inverse = inverse(a.group);
+  a.h_k_inverse = inverse(p.c.h_k);
+  a.p.max_seqlen_q = std::max(a.p.max_seqlen_q, 1);
   a.list_chunks = pl.list_chunks;
   a.ctas = pl.ctas;
   a.scale_log2 = p.softmax_scale * kLog2e;
@@ -1041,13 +1099,13 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
     if (status) return status;
     a.prompts = reinterpret_cast<const int32_t*>(static_cast<char*>(p.workspace) + pl.prompt_off + cache_prompt_keys(p));
   }
-  a.pre = p.c.cu_chunks;
+  a.pre = reinterpret_cast<int32_t*>(static_cast<char*>(p.workspace) + pl.sums_off);
   if (pl.sums) {
-    int32_t* pre = reinterpret_cast<int32_t*>(static_cast<char*>(p.workspace) + pl.sums_off);
-    cache_sums_kernel<<<1, 1024, 0, stream>>>(a, pre);
+    cache_sums_kernel<<<1, 1024, 0, stream>>>(a, a.pre);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return static_cast<int>(e);
-    a.pre = pre;
+  } else if (p.c.requests > kHeld) {  // a tile for each request: their chunks
+    a.pre = const_cast<int32_t*>(p.c.cu_chunks);
   }
   if (pl.D == 256) return pl.rows == 8 ? launch_t<256, 8>(a, pl, stream) : launch_t<256, 16>(a, pl, stream);
   if (pl.D == 128) return pl.rows == 8 ? launch_t<128, 8>(a, pl, stream) : launch_t<128, 16>(a, pl, stream);
