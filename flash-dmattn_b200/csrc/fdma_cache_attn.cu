@@ -262,7 +262,7 @@ struct Layout {
   static constexpr int kHalves = D > 128 ? 2 : 1;                   // 128-byte tiles side by side
   static constexpr int kTileBytes = kChunk * 128 * kHalves;         // K or V of a chunk
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = D > 128 ? 2 : 3;
+  static constexpr int kStages = D > 128 ? 2 : ROWS > 8 ? 4 : 3;
   static constexpr int kSteps = D / 16;                             // k steps of Q K^T
   static constexpr int kQBytes = ROWS / 8 * kSteps * 256;
   static constexpr int kBufFloats = ROWS * D;                       // one warp's sums
@@ -272,7 +272,9 @@ struct Layout {
   static constexpr int kBuf = kQ + kQBytes;
   static constexpr int kTotal = kBuf + kBufs * kBufFloats * 4 + 1024;
   static constexpr int kThreads = kWarps * 32 + (kGather ? 0 : 32);
-  static constexpr int kCtas = D > 128 ? 2 : 3;                     // per SM
+  // Per SM. Three with 16 rows, at 128 registers, spill: 8 requests of up to 65536 tokens, 4 new ones each, 32 heads over 8, d = 128:
+  // 105 us, two 93.
+  static constexpr int kCtas = D > 128 || ROWS > 8 ? 2 : 3;
 };
 
 template <int D, int ROWS, bool kGather, bool kBf16>
@@ -868,7 +870,7 @@ __global__ void __launch_bounds__(1024) cache_sums_kernel(const __grid_constant_
 // Joins the sums of units that several CTAs share, and writes the zeros of rows that nobody computes: a CTA per (token, head),
 // whose warps take a quarter of the sums each.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(128, D > 128 ? 6 : 10) cache_merge_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const __grid_constant__ AttnArgs a) {
   const fdma_cache_attention_params& p = a.p;
   const fdma_cache& c = p.c;
   __shared__ int s_request;
@@ -909,8 +911,8 @@ __global__ void __launch_bounds__(128, D > 128 ? 6 : 10) cache_merge_kernel(cons
       base = a.partial + static_cast<int64_t>(row - (tile << a.row_shift)) * (D + 4);
       if (c0 == c1) continue;  // written by that CTA
     }
-    // each warp takes every fourth sum, four at a time, and scales to its own maximum
-    constexpr int E = D / 32, kAhead = 4;  // elements per lane
+    // each warp takes every fourth sum, six at a time, and scales to its own maximum
+    constexpr int E = D / 32, kAhead = 6;  // elements per lane
     float acc[E], sum = 0.f, top = -CUDART_INF_F;
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = 0.f;
@@ -991,8 +993,10 @@ Plan plan_of(const fdma_cache_attention_params& p) {
   pl.prompts = cache_prompt_taken(p);
   const int64_t most = static_cast<int64_t>(std::min(p.max_seqlen_q, p.c.tokens)) * (p.h / p.c.h_k);
   pl.D = tile_dim(p.c.d);
-  pl.rows = most <= 8 ? 8 : 16;
-  pl.ctas = (pl.D == 256 ? 2 : 3) * sm_count();
+  // (at head dim 256, two tiles of 8 rows that read the same keys one after the other are faster than one of 16, whose accumulators
+  // do not fit: 8 requests of 16384 tokens, 4 new ones each, 32 heads over 8: 59 us against 70)
+  pl.rows = most <= 8 || pl.D == 256 ? 8 : 16;
+  pl.ctas = (pl.D == 256 || pl.rows > 8 ? 2 : 3) * sm_count();
   pl.list_chunks = p.kept_pos ? (p.kept_capacity + kChunk - 1) / kChunk : 0;
   pl.sums = p.c.requests > kHeld && (pl.list_chunks || most > pl.rows);
   const int64_t tiles = static_cast<int64_t>(p.c.tokens) * (p.h / p.c.h_k) / pl.rows + p.c.requests;
@@ -1107,7 +1111,7 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   } else if (p.c.requests > kHeld) {  // a tile for each request: their chunks
     a.pre = const_cast<int32_t*>(p.c.cu_chunks);
   }
-  if (pl.D == 256) return pl.rows == 8 ? launch_t<256, 8>(a, pl, stream) : launch_t<256, 16>(a, pl, stream);
+  if (pl.D == 256) return launch_t<256, 8>(a, pl, stream);
   if (pl.D == 128) return pl.rows == 8 ? launch_t<128, 8>(a, pl, stream) : launch_t<128, 16>(a, pl, stream);
   return pl.rows == 8 ? launch_t<64, 8>(a, pl, stream) : launch_t<64, 16>(a, pl, stream);
 }
