@@ -47,23 +47,31 @@ __device__ __forceinline__ uint32_t pack_scaled(uint16_t two, float scale) {
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant__ UnpackArgs a) {
   extern __shared__ int s_pre[];  // chunks, then rows, of the requests before
-  __shared__ long long s_warp[kThreads / 32];
-  __shared__ int s_block[4], s_tokens[kThreads / 32];
+  __shared__ long long s_warp[kThreads / 32], s_pairs[kThreads / 32];
+  __shared__ int s_block[4], s_longest[kThreads / 32];
   const fdma_cache& c = a.c;
   const int R = c.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int *pre_chunks = s_pre, *pre_rows = s_pre + R + 1;
-  long long carry = 0, tokens = 0;  // carry: rows << 32 | chunks
+  long long carry = 0, pairs = 0;  // carry: rows << 32 | chunks; pairs: of a new token and a key, see prompt_pays
+  int longest = 0;
   for (int base = 0; base < R; base += kThreads) {
     const int r = base + tid;
     long long x = 0;
-    int mine = 0;
+    long long my_pairs = 0;
+    int my_length = 0;
     if (r < R && c.cu_chunks[r + 1] > c.cu_chunks[r] && c.cu_seqlens[r + 1] - c.cu_seqlens[r] >= kPromptTokens) {
       const int n = max(0, min(min(c.lengths[r], a.max_keys), c.width << a.shift));
       x = (static_cast<long long>(n) << 32) | ((n + kChunk - 1) / kChunk);
-      mine = c.cu_seqlens[r + 1] - c.cu_seqlens[r];
+      my_length = n;
+      my_pairs = static_cast<long long>(n + kTileKeys) * (c.cu_seqlens[r + 1] - c.cu_seqlens[r]);
     }
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) s_tokens[warp] = mine;
+    my_length = __reduce_max_sync(0xffffffffu, my_length);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) my_pairs += __shfl_xor_sync(0xffffffffu, my_pairs, o);
+    if (lane == 0) {
+      s_pairs[warp] = my_pairs;
+      s_longest[warp] = my_length;
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long y = __shfl_up_sync(0xffffffffu, x, o);
@@ -75,7 +83,8 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
     for (int i = 0; i < kThreads / 32; ++i) {
       if (i < warp) before += s_warp[i];
       carry += s_warp[i];
-      tokens += s_tokens[i];
+      pairs += s_pairs[i];
+      longest = max(longest, s_longest[i]);
     }
     x += before;
     if (r < R) {
@@ -86,7 +95,8 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
   }
   if (tid == 0) pre_chunks[0] = pre_rows[0] = 0;
   __syncthreads();
-  const bool taken = tokens * a.heads >= prompt_work(c.d);
+  const int total_rows = pre_rows[R];
+  const bool taken = total_rows > 0 && prompt_pays(pairs * a.heads, longest, c.d);
   if (blockIdx.x == 0)
     for (int r = tid; r <= R; r += kThreads) a.cu_k[r] = taken ? pre_rows[r] : 0;
   const int total = taken ? pre_chunks[R] : 0;
@@ -173,7 +183,9 @@ fdma_fwd_params forward_params(const fdma_cache_attention_params& p, char* ws) {
 }  // namespace
 
 bool cache_prompt_taken(const fdma_cache_attention_params& p) {
-  if (std::min(p.max_seqlen_q, p.c.tokens) < kPromptTokens || static_cast<int64_t>(p.c.tokens) * p.h < prompt_work(p.c.d) || p.bias || p.kept_pos || p.c.requests > 8192) return false;
+  if (std::min(p.max_seqlen_q, p.c.tokens) < kPromptTokens || p.bias || p.kept_pos || p.c.requests > 8192) return false;
+  const int64_t keys = std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size);
+  if (!prompt_pays(static_cast<int64_t>(p.c.tokens) * p.h * (keys + kTileKeys), keys, p.c.d)) return false;
   const int64_t rows = most_rows(p);
   if (rows <= 0 || rows > kMostRows || scratch(p).total > static_cast<size_t>(kMostBytes)) return false;
   if (p.c.tokens > (1 << 19)) return false;

@@ -110,12 +110,14 @@ int create_mask(const fdma_mask_params& p, cudaStream_t stream);
 
 // ---- attention over the 8-bit cache ---------------------------------------------------------------
 // Requests with kPromptTokens or more new tokens have their keys converted to 16 bits once, for the tensor-core forward kernel
-// (fdma_cache_prompt.cu), if these are prompt_work() tokens x query heads in all; otherwise keys are read for 16 rows of queries at a
-// time (fdma_cache_attn.cu). The former needs 17 us per 1000 keys however few its CTAs are, the latter's time grows with the rows;
-// 32 heads over 8, d = 128, 32000 keys: 4 x 32 tokens 672 against 411 us, 4 x 64 672 against 803, 4 x 128 676 against 1650;
-// 16 heads over 1, d = 256: 4 x 64 tokens 715 against 750.
-constexpr int kPromptTokens = 32;
-__host__ __device__ inline int prompt_work(int d) { return d > 128 ? 4096 : 6144; }
+// (fdma_cache_prompt.cu), if there is enough work for it; otherwise keys are read for 16 rows of queries at a time
+// (fdma_cache_attn.cu). The former takes about 37 us and 17 us per 1000 keys, however few its CTAs are; the latter 14 us and 3.1 us for a
+// million tokens x heads x keys, a tile's beginning and end counting as 800 keys, and 15 us for having tried. 32 heads over 8, d =
+// 128, former and latter: 32000 keys, 4 x 32 tokens 672, 411 us; 4 x 64 672, 803; 1000 keys, 4 x 64 tokens 66, 68; 4 x 128 76, 115;
+// 8 heads over 2, 8 x up to 244 tokens over 43 41, 56; d = 256, 16 heads over 1, 32000 keys, 4 x 64 tokens 715, 750.
+constexpr int kPromptTokens = 32, kTileKeys = 800;
+// work: sum of tokens x heads x (keys + kTileKeys)
+__host__ __device__ inline bool prompt_pays(int64_t work, int64_t longest, int d) { return work >= 2600000 + (d > 128 ? 3700 : 5500) * longest; }
 int check_cache(const fdma_cache& c);
 // Whether the call may have such requests, and scratch and layouts for them. Then cache_prompt writes all rows, those of other
 // requests 0; what the device has found is at cache_prompt_keys in the scratch: the number of converted keys, 0 if the requests have
