@@ -83,6 +83,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Sets the NaN among four e4m3 numbers to 0; whether there was one.
+__device__ __forceinline__ uint32_t drop_nan(uint32_t& x) {
+  const uint32_t nan = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+  x &= ~((nan >> 7) * 0xFFu);
+  return nan != 0;
+}
 // An 8 x 8 matrix of 16-bit numbers, a row per four lanes, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -669,6 +675,35 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           grows |= v > m[nt][k & 1];
         }
       }
+      uint32_t poisoned = 0;  // scores, a bit each, whose value is NaN
+      if (!clean || with_bias) {
+        uint32_t seen = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * kTiles; ++i) seen |= static_cast<uint32_t>(x[i >> 2][i & 3] != -CUDART_INF_F) << i;
+        // Values that some query does not see must not reach it, which 0 times NaN would: NaN become 0 where they are, and who sees
+        // them gets NaN otherwise. What lies behind the last key may be anything, and becomes 0.
+        if (__any_sync(0xffffffffu, seen != (1u << (4 * kTiles)) - 1)) {
+          uint32_t nan_rows = 0;
+          const int there = kGather ? kSlice : meta.x != 0.f ? min(max(length - pos0, 0), kSlice) : 0;
+          for (int i = 0; i < 4 * L::kHalves; ++i) {
+            const int r = (i & 3) * 4 + (lane >> 3);
+            const uint32_t at = tile + L::kTileBytes + (i >> 2) * kChunk * 128 + r * 128 + (lane & 7) * 16;
+            uint4 v = lds128(at);
+            const bool used = D >= 128 || ((lane & 7) ^ (r & 7)) < D / 16;  // a row of 128 bytes may be half empty
+            const bool nan = (drop_nan(v.x) | drop_nan(v.y) | drop_nan(v.z) | drop_nan(v.w)) && r < there && used;
+            if (r >= there) v = make_uint4(0, 0, 0, 0);
+            if (nan || r >= there) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            const uint32_t lanes = __ballot_sync(0xffffffffu, nan);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) nan_rows |= static_cast<uint32_t>((lanes >> (8 * k) & 0xFF) != 0) << ((i & 3) * 4 + k);
+          }
+          fence_proxy_async_smem();  // before the next copy into this stage
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4 * kTiles; ++i)
+            if (nan_rows >> ((i >> 1 & 1) * 8 + key) & 1) poisoned |= seen & 1u << i;
+        }
+      }
       if (__any_sync(0xffffffffu, grows)) {  // a query's maxima are compared over its keys only when one of them grows
 #pragma unroll
         for (int nt = 0; nt < kTiles; ++nt) {
@@ -702,24 +737,22 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           l[nt][0] = fmaf(e[0] + e[2], meta.w, l[nt][0]);
           l[nt][1] = fmaf(e[1] + e[3], meta.w, l[nt][1]);
         }
+        if (poisoned) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (poisoned >> (nt * 4 + k) & 1) l[nt][k & 1] = CUDART_NAN_F;
+        }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float f = p_scale(kGather ? key_meta[k].z : meta.z);
           pb[nt][k] = transpose8(pack_f16(e[2 * k] * f, e[2 * k + 1] * f));
         }
       }
-      const bool whole = kGather || (pos0 + kSlice <= length && meta.x != 0.f);
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
         const uint32_t half = tile + (j >> 2) * kChunk * 128;
         const uint32_t at0 = half + (v_at0 ^ ((j & 3) << 5)), at1 = half + (v_at1 ^ ((j & 3) << 5));
-        uint32_t y0 = lds32<0>(at0), y1 = lds32<0>(at1), y2 = lds32<1024>(at0), y3 = lds32<1024>(at1);
-        if (!whole) {  // what lies behind the last key may be anything
-          if (meta.x == 0.f || pos0 + r0 >= length) y0 = 0;
-          if (meta.x == 0.f || pos0 + r1 >= length) y1 = 0;
-          if (meta.x == 0.f || pos0 + 8 + r0 >= length) y2 = 0;
-          if (meta.x == 0.f || pos0 + 8 + r1 >= length) y3 = 0;
-        }
+        const uint32_t y0 = lds32<0>(at0), y1 = lds32<0>(at1), y2 = lds32<1024>(at0), y3 = lds32<1024>(at1);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // bytes 0, 1 | 2, 3 of the words: rows g | g + 8 of the product
           const uint32_t first = __byte_perm(y0, y1, h ? 0x7362 : 0x5140), second = __byte_perm(y2, y3, h ? 0x7362 : 0x5140);

@@ -447,6 +447,35 @@ def test_not_a_number_stays_in_its_request(dev):
     assert torch.equal(got[1:3, :2, others], want[1:3, :2, others])
 
 
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("H,n,d,bs", [(2, 3, 64, 16), (8, 6, 128, 64), (16, 5, 256, 32)])
+def test_not_a_number_is_not_seen_through_a_mask(dev, kept, H, n, d, bs):
+    """Values and keys that are NaN at a later token of a draft, or behind a bias of -inf, leave the queries that do not see them as
+    they are; those that do become NaN."""
+    tables, cache, step, g = filled(dev, 2, [100, 61], [n, n], 2, d, bs, 19)
+    kv = torch.randn((2, 2 * n, 2, d), generator=g, device=dev, dtype=torch.bfloat16)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    q = torch.randn((2 * n, H, d), generator=g, device=dev, dtype=torch.bfloat16)
+    bias = torch.zeros((2, 2, 1, 128), device=dev, dtype=torch.bfloat16)
+    bias[0, :, :, 40:60] = -math.inf
+    keep = None
+    if kept:
+        keep = fsa.KeptKeys(torch.arange(128, dtype=torch.int32, device=dev).expand(2, 2, 128).contiguous(), ints([[128, 128]] * 2, dev), None, 128)
+    args = dict(attn_mask=keep, attn_bias=bias, max_seqlen_q=n)
+    want = fsa.flash_sparse_attn_cache_func(q, cache, tables, step, **args)
+    at = step.slots[[n - 1, 2 * n - 2]].tolist()  # the last token of one request, the last but one of the other
+    for slot, x in zip(at, (cache.v, cache.k)):
+        x.view(torch.uint8)[slot // bs, 0, slot % bs, 5] = 0xFF
+    hidden = tables.table[0, 40 // bs:60 // bs + 1].tolist()
+    for pos in range(40, 60):
+        cache.v.view(torch.uint8)[hidden[pos // bs - 40 // bs], :, pos % bs] = 0x7F
+    got = fsa.flash_sparse_attn_cache_func(q, cache, tables, step, **args)
+    G = H // 2
+    assert torch.equal(got[:n - 1], want[:n - 1]) and torch.equal(got[n:2 * n - 2], want[n:2 * n - 2])
+    assert torch.equal(got[n - 1, G:], want[n - 1, G:]) and torch.equal(got[2 * n - 2:, G:], want[2 * n - 2:, G:])
+    assert bool(got[n - 1, :G, 5].isnan().all()) and bool(got[2 * n - 2:, :G].isnan().all())
+
+
 def test_refused_and_padded_tokens_are_zero(dev):
     tables = fsa.block_tables(4, 3, 4, 16, device=dev)
     cache = fsa.quantized_cache(4, 1, 64, 16, device=dev)
