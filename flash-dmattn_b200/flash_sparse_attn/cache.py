@@ -38,7 +38,8 @@ class CacheStep(NamedTuple):
 
 
 class BlockTables(NamedTuple):
-    """Which blocks of a cache each request holds. The tensors live on the GPU and are updated in place, in stream order."""
+    """Which blocks of a cache each request holds, a block one request. The tensors live on the GPU and are updated in place, in stream
+    order; two calls on the same tables must not run at once."""
 
     table: torch.Tensor       # int32 (requests, blocks per request): a request's blocks in order, -1 behind them
     lengths: torch.Tensor     # int32 (requests,): tokens that each request holds
@@ -166,10 +167,12 @@ def flash_sparse_attn_cache_func(
     a `KeptKeys` ({1|requests}, {1|Hk}) or a bool tensor ({1|requests}, {1|Hk}, 1, keys), False or beyond its keys = masked out.
     attn_bias ({1|requests}, {1|Hk|H}, 1, keys), dtype of query, added to the scaled scores; 0 beyond its keys. softmax_scale
     defaults to d ** -0.5. max_seqlen_q, max_seqlen_k: bounds on the new tokens and on the length of any request, where the
-    host knows them (default: the step's tokens, the tables' width); what lies beyond a bound is not looked at. They help to choose
-    how the work is split.
+    host knows them (default: the step's tokens, the tables' width); what lies beyond a bound may be left out. They choose how the
+    work is split and how much scratch a call takes: pass them where you can.
 
-    Returns (tokens, H, d). Rows of tokens behind the last request, of refused requests and of queries that see no key are 0.
+    Returns (tokens, H, d). Rows of tokens behind the last request, of refused requests and of queries that see no key are 0. A key or
+    value that is NaN reaches the queries that see it (of a request with 32 or more new tokens, earlier ones of its tile as well) and no
+    other request.
     Scores, probabilities' sums and outputs are accumulated in 32 bits; probabilities enter the second product in 16 bits.
     There are no gradients: a call that would need them raises."""
     args = _cache_args(cache, tables, step)

@@ -5,7 +5,7 @@ from typing import Optional
 
 import torch
 
-from .modeling_flash_sparse_attention_utils import _flash_sparse_attention_forward
+from .modeling_flash_sparse_attention_utils import _cached_attention_forward, _flash_sparse_attention_forward
 
 
 def _half_dtype_of(module: torch.nn.Module) -> Optional[torch.dtype]:
@@ -34,6 +34,8 @@ def flash_sparse_attention_forward(
     softcap: Optional[float] = None,
     **kwargs,
 ):
+    """kv_cache (keyword, not in the reference): the layer's `CachedLayer`; query, key and value are then the step's new tokens
+    (1, H, tokens, d) of all requests, attention_bias is ({1|requests}, {1|Hk|H}, 1, keys), and attention runs over the 8-bit cache."""
     query_len, key_len = query.shape[2], key.shape[2]
     if any(dim == 0 for dim in query.shape):
         raise ValueError("FlashSparseAttention does not support inputs with a zero dimension; check the input "
@@ -45,6 +47,12 @@ def flash_sparse_attention_forward(
         is_causal = module.is_causal
     for dropped in ("output_attentions", "head_mask"):  # not supported by the fused path, as in the reference
         kwargs.pop(dropped, None)
+    kv_cache = kwargs.pop("kv_cache", None)
+    if kv_cache is not None:
+        if softcap:
+            raise NotImplementedError("softcap > 0 is not built into the B200 kernels")
+        return _cached_attention_forward(query, key, value, attention_mask, attention_bias, kv_cache, softmax_scale=scaling,
+                                         window_size=window_size, is_causal=is_causal, target_dtype=target_dtype), None
     out = _flash_sparse_attention_forward(
         query, key, value, attention_mask, attention_bias,
         query_length=query_len, key_length=key_len, is_causal=is_causal, softmax_scale=scaling, softcap=softcap,

@@ -17,12 +17,14 @@ alignment of its own lengths), which the full-range kernels skip tile by tile --
 there are; larger packs go through `flash_sparse_attn_varlen_func`, which runs every example as a zero-copy slice.
 """
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
+from ..cache import BlockTables, CacheStep, QuantizedCache, cache_append, flash_sparse_attn_cache_func
 from ..flash_sparse_attn_interface import flash_sparse_attn_func, flash_sparse_attn_varlen_func
-from ..utils.mask import create_mask
+from ..rotary import RotaryFrequencies
+from ..utils.mask import create_kept_keys, create_mask
 
 
 def fsa_peft_integration_check(q, k, v, bias, target_dtype: Optional[torch.dtype] = None):
@@ -155,3 +157,39 @@ def _flash_sparse_attention_forward(
         softmax_scale=softmax_scale, is_causal=is_causal and query_length != 1,
         softcap=softcap, deterministic=deterministic)
     return out[0] if isinstance(out, tuple) else out
+
+
+class CachedLayer(NamedTuple):
+    """What a layer needs to attend over the paged 8-bit cache in a step."""
+
+    cache: QuantizedCache                             # the layer's own
+    tables: BlockTables                               # of all layers
+    step: CacheStep                                   # of this step, from `tables.extend`
+    frequencies: Optional[RotaryFrequencies] = None   # query and key are turned here; None: they are already
+    max_seqlen_q: Optional[int] = None                # bounds on the requests' new tokens and lengths, where the host knows them
+    max_seqlen_k: Optional[int] = None
+
+
+def _cached_attention_forward(query_states, key_states, value_states, attention_mask, attention_bias, kv_cache: CachedLayer,
+                              softmax_scale: Optional[float] = None, window_size: Optional[int] = None, is_causal: bool = True,
+                              target_dtype: Optional[torch.dtype] = None):
+    """The step's keys and values (1, tokens, Hk, d) go into the cache, and its queries (1, tokens, H, d) attend over it: everything, or
+    with a bias of more than `window_size` keys the `window_size` keys of each request and kv head that it ranks highest. Returns
+    (1, tokens, H, d)."""
+    if attention_mask is not None:
+        raise ValueError("attention over a cache takes no attention_mask: the requests' lengths are in the step.")
+    if query_states.shape[0] != 1 or key_states.shape[0] != 1:
+        raise ValueError("attention over a cache takes the step's tokens as one row.")
+    q, k, v, bias = fsa_peft_integration_check(query_states[0], key_states[0], value_states[0], attention_bias, target_dtype)
+    cache, tables, step, frequencies, max_q, max_k = kv_cache
+    turned = cache_append(cache, tables, step, k, v, query=q if frequencies is not None else None, frequencies=frequencies)
+    q = q if turned is None else turned
+    kept = None
+    if bias is not None and window_size is not None and bias.shape[-1] > window_size:
+        keys = bias.shape[-1]
+        valid = torch.arange(keys, device=bias.device) < step.lengths[:, None]
+        kept = create_kept_keys(bias.expand(step.lengths.shape[0], -1, -1, -1), valid, step.lengths.shape[0], 1, keys, window_size,
+                                torch.finfo(bias.dtype).min)
+    out = flash_sparse_attn_cache_func(q, cache, tables, step, attn_mask=kept, attn_bias=bias, softmax_scale=softmax_scale,
+                                       is_causal=is_causal, max_seqlen_q=max_q, max_seqlen_k=max_k)
+    return out[None]
