@@ -665,10 +665,13 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             float add = km.x;
             if (head_bias && pos >= 0 && pos < p.bias_keys) add = bias_log2(raw_to_f<kBf16>(__ldg(bias_row[nt][k & 1] + pos)));
             v = fmaf(s[nt][k], row_scale[nt][k & 1] * km.y, add) + km.z;
-            if (pos < 0 || pos > newest[nt][k & 1]) v = -CUDART_INF_F;
+            if (add == -CUDART_INF_F || pos > newest[nt][k & 1]) v = -CUDART_INF_F;  // even where the key is NaN
           } else {
             v = s[nt][k] * (row_scale[nt][k & 1] * meta.y);
-            if (with_bias) v += bias_log2(raw_to_f<kBf16>(raw_bias[nt][k >> 1][k & 1]));
+            if (with_bias) {
+              const float add = bias_log2(raw_to_f<kBf16>(raw_bias[nt][k >> 1][k & 1]));
+              v = add == -CUDART_INF_F ? add : v + add;
+            }
             v += meta.z;
             if (!clean && (pos0 + (k >> 1) * 8 + key > newest[nt][k & 1] || meta.x == 0.f)) v = -CUDART_INF_F;
           }
@@ -1024,7 +1027,7 @@ struct Plan {
 Plan plan_of(const fdma_cache_attention_params& p) {
   Plan pl;
   pl.prompts = cache_prompt_taken(p);
-  const int64_t most = static_cast<int64_t>(std::min(p.max_seqlen_q, p.c.tokens)) * (p.h / p.c.h_k);
+  const int64_t most = static_cast<int64_t>(std::max(std::min(p.max_seqlen_q, p.c.tokens), 1)) * (p.h / p.c.h_k);
   pl.D = tile_dim(p.c.d);
   // (at head dim 256, two tiles of 8 rows that read the same keys one after the other are faster than one of 16, whose accumulators
   // do not fit: 8 requests of 16384 tokens, 4 new ones each, 32 heads over 8: 59 us against 70)

@@ -476,6 +476,37 @@ def test_not_a_number_is_not_seen_through_a_mask(dev, kept, H, n, d, bs):
     assert bool(got[n - 1, :G, 5].isnan().all()) and bool(got[2 * n - 2:, :G].isnan().all())
 
 
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("heads", [1, 2, 4])
+def test_not_a_number_in_a_key_is_not_seen_through_a_bias(dev, kept, heads):
+    tables, cache, step, g = filled(dev, 2, [100, 61], [1, 1], 2, 64, 16, 23)
+    kv = torch.randn((2, 2, 2, 64), generator=g, device=dev, dtype=torch.bfloat16)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    q = torch.randn((2, 4, 64), generator=g, device=dev, dtype=torch.bfloat16)
+    bias = torch.randn((2, heads, 1, 128), generator=g, device=dev, dtype=torch.bfloat16)
+    bias[:, :, :, 16:48] = -math.inf
+    keep = None
+    if kept:
+        keep = fsa.KeptKeys(torch.arange(128, dtype=torch.int32, device=dev).expand(2, 2, 128).contiguous(), ints([[128, 128]] * 2, dev), None, 128)
+    want = fsa.flash_sparse_attn_cache_func(q, cache, tables, step, keep, bias)
+    for block in tables.table[:, 1:3].flatten().tolist():
+        cache.k.view(torch.uint8)[block] = 0x7F
+        cache.v.view(torch.uint8)[block] = 0xFF
+    got = fsa.flash_sparse_attn_cache_func(q, cache, tables, step, keep, bias)
+    assert bool(want.isfinite().all()) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("bound", [0, 1])
+def test_a_bound_of_no_tokens_is_one_of_one(dev, bound):
+    """More requests than a CTA holds, and more heads per kv head than a tile has rows."""
+    requests, H, d = 130, 16, 64
+    tables, cache, step, g = filled(dev, requests, [(37 * r) % 150 for r in range(requests)], [1] * requests, 1, d, 16, 24)
+    kv = torch.randn((2, requests, 1, d), generator=g, device=dev, dtype=torch.float16)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    q = torch.randn((requests, H, d), generator=g, device=dev, dtype=torch.float16)
+    check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, max_seqlen_q=bound), *attend(q, cache, tables, step))
+
+
 def test_refused_and_padded_tokens_are_zero(dev):
     tables = fsa.block_tables(4, 3, 4, 16, device=dev)
     cache = fsa.quantized_cache(4, 1, 64, 16, device=dev)
@@ -699,6 +730,22 @@ def test_inference_mode(dev):
         check(fsa.flash_sparse_attn_cache_func(x, cache, tables, step), *attend(x, cache, tables, step))
         tables.truncate(ints([0], dev))
     assert tables.free_count.item() == 4
+
+
+def test_bool_masks_in_inference_mode(dev):
+    from flash_sparse_attn.utils.mask import create_kept_keys, create_mask
+
+    tables, cache, step, g = filled(dev, 2, [90, 40], [1, 1], 2, 64, 16, 25)
+    x = torch.randn((2, 4, 64), generator=g, device=dev, dtype=torch.bfloat16)
+    bias = torch.randn((2, 2, 1, 96), generator=g, device=dev, dtype=torch.bfloat16)
+    low = torch.finfo(bias.dtype).min
+    mask = create_mask(bias, None, 2, 1, 96, 32, low)
+    with torch.inference_mode():
+        kept = create_kept_keys(bias, None, 2, 1, 96, 32, low)
+        fsa.cache_append(cache, tables, step, x[:, :2], x[:, 2:])
+        got = [fsa.flash_sparse_attn_cache_func(x, cache, tables, step, m, bias) for m in (kept, mask, mask & True)]
+        check(got[0], *attend(x, cache, tables, step, kept, bias))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
 
 
 def test_compiled_step(dev):
