@@ -680,31 +680,39 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
       uint32_t poisoned = 0;  // scores, a bit each, whose value is NaN
       if (!clean || with_bias) {
-        uint32_t seen = 0;
+        float least = x[0][0];
 #pragma unroll
-        for (int i = 0; i < 4 * kTiles; ++i) seen |= static_cast<uint32_t>(x[i >> 2][i & 3] != -CUDART_INF_F) << i;
+        for (int i = 1; i < 4 * kTiles; ++i) least = fminf(least, x[i >> 2][i & 3]);
         // Values that some query does not see must not reach it, which 0 times NaN would: NaN become 0 where they are, and who sees
-        // them gets NaN otherwise. What lies behind the last key may be anything, and becomes 0.
-        if (__any_sync(0xffffffffu, seen != (1u << (4 * kTiles)) - 1)) {
-          uint32_t nan_rows = 0;
-          const int there = kGather ? kSlice : meta.x != 0.f ? min(max(length - pos0, 0), kSlice) : 0;
+        // them gets NaN otherwise. What lies behind the last key may be anything.
+        if (__any_sync(0xffffffffu, least == -CUDART_INF_F)) {
+          uint32_t found = 0;  // a bit for each of this lane's 16-byte pieces
+#pragma unroll
           for (int i = 0; i < 4 * L::kHalves; ++i) {
             const int r = (i & 3) * 4 + (lane >> 3);
             const uint32_t at = tile + L::kTileBytes + (i >> 2) * kChunk * 128 + r * 128 + (lane & 7) * 16;
             uint4 v = lds128(at);
-            const bool used = D >= 128 || ((lane & 7) ^ (r & 7)) < D / 16;  // a row of 128 bytes may be half empty
-            const bool nan = (drop_nan(v.x) | drop_nan(v.y) | drop_nan(v.z) | drop_nan(v.w)) && r < there && used;
-            if (r >= there) v = make_uint4(0, 0, 0, 0);
-            if (nan || r >= there) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-            const uint32_t lanes = __ballot_sync(0xffffffffu, nan);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) nan_rows |= static_cast<uint32_t>((lanes >> (8 * k) & 0xFF) != 0) << ((i & 3) * 4 + k);
+            if (drop_nan(v.x) | drop_nan(v.y) | drop_nan(v.z) | drop_nan(v.w)) {
+              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+              found |= 1u << i;
+            }
           }
-          fence_proxy_async_smem();  // before the next copy into this stage
           __syncwarp();
+          if (__any_sync(0xffffffffu, found)) {
+            fence_proxy_async_smem();  // before the next copy into this stage
+            const int there = kGather ? kSlice : meta.x != 0.f ? min(max(length - pos0, 0), kSlice) : 0;
+            uint32_t nan_rows = 0;
+            for (int i = 0; i < 4 * L::kHalves; ++i) {
+              const bool used = D >= 128 || ((lane & 7) ^ (((i & 3) * 4 + (lane >> 3)) & 7)) < D / 16;  // a row of 128 bytes may be half empty
+              const uint32_t lanes = __ballot_sync(0xffffffffu, used && found >> i & 1);
 #pragma unroll
-          for (int i = 0; i < 4 * kTiles; ++i)
-            if (nan_rows >> ((i >> 1 & 1) * 8 + key) & 1) poisoned |= seen & 1u << i;
+              for (int k = 0; k < 4; ++k) nan_rows |= static_cast<uint32_t>((lanes >> (8 * k) & 0xFF) != 0) << ((i & 3) * 4 + k);
+            }
+            nan_rows &= (1u << there) - 1;
+#pragma unroll
+            for (int i = 0; i < 4 * kTiles; ++i)
+              if (x[i >> 2][i & 3] != -CUDART_INF_F && nan_rows >> ((i >> 1 & 1) * 8 + key) & 1) poisoned |= 1u << i;
+          }
         }
       }
       if (__any_sync(0xffffffffu, grows)) {  // a query's maxima are compared over its keys only when one of them grows

@@ -507,6 +507,28 @@ def test_a_bound_of_no_tokens_is_one_of_one(dev, bound):
     check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, max_seqlen_q=bound), *attend(q, cache, tables, step))
 
 
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("lengths,d,bs", [([1, 17, 100], 48, 16), ([3, 129, 64], 128, 64), ([33, 40, 65], 256, 128)])
+def test_what_was_in_a_block_before_does_not_matter(dev, kept, lengths, d, bs):
+    tables = fsa.block_tables(3, 9, 30, bs, device=dev)
+    cache = fsa.quantized_cache(30, 2, d, bs, device=dev)
+    for x, byte in ((cache.k, 0x7F), (cache.v, 0xFF)):
+        x.view(torch.uint8).fill_(byte)
+    cache.k_scale.fill_(math.nan)
+    cache.v_scale.fill_(math.nan)
+    g = torch.Generator(device=dev).manual_seed(26)
+    for new in (lengths, [2, 1, 3]):
+        T = sum(new)
+        step = tables.extend(ints(new, dev), T)
+        kv = torch.randn((2, T, 2, d), generator=g, device=dev, dtype=torch.float16)
+        fsa.cache_append(cache, tables, step, kv[0], kv[1])
+        q = torch.randn((T, 4, d), generator=g, device=dev, dtype=torch.float16)
+        keep = None
+        if kept:
+            keep = fsa.KeptKeys(torch.arange(0, 256, 2, dtype=torch.int32, device=dev).expand(3, 2, 128).contiguous(), ints([[128, 90]] * 3, dev), None, 256)
+        check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, keep), *attend(q, cache, tables, step, keep))
+
+
 def test_refused_and_padded_tokens_are_zero(dev):
     tables = fsa.block_tables(4, 3, 4, 16, device=dev)
     cache = fsa.quantized_cache(4, 1, 64, 16, device=dev)
