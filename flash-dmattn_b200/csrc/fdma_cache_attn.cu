@@ -13,6 +13,9 @@
 //  * A unit of work is a (request, kv head, tile of 8 or 16 rows), made of chunks of 64 keys. The chunks of all units form one row;
 //    every CTA takes an equal part of it, however long the requests are, and starts and ends in the middle of a unit where it
 //    must. Such partial results go through scratch and a second kernel; units that one CTA finishes are written directly.
+//  * Where units are few and short, latency is what counts: a unit is shared by the CTAs of a cluster (kCluster), which join their sums
+//    through each other's shared memory. No second kernel, and no sums over the requests before the first load. 1 request of 4096
+//    tokens, 32 heads over 8, d = 128: 7.7 us in a graph, 12.2 with equal shares and the second kernel; 50 of 1000, 8 over 2: 9.5, 13.7.
 //  * A warp of the CTA copies chunks to shared memory by TMA, three ahead; four warps take 16 keys of each. The 128-byte swizzle
 //    and the order in which keys are assigned to the columns of the products (`key_row`) make all reads free of bank conflicts:
 //    K fragments are 16-byte reads of a key's row, V fragments 4-byte reads of four keys whose bytes are then paired.
@@ -35,6 +38,7 @@ constexpr int kWarps = 4;  // that compute; each has 16 keys of a chunk
 constexpr int kSlice = kChunk / kWarps;
 constexpr int kHeld = 128;  // requests whose work a CTA holds in shared memory
 constexpr int kMinShare = 2;  // chunks per CTA
+constexpr int kMostCluster = 16, kMostClusterChunks = 20;  // CTAs that share a unit (kCluster), and chunks of one of them
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPScale = 16384.f;  // probabilities in fp16: normal numbers down to 2^-28
 
@@ -50,6 +54,7 @@ struct AttnArgs {
   bool q_vec;              // queries in 16-byte vectors
   const int32_t* prompts;  // not null: rows of no request are written already, and if it points to a number above 0, those of
                            // requests with kPromptTokens or more as well
+  int cluster, tiles;      // CTAs that share a unit, and tiles of a request, where there are few units (kCluster)
   bool merge_requests;     // CTAs of the second kernel: kPromptTokens - 1 for each request, not one for every token
   float* partial;          // [cta][2][rows][D + 4]: sums over the values, then maximum and sum
   int* status;
@@ -261,6 +266,55 @@ __device__ __forceinline__ Units make_units(const AttnArgs& a, Held& h) {
   __syncthreads();
   return Units{a, &h};
 }
+// The same of a CTA that knows its unit.
+struct OneUnit {
+  const AttnArgs& a;
+  Cursor x;
+  Request q;
+  __device__ Unit of(const Cursor&, const Request&) const { return Unit{x.r, x.hk, x.tile, q.chunks, 0}; }
+  __device__ Cursor at(int64_t, Request& request) const {
+    request = q;
+    return x;
+  }
+  __device__ void advance(Cursor& at, Request&) const { at.r = a.p.c.requests; }
+};
+__device__ __forceinline__ OneUnit make_one_unit(const AttnArgs& a) {
+  const int slot = static_cast<int>(blockIdx.x) / a.cluster, per_request = a.p.c.h_k * a.tiles;
+  Cursor x;
+  x.r = slot / per_request;
+  x.hk = (slot - x.r * per_request) / a.tiles;
+  x.tile = slot - (x.r * a.p.c.h_k + x.hk) * a.tiles;
+  OneUnit u{a, x, load_request(a, x.r)};
+  if (a.list_chunks && a.p.kept_count) {
+    const int kept = a.p.kept_count[x.r * a.p.count_batch_stride + x.hk * a.p.count_head_stride];
+    u.q.chunks = (max(0, min(kept, a.p.kept_capacity)) + kChunk - 1) / kChunk;
+  }
+  return u;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// of another CTA of the cluster
+__device__ __forceinline__ uint32_t shared_of(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ int64_t share_of(int64_t total, int ctas) { return max(static_cast<int64_t>(kMinShare), quotient(total + ctas - 1, ctas)); }
 
 template <int D, int ROWS, bool kGather>
@@ -283,7 +337,7 @@ struct Layout {
   static constexpr int kCtas = D > 128 || ROWS > 8 ? 2 : 3;
 };
 
-template <int D, int ROWS, bool kGather, bool kBf16>
+template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster>
 __global__ void __launch_bounds__(Layout<D, ROWS, kGather>::kThreads, Layout<D, ROWS, kGather>::kCtas)
 cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using L = Layout<D, ROWS, kGather>;
@@ -295,6 +349,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   // K scale, exponent of the V scale, position
   __shared__ float4 s_meta[L::kStages][kGather ? kChunk : kWarps];
   __shared__ Held s_held;
+  __shared__ __align__(8) float2 s_part[ROWS];  // kCluster: maximum and sum of this CTA's part; the sums over the values are in s_buf
   __shared__ float s_row_scale[ROWS], s_m[kWarps][ROWS], s_l[kWarps][ROWS];
   __shared__ int s_abort;
   unsigned char* smem = align_smem_1024(s_raw);
@@ -314,13 +369,25 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   }
   if (kGather && c.d < D)  // columns beyond the head dim stay zero in every stage
     for (int i = tid; i < L::kStages * L::kStageBytes / 16; i += L::kThreads) reinterpret_cast<uint4*>(smem + L::kRing)[i] = make_uint4(0, 0, 0, 0);
-  const Units units = make_units(a, s_held);
+  const auto units = [&] {
+    if constexpr (kCluster) return make_one_unit(a);
+    else return make_units(a, s_held);
+  }();
+  if (kCluster && tid < ROWS) s_part[tid] = make_float2(-CUDART_INF_F, 0.f);
   __syncthreads();
-  if (blockIdx.x == 0 && units.held)
-    for (int i = tid; i <= c.requests; i += L::kThreads) a.pre[i] = s_held.pre[i];
-  const int64_t total = units.total(), share = share_of(total, a.ctas);
-  const int64_t w0 = min(total, blockIdx.x * share), w1 = min(total, w0 + share);
-  if (w0 >= w1) return;
+  int64_t w0, w1;
+  if constexpr (kCluster) {
+    const int n = units.q.rows > units.x.tile * ROWS ? units.q.chunks : 0, rank = static_cast<int>(cluster_rank()), shift = 31 - __clz(a.cluster);
+    w0 = static_cast<int64_t>(n) * rank >> shift;
+    w1 = static_cast<int64_t>(n) * (rank + 1) >> shift;
+  } else {
+    if (blockIdx.x == 0 && units.held)
+      for (int i = tid; i <= c.requests; i += L::kThreads) a.pre[i] = s_held.pre[i];
+    const int64_t total = units.total(), share = share_of(total, a.ctas);
+    w0 = min(total, blockIdx.x * share);
+    w1 = min(total, w0 + share);
+    if (w0 >= w1) return;
+  }
   const WaitCtl ctl{&s_abort, a.status};
 
   if (!kGather && warp == kWarps) {
@@ -413,6 +480,11 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         st = st == 0 ? L::kStages - 1 : st - 1;
         mbar_wait_limit(&s_full[st], phase, WaitCtl{&s_abort, a.status}, 703, 1000000ull);
       }
+    }
+    if (kCluster) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
     }
     return;
   }
@@ -850,8 +922,9 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
     }
     if (warp != 0) continue;
-    const bool complete = first == 0 && last == u.n;
-    float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (first > 0 ? 0 : 1)) * ROWS * (D + 4);
+    if (kCluster) __syncwarp();  // (the sums are read no more)
+    const bool complete = !kCluster && first == 0 && last == u.n;
+    float* part = kCluster ? s_buf : a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (first > 0 ? 0 : 1)) * ROWS * (D + 4);
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
@@ -870,15 +943,77 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               *reinterpret_cast<uint2*>(dst + dd) = make_uint2(pack2<kBf16>(y[0][e] * inv, y[0][2 + e] * inv), pack2<kBf16>(y[1][e] * inv, y[1][2 + e] * inv));
           }
         } else {
-          float* dst = part + rr * (D + 4);
+          float* dst = part + rr * (kCluster ? D : D + 4);
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const float(&y)[2][4] = o[nt][j];
             *reinterpret_cast<float4*>(dst + 32 * j + 4 * g) = make_float4(y[0][e], y[0][2 + e], y[1][e], y[1][2 + e]);
           }
-          if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[nt][e], l[nt][e]);
+          if (g == 0) *(kCluster ? s_part + rr : reinterpret_cast<float2*>(dst + D)) = make_float2(m[nt][e], l[nt][e]);
         }
       }
+  }
+
+  if constexpr (kCluster) {
+    // ---- the CTAs' sums: each joins its share of the numbers, eight threads for four of them ----
+    cluster_sync();
+    const Request& q = units.q;
+    const int rank = static_cast<int>(cluster_rank()), row0 = units.x.tile * ROWS, nrows = min(ROWS, q.rows - row0), of = tid & 7;
+    for (int base = rank * 16; base < nrows * (D / 4); base += a.cluster * 16) {
+      const int v = base + (tid >> 3), rr = min(v / (D / 4), nrows - 1), col = v % (D / 4) * 4;
+      float2 ml[2];
+      float4 y[2];
+      float top = -CUDART_INF_F, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        ml[k] = make_float2(-CUDART_INF_F, 0.f);
+        if (of + 8 * k < a.cluster) {
+          ml[k] = ld_cluster2(shared_of(s_part + rr, of + 8 * k));
+          y[k] = ld_cluster(shared_of(s_buf + rr * D + col, of + 8 * k));
+        }
+        top = fmaxf(top, ml[k].x);
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float from = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (ml[k].x != -CUDART_INF_F || ml[k].y != 0.f) {  // (otherwise its sums are zeros, or were not written; NaN is not 0)
+          const float f = exp2_or_zero(ml[k].x - from);
+          sum = fmaf(ml[k].y, f, sum);
+          acc[0] = fmaf(y[k].x, f, acc[0]); acc[1] = fmaf(y[k].y, f, acc[1]);
+          acc[2] = fmaf(y[k].z, f, acc[2]); acc[3] = fmaf(y[k].w, f, acc[3]);
+        }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+      }
+      if (of == 0 && v < nrows * (D / 4) && col < c.d) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const uint2 th = token_head(a, row0 + rr);
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(q.token0 + th.x) * p.out_row_stride + (units.x.hk * a.group + th.y) * p.out_head_stride;
+        *reinterpret_cast<uint2*>(dst + col) = make_uint2(pack2<kBf16>(acc[0] * inv, acc[1] * inv), pack2<kBf16>(acc[2] * inv, acc[3] * inv));
+      }
+    }
+    // rows that nobody computes: of this request, and behind the last one
+    if (units.x.tile == 0) {
+      auto clear = [&](int token0, int64_t from, int64_t to) {
+        for (int64_t i = from * (c.d / 8) + rank * 128 + tid; i < to * (c.d / 8); i += a.cluster * 128) {
+          const int row = static_cast<int>(i / (c.d / 8));
+          const uint2 th = token_head(a, row);
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(token0 + th.x) * p.out_row_stride + (units.x.hk * a.group + th.y) * p.out_head_stride;
+          *reinterpret_cast<uint4*>(dst + (i - static_cast<int64_t>(row) * (c.d / 8)) * 8) = make_uint4(0, 0, 0, 0);
+        }
+      };
+      if (q.rows < q.n * a.group) clear(q.token0, q.rows, static_cast<int64_t>(q.n) * a.group);
+      if (units.x.r == c.requests - 1) {
+        const int end = max(0, min(c.cu_seqlens[c.requests], c.tokens));
+        if (end < c.tokens) clear(end, 0, static_cast<int64_t>(c.tokens - end) * a.group);
+      }
+    }
+    cluster_sync();  // nobody leaves while its shared memory may still be read
   }
 }
 
@@ -1030,6 +1165,7 @@ struct Plan {
   bool sums;  // by a kernel of their own: many requests, and not one tile of cu_chunks' chunks for each
   int64_t most_chunks;
   bool prompts;
+  int cluster, tiles, units;
   size_t sums_off, prompt_off, bytes;
 };
 Plan plan_of(const fdma_cache_attention_params& p) {
@@ -1045,13 +1181,36 @@ Plan plan_of(const fdma_cache_attention_params& p) {
   pl.sums = p.c.requests > kHeld && (pl.list_chunks || most > pl.rows);
   const int64_t tiles = static_cast<int64_t>(p.c.tokens) * (p.h / p.c.h_k) / pl.rows + p.c.requests;
   pl.most_chunks = tiles * (pl.list_chunks ? pl.list_chunks : (static_cast<int64_t>(p.c.width) * p.c.block_size + kChunk - 1) / kChunk);
+  pl.tiles = static_cast<int>((most + pl.rows - 1) / pl.rows);
+  const int64_t units = static_cast<int64_t>(p.c.requests) * p.c.h_k * pl.tiles;
+  const int64_t chunks = pl.list_chunks ? pl.list_chunks : (std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size) + kChunk - 1) / kChunk;
+  pl.units = static_cast<int>(std::min<int64_t>(units, 1 << 20));
+  pl.cluster = 0;
+  // Few and short enough units get a cluster each: as many CTAs as run at once (clusters leave places of a GPU's parts empty, 16 a
+  // quarter of them and 8 an eighth), but fewer than two for a chunk. From 24 chunks a CTA on equal shares are as fast (1 request of
+  // 24000 tokens, 32 heads over 8, d = 128: 20.5 us, 20.3); up to 16 they take longer (4096 tokens: 7.7, 12.2; 16384: 15.5, 16.9).
+  if (!pl.prompts && units > 0)
+    for (int n = kMostCluster; n > 1 && !pl.cluster; n /= 2)
+      if (units * n <= pl.ctas - pl.ctas * n / 64 && (n < 2 * chunks || n == 2) && chunks <= static_cast<int64_t>(kMostClusterChunks) * n) pl.cluster = n;
   pl.sums_off = align256(static_cast<size_t>(pl.ctas) * 2 * pl.rows * (pl.D + 4) * sizeof(float));
   pl.prompt_off = pl.sums_off + align256((static_cast<size_t>(p.c.requests) + 1) * sizeof(int32_t));
   pl.bytes = pl.prompt_off + (pl.prompts ? cache_prompt_workspace_bytes(p) : 0);
   return pl;
 }
 
-template <int D, int ROWS, bool kGather, bool kBf16>
+int allow_wide_clusters_once(const void* kernel, std::atomic<uint64_t>& prepared) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (prepared.load(std::memory_order_acquire) & bit)) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 64) prepared.fetch_or(bit, std::memory_order_release);
+  return 0;
+}
+
+template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster>
 int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
   using L = Layout<D, ROWS, kGather>;
   const fdma_cache& c = a.p.c;
@@ -1064,10 +1223,28 @@ int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
     if (!st) st = encode_tmap_4d(&map_v, c.v, 1, dims, strides, box);
     if (st) return st;
   }
-  auto kern = cache_attend_kernel<D, ROWS, kGather, kBf16>;
-  static std::atomic<uint64_t> prepared{0};
+  auto kern = cache_attend_kernel<D, ROWS, kGather, kBf16, kCluster>;
+  static std::atomic<uint64_t> prepared{0}, wide{0};
   const int st_smem = allow_smem_once(reinterpret_cast<const void*>(kern), L::kTotal, prepared);
   if (st_smem) return st_smem;
+  if constexpr (kCluster) {
+    a.cluster = pl.cluster;
+    a.tiles = pl.tiles;
+    const int st = pl.cluster > 8 ? allow_wide_clusters_once(reinterpret_cast<const void*>(kern), wide) : 0;
+    if (st) return st;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(pl.units) * pl.cluster);
+    cfg.blockDim = dim3(L::kThreads);
+    cfg.dynamicSmemBytes = L::kTotal;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = pl.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, a, map_k, map_v));
+  }
   kern<<<pl.ctas, L::kThreads, L::kTotal, stream>>>(a, map_k, map_v);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -1085,11 +1262,15 @@ int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
   cfg.numAttrs = 1;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, cache_merge_kernel<D, kBf16>, a));
 }
+template <int D, int ROWS, bool kCluster>
+int launch_c(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
+  const bool bf16 = a.p.dtype == FDMA_BF16;
+  if (a.list_chunks) return bf16 ? launch<D, ROWS, true, true, kCluster>(a, pl, stream) : launch<D, ROWS, true, false, kCluster>(a, pl, stream);
+  return bf16 ? launch<D, ROWS, false, true, kCluster>(a, pl, stream) : launch<D, ROWS, false, false, kCluster>(a, pl, stream);
+}
 template <int D, int ROWS>
 int launch_t(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
-  const bool bf16 = a.p.dtype == FDMA_BF16;
-  if (a.list_chunks) return bf16 ? launch<D, ROWS, true, true>(a, pl, stream) : launch<D, ROWS, true, false>(a, pl, stream);
-  return bf16 ? launch<D, ROWS, false, true>(a, pl, stream) : launch<D, ROWS, false, false>(a, pl, stream);
+  return pl.cluster ? launch_c<D, ROWS, true>(a, pl, stream) : launch_c<D, ROWS, false>(a, pl, stream);
 }
 
 int check_attention(const fdma_cache_attention_params* pp) {
@@ -1148,7 +1329,7 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
     a.prompts = reinterpret_cast<const int32_t*>(static_cast<char*>(p.workspace) + pl.prompt_off + cache_prompt_keys(p));
   }
   a.pre = reinterpret_cast<int32_t*>(static_cast<char*>(p.workspace) + pl.sums_off);
-  if (pl.sums) {
+  if (pl.sums && !pl.cluster) {
     cache_sums_kernel<<<1, 1024, 0, stream>>>(a, a.pre);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return static_cast<int>(e);

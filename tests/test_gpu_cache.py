@@ -529,6 +529,80 @@ def test_what_was_in_a_block_before_does_not_matter(dev, kept, lengths, d, bs):
         check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, keep), *attend(q, cache, tables, step, keep))
 
 
+def widen(tables):
+    """The same requests with rows for 40000 tokens: the work is then split for long requests, whatever their lengths are."""
+    more = 40000 // tables.block_size - tables.table.shape[1]
+    return tables._replace(table=torch.nn.functional.pad(tables.table, (0, more), value=-1))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cached,new,H,Hk,d,bs", ATTEND)
+def test_attention_under_wide_bounds(dev, dtype, cached, new, H, Hk, d, bs):
+    tables, cache, step, g = filled(dev, len(cached), cached, new, Hk, d, bs, 27)
+    T = sum(new)
+    kv = torch.randn((2, T, Hk, d), generator=g, device=dev).to(dtype)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    q = torch.randn((T, H, d), generator=g, device=dev).to(dtype)
+    tables = widen(tables)
+    check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step), *attend(q, cache, tables, step))
+    most = max(step.lengths.tolist())
+    pos = torch.arange(40000, dtype=torch.int32, device=dev) * 2
+    kept = fsa.KeptKeys(pos.expand(1, Hk, -1).contiguous(), torch.full((1, Hk), most // 2, dtype=torch.int32, device=dev), None, 80000)
+    bias = torch.randn((1, H, 1, most), generator=g, device=dev).to(dtype)
+    check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, kept, bias, max_seqlen_q=max(new)), *attend(q, cache, tables, step, kept, bias))
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("requests,length,Hk", [(1, 1, 1), (1, 70, 2), (2, 200, 1), (1, 1200, 1), (1, 20000, 1), (3, 5000, 8), (40, 600, 1),
+                                                (100, 130, 1), (210, 100, 1), (300, 100, 1)])
+def test_shared_units(dev, kept, requests, length, Hk):
+    """Units of one to sixteen CTAs and more, requests of one token and of the full length, refused ones, and tokens behind the last."""
+    d, bs = 64, 64
+    lengths = [1 + (length - 1) * (i % 3) // 2 for i in range(requests)]
+    lengths[-1] = length
+    tables, cache, _, g = filled(dev, requests, [n - 1 for n in lengths], [1] * requests, Hk, d, bs, 28)
+    tables.truncate(ints([n - 1 for n in lengths], dev))
+    new = [1] * requests
+    if requests > 1:
+        new[0] = tables.table.shape[1] * bs + 1  # is refused
+    T = sum(new) + 3
+    step = tables.extend(ints(new, dev), T)
+    assert step.granted.tolist() == [n == 1 for n in new]
+    kv = torch.randn((2, T, Hk, d), generator=g, device=dev, dtype=torch.bfloat16)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    q = torch.randn((T, 4 * Hk, d), generator=g, device=dev, dtype=torch.bfloat16)
+    keep = None
+    if kept:
+        n = (length + 2) // 3
+        count = torch.randint(0, n + 1, (requests, Hk), generator=g, device=dev, dtype=torch.int32)
+        keep = fsa.KeptKeys((3 * torch.arange(n, dtype=torch.int32, device=dev)).expand(requests, Hk, n).contiguous(), count, None, 3 * n)
+    out = fsa.flash_sparse_attn_cache_func(q, cache, tables, step, keep, max_seqlen_q=1, max_seqlen_k=length)
+    check(out, *attend(q, cache, tables, step, keep))
+    assert not out[-3:].any() and (requests == 1 or not out[:new[0]].any())
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("wide", [False, True])
+def test_not_a_number_in_every_key(dev, kept, wide):
+    """Scores that are all NaN are larger than no maximum; the result is NaN all the same, and only there."""
+    tables, cache, step, g = filled(dev, 3, [300, 90, 500], [1, 3, 2], 2, 128, 32, 29)
+    kv = torch.randn((2, 6, 2, 128), generator=g, device=dev, dtype=torch.bfloat16)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    q = torch.randn((6, 8, 128), generator=g, device=dev, dtype=torch.bfloat16)
+    keep = None
+    if kept:
+        keep = fsa.KeptKeys(torch.arange(512, dtype=torch.int32, device=dev).expand(1, 1, 512).contiguous(), ints([[512]], dev), None, 512)
+    if wide:
+        tables = widen(tables)
+        if kept:
+            keep = keep._replace(key_pos=torch.nn.functional.pad(keep.key_pos, (0, 40000)))
+    want = fsa.flash_sparse_attn_cache_func(q, cache, tables, step, keep)
+    cache.k.view(torch.uint8)[tables.table[1, :3].long(), 1] = 0x7F
+    got = fsa.flash_sparse_attn_cache_func(q, cache, tables, step, keep)
+    assert bool(got[1:4, 4:].isnan().all())
+    assert torch.equal(got[1:4, :4], want[1:4, :4]) and torch.equal(got[[0, 4, 5]], want[[0, 4, 5]])
+
+
 def test_refused_and_padded_tokens_are_zero(dev):
     tables = fsa.block_tables(4, 3, 4, 16, device=dev)
     cache = fsa.quantized_cache(4, 1, 64, 16, device=dev)
