@@ -1194,7 +1194,7 @@ Plan plan_of(const fdma_cache_attention_params& p) {
       if (units * n <= pl.ctas - pl.ctas * n / 64 && (n < 2 * chunks || n == 2) && chunks <= static_cast<int64_t>(kMostClusterChunks) * n) pl.cluster = n;
   pl.sums_off = align256(static_cast<size_t>(pl.ctas) * 2 * pl.rows * (pl.D + 4) * sizeof(float));
   pl.prompt_off = pl.sums_off + align256((static_cast<size_t>(p.c.requests) + 1) * sizeof(int32_t));
-  pl.bytes = pl.prompt_off + (pl.prompts ? cache_prompt_workspace_bytes(p) : 0);
+  pl.bytes = pl.cluster ? 0 : pl.prompt_off + (pl.prompts ? cache_prompt_workspace_bytes(p) : 0);
   return pl;
 }
 
@@ -1305,7 +1305,7 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   if ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uint64_t>(p.out_row_stride | p.out_head_stride) * 2) % 16) return FDMA_ERR_UNSUPPORTED;
   const Plan pl = plan_of(p);
   if (pl.most_chunks > 0x7FFFFFFF) return FDMA_ERR_TOO_LARGE;
-  if (!p.workspace || p.workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(p.workspace) & 255)) return FDMA_ERR_WORKSPACE;
+  if (pl.bytes && (!p.workspace || p.workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(p.workspace) & 255))) return FDMA_ERR_WORKSPACE;
   AttnArgs a = {};
   a.p = p;
   a.shift = p.c.block_size == 16 ? 4 : p.c.block_size == 32 ? 5 : p.c.block_size == 64 ? 6 : 7;
@@ -1319,22 +1319,25 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   a.ctas = pl.ctas;
   a.scale_log2 = p.softmax_scale * kLog2e;
   a.q_vec = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uint64_t>(p.query_row_stride | p.query_head_stride) * 2) % 16 == 0;
-  a.partial = static_cast<float*>(p.workspace);
   a.status = kernel_status_ptr();
   if (!a.status) return FDMA_ERR_DRIVER;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (pl.prompts) {
-    const int status = cache_prompt(p, a.shift, static_cast<char*>(p.workspace) + pl.prompt_off, stream);
-    if (status) return status;
-    a.prompts = reinterpret_cast<const int32_t*>(static_cast<char*>(p.workspace) + pl.prompt_off + cache_prompt_keys(p));
-  }
-  a.pre = reinterpret_cast<int32_t*>(static_cast<char*>(p.workspace) + pl.sums_off);
-  if (pl.sums && !pl.cluster) {
-    cache_sums_kernel<<<1, 1024, 0, stream>>>(a, a.pre);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return static_cast<int>(e);
-  } else if (p.c.requests > kHeld) {  // a tile for each request: their chunks
-    a.pre = const_cast<int32_t*>(p.c.cu_chunks);
+  if (!pl.cluster) {
+    char* const ws = static_cast<char*>(p.workspace);
+    a.partial = static_cast<float*>(p.workspace);
+    if (pl.prompts) {
+      const int status = cache_prompt(p, a.shift, ws + pl.prompt_off, stream);
+      if (status) return status;
+      a.prompts = reinterpret_cast<const int32_t*>(ws + pl.prompt_off + cache_prompt_keys(p));
+    }
+    a.pre = reinterpret_cast<int32_t*>(ws + pl.sums_off);
+    if (pl.sums) {
+      cache_sums_kernel<<<1, 1024, 0, stream>>>(a, a.pre);
+      const cudaError_t e = cudaGetLastError();
+      if (e != cudaSuccess) return static_cast<int>(e);
+    } else if (p.c.requests > kHeld) {  // a tile for each request: their chunks
+      a.pre = const_cast<int32_t*>(p.c.cu_chunks);
+    }
   }
   if (pl.D == 256) return launch_t<256, 8>(a, pl, stream);
   if (pl.D == 128) return pl.rows == 8 ? launch_t<128, 8>(a, pl, stream) : launch_t<128, 16>(a, pl, stream);

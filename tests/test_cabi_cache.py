@@ -136,10 +136,18 @@ def test_append(change, status):
     (dict(bias=ADDR, h_bias=3, bias_keys=1), -1), (dict(bias=ADDR, h_bias=1, bias_keys=0), -1), (dict(kept_pos=ADDR, kept_capacity=0), -1),
     (dict(dtype=2), -2), (dict(out=ADDR + 2), -2), (dict(out_row_stride=3), -2), ({}, -3), (dict(workspace=ADDR + 16, workspace_bytes=1 << 30), -3)])
 def test_attention(change, status):
-    p = fill(Attention(), ["query", "out"], c=cache(), h=1, max_seqlen_q=1, max_seqlen_k=1, softmax_scale=1.0)
+    p = fill(Attention(), ["query", "out"], c=cache(requests=500), h=1, max_seqlen_q=1, max_seqlen_k=1, softmax_scale=1.0)
     for k, v in change.items():
         setattr(p, k, v)
     assert call("fdma_cache_attention", p) == status
+
+
+def test_workspace_of_few_requests():
+    fn = _lib.load().fdma_cache_attention_workspace_bytes
+    fn.restype, fn.argtypes = ctypes.c_size_t, [ctypes.c_void_p]
+    for requests, some in ((1, False), (500, True)):
+        p = fill(Attention(), ["query", "out"], c=cache(requests=requests), h=1, max_seqlen_q=1, max_seqlen_k=1, softmax_scale=1.0)
+        assert (fn(ctypes.byref(p)) > 0) == some
 
 
 def test_heads_must_divide():
