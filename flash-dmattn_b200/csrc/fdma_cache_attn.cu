@@ -56,7 +56,7 @@ struct AttnArgs {
                            // requests with kPromptTokens or more as well
   int cluster, tiles;      // CTAs that share a unit, and tiles of a request, where there are few units (kCluster)
   bool merge_requests;     // CTAs of the second kernel: kPromptTokens - 1 for each request, not one for every token
-  float* partial;          // [cta][2][rows][D + 4]: sums over the values, then maximum and sum
+  float* partial;          // [cta][2][rows][D + 4]: sums over the values, then maximum, sum and the maximum's exponent
   int* status;
 };
 
@@ -146,7 +146,24 @@ __device__ __forceinline__ float bias_log2(float b) {
 __device__ __forceinline__ float value_scale(float x) { return x < 0x1p-100f ? 0x1p-101f : x; }
 __device__ __forceinline__ float p_scale(float exponent) { return exponent < -100.f ? 0.f : kPScale; }
 __device__ __forceinline__ float exponent_of(float x) { return static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) - 127); }
-__device__ __forceinline__ float exp2_or_zero(float x) { return x == -CUDART_INF_F ? 0.f : exp2f(x); }
+// A running maximum over scores times V scales, 2^(m + z): the score m and the scale's exponent z are kept apart, because a bias can make
+// m so large that the sum would lose z, and the values of blocks with other scales would then count by the wrong factor. Differences
+// are small where they matter: of equal scores exactly 0.
+struct Peak {
+  float m, z;
+};
+// log2 of a's ratio to b; NaN where neither has seen a key
+__device__ __forceinline__ float above(const Peak& a, const Peak& b) { return (a.m - b.m) + (a.z - b.z); }
+__device__ __forceinline__ Peak higher(const Peak& a, const Peak& b) { return above(b, a) > 0.f ? b : a; }
+// what sums up to `from` are multiplied by in sums up to `to`, which is no lower
+__device__ __forceinline__ float rescale(const Peak& from, const Peak& to) { return from.m == -CUDART_INF_F ? 0.f : exp2f(above(from, to)); }
+__device__ __forceinline__ Peak shuffled(const Peak& x, int mask) {
+  return Peak{__shfl_xor_sync(0xffffffffu, x.m, mask), __shfl_xor_sync(0xffffffffu, x.z, mask)};
+}
+// (lanes that compared in different orders may hold different ones of two equal peaks)
+__device__ __forceinline__ Peak of_lane(const Peak& x, int lane) {
+  return Peak{__shfl_sync(0xffffffffu, x.m, lane), __shfl_sync(0xffffffffu, x.z, lane)};
+}
 
 __device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
   const fdma_cache& c = a.p.c;
@@ -310,11 +327,6 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ int64_t share_of(int64_t total, int ctas) { return max(static_cast<int64_t>(kMinShare), quotient(total + ctas - 1, ctas)); }
 
 template <int D, int ROWS, bool kGather>
@@ -349,8 +361,10 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   // K scale, exponent of the V scale, position
   __shared__ float4 s_meta[L::kStages][kGather ? kChunk : kWarps];
   __shared__ Held s_held;
-  __shared__ __align__(8) float2 s_part[ROWS];  // kCluster: maximum and sum of this CTA's part; the sums over the values are in s_buf
-  __shared__ float s_row_scale[ROWS], s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+  // kCluster: maximum, sum and the maximum's exponent of this CTA's part; the sums over the values are in s_buf
+  __shared__ __align__(16) float4 s_part[ROWS];
+  __shared__ float s_row_scale[ROWS], s_l[kWarps][ROWS];
+  __shared__ Peak s_m[kWarps][ROWS];
   __shared__ int s_abort;
   unsigned char* smem = align_smem_1024(s_raw);
   const fdma_cache_attention_params& p = a.p;
@@ -373,7 +387,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     if constexpr (kCluster) return make_one_unit(a);
     else return make_units(a, s_held);
   }();
-  if (kCluster && tid < ROWS) s_part[tid] = make_float2(-CUDART_INF_F, 0.f);
+  if (kCluster && tid < ROWS) s_part[tid] = make_float4(-CUDART_INF_F, 0.f, 0.f, 0.f);
   __syncthreads();
   int64_t w0, w1;
   if constexpr (kCluster) {
@@ -578,14 +592,15 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 
     // of queries 8 tile + 2 t, + 1: sums over the values (elements 32 j + 4 g + 2 half + {0: [0, 1], 1: [2, 3]}), maximum, this lane's
     // share of the softmax's sum, factor of the scores, newest position seen
-    float o[kTiles][D / 32][2][4], m[kTiles][2], l[kTiles][2], row_scale[kTiles][2];
+    float o[kTiles][D / 32][2][4], l[kTiles][2], row_scale[kTiles][2];
+    Peak top[kTiles][2];
     int newest[kTiles][2];
     const uint16_t* bias_row[kTiles][2];
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m[nt][e] = -CUDART_INF_F;
+        top[nt][e] = Peak{-CUDART_INF_F, 0.f};
         l[nt][e] = 0.f;
         const int rr = min(8 * nt + 2 * t + e, nrows - 1), row = row0 + rr;
         row_scale[nt][e] = s_row_scale[rr];
@@ -725,7 +740,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       // all 16 keys are there and seen by every row
       const bool clean = !kGather && pos0 + kSlice <= sure && meta.x != 0.f;
       float x[kTiles][4];
-      bool grows = false;
+      auto z_of = [&](int k) { return kGather ? key_meta[k >> 1].z : meta.z; };  // exponent of the V scale of score k
+      bool grows = false;  // (rounded down, so that no score above the maximum is missed)
 #pragma unroll
       for (int nt = 0; nt < kTiles; ++nt) {
 #pragma unroll
@@ -736,7 +752,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             const int pos = __float_as_int(km.w);
             float add = km.x;
             if (head_bias && pos >= 0 && pos < p.bias_keys) add = bias_log2(raw_to_f<kBf16>(__ldg(bias_row[nt][k & 1] + pos)));
-            v = fmaf(s[nt][k], row_scale[nt][k & 1] * km.y, add) + km.z;
+            v = fmaf(s[nt][k], row_scale[nt][k & 1] * km.y, add);
             if (add == -CUDART_INF_F || pos > newest[nt][k & 1]) v = -CUDART_INF_F;  // even where the key is NaN
           } else {
             v = s[nt][k] * (row_scale[nt][k & 1] * meta.y);
@@ -744,10 +760,9 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               const float add = bias_log2(raw_to_f<kBf16>(raw_bias[nt][k >> 1][k & 1]));
               v = add == -CUDART_INF_F ? add : v + add;
             }
-            v += meta.z;
             if (!clean && (pos0 + (k >> 1) * 8 + key > newest[nt][k & 1] || meta.x == 0.f)) v = -CUDART_INF_F;
           }
-          grows |= v > m[nt][k & 1];
+          grows |= v > __fadd_rd(top[nt][k & 1].m, top[nt][k & 1].z - z_of(k));
         }
       }
       uint32_t poisoned = 0;  // scores, a bit each, whose value is NaN
@@ -793,12 +808,20 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           float corr[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(x[nt][e], x[nt][2 + e]);
+            Peak now;
+            if (kGather) {
+              now = higher(Peak{x[nt][e], z_of(e)}, Peak{x[nt][2 + e], z_of(2 + e)});
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            const float m_new = fmaxf(m[nt][e], mx);
-            corr[e] = exp2_or_zero(m[nt][e] - (m_new == -CUDART_INF_F ? 0.f : m_new));
-            m[nt][e] = m_new;
+              for (int off = 4; off < 32; off <<= 1) now = higher(now, shuffled(now, off));
+              now = of_lane(now, t);
+            } else {  // one block: the scores alone
+              now = Peak{fmaxf(x[nt][e], x[nt][2 + e]), meta.z};
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) now.m = fmaxf(now.m, __shfl_xor_sync(0xffffffffu, now.m, off));
+            }
+            now = higher(top[nt][e], now);
+            corr[e] = rescale(top[nt][e], now);
+            top[nt][e] = now;
             l[nt][e] *= corr[e];
           }
 #pragma unroll
@@ -812,7 +835,10 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       for (int nt = 0; nt < kTiles; ++nt) {
         float e[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = exp2f(x[nt][k] - (m[nt][k & 1] == -CUDART_INF_F ? 0.f : m[nt][k & 1]));
+        for (int k = 0; k < 4; ++k) {
+          const Peak& y = top[nt][k & 1];
+          e[k] = exp2f((x[nt][k] - (y.m == -CUDART_INF_F ? 0.f : y.m)) + (z_of(k) - y.z));
+        }
         if (kGather) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) l[nt][k & 1] = fmaf(e[k], exp2f(-key_meta[k >> 1].z), l[nt][k & 1]);
@@ -860,7 +886,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
         if (g == 0) {
-          s_m[warp][8 * nt + 2 * t + e] = m[nt][e];
+          s_m[warp][8 * nt + 2 * t + e] = top[nt][e];
           s_l[warp][8 * nt + 2 * t + e] = l[nt][e];
         }
       }
@@ -871,14 +897,14 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int rr = 8 * nt + 2 * t + e;
-        float cm = -CUDART_INF_F, cl = 0.f;
+        Peak all = s_m[0][rr];
+        float cl = 0.f;
 #pragma unroll
-        for (int x = 0; x < kWarps; ++x) cm = fmaxf(cm, s_m[x][rr]);
-        const float base = cm == -CUDART_INF_F ? 0.f : cm;
+        for (int x = 1; x < kWarps; ++x) all = higher(all, s_m[x][rr]);
 #pragma unroll
-        for (int x = 0; x < kWarps; ++x) cl = fmaf(s_l[x][rr], exp2_or_zero(s_m[x][rr] - base), cl);
-        f[e] = exp2_or_zero(m[nt][e] - base) * (1.f / kPScale);
-        m[nt][e] = cm;
+        for (int x = 0; x < kWarps; ++x) cl = fmaf(s_l[x][rr], rescale(s_m[x][rr], all), cl);
+        f[e] = rescale(top[nt][e], all) * (1.f / kPScale);
+        top[nt][e] = all;
         l[nt][e] = cl;
       }
 #pragma unroll
@@ -949,7 +975,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             const float(&y)[2][4] = o[nt][j];
             *reinterpret_cast<float4*>(dst + 32 * j + 4 * g) = make_float4(y[0][e], y[0][2 + e], y[1][e], y[1][2 + e]);
           }
-          if (g == 0) *(kCluster ? s_part + rr : reinterpret_cast<float2*>(dst + D)) = make_float2(m[nt][e], l[nt][e]);
+          if (g == 0) *(kCluster ? s_part + rr : reinterpret_cast<float4*>(dst + D)) = make_float4(top[nt][e].m, l[nt][e], top[nt][e].z, 0.f);
         }
       }
   }
@@ -961,25 +987,25 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const int rank = static_cast<int>(cluster_rank()), row0 = units.x.tile * ROWS, nrows = min(ROWS, q.rows - row0), of = tid & 7;
     for (int base = rank * 16; base < nrows * (D / 4); base += a.cluster * 16) {
       const int v = base + (tid >> 3), rr = min(v / (D / 4), nrows - 1), col = v % (D / 4) * 4;
-      float2 ml[2];
-      float4 y[2];
-      float top = -CUDART_INF_F, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+      float4 ml[2], y[2];
+      Peak top{-CUDART_INF_F, 0.f};
+      float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        ml[k] = make_float2(-CUDART_INF_F, 0.f);
+        ml[k] = make_float4(-CUDART_INF_F, 0.f, 0.f, 0.f);
         if (of + 8 * k < a.cluster) {
-          ml[k] = ld_cluster2(shared_of(s_part + rr, of + 8 * k));
+          ml[k] = ld_cluster(shared_of(s_part + rr, of + 8 * k));
           y[k] = ld_cluster(shared_of(s_buf + rr * D + col, of + 8 * k));
         }
-        top = fmaxf(top, ml[k].x);
+        top = higher(top, Peak{ml[k].x, ml[k].z});
       }
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float from = top == -CUDART_INF_F ? 0.f : top;
+      for (int o = 1; o < 8; o <<= 1) top = higher(top, shuffled(top, o));
+      top = of_lane(top, lane & ~7);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         if (ml[k].x != -CUDART_INF_F || ml[k].y != 0.f) {  // (otherwise its sums are zeros, or were not written; NaN is not 0)
-          const float f = exp2_or_zero(ml[k].x - from);
+          const float f = rescale(Peak{ml[k].x, ml[k].z}, top);
           sum = fmaf(ml[k].y, f, sum);
           acc[0] = fmaf(y[k].x, f, acc[0]); acc[1] = fmaf(y[k].y, f, acc[1]);
           acc[2] = fmaf(y[k].z, f, acc[2]); acc[3] = fmaf(y[k].w, f, acc[3]);
@@ -1053,7 +1079,8 @@ __global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const
   const fdma_cache_attention_params& p = a.p;
   const fdma_cache& c = p.c;
   __shared__ int s_request;
-  __shared__ float s_top[4], s_sum[4], s_acc[4][D];
+  __shared__ Peak s_top[4];
+  __shared__ float s_sum[4], s_acc[4][D];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slot = static_cast<int>(blockIdx.x / p.h), head = static_cast<int>(blockIdx.x - static_cast<unsigned>(slot) * p.h);
   int r, token = slot, end = slot + 1;
@@ -1090,28 +1117,30 @@ __global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const
       base = a.partial + static_cast<int64_t>(row - (tile << a.row_shift)) * (D + 4);
       if (c0 == c1) continue;  // written by that CTA
     }
-    // each warp takes every fourth sum, six at a time, and scales to its own maximum
-    constexpr int E = D / 32, kAhead = 6;  // elements per lane
-    float acc[E], sum = 0.f, top = -CUDART_INF_F;
+    // each warp takes every fourth sum, four at a time, and scales to its own maximum
+    constexpr int E = D / 32, kAhead = 4;  // elements per lane
+    float acc[E], sum = 0.f;
+    Peak top{-CUDART_INF_F, 0.f};
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = 0.f;
     for (int x0 = c0 + warp; x0 <= c1; x0 += 4 * kAhead) {
-      float2 ml[kAhead], y[kAhead][E / 2];
+      float4 ml[kAhead];
+      float2 y[kAhead][E / 2];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int x = x0 + 4 * k;
-        ml[k] = make_float2(-CUDART_INF_F, 0.f);
+        ml[k] = make_float4(-CUDART_INF_F, 0.f, 0.f, 0.f);
         if (x <= c1) {
           const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
-          ml[k] = *reinterpret_cast<const float2*>(src + D);
+          ml[k] = *reinterpret_cast<const float4*>(src + D);
 #pragma unroll
           for (int i = 0; i < E / 2; ++i) y[k][i] = *reinterpret_cast<const float2*>(src + lane * E + 2 * i);
         }
       }
-      float now = top;
+      Peak now = top;
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) now = fmaxf(now, ml[k].x);
-      const float from = now == -CUDART_INF_F ? 0.f : now, f0 = exp2_or_zero(top - from);
+      for (int k = 0; k < kAhead; ++k) now = higher(now, Peak{ml[k].x, ml[k].z});
+      const float f0 = rescale(top, now);
       top = now;
       sum *= f0;
 #pragma unroll
@@ -1119,7 +1148,7 @@ __global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
         if (x0 + 4 * k <= c1) {
-          const float f = exp2_or_zero(ml[k].x - from);
+          const float f = rescale(Peak{ml[k].x, ml[k].z}, now);
           sum = fmaf(ml[k].y, f, sum);
 #pragma unroll
           for (int i = 0; i < E / 2; ++i) {
@@ -1135,13 +1164,12 @@ __global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const
 #pragma unroll
     for (int i = 0; i < E; ++i) s_acc[warp][lane * E + i] = acc[i];
     __syncthreads();
-    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-    const float from = top == -CUDART_INF_F ? 0.f : top;
+    top = higher(higher(s_top[0], s_top[1]), higher(s_top[2], s_top[3]));
     float f[4];
     sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      f[x] = exp2_or_zero(s_top[x] - from);
+      f[x] = rescale(s_top[x], top);
       sum = fmaf(s_sum[x], f[x], sum);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
