@@ -220,10 +220,9 @@ int check_tables(const fdma_tables_params* p) {
 int table_threads(int64_t n) { return static_cast<int>(std::min<int64_t>(kTableThreads, std::max<int64_t>(128, (n + 31) / 32 * 32))); }
 
 template <typename K>
-int table_smem(K kernel, int requests, size_t* bytes) {
+int table_smem(K kernel, int requests, std::atomic<uint64_t>& prepared, size_t* bytes) {
   *bytes = static_cast<size_t>(requests) * 12;
-  if (*bytes <= 40 * 1024) return 0;
-  return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(*bytes)));
+  return *bytes <= 40 * 1024 ? 0 : allow_smem_once(reinterpret_cast<const void*>(kernel), kMaxRequests * 12, prepared);
 }
 
 // ---- the writer ---------------------------------------------------------------------------------------------------
@@ -233,6 +232,7 @@ int table_smem(K kernel, int requests, size_t* bytes) {
 // 6 prompts of up to 2700 tokens (8 300 in all), 32 + 8 heads, d = 128 (176 MB): 49 us; without the queries 29, the queries alone 28.
 constexpr int kAppendThreads = kRotaryWarps * 32;
 constexpr int kAppendCtas = 4;  // per SM
+constexpr int kMaxBlock = 128, kMaxDim = 256;  // tokens of a block, head dimension
 struct AppendArgs {
   fdma_cache_append_params p;
   RotaryUnits key_units;    // of keys that are turned
@@ -460,8 +460,10 @@ int launch_append(AppendArgs a, cudaStream_t stream) {
   }
   auto kern = append_kernel<T, N, kInterleaved>;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return static_cast<int>(e);
+    static std::atomic<uint64_t> prepared{0};
+    const int most = kMaxBlock * factor_pitch<N>(kMaxDim / 2) * static_cast<int>(sizeof(float2));  // (what queries need is less)
+    const int st = allow_smem_once(reinterpret_cast<const void*>(kern), most, prepared);
+    if (st) return st;
   }
   const int64_t ctas = a.cache_ctas + query_ctas;
   if (ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
@@ -504,7 +506,8 @@ extern "C" int fdma_tables_extend(const fdma_tables_params* p, void* stream) {
   if (!p->cu_seqlens || !p->cu_blocks || !p->cu_chunks || (p->tokens && (!p->positions || !p->slots))) return FDMA_ERR_BAD_ARG;
   if (p->requests == 0 || !p->lengths_after || !p->granted) return FDMA_ERR_BAD_ARG;
   size_t smem;
-  st = table_smem(extend_kernel, p->requests, &smem);
+  static std::atomic<uint64_t> prepared{0};
+  st = table_smem(extend_kernel, p->requests, prepared, &smem);
   if (st) return st;
   // a CTA for 2048 tokens: beyond that filling takes longer than another CTA's sums
   const int ctas = std::max(1, std::min(sm_count(), p->tokens / 2048));
@@ -517,7 +520,8 @@ extern "C" int fdma_tables_truncate(const fdma_tables_params* p, void* stream) {
   if (st) return st;
   if (p->requests == 0) return FDMA_OK;
   size_t smem;
-  st = table_smem(truncate_kernel, p->requests, &smem);
+  static std::atomic<uint64_t> prepared{0};
+  st = table_smem(truncate_kernel, p->requests, prepared, &smem);
   if (st) return st;
   truncate_kernel<<<1, kTableThreads, smem, static_cast<cudaStream_t>(stream)>>>(*p, block_shift(p->block_size));
   return static_cast<int>(cudaGetLastError());

@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 64;
+constexpr int kMostRequests = 8192;
 constexpr int64_t kMostRows = 1 << 20;               // keys of all requests, what the forward kernel's tables hold
 constexpr int64_t kMostBytes = int64_t{1} << 32;     // of scratch
 
@@ -183,7 +184,7 @@ fdma_fwd_params forward_params(const fdma_cache_attention_params& p, char* ws) {
 }  // namespace
 
 bool cache_prompt_taken(const fdma_cache_attention_params& p) {
-  if (std::min(p.max_seqlen_q, p.c.tokens) < kPromptTokens || p.bias || p.kept_pos || p.c.requests > 8192) return false;
+  if (std::min(p.max_seqlen_q, p.c.tokens) < kPromptTokens || p.bias || p.kept_pos || p.c.requests > kMostRequests) return false;
   const int64_t keys = std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size);
   if (!prompt_pays(static_cast<int64_t>(p.c.tokens) * p.h * (keys + kTileKeys), keys, p.c.d)) return false;
   const int64_t rows = most_rows(p);
@@ -210,8 +211,10 @@ int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspac
   const size_t smem = (static_cast<size_t>(p.c.requests) + 1) * 8;
   const bool bf16 = p.dtype == FDMA_BF16;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(bf16 ? unpack_kernel<true> : unpack_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return static_cast<int>(e);
+    static std::atomic<uint64_t> prepared[2] = {};
+    const void* kern = bf16 ? reinterpret_cast<const void*>(unpack_kernel<true>) : reinterpret_cast<const void*>(unpack_kernel<false>);
+    const int st = allow_smem_once(kern, (kMostRequests + 1) * 8, prepared[bf16]);
+    if (st) return st;
   }
   const int64_t most_chunks = a.rows / kChunk + std::min<int64_t>(p.c.requests, p.c.tokens / kPromptTokens);
   const int ctas = static_cast<int>(std::min<int64_t>(most_chunks, 8 * sm_count()));

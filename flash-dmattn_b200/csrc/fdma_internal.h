@@ -138,7 +138,9 @@ int export_softmax_d(const fdma_bwd_params& bp, const float* dsum, int sq_r, cud
 // Number of SMs of the current device (cudaDevAttrMultiProcessorCount, cached per device).
 int sm_count();
 
-// Allows a kernel `bytes` of dynamic shared memory on the current device, once per device (`prepared`: a bit each).
+// Allows a kernel `bytes` of dynamic shared memory on the current device, once per device (`prepared`: a bit each). The limit belongs to
+// the kernel, whoever calls it: `bytes` is the most that any call needs, since one that set its own size could lower the limit
+// between another thread's setting and its launch.
 inline int allow_smem_once(const void* kernel, int bytes, std::atomic<uint64_t>& prepared) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);

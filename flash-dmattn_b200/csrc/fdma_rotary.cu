@@ -16,6 +16,8 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 4) rotary_kernel(const __gr
   rotate_tokens<T, N, kInterleaved>(a, static_cast<int64_t>(blockIdx.x) * kRotaryWarps + warp, s_factors + warp * rotary_warp_pairs<N>(a));
 }
 
+constexpr int kMaxRotaryDim = 4096;  // a CTA's factors are held in 160 KB, 192 KB in fp32
+
 template <typename T, int N, bool kInterleaved>
 int launch(const fdma_rotary_params& p, cudaStream_t stream) {
   const RotaryArgs a = rotary_args(p, N);
@@ -23,8 +25,10 @@ int launch(const fdma_rotary_params& p, cudaStream_t stream) {
   if (ctas > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
   const size_t smem = rotary_smem<N>(a);
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(rotary_kernel<T, N, kInterleaved>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return static_cast<int>(e);
+    static std::atomic<uint64_t> prepared{0};
+    const int most = kRotaryWarps * factor_pitch<N>(kMaxRotaryDim / 2) * static_cast<int>(sizeof(float2));
+    const int st = allow_smem_once(reinterpret_cast<const void*>(rotary_kernel<T, N, kInterleaved>), most, prepared);
+    if (st) return st;
   }
   rotary_kernel<T, N, kInterleaved><<<static_cast<unsigned>(ctas), kRotaryWarps * 32, smem, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
@@ -50,7 +54,7 @@ extern "C" int fdma_rotary(const fdma_rotary_params* pp, void* stream_) {
   if (p.h_k && (!p.k || !p.k_out)) return FDMA_ERR_BAD_ARG;
   if (p.rotary_dim <= 0 || p.rotary_dim % 2 || p.rotary_dim > p.d) return FDMA_ERR_BAD_ARG;
   if (p.positions && p.position_bits != 32 && p.position_bits != 64) return FDMA_ERR_BAD_ARG;
-  if (p.rotary_dim > 4096) return FDMA_ERR_UNSUPPORTED;  // a CTA's factors are held in 160 KB
+  if (p.rotary_dim > kMaxRotaryDim) return FDMA_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(p.h + p.h_k) * p.d > (1 << 24)) return FDMA_ERR_UNSUPPORTED;
   if (p.b == 0 || p.seqlen == 0) return FDMA_OK;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
