@@ -16,6 +16,7 @@ sequence under a per-query visibility mask (same example, and causal inside the 
 alignment of its own lengths), which the full-range kernels skip tile by tile -- one launch however many examples
 there are; larger packs go through `flash_sparse_attn_varlen_func`, which runs every example as a zero-copy slice.
 """
+import math
 import os
 from typing import NamedTuple, Optional
 
@@ -174,22 +175,40 @@ def _cached_attention_forward(query_states, key_states, value_states, attention_
                               softmax_scale: Optional[float] = None, window_size: Optional[int] = None, is_causal: bool = True,
                               target_dtype: Optional[torch.dtype] = None):
     """The step's keys and values (1, tokens, Hk, d) go into the cache, and its queries (1, tokens, H, d) attend over it: everything, or
-    with a bias of more than `window_size` keys the `window_size` keys of each request and kv head that it ranks highest. Returns
-    (1, tokens, H, d)."""
+    with a bias of more than `window_size` keys the `window_size` keys of each request that each row of the bias ranks highest: one
+    row for all heads, or one per kv head or query head. Returns (1, tokens, H, d). What the attention would refuse is refused here,
+    before anything is written."""
     if attention_mask is not None:
         raise ValueError("attention over a cache takes no attention_mask: the requests' lengths are in the step.")
     if query_states.shape[0] != 1 or key_states.shape[0] != 1:
         raise ValueError("attention over a cache takes the step's tokens as one row.")
     q, k, v, bias = fsa_peft_integration_check(query_states[0], key_states[0], value_states[0], attention_bias, target_dtype)
     cache, tables, step, frequencies, max_q, max_k = kv_cache
-    turned = cache_append(cache, tables, step, k, v, query=q if frequencies is not None else None, frequencies=frequencies)
-    q = q if turned is None else turned
+    R, H, Hk = step.lengths.shape[0], q.shape[1], k.shape[1]
+    if Hk == 0 or H % Hk:
+        raise ValueError("attention over a cache takes as many query heads for each kv head.")
+    if any(bound is not None and bound < 0 for bound in (max_q, max_k)):
+        raise ValueError("max_seqlen_q and max_seqlen_k must not be negative.")
+    if bias is not None:
+        if bias.dim() != 4 or bias.shape[0] not in (1, R) or bias.shape[1] not in (1, Hk, H) or bias.shape[2] != 1 or bias.shape[3] == 0:
+            raise ValueError("attention over a cache takes a bias ({1|requests}, {1|Hk|H}, 1, keys).")
+        if bias.dtype != q.dtype or bias.device != q.device:
+            raise ValueError("attention over a cache takes a bias of the query's dtype and device.")
+        if torch.is_grad_enabled() and bias.requires_grad:
+            raise ValueError("attention over a cache has no gradients: call it under torch.no_grad().")
     kept = None
     if bias is not None and window_size is not None and bias.shape[-1] > window_size:
-        keys = bias.shape[-1]
+        keys, low = bias.shape[-1], torch.finfo(bias.dtype).min
         valid = torch.arange(keys, device=bias.device) < step.lengths[:, None]
-        kept = create_kept_keys(bias.expand(step.lengths.shape[0], -1, -1, -1), valid, step.lengths.shape[0], 1, keys, window_size,
-                                torch.finfo(bias.dtype).min)
+        rows = bias.expand(R, -1, -1, -1)
+        if bias.shape[1] in (1, Hk):
+            kept = create_kept_keys(rows, valid, R, 1, keys, window_size, low)
+        else:  # the attention takes one list for each kv head: keys that any of its query heads keeps, hidden from the others
+            mask = create_mask(rows, valid, R, 1, keys, window_size, low)
+            bias = rows.masked_fill(~mask, -math.inf)
+            kept = mask.view(R, Hk, H // Hk, 1, keys).any(2)
+    turned = cache_append(cache, tables, step, k, v, query=q if frequencies is not None else None, frequencies=frequencies)
+    q = q if turned is None else turned
     out = flash_sparse_attn_cache_func(q, cache, tables, step, attn_mask=kept, attn_bias=bias, softmax_scale=softmax_scale,
                                        is_causal=is_causal, max_seqlen_q=max_q, max_seqlen_k=max_k)
     return out[None]
