@@ -1,0 +1,108 @@
+"""Attention of prompt parts over the 8-bit cache, in steps with enough work for the conversion to 16 bits. Every case says how many
+keys have to be converted, and the call through the C interface, whose scratch the test can read, says how many were: a threshold
+that is tuned cannot empty these tests."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import flash_sparse_attn as fsa
+from flash_sparse_attn import _lib
+from test_cabi_cache import Attention, Cache
+from test_gpu_cache import attend, check, dev, filled, ints  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def through_c(q, cache, tables, step, max_q=None, max_k=None, causal=True):
+    """(result, converted keys) of the call through the C interface; the last 256-byte piece of the scratch that holds requests + 1 numbers
+    is the converted keys, summed up."""
+    T, H, d = q.shape
+    R, width = tables.table.shape
+    c = Cache(k=cache.k.data_ptr(), v=cache.v.data_ptr(), k_scale=cache.k_scale.data_ptr(), v_scale=cache.v_scale.data_ptr(),
+              table=tables.table.data_ptr(), requests=R, width=width, num_blocks=cache.k.shape[0], block_size=tables.block_size, tokens=T,
+              h_k=cache.k.shape[1], d=d, **{n: getattr(step, n).data_ptr() for n in ("cu_seqlens", "lengths", "cu_blocks", "cu_chunks", "positions")})
+    out = torch.full_like(q, math.nan)
+    p = Attention(c=c, query=q.data_ptr(), out=out.data_ptr(), query_row_stride=q.stride(0), query_head_stride=q.stride(1),
+                  out_row_stride=out.stride(0), out_head_stride=out.stride(1), h=H, dtype=_lib.FDMA_BF16 if q.dtype == torch.bfloat16 else _lib.FDMA_FP16,
+                  is_causal=int(causal), max_seqlen_q=T if max_q is None else max_q, max_seqlen_k=width * tables.block_size if max_k is None else max_k,
+                  softmax_scale=d ** -0.5)
+    lib = _lib.load()
+    size, run = lib.fdma_cache_attention_workspace_bytes, lib.fdma_cache_attention
+    size.restype, size.argtypes = ctypes.c_size_t, [ctypes.c_void_p]
+    run.restype, run.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]
+    n = size(ctypes.byref(p))
+    ws = torch.full((max(n, 256),), 0xFF, dtype=torch.uint8, device=q.device)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), n
+    assert run(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == 0
+    at = n - -(-(R + 1) * 4 // 256) * 256
+    return out, int(ws[at:at + 4 * (R + 1)].view(torch.int32)[R]) if n else 0
+
+
+def prompts(dev, cached, new, H, Hk, d, bs, dtype, seed):  # noqa: F811
+    tables, cache, step, g = filled(dev, len(cached), cached, new, Hk, d, bs, seed)
+    T = sum(new)
+    kv = torch.randn((2, T, Hk, d), generator=g, device=dev).to(dtype)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    return tables, cache, step, torch.randn((T, H, d), generator=g, device=dev).to(dtype), g
+
+
+CASES = [  # cached, new, heads, kv heads, head dim, block size
+    ([500, 37, 0], [200, 260, 300], 32, 8, 128, 64), ([900, 3], [400, 33], 32, 4, 64, 16), ([700, 100, 0, 250], [310, 1, 420, 7], 32, 8, 80, 32),
+    ([1000, 0], [256, 1000], 16, 16, 96, 128), ([1500], [300], 16, 1, 256, 128), ([40, 5, 1300, 800], [1, 31, 1, 600], 32, 8, 128, 16),
+    ([60] * 40, [1] * 38 + [500, 300], 32, 8, 64, 32), ([0, 511, 77], [513, 32, 5], 16, 2, 256, 64), ([130, 0], [0, 700], 12, 12, 48, 16)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cached,new,H,Hk,d,bs", CASES)
+def test_prompt_parts(dev, dtype, cached, new, H, Hk, d, bs):  # noqa: F811
+    tables, cache, step, q, _ = prompts(dev, cached, new, H, Hk, d, bs, dtype, 41)
+    want = attend(q, cache, tables, step)
+    got, keys = through_c(q, cache, tables, step)
+    assert keys == sum(a + b for a, b in zip(cached, new) if b >= 32)
+    check(got, *want)
+    most = max(a + b for a, b in zip(cached, new))
+    assert through_c(q, cache, tables, step, max(new), most)[1] == keys
+    check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step), *want)
+    check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, max_seqlen_q=max(new), max_seqlen_k=most), *want)
+    check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, is_causal=False, softmax_scale=0.05),
+          *attend(q, cache, tables, step, scale=0.05, causal=False))
+
+
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 64), (256, 32)])
+def test_refused_requests_and_padding(dev, d, bs):  # noqa: F811
+    """A refused request of many tokens, padding behind the last one, and single tokens, beside converted ones."""
+    H, Hk, dtype = 16, 2, torch.bfloat16
+    cached, new = [600, 20, 10, 300], [280, 200, 1, 350]
+    tables, cache, _, g = filled(dev, 4, cached, new, Hk, d, bs, 42)
+    tables.truncate(ints(cached, dev))
+    new[1] = tables.table.shape[1] * bs + 1 - 20  # outgrows its row
+    T = sum(new) + 77
+    step = tables.extend(ints(new, dev), T)
+    assert step.granted.tolist() == [True, False, True, True]
+    kv = torch.randn((2, T, Hk, d), generator=g, device=dev).to(dtype)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    q = torch.randn((T, H, d), generator=g, device=dev).to(dtype)
+    got, keys = through_c(q, cache, tables, step)
+    assert keys == 880 + 650
+    check(got, *attend(q, cache, tables, step))
+    assert not bool(got[280:280 + new[1]].any()) and not bool(got[-77:].any())
+
+
+def test_captured_and_replayed(dev):  # noqa: F811
+    """In a CUDA graph, with contents that change between replays."""
+    tables, cache, step, q, g = prompts(dev, [400, 30], [250, 300], 32, 8, 128, 64, torch.bfloat16, 43)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fsa.flash_sparse_attn_cache_func(q, cache, tables, step)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fsa.flash_sparse_attn_cache_func(q, cache, tables, step)
+    for _ in range(3):
+        q.copy_(torch.randn(q.shape, generator=g, device=dev))
+        graph.replay()
+        assert torch.equal(out, fsa.flash_sparse_attn_cache_func(q, cache, tables, step))
+        check(out, *attend(q, cache, tables, step))
