@@ -25,7 +25,7 @@ struct UnpackArgs {
   fdma_cache c;
   int32_t* cu_k;
   void *k, *v;  // (rows, h_k, d)
-  int shift, max_keys, rows, heads;
+  int shift, max_keys, max_queries, rows, heads;
 };
 
 template <bool kBf16>
@@ -51,11 +51,14 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
   extern __shared__ int s_pre[];  // chunks, then rows, of the requests before
   __shared__ long long s_warp[kThreads / 32], s_pairs[kThreads / 32];
   __shared__ int s_block[4], s_longest[kThreads / 32];
+  __shared__ bool s_beyond;  // a request is beyond the caller's bounds, which this path does not cut as the other one does: none are converted
   const fdma_cache& c = a.c;
   const int R = c.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int *pre_chunks = s_pre, *pre_rows = s_pre + R + 1;
   long long carry = 0, pairs = 0;  // carry: rows << 32 | chunks; pairs: of a new token and a key, see prompt_pays
   int longest = 0;
+  if (tid == 0) s_beyond = false;
+  __syncthreads();
   for (int base = 0; base < R; base += kThreads) {
     const int r = base + tid;
     long long x = 0;
@@ -65,7 +68,9 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
       const int n = max(0, min(min(c.lengths[r], a.max_keys), c.width << a.shift));
       x = (static_cast<long long>(n) << 32) | ((n + kChunk - 1) / kChunk);
       my_length = n;
-      my_pairs = static_cast<long long>(n + kTileKeys) * (c.cu_seqlens[r + 1] - c.cu_seqlens[r]);
+      const int queries = c.cu_seqlens[r + 1] - c.cu_seqlens[r];
+      my_pairs = static_cast<long long>(n + kTileKeys) * queries;
+      if (c.lengths[r] > a.max_keys || queries > a.max_queries) s_beyond = true;
     }
     my_length = __reduce_max_sync(0xffffffffu, my_length);
 #pragma unroll
@@ -98,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
   if (tid == 0) pre_chunks[0] = pre_rows[0] = 0;
   __syncthreads();
   const int total_rows = pre_rows[R];
-  const bool taken = total_rows > 0 && prompt_pays(pairs * a.heads, longest, c.d);
+  const bool taken = total_rows > 0 && !s_beyond && prompt_pays(pairs * a.heads, longest, c.d);
   if (blockIdx.x == 0)
     for (int r = tid; r <= R; r += kThreads) a.cu_k[r] = taken ? pre_rows[r] : 0;
   const int total = taken ? pre_chunks[R] : 0;
@@ -206,6 +211,7 @@ int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspac
   a.v = ws + s.v;
   a.shift = shift;
   a.max_keys = p.max_seqlen_k;
+  a.max_queries = p.max_seqlen_q;
   a.rows = static_cast<int>(most_rows(p));
   a.heads = p.h;
   const size_t smem = (static_cast<size_t>(p.c.requests) + 1) * 8;

@@ -167,8 +167,9 @@ def flash_sparse_attn_cache_func(
     a `KeptKeys` ({1|requests}, {1|Hk}) or a bool tensor ({1|requests}, {1|Hk}, 1, keys), False or beyond its keys = masked out.
     attn_bias ({1|requests}, {1|Hk|H}, 1, keys), dtype of query, added to the scaled scores; 0 beyond its keys. softmax_scale
     defaults to d ** -0.5. max_seqlen_q, max_seqlen_k: bounds on the new tokens and on the length of any request, where the
-    host knows them (default: the step's tokens, the tables' width); what lies beyond a bound may be left out. They choose how the
-    work is split and how much scratch a call takes: pass them where you can.
+    host knows them (default: the step's tokens, the tables' width). They choose how the work is split and how much scratch a call
+    takes: pass them where you can. Where a request goes beyond them, its queries from max_seqlen_q on are 0 (the first always counts), and
+    keys from max_seqlen_k on are not seen; queries' positions stay those in the whole request.
 
     Returns (tokens, H, d). Rows of tokens behind the last request, of refused requests and of queries that see no key are 0. A key or
     value that is NaN reaches the queries that see it (of a request with 32 or more new tokens, earlier ones of its tile as well) and no

@@ -475,9 +475,9 @@ int fdma_cache_append(const fdma_cache_append_params* p, void* stream);
  * positions up to L - n + i (is_causal = 0: all L). bias, if given: dtype of query, ({requests|1}, {h|h_k|1}, 1, bias_keys), added
  * to the scaled scores, 0 for keys at bias_keys and beyond. kept_pos, if given: ascending positions ({requests|1}, {h_k|1},
  * kept_capacity) of the keys that are attended to, kept_count of them or as many as are below L. Rows of tokens that belong to
- * no request, of refused requests and of queries that see no key are 0. max_seqlen_q, max_seqlen_k: no request has more new
- * tokens, or more tokens; queries and keys beyond may be left out. workspace: 256-byte aligned; few, short requests
- * need none.
+ * no request, of refused requests and of queries that see no key are 0. max_seqlen_q, max_seqlen_k: bounds on a request's new
+ * tokens, and on its tokens: a query at max_seqlen_q (at least 1) or beyond is 0, and keys at max_seqlen_k or beyond are not
+ * seen, while the queries' positions are those in the whole request. workspace: 256-byte aligned; few, short requests need none.
  */
 typedef struct fdma_cache_attention_params {
   fdma_cache c;

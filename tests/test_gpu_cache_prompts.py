@@ -106,3 +106,17 @@ def test_captured_and_replayed(dev):  # noqa: F811
         graph.replay()
         assert torch.equal(out, fsa.flash_sparse_attn_cache_func(q, cache, tables, step))
         check(out, *attend(q, cache, tables, step))
+
+
+@pytest.mark.parametrize("cached,new,H,Hk,d,bs,max_q,max_k", [
+    ([600, 37], [300, 260], 32, 8, 128, 64, 300, 500), ([600, 37], [300, 260], 32, 8, 128, 64, 200, 900), ([500], [400], 16, 2, 64, 16, 400, 700),
+    ([700, 100], [310, 1], 32, 8, 80, 32, 300, 1000), ([5, 9], [3, 2], 8, 2, 64, 16, 2, 9)])
+def test_requests_beyond_the_bounds(dev, cached, new, H, Hk, d, bs, max_q, max_k):  # noqa: F811
+    """Queries from max_seqlen_q on are 0, keys from max_seqlen_k on are not seen, and the causal edge stays where the request's length
+    puts it: the same rule for few new tokens and for many."""
+    tables, cache, step, q, _ = prompts(dev, cached, new, H, Hk, d, bs, torch.bfloat16, 44)
+    seen = fsa.KeptKeys(torch.arange(max_k, dtype=torch.int32, device=dev).expand(1, 1, -1).contiguous(), ints([[max_k]], dev), None, max_k)
+    want, tol = attend(q, cache, tables, step, seen)
+    for first, n in zip(step.cu_seqlens.tolist(), new):
+        want[first + max_q:first + n] = 0
+    check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, max_seqlen_q=max_q, max_seqlen_k=max_k), want, tol)
