@@ -53,7 +53,8 @@ struct AttnArgs {
   float scale_log2;
   bool q_vec;              // queries in 16-byte vectors
   const int32_t* prompts;  // not null: rows of no request are written already, and if it points to a number above 0, those of
-                           // requests with kPromptTokens or more as well
+                           // requests with kPromptTokens or more as well, unless what was found says that they do not hold
+  const PromptFound* found;
   int cluster, tiles;      // CTAs that share a unit, and tiles of a request, where there are few units (kCluster)
   bool merge_requests;     // CTAs of the second kernel: kPromptTokens - 1 for each request, not one for every token
   float* partial;          // [cta][2][rows][D + 4]: sums over the values, then maximum, sum and the maximum's exponent
@@ -174,7 +175,7 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
   q.n = max(0, min(end, c.tokens) - q.token0);
   q.chunks = max(0, chunk1 - chunk0);
   q.rows = q.chunks ? min(q.n, a.p.max_seqlen_q) * a.group : 0;  // no chunks: refused
-  if (a.prompts && q.n >= kPromptTokens && *a.prompts > 0) q.rows = -1;
+  if (a.prompts && q.n >= kPromptTokens && *a.prompts > 0 && prompt_holds(*a.found)) q.rows = -1;
   if (a.list_chunks) q.chunks = a.list_chunks;
   return q;
 }
@@ -1357,6 +1358,7 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
       const int status = cache_prompt(p, a.shift, ws + pl.prompt_off, stream);
       if (status) return status;
       a.prompts = reinterpret_cast<const int32_t*>(ws + pl.prompt_off + cache_prompt_keys(p));
+      a.found = reinterpret_cast<const PromptFound*>(ws + pl.prompt_off + cache_prompt_found(p));
     }
     a.pre = reinterpret_cast<int32_t*>(ws + pl.sums_off);
     if (pl.sums) {

@@ -1,9 +1,10 @@
 // Attention of prompt parts over the paged 8-bit cache: requests with many new tokens at once.
 //
 // Tensor-bound: with n queries per key the keys are worth converting once. One kernel turns the requests' blocks into 16-bit keys and
-// values, packed request after request (8-bit numbers times a power of two: exact in bf16, and in fp16 as far as it reaches: what
-// is larger becomes its largest number); the packed-sequence forward kernel does the rest with tcgen05. The conversion is
-// memory-bound, 6 d bytes per key and kv head (read 2 d, write 4 d).
+// values, packed request after request; the packed-sequence forward kernel does the rest with tcgen05. The conversion is
+// memory-bound, 6 d bytes per key and kv head (read 2 d, write 4 d). 8-bit numbers times a power of two are exact in bf16. In fp16 they
+// are rounded to multiples of 2^-24 where they are that small, which is no coarser than fp16 keys and values are before they
+// enter the cache. What fp16 cannot hold is left to the other kernel (PromptFound): the call is then computed again from the 8 bits.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -24,6 +25,7 @@ constexpr int64_t kMostBytes = int64_t{1} << 32;     // of scratch
 struct UnpackArgs {
   fdma_cache c;
   int32_t* cu_k;
+  PromptFound* found;  // zeros before
   void *k, *v;  // (rows, h_k, d)
   int shift, max_keys, max_queries, rows, heads;
 };
@@ -38,10 +40,20 @@ __device__ __forceinline__ uint32_t pack_scaled(uint16_t two, float scale) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  if (fabsf(f.x) > 65504.f) f.x = copysignf(65504.f, f.x);
-  if (fabsf(f.y) > 65504.f) f.y = copysignf(65504.f, f.y);
   const __half2 v = __floats2half2_rn(f.x, f.y);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Whether eight 8-bit numbers times the scale are in fp16's range.
+__device__ __forceinline__ bool fits_fp16(uint2 x, float scale) {
+  bool fits = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint16_t two = static_cast<uint16_t>((i < 2 ? x.x : x.y) >> (16 * (i & 1)));
+    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+    fits &= fabsf(f.x * scale) <= 65504.f && fabsf(f.y * scale) <= 65504.f;
+  }
+  return fits;
 }
 
 // A CTA converts a 64-key chunk of a request, all heads of K and V, at a time. 2 x 16 048 keys, 8 heads, d = 128 (197 MB): 42 us, of which
@@ -51,6 +63,7 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
   extern __shared__ int s_pre[];  // chunks, then rows, of the requests before
   __shared__ long long s_warp[kThreads / 32], s_pairs[kThreads / 32];
   __shared__ int s_block[4], s_longest[kThreads / 32];
+  __shared__ uint32_t s_scales[2];
   __shared__ bool s_beyond;  // a request is beyond the caller's bounds, which this path does not cut as the other one does: none are converted
   const fdma_cache& c = a.c;
   const int R = c.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -107,6 +120,8 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
   if (blockIdx.x == 0)
     for (int r = tid; r <= R; r += kThreads) a.cu_k[r] = taken ? pre_rows[r] : 0;
   const int total = taken ? pre_chunks[R] : 0;
+  bool fits = true;
+  uint32_t largest = 0, smallest = 0;  // bits of V scales, the latter inverted
   // A thread keeps its eight columns and walks rows, and heads within a row: the loads of eight do not wait for one another.
   const int pieces = c.d / 8, row_step = kThreads / pieces, my_row = tid / pieces, column = (tid - my_row * pieces) * 8;
   for (int w = blockIdx.x; w < total; w += gridDim.x) {
@@ -135,6 +150,11 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
           for (int v = 0; v < 2; ++v) {
             const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v ? c.v : c.k) + from + head * head_step));
             const float scale = __ldg((v ? c.v_scale : c.k_scale) + at + head);
+            if (!kBf16 && scale > 65504.f / 448.f) fits &= fits_fp16(x, scale);
+            if (!kBf16 && v && scale > 0x1p-100f) {
+              largest = max(largest, __float_as_uint(scale));
+              smallest = max(smallest, ~__float_as_uint(scale));
+            }
             y[v] = make_uint4(pack_scaled<kBf16>(static_cast<uint16_t>(x.x), scale), pack_scaled<kBf16>(static_cast<uint16_t>(x.x >> 16), scale),
                               pack_scaled<kBf16>(static_cast<uint16_t>(x.y), scale), pack_scaled<kBf16>(static_cast<uint16_t>(x.y >> 16), scale));
           }
@@ -145,6 +165,19 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
     }
     __syncthreads();
   }
+  if (!fits) atomicOr(&a.found->unfit, 1);
+  if (!kBf16 && total > 0) {
+    if (tid == 0) s_scales[0] = s_scales[1] = 0;
+    __syncthreads();
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    smallest = __reduce_max_sync(0xffffffffu, smallest);
+    if (lane == 0) {
+      atomicMax(&s_scales[0], largest);
+      atomicMax(&s_scales[1], smallest);
+    }
+    __syncthreads();
+    if (tid < 2) atomicMax(tid ? &a.found->smallest : &a.found->largest, s_scales[tid]);
+  }
 }
 
 // At most so many keys: requests that have kPromptTokens new ones each, of the longest length.
@@ -153,14 +186,15 @@ int64_t most_rows(const fdma_cache_attention_params& p) {
   return requests * std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size);
 }
 struct Scratch {
-  size_t v, lse, cu_k, total;
+  size_t v, lse, found, cu_k, total;
 };
 Scratch scratch(const fdma_cache_attention_params& p) {
   Scratch s;
   const size_t kv = align256(static_cast<size_t>(most_rows(p)) * p.c.h_k * p.c.d * 2);
   s.v = kv;
   s.lse = 2 * kv;
-  s.cu_k = s.lse + align256(static_cast<size_t>(p.h) * p.c.tokens * sizeof(float));
+  s.found = s.lse + align256(static_cast<size_t>(p.h) * p.c.tokens * sizeof(float));
+  s.cu_k = s.found + align256(sizeof(PromptFound));
   s.total = s.cu_k + align256((static_cast<size_t>(p.c.requests) + 1) * sizeof(int32_t));
   return s;
 }
@@ -200,6 +234,7 @@ bool cache_prompt_taken(const fdma_cache_attention_params& p) {
 }
 size_t cache_prompt_workspace_bytes(const fdma_cache_attention_params& p) { return scratch(p).total; }
 size_t cache_prompt_keys(const fdma_cache_attention_params& p) { return scratch(p).cu_k + static_cast<size_t>(p.c.requests) * sizeof(int32_t); }
+size_t cache_prompt_found(const fdma_cache_attention_params& p) { return scratch(p).found; }
 
 int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspace, cudaStream_t stream) {
   char* ws = static_cast<char*>(workspace);
@@ -207,6 +242,7 @@ int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspac
   UnpackArgs a;
   a.c = p.c;
   a.cu_k = reinterpret_cast<int32_t*>(ws + s.cu_k);
+  a.found = reinterpret_cast<PromptFound*>(ws + s.found);
   a.k = ws;
   a.v = ws + s.v;
   a.shift = shift;
@@ -224,9 +260,11 @@ int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspac
   }
   const int64_t most_chunks = a.rows / kChunk + std::min<int64_t>(p.c.requests, p.c.tokens / kPromptTokens);
   const int ctas = static_cast<int>(std::min<int64_t>(most_chunks, 8 * sm_count()));
+  cudaError_t e = cudaMemsetAsync(a.found, 0, sizeof(PromptFound), stream);
+  if (e != cudaSuccess) return static_cast<int>(e);
   if (bf16) unpack_kernel<true><<<ctas, kThreads, smem, stream>>>(a);
   else unpack_kernel<false><<<ctas, kThreads, smem, stream>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
   return tc_fwd(forward_params(p, ws), stream, PackedSeqs{p.c.cu_seqlens, a.cu_k, p.c.requests});
 }

@@ -16,8 +16,9 @@ pytestmark = pytest.mark.gpu
 
 
 def through_c(q, cache, tables, step, max_q=None, max_k=None, causal=True):
-    """(result, converted keys) of the call through the C interface; the last 256-byte piece of the scratch that holds requests + 1 numbers
-    is the converted keys, summed up."""
+    """(result, converted keys whose results were used) of the call through the C interface; the scratch ends with what the conversion
+    came upon (256 bytes; not 0 at first: a number that does not fit; then the largest and inverted smallest V scale) and the
+    converted keys of the requests, summed up (requests + 1, in whole 256 bytes)."""
     T, H, d = q.shape
     R, width = tables.table.shape
     c = Cache(k=cache.k.data_ptr(), v=cache.v.data_ptr(), k_scale=cache.k_scale.data_ptr(), v_scale=cache.v_scale.data_ptr(),
@@ -37,7 +38,11 @@ def through_c(q, cache, tables, step, max_q=None, max_k=None, causal=True):
     p.workspace, p.workspace_bytes = ws.data_ptr(), n
     assert run(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == 0
     at = n - -(-(R + 1) * 4 // 256) * 256
-    return out, int(ws[at:at + 4 * (R + 1)].view(torch.int32)[R]) if n else 0
+    if not n:
+        return out, 0
+    unfit, largest, smallest = ws[at - 256:at - 244].view(torch.int32).tolist()
+    holds = unfit == 0 and (largest >> 23) - (~smallest >> 23) <= 8
+    return out, int(ws[at:at + 4 * (R + 1)].view(torch.int32)[R]) if holds else 0
 
 
 def prompts(dev, cached, new, H, Hk, d, bs, dtype, seed):  # noqa: F811
@@ -120,3 +125,26 @@ def test_requests_beyond_the_bounds(dev, cached, new, H, Hk, d, bs, max_q, max_k
     for first, n in zip(step.cu_seqlens.tolist(), new):
         want[first + max_q:first + n] = 0
     check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step, max_seqlen_q=max_q, max_seqlen_k=max_k), want, tol)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("scale", [2.0 ** -1, 2.0 ** 7, 2.0 ** 10])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_numbers_beyond_the_range_of_fp16(dev, dtype, scale, which):  # noqa: F811
+    """Keys or values of one block that are larger than fp16 holds count as they are, with fp16 queries too, and so do values that are large
+    beside others: results of converted ones are not used then."""
+    tables, cache, step, q, _ = prompts(dev, [600, 37], [300, 260], 32, 8, 128, 64, dtype, 45)
+    block = tables.table[0, 3].item()
+    (cache.k_scale if which == "k" else cache.v_scale)[block] = scale
+    x = getattr(cache, which).view(torch.uint8)[block]
+    x[:, 5, 7] = 0x7E  # 448
+    if which == "k":
+        q.mul_(2.0 ** -12)  # (scores near one another)
+    want, tol = attend(q, cache, tables, step)
+    got, keys = through_c(q, cache, tables, step)
+    beyond = want.abs() + tol > 65504  # results that are infinite, or nearly, when they are rounded to fp16
+    assert beyond.float().mean() < 0.01
+    for out in (got, fsa.flash_sparse_attn_cache_func(q, cache, tables, step)):
+        check(out.masked_fill(beyond, 0), want.masked_fill(beyond, 0), tol)
+    far = 448 * scale > 65504 or (which == "v" and scale > 2.0 ** -9 * 2.0 ** 8)
+    assert (keys == 0) == (dtype == torch.float16 and far)
