@@ -4,7 +4,8 @@
 // values, packed request after request; the packed-sequence forward kernel does the rest with tcgen05. The conversion is
 // memory-bound, 6 d bytes per key and kv head (read 2 d, write 4 d). 8-bit numbers times a power of two are exact in bf16. In fp16 they
 // are rounded to multiples of 2^-24 where they are that small, which is no coarser than fp16 keys and values are before they
-// enter the cache. What fp16 cannot hold is left to the other kernel (PromptFound): the call is then computed again from the 8 bits.
+// enter the cache. What fp16 cannot hold is left to the other kernel (PromptFound): the call is then computed again from the 8 bits. So
+// are NaN: in the forward kernel one in a value reaches the queries of its tile that do not see it, and one in a key may be lost.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -44,6 +45,9 @@ __device__ __forceinline__ uint32_t pack_scaled(uint16_t two, float scale) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+__device__ __forceinline__ bool has_nan(uint2 x) {
+  return ((((x.x & 0x7F7F7F7Fu) + 0x01010101u) | ((x.y & 0x7F7F7F7Fu) + 0x01010101u)) & 0x80808080u) != 0;
+}
 // Whether eight 8-bit numbers times the scale are in fp16's range.
 __device__ __forceinline__ bool fits_fp16(uint2 x, float scale) {
   bool fits = true;
@@ -150,6 +154,7 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
           for (int v = 0; v < 2; ++v) {
             const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v ? c.v : c.k) + from + head * head_step));
             const float scale = __ldg((v ? c.v_scale : c.k_scale) + at + head);
+            fits &= !has_nan(x) && scale <= 0x1p119f;
             if (!kBf16 && scale > 65504.f / 448.f) fits &= fits_fp16(x, scale);
             if (!kBf16 && v && scale > 0x1p-100f) {
               largest = max(largest, __float_as_uint(scale));

@@ -172,8 +172,7 @@ def flash_sparse_attn_cache_func(
     keys from max_seqlen_k on are not seen; queries' positions stay those in the whole request.
 
     Returns (tokens, H, d). Rows of tokens behind the last request, of refused requests and of queries that see no key are 0. A key or
-    value that is NaN reaches the queries that see it (of a request with 32 or more new tokens, earlier ones of its tile as well) and no
-    other request.
+    value that is NaN reaches the queries that see it and no others.
     Scores, probabilities' sums and outputs are accumulated in 32 bits; probabilities enter the second product in 16 bits.
     There are no gradients: a call that would need them raises."""
     args = _cache_args(cache, tables, step)

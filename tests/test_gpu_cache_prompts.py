@@ -148,3 +148,37 @@ def test_numbers_beyond_the_range_of_fp16(dev, dtype, scale, which):  # noqa: F8
         check(out.masked_fill(beyond, 0), want.masked_fill(beyond, 0), tol)
     far = 448 * scale > 65504 or (which == "v" and scale > 2.0 ** -9 * 2.0 ** 8)
     assert (keys == 0) == (dtype == torch.float16 and far)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,Hk,d,bs", [(32, 8, 128, 64), (32, 4, 64, 16), (16, 2, 256, 32)])
+def test_not_a_number_reaches_who_sees_it(dev, dtype, H, Hk, d, bs, which):  # noqa: F811
+    """NaN among the last tokens of a prompt: later queries of that request and head become NaN, all others stay as they are."""
+    cached, new, G = [500, 37, 700], [300, 260, 310], H // Hk
+    tables, cache, step, q, _ = prompts(dev, cached, new, H, Hk, d, bs, dtype, 46)
+    want, tol = attend(q, cache, tables, step)
+    assert through_c(q, cache, tables, step)[1] == sum(cached) + sum(new)
+    for r, token, head in ((0, 270, 0), (1, 101, 1), (1, 200, 1), (2, 309, 0)):
+        pos = cached[r] + token
+        getattr(cache, which).view(torch.uint8)[tables.table[r, pos // bs], head, pos % bs, 9] = 0xFF
+    assert through_c(q, cache, tables, step)[1] == 0
+    got = fsa.flash_sparse_attn_cache_func(q, cache, tables, step)
+    first = step.cu_seqlens.tolist()
+    hit = torch.zeros(got.shape[:2], dtype=torch.bool, device=dev)
+    for r, token, head in ((0, 270, 0), (1, 101, 1), (2, 309, 0)):
+        hit[first[r] + token:first[r + 1], head * G:(head + 1) * G] = True
+    assert bool(got[hit][:, 9].isnan().all()) and (which == "v" or bool(got[hit].isnan().all()))
+    assert bool(got[~hit].isfinite().all())
+    check(got[~hit], want[~hit], tol[~hit])
+
+
+def test_scales_that_16_bits_cannot_hold(dev):  # noqa: F811
+    """V scales up to 2^127: results that are in bf16's range are what they are with single tokens."""
+    tables, cache, step, q, _ = prompts(dev, [600, 37], [300, 260], 32, 8, 128, 64, torch.bfloat16, 47)
+    cache.v_scale.mul_(2.0 ** 100)
+    cache.v_scale[tables.table[0, 2], 3] = 2.0 ** 123
+    cache.v.view(torch.uint8)[tables.table[0, 2], 3] &= 0xB7  # (at most 15, so that 32 bits hold the numbers)
+    want, tol = attend(q, cache, tables, step)
+    check(fsa.flash_sparse_attn_cache_func(q, cache, tables, step), want, tol)
+    assert through_c(q, cache, tables, step)[1] == 0
