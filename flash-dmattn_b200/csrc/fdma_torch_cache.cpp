@@ -290,6 +290,8 @@ fdma_cache cache_params(const Cache& t, int64_t tokens) {
     need(x->scalar_type() == at::kFloat && x->dim() == 2 && x->is_contiguous() && x->size(0) == t.k.size(0) && x->size(1) == t.k.size(1) &&
              x->device() == t.k.device(),
          "the cache's scales must be two contiguous float32 tensors (blocks, kv heads)");
+  need(!(at::GradMode::is_enabled() && (t.k.requires_grad() || t.v.requires_grad() || t.k_scale.requires_grad() || t.v_scale.requires_grad())),
+       "the 8-bit cache has no gradients: call it under torch.no_grad()");
   check_block_size(t.k.size(2));
   need(t.k.size(3) > 0 && t.k.size(3) % 16 == 0 && t.k.size(3) <= 256, "the cache supports head dimensions that are multiples of 16 up to 256");
   need(t.k.size(0) > 0 && t.k.size(1) > 0, "the cache is empty");
