@@ -173,7 +173,11 @@ def flash_sparse_attn_cache_func(
 
     Returns (tokens, H, d). Rows of tokens behind the last request, of refused requests and of queries that see no key are 0. A key or
     value that is NaN reaches the queries that see it and no others.
-    Scores, probabilities' sums and outputs are accumulated in 32 bits; probabilities enter the second product in 16 bits.
+    Scores, probabilities' sums and outputs are accumulated in 32 bits. Probabilities enter the second product in fp16 (2^-11 of
+    themselves). Requests with 32 or more new tokens, without mask or bias, have their keys converted to the query's type where the step
+    has enough work for it; their probabilities are of that type (bf16: 2^-9). So what else is in a step can change how a result is
+    rounded. The conversion takes up to 2^20 keys, counted as requests that can have so many new tokens times max_seqlen_k, and 4 GiB
+    of scratch: a call whose bounds allow for more reads the 8 bits, as one does that comes upon NaN or numbers that 16 bits do not hold.
     There are no gradients: a call that would need them raises."""
     args = _cache_args(cache, tables, step)
     key_pos = count = None

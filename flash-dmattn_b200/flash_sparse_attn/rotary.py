@@ -111,8 +111,8 @@ def apply_rotary(
     tensors (key None: (query, None)); gradients flow to query and key, any number of times.
 
     bf16, fp16 or fp32, any strides with a head's elements side by side (others are copied first). positions: int32 or int64,
-    ({1|B}, S) or (S,), any value; None: 0 .. S - 1. Angles are exact to 2^-53 of the frequency at every position, sums are
-    32-bit and the results are rounded once."""
+    ({1|B}, S) or (S,), any value; None: 0 .. S - 1. Frequencies are held to 2^-65 of a turn per position and angles to
+    2^-32 of a turn (at position 10^6, too), sums are 32-bit and the results are rounded once."""
     native = _native.load()
     if not torch.compiler.is_compiling():
         out = native.rotary((query, key, positions, frequencies.turns), frequencies.interleaved, frequencies.amplitude, False)

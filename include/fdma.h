@@ -384,7 +384,7 @@ int fdma_merge_partials(const fdma_merge_params* p, void* stream);
  *   y1 = amplitude (x1 cos - x2 sin),  y2 = amplitude (x2 cos + x1 sin),  angle = position * frequency of the pair;
  * the rest is copied. Pairs are (i, i + rotary_dim / 2), or with `interleaved` (2 i, 2 i + 1). q (b, seqlen, h, d), k (b, seqlen,
  * h_k, d), h_k = 0: queries alone; strides in elements, innermost 1. turns (rotary_dim / 2): the frequencies in turns per
- * position as 64-bit fractions, frequency / (2 pi) * 2^64 (angles are then exact at any position). positions: int32 or int64
+ * position as 64-bit fractions, frequency / (2 pi) * 2^64 (angles are the exact products, modulo a turn, less at most 2^-32 turn). positions: int32 or int64
  * (position_bits) with the strides given, NULL: 0 .. seqlen - 1. inverse: by the negative angle, which is the gradient.
  * dtype BF16, FP16 or FP32; q_out and k_out do not overlap the inputs.
  */
