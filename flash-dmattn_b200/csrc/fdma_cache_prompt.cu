@@ -5,7 +5,8 @@
 // memory-bound, 6 d bytes per key and kv head (read 2 d, write 4 d). 8-bit numbers times a power of two are exact in bf16. In fp16 they
 // are rounded to multiples of 2^-24 where they are that small, which is no coarser than fp16 keys and values are before they
 // enter the cache. What fp16 cannot hold is left to the other kernel (PromptFound): the call is then computed again from the 8 bits. So
-// are NaN: in the forward kernel one in a value reaches the queries of its tile that do not see it, and one in a key may be lost.
+// are NaN in values: in the forward kernel one of them reaches the queries of its tile that do not see it. (In a key it does not: scores
+// are masked, not multiplied by 0.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
           for (int v = 0; v < 2; ++v) {
             const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v ? c.v : c.k) + from + head * head_step));
             const float scale = __ldg((v ? c.v_scale : c.k_scale) + at + head);
-            fits &= !has_nan(x) && scale <= 0x1p119f;
+            fits &= !(v && has_nan(x)) && scale <= 0x1p119f;
             if (!kBf16 && scale > 65504.f / 448.f) fits &= fits_fp16(x, scale);
             if (!kBf16 && v && scale > 0x1p-100f) {
               largest = max(largest, __float_as_uint(scale));

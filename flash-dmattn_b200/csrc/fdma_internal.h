@@ -126,7 +126,7 @@ bool cache_prompt_taken(const fdma_cache_attention_params& p);
 size_t cache_prompt_workspace_bytes(const fdma_cache_attention_params& p);
 size_t cache_prompt_keys(const fdma_cache_attention_params& p);
 // What the conversion comes upon, at cache_prompt_found in the scratch. The rows of the requests that were converted are to be
-// computed again where prompt_holds is false: a number is NaN or too large, or, in fp16, V scales are more than 2^8 apart. The forward
+// computed again where prompt_holds is false: a value is NaN, a number is too large, or, in fp16, V scales are more than 2^8 apart. The forward
 // kernel's probabilities are fp16 there, multiples of 2^-24 when small, and the values that such a probability meets must not be large beside
 // those of the likely keys: scales 2^8 apart add up to 2^-11 of a result over 64 large keys, 2^16 apart 2^-3.
 struct PromptFound {

@@ -177,7 +177,7 @@ def flash_sparse_attn_cache_func(
     themselves). Requests with 32 or more new tokens, without mask or bias, have their keys converted to the query's type where the step
     has enough work for it; their probabilities are of that type (bf16: 2^-9). So what else is in a step can change how a result is
     rounded. The conversion takes up to 2^20 keys, counted as requests that can have so many new tokens times max_seqlen_k, and 4 GiB
-    of scratch: a call whose bounds allow for more reads the 8 bits, as one does that comes upon NaN or numbers that 16 bits do not hold.
+    of scratch: a call whose bounds allow for more reads the 8 bits, as one does that comes upon NaN in a value or numbers that 16 bits do not hold.
     There are no gradients: a call that would need them raises."""
     args = _cache_args(cache, tables, step)
     key_pos = count = None
