@@ -165,6 +165,12 @@ def _reshape_padding_mask(attention_mask, batch_size, query_len, key_len):
     return attention_mask
 
 
+def _attach(mask, name, cache):
+    """Ties a cache to the mask's present contents. A tensor made in inference mode counts no edits, so nothing can be tied to it."""
+    if not mask.is_inference():
+        setattr(mask, name, (cache, mask._version))
+
+
 def _native_topk(attention_bias, attention_mask, window_size, min_dtype):
     """The plain top-k mask through the native host path (csrc/fdma_torch.cpp), with the caches `create_mask` attaches
     to it; None for inputs that path does not take."""
@@ -173,9 +179,9 @@ def _native_topk(attention_bias, attention_mask, window_size, min_dtype):
         return None
     mask = res[0]
     if len(res) == 4:
-        mask._fdma_kept = (KeptKeys(res[1], res[2], res[3], mask.shape[3]), mask._version)
+        _attach(mask, "_fdma_kept", KeptKeys(res[1], res[2], res[3], mask.shape[3]))
     elif len(res) == 3:
-        mask._fdma_packed = (PackedMask(res[1], res[2], mask.shape[3]), mask._version)
+        _attach(mask, "_fdma_packed", PackedMask(res[1], res[2], mask.shape[3]))
     return mask
 
 
@@ -214,7 +220,7 @@ def create_mask(
             # re-reading the bool mask and without a device read-back; the tensor's version counter ties the cache
             # to the mask's current contents (any in-place edit invalidates it).
             mask, kept = _topk_mask_with_positions(attention_bias, attention_mask, window_size, min_dtype)
-            mask._fdma_kept = (kept, mask._version)
+            _attach(mask, "_fdma_kept", kept)
             return mask
         if (rows > 1 and (block_size is None or block_size <= 1) and 0 < window_size <= attention_bias.shape[-1]
                 and attention_bias.is_cuda and attention_bias.dim() == 4):
@@ -225,7 +231,7 @@ def create_mask(
             mask, packed = _launch(attention_bias, attention_mask, window_size, min_dtype, None, _lib.MASK_TOPK,
                                    positions="bits_also")
             if packed is not None:
-                mask._fdma_packed = (packed, mask._version)
+                _attach(mask, "_fdma_packed", packed)
             return mask
         return topk_mask(attention_bias, attention_mask, window_size, min_dtype, block_size)
     if type == "relu":
