@@ -52,9 +52,8 @@ struct AttnArgs {
   int ctas;                // along the row of chunks
   float scale_log2;
   bool q_vec;              // queries in 16-byte vectors
-  const int32_t* prompts;  // not null: rows of no request are written already, and if it points to a number above 0, those of
-                           // requests with kPromptTokens or more as well, unless what was found says that they do not hold
-  const PromptFound* found;
+  const int32_t* prompts;  // not null: rows of no request are written already, and if it points to 0, those of requests with
+                           // kPromptTokens or more as well (one word: look-ups that read three more took 10 us of 340)
   int cluster, tiles;      // CTAs that share a unit, and tiles of a request, where there are few units (kCluster)
   bool merge_requests;     // CTAs of the second kernel: kPromptTokens - 1 for each request, not one for every token
   float* partial;          // [cta][2][rows][D + 4]: sums over the values, then maximum, sum and the maximum's exponent
@@ -153,13 +152,21 @@ __device__ __forceinline__ float exponent_of(float x) { return static_cast<float
 struct Peak {
   float m, z;
 };
-// log2 of a's ratio to b; NaN where neither has seen a key
+// No key seen yet: below any score of one that is (see bias_log2), and finite, so that differences are numbers.
+constexpr float kNone = -3.2e38f;
+// log2 of a's ratio to b
 __device__ __forceinline__ float above(const Peak& a, const Peak& b) { return (a.m - b.m) + (a.z - b.z); }
 __device__ __forceinline__ Peak higher(const Peak& a, const Peak& b) { return above(b, a) > 0.f ? b : a; }
 // what sums up to `from` are multiplied by in sums up to `to`, which is no lower
-__device__ __forceinline__ float rescale(const Peak& from, const Peak& to) { return from.m == -CUDART_INF_F ? 0.f : exp2f(above(from, to)); }
+__device__ __forceinline__ float rescale(const Peak& from, const Peak& to) { return exp2f(above(from, to)); }
 __device__ __forceinline__ Peak shuffled(const Peak& x, int mask) {
   return Peak{__shfl_xor_sync(0xffffffffu, x.m, mask), __shfl_xor_sync(0xffffffffu, x.z, mask)};
+}
+// Of eight lanes.
+__device__ __forceinline__ float largest8(float x) {
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
 }
 // (lanes that compared in different orders may hold different ones of two equal peaks)
 __device__ __forceinline__ Peak of_lane(const Peak& x, int lane) {
@@ -175,7 +182,7 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
   q.n = max(0, min(end, c.tokens) - q.token0);
   q.chunks = max(0, chunk1 - chunk0);
   q.rows = q.chunks ? min(q.n, a.p.max_seqlen_q) * a.group : 0;  // no chunks: refused
-  if (a.prompts && q.n >= kPromptTokens && *a.prompts > 0 && prompt_holds(*a.found)) q.rows = -1;
+  if (a.prompts && q.n >= kPromptTokens && *a.prompts == 0) q.rows = -1;
   if (a.list_chunks) q.chunks = a.list_chunks;
   return q;
 }
@@ -350,7 +357,9 @@ struct Layout {
   static constexpr int kCtas = D > 128 || ROWS > 8 ? 2 : 3;
 };
 
-template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster>
+// kBias: with a bias, dense (without one the loop is shorter by its loads: 14.2 us instead of 14.7 for 16 requests of drafts). With a list
+// of kept keys the bias is looked for when it runs.
+template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster, bool kBias>
 __global__ void __launch_bounds__(Layout<D, ROWS, kGather>::kThreads, Layout<D, ROWS, kGather>::kCtas)
 cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using L = Layout<D, ROWS, kGather>;
@@ -370,6 +379,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   unsigned char* smem = align_smem_1024(s_raw);
   const fdma_cache_attention_params& p = a.p;
   const fdma_cache& c = p.c;
+  const bool biased = kGather ? p.bias != nullptr : kBias;
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
@@ -388,7 +398,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     if constexpr (kCluster) return make_one_unit(a);
     else return make_units(a, s_held);
   }();
-  if (kCluster && tid < ROWS) s_part[tid] = make_float4(-CUDART_INF_F, 0.f, 0.f, 0.f);
+  if (kCluster && tid < ROWS) s_part[tid] = make_float4(kNone, 0.f, 0.f, 0.f);
   __syncthreads();
   int64_t w0, w1;
   if constexpr (kCluster) {
@@ -601,14 +611,14 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     for (int nt = 0; nt < kTiles; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[nt][e] = Peak{-CUDART_INF_F, 0.f};
+        top[nt][e] = Peak{kNone, 0.f};
         l[nt][e] = 0.f;
         const int rr = min(8 * nt + 2 * t + e, nrows - 1), row = row0 + rr;
         row_scale[nt][e] = s_row_scale[rr];
         const uint2 th = token_head(a, row);
         newest[nt][e] = p.is_causal ? min(length - 1, q.length - q.n + static_cast<int>(th.x)) : length - 1;
         const int head = u.hk * a.group + th.y;
-        bias_row[nt][e] = p.bias ? static_cast<const uint16_t*>(p.bias) + u.r * p.bias_batch_stride +
+        bias_row[nt][e] = biased ? static_cast<const uint16_t*>(p.bias) + u.r * p.bias_batch_stride +
                                        (p.h_bias == p.h ? head : p.h_bias == c.h_k ? u.hk : 0) * p.bias_head_stride
                                  : nullptr;
       }
@@ -626,7 +636,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     float g_scale_k = 0.f, g_scale_v = 1.f;  // as loaded: a conversion beside a load would wait for it
     uint16_t g_bias = 0;
     int g_pos = -1;
-    const bool head_bias = p.bias && p.h_bias == p.h && a.group > 1;
+    const bool head_bias = biased && p.h_bias == p.h && a.group > 1;
     auto load_pos = [&](int chunk) {
       const int slot = chunk * kChunk + warp * kSlice + (lane & 15);
       return chunk < last && slot < slots ? __ldg(list + slot) : -1;
@@ -655,7 +665,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const int64_t at = static_cast<int64_t>(block2) * c.h_k + u.hk;
         g_scale_k = __ldg(c.k_scale + at);
         g_scale_v = __ldg(c.v_scale + at);
-        g_bias = p.bias && !head_bias && pos2 < p.bias_keys ? __ldg(bias_row[0][0] + pos2) : static_cast<uint16_t>(0);
+        g_bias = biased && !head_bias && pos2 < p.bias_keys ? __ldg(bias_row[0][0] + pos2) : static_cast<uint16_t>(0);
       }
       if (i + kAhead < last) {
         constexpr int kLanes = D / 16;  // 16-byte pieces of a row
@@ -695,7 +705,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       if (kGather) gather(chunk);
       const int key = key_row(g);  // this lane's scores: keys pos0 + key, + 8
       uint16_t raw_bias[kTiles][2][2];
-      const bool with_bias = !kGather && p.bias, head_bias_dense = with_bias && head_bias;
+      constexpr bool with_bias = kBias;
+      const bool head_bias_dense = with_bias && head_bias;
       if (with_bias) {
 #pragma unroll
         for (int nt = 0; nt < kTiles; ++nt)
@@ -742,7 +753,13 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       const bool clean = !kGather && pos0 + kSlice <= sure && meta.x != 0.f;
       float x[kTiles][4];
       auto z_of = [&](int k) { return kGather ? key_meta[k >> 1].z : meta.z; };  // exponent of the V scale of score k
-      bool grows = false;  // (rounded down, so that no score above the maximum is missed)
+      // log2 of its ratio to the maximum
+      auto ratio = [&](int nt, int k) {
+        const float diff = x[nt][k] - top[nt][k & 1].m;
+        return diff + (z_of(k) - top[nt][k & 1].z);
+      };
+      float d[kTiles][4];
+      bool grows = false;
 #pragma unroll
       for (int nt = 0; nt < kTiles; ++nt) {
 #pragma unroll
@@ -763,7 +780,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             }
             if (!clean && (pos0 + (k >> 1) * 8 + key > newest[nt][k & 1] || meta.x == 0.f)) v = -CUDART_INF_F;
           }
-          grows |= v > __fadd_rd(top[nt][k & 1].m, top[nt][k & 1].z - z_of(k));
+          d[nt][k] = ratio(nt, k);
+          grows |= d[nt][k] > 0.f;
         }
       }
       uint32_t poisoned = 0;  // scores, a bit each, whose value is NaN
@@ -815,8 +833,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) now = higher(now, shuffled(now, off));
               now = of_lane(now, t);
-            } else {  // one block: the scores alone
-              now = Peak{fmaxf(x[nt][e], x[nt][2 + e]), meta.z};
+            } else {  // the scores alone: of one block, or with the exponents in them
+              now = Peak{fmaxf(x[nt][e], x[nt][2 + e]), z_of(e)};
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) now.m = fmaxf(now.m, __shfl_xor_sync(0xffffffffu, now.m, off));
             }
@@ -829,6 +847,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[nt][j][i >> 2][i & 3] *= corr[i & 1];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) d[nt][k] = ratio(nt, k);
         }
       }
       uint32_t pb[kTiles][2];  // P^T: queries' probabilities, keys 0-7 | 8-15
@@ -836,10 +856,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       for (int nt = 0; nt < kTiles; ++nt) {
         float e[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const Peak& y = top[nt][k & 1];
-          e[k] = exp2f((x[nt][k] - (y.m == -CUDART_INF_F ? 0.f : y.m)) + (z_of(k) - y.z));
-        }
+        for (int k = 0; k < 4; ++k) e[k] = exp2f(d[nt][k]);
         if (kGather) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) l[nt][k & 1] = fmaf(e[k], exp2f(-key_meta[k >> 1].z), l[nt][k & 1]);
@@ -989,24 +1006,22 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     for (int base = rank * 16; base < nrows * (D / 4); base += a.cluster * 16) {
       const int v = base + (tid >> 3), rr = min(v / (D / 4), nrows - 1), col = v % (D / 4) * 4;
       float4 ml[2], y[2];
-      Peak top{-CUDART_INF_F, 0.f};
       float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        ml[k] = make_float4(-CUDART_INF_F, 0.f, 0.f, 0.f);
+        ml[k] = make_float4(kNone, 0.f, 0.f, 0.f);
         if (of + 8 * k < a.cluster) {
           ml[k] = ld_cluster(shared_of(s_part + rr, of + 8 * k));
           y[k] = ld_cluster(shared_of(s_buf + rr * D + col, of + 8 * k));
         }
-        top = higher(top, Peak{ml[k].x, ml[k].z});
       }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) top = higher(top, shuffled(top, o));
-      top = of_lane(top, lane & ~7);
+      // maxima relative to about the largest, and the largest of those
+      const float about = largest8(fmaxf(ml[0].x + ml[0].z, ml[1].x + ml[1].z));
+      const float rel[2] = {(ml[0].x - about) + ml[0].z, (ml[1].x - about) + ml[1].z}, most = largest8(fmaxf(rel[0], rel[1]));
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (ml[k].x != -CUDART_INF_F || ml[k].y != 0.f) {  // (otherwise its sums are zeros, or were not written; NaN is not 0)
-          const float f = rescale(Peak{ml[k].x, ml[k].z}, top);
+        if (ml[k].x != kNone || ml[k].y != 0.f) {  // (otherwise its sums are zeros, or were not written; NaN is not 0)
+          const float f = exp2f(rel[k] - most);
           sum = fmaf(ml[k].y, f, sum);
           acc[0] = fmaf(y[k].x, f, acc[0]); acc[1] = fmaf(y[k].y, f, acc[1]);
           acc[2] = fmaf(y[k].z, f, acc[2]); acc[3] = fmaf(y[k].w, f, acc[3]);
@@ -1121,7 +1136,7 @@ __global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const
     // each warp takes every fourth sum, four at a time, and scales to its own maximum
     constexpr int E = D / 32, kAhead = 4;  // elements per lane
     float acc[E], sum = 0.f;
-    Peak top{-CUDART_INF_F, 0.f};
+    Peak top{kNone, 0.f};
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = 0.f;
     for (int x0 = c0 + warp; x0 <= c1; x0 += 4 * kAhead) {
@@ -1130,7 +1145,7 @@ __global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int x = x0 + 4 * k;
-        ml[k] = make_float4(-CUDART_INF_F, 0.f, 0.f, 0.f);
+        ml[k] = make_float4(kNone, 0.f, 0.f, 0.f);
         if (x <= c1) {
           const float* src = base + (2 * static_cast<int64_t>(x) + (x == c0)) * step;
           ml[k] = *reinterpret_cast<const float4*>(src + D);
@@ -1239,7 +1254,7 @@ int allow_wide_clusters_once(const void* kernel, std::atomic<uint64_t>& prepared
   return 0;
 }
 
-template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster>
+template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster, bool kBias>
 int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
   using L = Layout<D, ROWS, kGather>;
   const fdma_cache& c = a.p.c;
@@ -1252,7 +1267,7 @@ int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
     if (!st) st = encode_tmap_4d(&map_v, c.v, 1, dims, strides, box);
     if (st) return st;
   }
-  auto kern = cache_attend_kernel<D, ROWS, kGather, kBf16, kCluster>;
+  auto kern = cache_attend_kernel<D, ROWS, kGather, kBf16, kCluster, kBias>;
   static std::atomic<uint64_t> prepared{0}, wide{0};
   const int st_smem = allow_smem_once(reinterpret_cast<const void*>(kern), L::kTotal, prepared);
   if (st_smem) return st_smem;
@@ -1291,15 +1306,15 @@ int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
   cfg.numAttrs = 1;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, cache_merge_kernel<D, kBf16>, a));
 }
-template <int D, int ROWS, bool kCluster>
+template <int D, int ROWS, bool kCluster, bool kBf16>
 int launch_c(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
-  const bool bf16 = a.p.dtype == FDMA_BF16;
-  if (a.list_chunks) return bf16 ? launch<D, ROWS, true, true, kCluster>(a, pl, stream) : launch<D, ROWS, true, false, kCluster>(a, pl, stream);
-  return bf16 ? launch<D, ROWS, false, true, kCluster>(a, pl, stream) : launch<D, ROWS, false, false, kCluster>(a, pl, stream);
+  if (a.list_chunks) return launch<D, ROWS, true, kBf16, kCluster, false>(a, pl, stream);
+  return a.p.bias ? launch<D, ROWS, false, kBf16, kCluster, true>(a, pl, stream) : launch<D, ROWS, false, kBf16, kCluster, false>(a, pl, stream);
 }
 template <int D, int ROWS>
 int launch_t(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
-  return pl.cluster ? launch_c<D, ROWS, true>(a, pl, stream) : launch_c<D, ROWS, false>(a, pl, stream);
+  if (a.p.dtype == FDMA_BF16) return pl.cluster ? launch_c<D, ROWS, true, true>(a, pl, stream) : launch_c<D, ROWS, false, true>(a, pl, stream);
+  return pl.cluster ? launch_c<D, ROWS, true, false>(a, pl, stream) : launch_c<D, ROWS, false, false>(a, pl, stream);
 }
 
 int check_attention(const fdma_cache_attention_params* pp) {
@@ -1357,8 +1372,7 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
     if (pl.prompts) {
       const int status = cache_prompt(p, a.shift, ws + pl.prompt_off, stream);
       if (status) return status;
-      a.prompts = reinterpret_cast<const int32_t*>(ws + pl.prompt_off + cache_prompt_keys(p));
-      a.found = reinterpret_cast<const PromptFound*>(ws + pl.prompt_off + cache_prompt_found(p));
+      a.prompts = reinterpret_cast<const int32_t*>(ws + pl.prompt_off + cache_prompt_again(p));
     }
     a.pre = reinterpret_cast<int32_t*>(ws + pl.sums_off);
     if (pl.sums) {

@@ -4,7 +4,7 @@
 // values, packed request after request; the packed-sequence forward kernel does the rest with tcgen05. The conversion is
 // memory-bound, 6 d bytes per key and kv head (read 2 d, write 4 d). 8-bit numbers times a power of two are exact in bf16. In fp16 they
 // are rounded to multiples of 2^-24 where they are that small, which is no coarser than fp16 keys and values are before they
-// enter the cache. What fp16 cannot hold is left to the other kernel (PromptFound): the call is then computed again from the 8 bits. So
+// enter the cache. What fp16 cannot hold is left to the other kernel (PromptFound): the rows are then computed again from the 8 bits. So
 // are NaN in values: in the forward kernel one of them reaches the queries of its tile that do not see it. (In a key it does not: scores
 // are masked, not multiplied by 0.)
 #include <cuda_bf16.h>
@@ -12,6 +12,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <cstddef>
 
 #include "fdma_internal.h"
 
@@ -23,6 +24,15 @@ constexpr int kChunk = 64;
 constexpr int kMostRequests = 8192;
 constexpr int64_t kMostRows = 1 << 20;               // keys of all requests, what the forward kernel's tables hold
 constexpr int64_t kMostBytes = int64_t{1} << 32;     // of scratch
+
+// What the conversion comes upon. In fp16, V scales may be up to 2^8 apart: the forward kernel's probabilities are fp16 then, multiples
+// of 2^-24 when small, and values that such a probability meets must not be large beside those of the likely keys (scales 2^8 apart
+// add up to 2^-11 of a result over 64 large keys, 2^16 apart 2^-3).
+struct PromptFound {
+  int32_t again;               // not 0: the rows are to be computed from the 8 bits
+  uint32_t largest, smallest;  // bits of the V scales, the latter inverted
+};
+constexpr int kMostApart = 8;
 
 struct UnpackArgs {
   fdma_cache c;
@@ -171,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
     }
     __syncthreads();
   }
-  if (!fits) atomicOr(&a.found->unfit, 1);
+  if (!fits || (!taken && blockIdx.x == 0 && tid == 0)) atomicOr(&a.found->again, 1);
   if (!kBf16 && total > 0) {
     if (tid == 0) s_scales[0] = s_scales[1] = 0;
     __syncthreads();
@@ -182,7 +192,13 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
       atomicMax(&s_scales[1], smallest);
     }
     __syncthreads();
-    if (tid < 2) atomicMax(tid ? &a.found->smallest : &a.found->largest, s_scales[tid]);
+    if (tid == 0) {  // of two CTAs whose scales are too far apart, the one that looks later sees both
+      atomicMax(&a.found->largest, s_scales[0]);
+      atomicMax(&a.found->smallest, s_scales[1]);
+      __threadfence();
+      const uint32_t high = atomicMax(&a.found->largest, 0u), low = ~atomicMax(&a.found->smallest, 0u);
+      if (static_cast<int>(high >> 23) - static_cast<int>(low >> 23) > kMostApart) atomicOr(&a.found->again, 1);
+    }
   }
 }
 
@@ -239,8 +255,7 @@ bool cache_prompt_taken(const fdma_cache_attention_params& p) {
   return tc_fwd_supported(forward_params(p, reinterpret_cast<char*>(uintptr_t{256})));
 }
 size_t cache_prompt_workspace_bytes(const fdma_cache_attention_params& p) { return scratch(p).total; }
-size_t cache_prompt_keys(const fdma_cache_attention_params& p) { return scratch(p).cu_k + static_cast<size_t>(p.c.requests) * sizeof(int32_t); }
-size_t cache_prompt_found(const fdma_cache_attention_params& p) { return scratch(p).found; }
+size_t cache_prompt_again(const fdma_cache_attention_params& p) { return scratch(p).found + offsetof(PromptFound, again); }
 
 int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspace, cudaStream_t stream) {
   char* ws = static_cast<char*>(workspace);

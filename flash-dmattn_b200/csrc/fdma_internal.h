@@ -120,23 +120,11 @@ constexpr int kPromptTokens = 32, kTileKeys = 800;
 __host__ __device__ inline bool prompt_pays(int64_t work, int64_t longest, int d) { return work >= 2600000 + (d > 128 ? 3700 : 5500) * longest; }
 int check_cache(const fdma_cache& c);
 // Whether the call may have such requests, and scratch and layouts for them. Then cache_prompt writes all rows, those of other
-// requests 0; the number of converted keys is at cache_prompt_keys in the scratch, 0 if the requests have too few tokens together and
-// none are converted.
+// requests 0; at cache_prompt_again in the scratch is 0, or a number above 0 if the rows of the requests with so many tokens are still
+// to be computed: they have too few tokens together, and none are converted, or the conversion came upon numbers that it cannot hold.
 bool cache_prompt_taken(const fdma_cache_attention_params& p);
 size_t cache_prompt_workspace_bytes(const fdma_cache_attention_params& p);
-size_t cache_prompt_keys(const fdma_cache_attention_params& p);
-// What the conversion comes upon, at cache_prompt_found in the scratch. The rows of the requests that were converted are to be
-// computed again where prompt_holds is false: a value is NaN, a number is too large, or, in fp16, V scales are more than 2^8 apart. The forward
-// kernel's probabilities are fp16 there, multiples of 2^-24 when small, and the values that such a probability meets must not be large beside
-// those of the likely keys: scales 2^8 apart add up to 2^-11 of a result over 64 large keys, 2^16 apart 2^-3.
-struct PromptFound {
-  int32_t unfit;
-  uint32_t largest, smallest;  // bits of the V scales, the latter inverted
-};
-__host__ __device__ inline bool prompt_holds(const PromptFound& f) {
-  return f.unfit == 0 && static_cast<int>(f.largest >> 23) - static_cast<int>(~f.smallest >> 23) <= 8;
-}
-size_t cache_prompt_found(const fdma_cache_attention_params& p);
+size_t cache_prompt_again(const fdma_cache_attention_params& p);
 int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspace, cudaStream_t stream);
 
 // ---- helpers -----------------------------------------------------------------------------------

@@ -17,8 +17,8 @@ pytestmark = pytest.mark.gpu
 
 def through_c(q, cache, tables, step, max_q=None, max_k=None, causal=True):
     """(result, converted keys whose results were used) of the call through the C interface; the scratch ends with what the conversion
-    came upon (256 bytes; not 0 at first: a number that does not fit; then the largest and inverted smallest V scale) and the
-    converted keys of the requests, summed up (requests + 1, in whole 256 bytes)."""
+    came upon (256 bytes; not 0 at first: they are computed again) and the converted keys of the requests, summed up (requests + 1,
+    in whole 256 bytes)."""
     T, H, d = q.shape
     R, width = tables.table.shape
     c = Cache(k=cache.k.data_ptr(), v=cache.v.data_ptr(), k_scale=cache.k_scale.data_ptr(), v_scale=cache.v_scale.data_ptr(),
@@ -40,9 +40,9 @@ def through_c(q, cache, tables, step, max_q=None, max_k=None, causal=True):
     at = n - -(-(R + 1) * 4 // 256) * 256
     if not n:
         return out, 0
-    unfit, largest, smallest = ws[at - 256:at - 244].view(torch.int32).tolist()
-    holds = unfit == 0 and (largest >> 23) - (~smallest >> 23) <= 8
-    return out, int(ws[at:at + 4 * (R + 1)].view(torch.int32)[R]) if holds else 0
+    again, keys = int(ws[at - 256:at - 252].view(torch.int32)), int(ws[at:at + 4 * (R + 1)].view(torch.int32)[R])
+    assert keys > 0 or again
+    return out, 0 if again else keys
 
 
 def prompts(dev, cached, new, H, Hk, d, bs, dtype, seed):  # noqa: F811
