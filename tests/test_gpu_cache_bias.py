@@ -17,7 +17,7 @@ LAYOUTS = [  # cached, new, heads, kv heads, head dim, block size
     ([200, 130, 64], [1, 1, 1], 4, 2, 64, 32), ([5000], [1], 8, 2, 128, 64), ([700, 0, 12], [5, 9, 1], 12, 4, 128, 16),
     ([300, 90], [3, 40], 8, 2, 256, 32), ([150] * 140, [1] * 140, 2, 1, 16, 16)]
 BIASES = [  # type, bias, whether queries may be other than 0: next to the type's lowest number their scores count for nothing
-    (torch.bfloat16, torch.finfo(torch.bfloat16).min, True), (torch.bfloat16, -1e9, False), (torch.bfloat16, -1.2e7, False),
+    (torch.bfloat16, torch.finfo(torch.bfloat16).min, True), (torch.bfloat16, torch.finfo(torch.bfloat16).max, True), (torch.bfloat16, -1e9, False), (torch.bfloat16, -1.2e7, False),
     (torch.float16, torch.finfo(torch.float16).min, False)]
 
 
@@ -70,7 +70,7 @@ def test_rows_of_one_large_bias_are_averages(dev, cached, new, H, Hk, d, bs, dty
     assert not bool(got[(number == 0).expand_as(got)].any())
 
 
-@pytest.mark.parametrize("value", [-1e9, -3e4, 3e4, 1e9])
+@pytest.mark.parametrize("value", [-1e9, -3e4, 3e4, 1e9, torch.finfo(torch.bfloat16).min, torch.finfo(torch.bfloat16).max])
 def test_keys_without_the_large_bias(dev, value):  # noqa: F811
     """Keys of two biases far apart: those of the larger one alone count, an average over them with queries of 0."""
     tables, cache, step, g = filled(dev, 2, [900, 70], [1, 3], 2, 128, 16, 32)
@@ -82,6 +82,23 @@ def test_keys_without_the_large_bias(dev, value):  # noqa: F811
     visible = bias[:, :, 0] == bias.amax()
     mean, size, number = averages(cache, tables, step, 8, visible)
     q = torch.zeros((4, 8, 128), device=dev, dtype=torch.bfloat16)
+    for t in (tables, widen(tables)):
+        got = fsa.flash_sparse_attn_cache_func(q, cache, t, step, None, bias).double()
+        tol = 2.0 ** -8 * mean.abs() + (2.0 ** -11 + number * 2.0 ** -23) * size + 1e-38
+        assert bool(((got - mean).abs() <= tol).all())
+
+
+def test_the_lowest_beside_the_highest(dev):  # noqa: F811
+    """Half of the keys at the type's lowest number, the others at its highest: the latter alone count; -inf beside both hides."""
+    tables, cache, step, g = filled(dev, 2, [900, 70], [1, 3], 2, 128, 16, 35)
+    kv = torch.randn((2, 4, 2, 128), generator=g, device=dev).to(torch.bfloat16)
+    fsa.cache_append(cache, tables, step, kv[0], kv[1])
+    cache.v_scale.copy_(torch.exp2(torch.randint(-12, -2, cache.v_scale.shape, generator=g, device=dev).float()))
+    bias = torch.full((2, 2, 1, 901), torch.finfo(torch.bfloat16).min, device=dev, dtype=torch.bfloat16)
+    bias[..., 1::4] = torch.finfo(torch.bfloat16).max
+    bias[..., 3::4] = -math.inf
+    mean, size, number = averages(cache, tables, step, 8, bias[:, :, 0] > 0)
+    q = torch.randn((4, 8, 128), generator=g, device=dev).to(torch.bfloat16)
     for t in (tables, widen(tables)):
         got = fsa.flash_sparse_attn_cache_func(q, cache, t, step, None, bias).double()
         tol = 2.0 ** -8 * mean.abs() + (2.0 ** -11 + number * 2.0 ** -23) * size + 1e-38

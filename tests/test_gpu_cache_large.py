@@ -37,6 +37,24 @@ def test_blocks_beyond_4_gib(dev):  # noqa: F811
         assert torch.equal(a.view(torch.uint8), b[many - few:].view(torch.uint8))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_beyond_2_to_the_31_elements(dev, interleaved):  # noqa: F811
+    S, H, d = 70000, 256, 128
+    assert S * H * d > 2 ** 31
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    f = fsa.rotary_frequencies(96, interleaved=interleaved, device=dev)
+    x = torch.empty((1, S, H, d), device=dev, dtype=torch.bfloat16)
+    g = torch.Generator(device=dev).manual_seed(63)
+    for at in (0, S // 2, S - 3):
+        x[:, at:at + 3] = torch.randn((1, 3, H, d), generator=g, device=dev).to(torch.bfloat16)
+    out = fsa.apply_rotary(x, x[:, :, :1], f)
+    for at in (0, S // 2, S - 3):
+        part = x[:, at:at + 3].contiguous()
+        want = fsa.apply_rotary(part, part[:, :, :1].contiguous(), f, torch.arange(at, at + 3, device=dev))
+        assert torch.equal(out[0][:, at:at + 3], want[0]) and torch.equal(out[1][:, at:at + 3], want[1])
+
+
 def test_tensors_without_elements(dev):  # noqa: F811
     f = fsa.rotary_frequencies(64, device=dev)
     for shape in ((0, 5, 2, 64), (3, 0, 2, 64), (0, 2, 64)):
