@@ -833,7 +833,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) now = higher(now, shuffled(now, off));
               now = of_lane(now, t);
-            } else {  // the scores alone: of one block, or with the exponents in them
+            } else {  // of one block: the scores alone
               now = Peak{fmaxf(x[nt][e], x[nt][2 + e]), z_of(e)};
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) now.m = fmaxf(now.m, __shfl_xor_sync(0xffffffffu, now.m, off));
