@@ -1,7 +1,7 @@
 """Attention with a sliding window and sink tokens, in training, on packed sequences and over the paged 8-bit cache, and the verification
 of drafted tokens. Each case is a dict of plain values:
 
-  op        "window"  flash_sparse_attn_func           "packed"  flash_sparse_attn_varlen_func
+  op        "window"  flash_sparse_attn_window_func    "packed"  flash_sparse_attn_window_varlen_func
             "cache"   flash_sparse_attn_cache_func     "verify"  verify_drafts
   heads, kv_heads, head_dim, dtype; window (keys that a query sees, its own among them), sinks (first keys that stay visible)
   batch, seqlen, past (keys before the first query), padded (a mask of the keys that are there), train: with the gradients     window
@@ -402,11 +402,10 @@ def _own(s):
     fsa, c = _package(), s["case"]
     if c["op"] in ("window", "packed"):
         if c["op"] == "window":
-            out = fsa.flash_sparse_attn_func(s["q"], s["k"], s["v"], attn_mask=s.get("mask"), is_causal=True, sliding_window=c["window"],
-                                             sink_tokens=c["sinks"])
+            out = fsa.flash_sparse_attn_window_func(s["q"], s["k"], s["v"], c["window"], c["sinks"], attn_mask=s.get("mask"))
         else:
-            out = fsa.flash_sparse_attn_varlen_func(s["q"], s["k"], s["v"], s["cu"], s["cu"], s["longest"], s["longest"], is_causal=True,
-                                                    sliding_window=c["window"], sink_tokens=c["sinks"])
+            out = fsa.flash_sparse_attn_window_varlen_func(s["q"], s["k"], s["v"], s["cu"], s["cu"], s["longest"], s["longest"],
+                                                           c["window"], c["sinks"])
         return [out, *torch.autograd.grad(out, (s["q"], s["k"], s["v"]), s["dout"])] if c["train"] else [out]
     step = fsa.CacheStep(**s["step"])
     if c["op"] == "verify":
