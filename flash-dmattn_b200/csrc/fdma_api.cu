@@ -84,6 +84,20 @@ bool packed_ok(const fdma_fwd_params& p, const PackedSeqs& s) {
   return s.cu_q && s.cu_k && s.n > 0 && s.n <= (1 << 24) && p.b == 1 && !p.mask && !p.bias && !p.key_pos && (p.path == FDMA_PATH_AUTO || p.path == FDMA_PATH_TCGEN05);
 }
 
+// Sliding window: causal, a mask broadcast over the queries or none, no bias, no gathered keys; packed sequences take no mask.
+int check_window(const fdma_fwd_params& p, int32_t window, int32_t sinks, const int32_t* cu_q, const int32_t* cu_k, int32_t n) {
+  if (window <= 0 || sinks < 0 || n < 0 || (n > 0) != (cu_q != nullptr) || (n > 0) != (cu_k != nullptr) || !p.is_causal) return FDMA_ERR_BAD_ARG;
+  if (p.bias || p.key_pos || p.mask_bits || (p.mask && p.mask_row_stride != 0 && p.seqlen_q != 1)) return FDMA_ERR_UNSUPPORTED;
+  if (p.path != FDMA_PATH_AUTO && p.path != FDMA_PATH_TCGEN05) return FDMA_ERR_UNSUPPORTED;
+  return n > 0 && !packed_ok(p, PackedSeqs{cu_q, cu_k, n}) ? FDMA_ERR_UNSUPPORTED : 0;
+}
+// What the kernels compare positions with. At most seqlen_k each: more makes no difference.
+Window window_of(const fdma_fwd_params& p, int32_t window, int32_t sinks) {
+  Window w;
+  w.keys = window < p.seqlen_k ? window : (p.seqlen_k > 0 ? p.seqlen_k : 1);
+  w.sinks = sinks < p.seqlen_k ? sinks : p.seqlen_k;
+  return w;
+}
 // Normalised copy: absent mask/bias get head count 1 so head-ratio arithmetic never divides by zero, and
 // causal is dropped for single-query calls (flash_api.cpp:441).
 fdma_fwd_params normalise(const fdma_fwd_params& in) {
@@ -96,6 +110,13 @@ fdma_fwd_params normalise(const fdma_fwd_params& in) {
     p.key_pos = nullptr;
     p.h_pos = 1;
   }
+  return p;
+}
+
+// The same for a sliding window. A single query stays causal: it has a position.
+fdma_fwd_params normalise_window(const fdma_fwd_params& in) {
+  fdma_fwd_params p = normalise(in);
+  p.is_causal = 1;
   return p;
 }
 
@@ -301,6 +322,40 @@ int fdma_bwd_varlen(const fdma_bwd_params* pp, const int32_t* cu_q, const int32_
   const PackedSeqs seqs = {cu_q, cu_k, n};
   if (!packed_ok(p.f, seqs) || p.dbias || p.scatter_pos || p.f.d > 128 || !tc_bwd_supported(p)) return FDMA_ERR_UNSUPPORTED;
   return tc_bwd(p, static_cast<cudaStream_t>(stream_), seqs);
+}
+
+int fdma_fwd_window(const fdma_fwd_params* pp, int32_t window, int32_t sinks, const int32_t* cu_q, const int32_t* cu_k, int32_t n, void* stream_) {
+  if (!pp) return FDMA_ERR_BAD_ARG;
+  int st = validate_fwd(*pp);
+  if (!st) st = check_window(*pp, window, sinks, cu_q, cu_k, n);
+  if (st) return st;
+  st = check_arch();
+  if (st) return st;
+  const fdma_fwd_params p = normalise_window(*pp);
+  if (!tc_fwd_supported(p)) return FDMA_ERR_UNSUPPORTED;
+  return tc_fwd(p, static_cast<cudaStream_t>(stream_), PackedSeqs{cu_q, cu_k, n}, window_of(p, window, sinks));
+}
+
+size_t fdma_bwd_window_workspace_bytes(const fdma_bwd_params* pp, int32_t window, int32_t sinks, int32_t n) {
+  if (!pp || window <= 0 || sinks < 0 || n < 0 || validate_bwd(*pp)) return 0;
+  fdma_bwd_params p = *pp;
+  p.f = normalise_window(pp->f);
+  const Window w = window_of(p.f, window, sinks);
+  return tc_bwd_window_supported(p, w, n) ? tc_bwd_window_workspace_bytes(p, w, n) : 0;
+}
+
+int fdma_bwd_window(const fdma_bwd_params* pp, int32_t window, int32_t sinks, const int32_t* cu_q, const int32_t* cu_k, int32_t n, void* stream_) {
+  if (!pp) return FDMA_ERR_BAD_ARG;
+  int st = validate_bwd(*pp);
+  if (!st) st = check_window(pp->f, window, sinks, cu_q, cu_k, n);
+  if (st) return st;
+  st = check_arch();
+  if (st) return st;
+  fdma_bwd_params p = *pp;
+  p.f = normalise_window(pp->f);
+  const Window w = window_of(p.f, window, sinks);
+  if (!tc_bwd_window_supported(p, w, n)) return FDMA_ERR_UNSUPPORTED;
+  return tc_bwd_window(p, static_cast<cudaStream_t>(stream_), PackedSeqs{cu_q, cu_k, n}, w);
 }
 
 int fdma_create_mask(const fdma_mask_params* p, void* stream_) {

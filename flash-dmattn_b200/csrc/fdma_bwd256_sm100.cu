@@ -44,6 +44,7 @@ constexpr int kBN = 128;  // stationary rows per CTA
 constexpr int kBM = 64;   // streamed rows per step
 constexpr int kThreads = 384;
 constexpr int kFlush = 64;  // 64-key steps whose dQ the tensor core sums up (4096 keys)
+constexpr int kFarRows = 2048;  // sliding windows: queries beyond the window that a CTA works on for a tile of sink keys
 constexpr int kMaxBits = 4096;  // 64-key tiles the activity bits of a dQ pass can hold; beyond, every tile is worked on
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -78,6 +79,11 @@ struct Bwd256Params {
   const int32_t* key_pos;
   int64_t pos_batch_stride, pos_head_stride;
   int h_pos, causal_shift;
+  // Sliding window (kWindow): as in fdma_bwd_rows_sm100.cu, near and far CTAs of the tiles that hold sinks leave fp32 sums,
+  // [2: dV, dK][near of each batch element, then its parts of kFarRows queries][h_k][sink_tiles * 128][256]
+  Window window;
+  float* sink_sums;
+  int sink_tiles, far_slots, n_far_ctas;  // far CTAs of a pass
   float scale_log2, scale;
 };
 
@@ -108,7 +114,12 @@ __device__ __forceinline__ uint16_t f_to_raw16(float x) {
   return static_cast<uint16_t>(pack_16x2<kBf16>(x, 0.f) & 0xFFFFu);
 }
 
-template <bool kBf16, int kPass>
+// Whether the queries [q_lo, q_hi) hold one that sees the tile from key0 on as sinks alone, beyond its window. query + coff: its position
+__device__ __forceinline__ bool far_part(int key0, int q_lo, int q_hi, int coff, const Window& window) {
+  return q_lo < q_hi && q_hi - 1 >= key0 + window.keys - coff;
+}
+
+template <bool kBf16, int kPass, bool kWindow>
 __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* smem, int item) {
   using L = Smem256;
   constexpr bool kKeys = kPass != kDq;     // stationary rows are keys
@@ -138,7 +149,21 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
   const bool causal = p.is_causal != 0;
   // the CTA's stationary tile n, its (kv) head and batch element; key passes: its range of 64-row query tiles
   int n, hk, b, h = 0, split = 0;
-  if (kKeys) {
+  const bool far = kWindow && kKeys && item < p.n_far_ctas;
+  int slot = 0;
+  if (kWindow && kKeys) {
+    if (far) {  // they run first
+      n = item % p.sink_tiles;
+      hk = item / p.sink_tiles % p.h_k;
+      slot = item / (p.sink_tiles * p.h_k) % p.far_slots;
+      b = item / (p.sink_tiles * p.h_k * p.far_slots);
+    } else {
+      item -= p.n_far_ctas;
+      n = item % NT;
+      hk = item / NT % p.h_k;
+      b = item / NT / p.h_k;
+    }
+  } else if (kKeys) {
     // (query-range split, key tile): with more than one split the CTA covers the query tiles [m_start, M64) of its key tile
     // and leaves fp32 partials. The last ranges, never emptied by causal masking, run first.
     const int per = NT * p.nsplit;
@@ -174,7 +199,21 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
       m_start = max(0, (n * kBN - coff) / kBM);
     }
     m_start = max(m_start, split * m_chunk);
+    if (kWindow) {
+      if (far) {
+        const int q_lo = slot * kFarRows, q_hi = min(Sq, q_lo + kFarRows);
+        if (!far_part(n * kBN, q_lo, q_hi, coff, p.window)) return;  // (the whole CTA agrees)
+        m_start = max(q_lo, n * kBN + p.window.keys - coff) / kBM;
+        M64 = (q_hi + kBM - 1) / kBM;
+      } else {
+        M64 = max(0, min(M64, (min(n * kBN + kBN, Sk) - 1 + p.window.keys - coff + kBM - 1) / kBM));
+      }
+    }
   }
+  // Sliding window, dQ pass: the key tiles of the sinks and those of the window, numbered without the gap between
+  const int sink_subs = kWindow ? (min(p.window.sinks, Sk) + kBM - 1) / kBM : 0;
+  int gap = 0;
+  auto tile_of = [&](int m) { return kWindow && !kKeys && m >= sink_subs ? m + gap : m; };
   const WaitCtl ctl{s_abort, p.status};
 
   // ---------------- set-up ----------------
@@ -252,8 +291,15 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
     if (pos_row) vis = s_count[1];
     else if (causal) vis = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(Sk), static_cast<int64_t>(q_last) + coff + 1)));
     n_sub = (vis + kBM - 1) / kBM;
+    if (kWindow) {
+      gap = max(0, min(max(0, n * kBN + coff - p.window.keys + 1) / kBM, n_sub) - sink_subs);
+      n_sub -= gap;
+    }
     n_steps = n_sub;
-    if (use_bits) {
+    if (kWindow && use_bits) {
+      n_steps = 0;
+      for (int i = 0; i < n_sub; ++i) n_steps += (s_bits[tile_of(i) >> 5] >> (tile_of(i) & 31)) & 1u;
+    } else if (use_bits) {
       n_steps = 0;
       for (int w = 0; w * 32 < n_sub; ++w)
         n_steps += __popc(s_bits[w] & (n_sub - w * 32 >= 32 ? 0xFFFFFFFFu : (1u << (n_sub - w * 32)) - 1u));
@@ -270,7 +316,7 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
       }
     } else {
       do ++m;
-      while (use_bits && m < n_sub && !((s_bits[m >> 5] >> (m & 31)) & 1u));
+      while (use_bits && m < n_sub && !((s_bits[tile_of(m) >> 5] >> (tile_of(m) & 31)) & 1u));
     }
   };
   if (!kKeys) next();  // to the first active tile
@@ -294,7 +340,7 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
       const CUtensorMap* tm_b = kPass == kDk ? &p.tm_do : kPass == kDv ? &p.tm_q : &p.tm_v;
       bool ok = true;
       for (int i = 0; i < n_steps && ok; ++i, next()) {
-        const int head = kKeys ? hk * G + g : hk, row = m * kBM;
+        const int head = kKeys ? hk * G + g : hk, row = tile_of(m) * kBM;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           // in the order the products want them: kDv computes its scores from the other operand
@@ -381,7 +427,7 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
         const int64_t row0 = (static_cast<int64_t>(b) * p.h + hk * G + g) * p.sq_r + m * kBM;
         v = *reinterpret_cast<const uint4*>((lane < 16 ? p.lse2 : p.dsum) + row0 + (lane & 15) * 4);
       } else {  // addend (bias in log2 units, or -inf where masked out) and position of two keys per lane
-        const int k = m * kBM + lane * 2;
+        const int k = tile_of(m) * kBM + lane * 2;
         const uint32_t mb = mrow ? *reinterpret_cast<const uint16_t*>(mrow + k) : 0x0101u;
         const uint32_t bb = brow ? *reinterpret_cast<const uint32_t*>(brow + k) : 0u;
         v.x = __float_as_uint(k < Sk && (mb & 0xFFu) ? raw16_to_f<kBf16>(static_cast<uint16_t>(bb & 0xFFFFu)) * kLog2e : -CUDART_INF_F);
@@ -407,7 +453,7 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
     const int row = n * kBN + (warp & 3) * 32 + lane;
     const int warp_row = n * kBN + (warp & 3) * 32;
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const bool row_ok = row < (kKeys ? Sk : Sq);
+    const bool row_ok = row < (kKeys ? (far ? min(p.window.sinks, Sk) : Sk) : Sq);
     // key passes: addend of this key, and the value compared with q + coff in the causal test, its position
     // (clamped so that ckey - coff cannot overflow; padding slots hold INT_MAX and are masked out anyway)
     float bv = -CUDART_INF_F;
@@ -431,6 +477,11 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
         qlim_wmin = clamp(static_cast<int64_t>(warp_row) + coff);
       }
     }
+    // Sliding window. Key passes: the queries [qlo, qhi) see this key, [qlo_max, qhi_min) all keys of the warp; dQ pass: the first key this
+    // row (and the warp's last row) sees in its window
+    const int qlo = ckey - coff + (far ? p.window.keys : 0), qhi = far ? 0x7FFFFFFF : ckey - coff + p.window.keys;
+    const int qlo_max = ckey_wmax - coff + (far ? p.window.keys : 0), qhi_min = far ? 0x7FFFFFFF : warp_row - coff + p.window.keys;
+    const int kfirst = row + coff - p.window.keys + 1, kfirst_wmax = warp_row + 31 + coff - p.window.keys + 1;
     float colsum = 0.f;
     bool ok = true;
     int flushed = 0;  // dQ pass: sums moved to memory so far
@@ -450,8 +501,10 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
       tmem_wait_ld();
       const int* pos = reinterpret_cast<const int*>(vec + 64);
       const int q0 = m * kBM + half * 32;
-      const bool diag = causal && (kKeys ? static_cast<int64_t>(ckey_wmax) > static_cast<int64_t>(q0) + coff
-                                         : pos[31] > qlim_wmin);  // warp-uniform
+      const bool diag = kWindow ? (kKeys ? qlo_max > q0 || qhi_min < q0 + 32
+                                         : pos[31] > qlim_wmin || (pos[0] < kfirst_wmax && pos[31] >= p.window.sinks))
+                                : causal && (kKeys ? static_cast<int64_t>(ckey_wmax) > static_cast<int64_t>(q0) + coff
+                                                   : pos[31] > qlim_wmin);  // warp-uniform
       float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int j4 = 0; j4 < 8; ++j4) {
@@ -466,7 +519,10 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
           float2 add;  // bias - LSE, or -inf
           if (kKeys) {
             float2 b2 = make_float2(bv, bv);
-            if (diag) {
+            if (kWindow && diag) {
+              if (q0 + 2 * j < qlo || q0 + 2 * j >= qhi) b2.x = -CUDART_INF_F;
+              if (q0 + 2 * j + 1 < qlo || q0 + 2 * j + 1 >= qhi) b2.y = -CUDART_INF_F;
+            } else if (diag) {
               if (ckey - coff > q0 + 2 * j) b2.x = -CUDART_INF_F;
               if (ckey - coff > q0 + 2 * j + 1) b2.y = -CUDART_INF_F;
             }
@@ -474,8 +530,8 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
           } else {
             add = __fadd2_rn(vv, make_float2(-lse, -lse));
             if (diag) {
-              if (pos[2 * j] > qlim) add.x = -CUDART_INF_F;
-              if (pos[2 * j + 1] > qlim) add.y = -CUDART_INF_F;
+              if (pos[2 * j] > qlim || (kWindow && pos[2 * j] < kfirst && pos[2 * j] >= p.window.sinks)) add.x = -CUDART_INF_F;
+              if (pos[2 * j + 1] > qlim || (kWindow && pos[2 * j + 1] < kfirst && pos[2 * j + 1] >= p.window.sinks)) add.y = -CUDART_INF_F;
             }
           }
           const float2 x = __ffma2_rn(make_float2(__uint_as_float(rs[2 * j]), __uint_as_float(rs[2 * j + 1])), sc2, add);
@@ -547,8 +603,11 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
                       : kPass == kDk ? reinterpret_cast<uint16_t*>(p.dk) + b * p.dk_batch_stride + hk * p.dk_head_stride + row_g * p.dk_row_stride
                                      : reinterpret_cast<uint16_t*>(p.dq) + b * p.dq_batch_stride + h * p.dq_head_stride + row_g * p.dq_row_stride;
       // partial: part[dv|dk][split][b][hk][key][256]
-      float* part = p.dkv_part + ((((static_cast<int64_t>(kPass == kDk ? 1 : 0) * p.nsplit + split) * p.b + b) * p.h_k + hk) *
-                                      (NT * kBN) + row) * kD;
+      const int64_t unit = far ? p.b + b * p.far_slots + slot : b;
+      float* part = kWindow ? p.sink_sums + (((static_cast<int64_t>(kPass == kDk ? 1 : 0) * (p.b + p.b * p.far_slots) + unit) * p.h_k + hk) *
+                                                 (p.sink_tiles * kBN) + row) * kD
+                            : p.dkv_part + ((((static_cast<int64_t>(kPass == kDk ? 1 : 0) * p.nsplit + split) * p.b + b) * p.h_k + hk) *
+                                                (NT * kBN) + row) * kD;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {  // this warpgroup's 128 of the 256 columns
         const int col = half * 128 + c * 32;
@@ -570,7 +629,8 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
             r[v4 * 4 + 3] = __float_as_uint(__uint_as_float(r[v4 * 4 + 3]) + y.w);
           }
         }
-        if (kKeys && p.dkv_part) {
+        if (kKeys && (kWindow ? n < p.sink_tiles : p.dkv_part != nullptr)) {
+          if (kWindow && !row_ok) continue;  // (after the warp-wide load)
 #pragma unroll
           for (int v4 = 0; v4 < 8; ++v4)
             *reinterpret_cast<float4*>(part + col + v4 * 4) =
@@ -601,21 +661,49 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
   }
 }
 
-template <bool kBf16>
+template <bool kBf16, bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1) bwd256_kernel(const __grid_constant__ Bwd256Params p) {
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = align_smem_1024(smem_dyn);
   const int item = blockIdx.x;
-  if (item < p.n_kv_ctas) pass256<kBf16, kDk>(p, smem, item);
-  else if (item < 2 * p.n_kv_ctas) pass256<kBf16, kDv>(p, smem, item - p.n_kv_ctas);
-  else pass256<kBf16, kDq>(p, smem, item - 2 * p.n_kv_ctas);
+  if (item < p.n_kv_ctas) pass256<kBf16, kDk, kWindow>(p, smem, item);
+  else if (item < 2 * p.n_kv_ctas) pass256<kBf16, kDv, kWindow>(p, smem, item - p.n_kv_ctas);
+  else pass256<kBf16, kDq, kWindow>(p, smem, item - 2 * p.n_kv_ctas);
+}
+
+// Sliding window, tiles that hold sinks: dV and dK as the sum of what the CTAs of the queries near them and of those beyond have left, in
+// the order of the queries. A warp per key row.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) sinks256_kernel(const __grid_constant__ Bwd256Params p) {
+  const int lane = threadIdx.x & 31, rows = p.sink_tiles * kBN, coff = p.seqlen_k - p.seqlen_q;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int b = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * rows)), hk = static_cast<int>(w / rows % p.h_k), row = static_cast<int>(w % rows);
+  if (b >= p.b || row >= p.seqlen_k) return;
+  const int64_t units = p.b + static_cast<int64_t>(p.b) * p.far_slots;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {  // dV, dK
+    float acc[kD / 32];
+    auto add = [&](int64_t u, bool fresh) {
+      const float* src = p.sink_sums + (((x * units + u) * p.h_k + hk) * rows + row) * kD + lane * (kD / 32);
+#pragma unroll
+      for (int i = 0; i < kD / 32; ++i) acc[i] = src[i] + (fresh ? 0.f : acc[i]);
+    };
+    add(b, true);
+    for (int c = 0; row < p.window.sinks && c < p.far_slots; ++c)
+      if (far_part(row / kBN * kBN, c * kFarRows, min((c + 1) * kFarRows, p.seqlen_q), coff, p.window)) add(p.b + b * p.far_slots + c, false);
+    uint16_t* dst = x == 0 ? reinterpret_cast<uint16_t*>(p.dv) + b * p.dv_batch_stride + hk * p.dv_head_stride + row * p.dv_row_stride
+                           : reinterpret_cast<uint16_t*>(p.dk) + b * p.dk_batch_stride + hk * p.dk_head_stride + row * p.dk_row_stride;
+#pragma unroll
+    for (int i = 0; i < kD / 32; ++i)
+      if (lane * (kD / 32) + i < p.d) dst[lane * (kD / 32) + i] = f_to_raw16<kBf16>(acc[i]);
+  }
 }
 
 struct Plan256 {
-  int sq_r, nsplit;
+  int sq_r, nsplit, sink_tiles, far_slots;
   bool want_dbias;
   bool part;  // dK, dV and column sums leave the main kernel as fp32 partials
-  size_t lse2_off, dsum_off, dq_off, part_off, dbpart_off, total;
+  size_t lse2_off, dsum_off, dq_off, part_off, dbpart_off, sinks_off, total;
 };
 
 // Query-range splits per key tile: a grid that cannot fill the GPU twice is cut along the query dimension until each of the
@@ -630,11 +718,13 @@ int pick_nsplit256(const fdma_fwd_params& p) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(want, cap), 64)));
 }
 
-Plan256 plan256(const fdma_bwd_params& bp) {
+Plan256 plan256(const fdma_bwd_params& bp, const Window& window) {
   const fdma_fwd_params& p = bp.f;
   Plan256 pl;
   pl.sq_r = static_cast<int>(round_up(p.seqlen_q, kBM));
-  pl.nsplit = pick_nsplit256(p);
+  pl.nsplit = window.keys ? 1 : pick_nsplit256(p);
+  pl.sink_tiles = window.keys ? (std::min(window.sinks, p.seqlen_k) + kBN - 1) / kBN : 0;
+  pl.far_slots = pl.sink_tiles ? (p.seqlen_q + kFarRows - 1) / kFarRows : 0;
   pl.want_dbias = bp.dbias != nullptr;
   size_t o = 0;
   const size_t rows = static_cast<size_t>(p.b) * p.h * pl.sq_r;
@@ -650,6 +740,8 @@ Plan256 plan256(const fdma_bwd_params& bp) {
     pl.dbpart_off = o;
     if (pl.want_dbias) o += align256(static_cast<size_t>(pl.nsplit) * p.b * p.h_k * keys_r * 4);
   }
+  pl.sinks_off = o;
+  o += align256(static_cast<size_t>(2) * p.b * (1 + pl.far_slots) * p.h_k * pl.sink_tiles * kBN * kD * 4);
   pl.total = o;
   return pl;
 }
@@ -657,7 +749,7 @@ Plan256 plan256(const fdma_bwd_params& bp) {
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
 template <bool kBf16>
-int launch256(const fdma_bwd_params& bp, const Plan256& pl, cudaStream_t stream) {
+int launch256(const fdma_bwd_params& bp, const Plan256& pl, const Window& window, cudaStream_t stream) {
   const fdma_fwd_params& p = bp.f;
   if (!p.workspace || p.workspace_bytes < pl.total) return FDMA_ERR_WORKSPACE;
   char* ws = static_cast<char*>(p.workspace);
@@ -729,10 +821,15 @@ int launch256(const fdma_bwd_params& bp, const Plan256& pl, cudaStream_t stream)
   kp.scale_log2 = p.softmax_scale * kLog2e;
   kp.scale = p.softmax_scale;
 
-  auto kern = bwd256_kernel<kBf16>;
+  kp.window = window;
+  kp.sink_sums = reinterpret_cast<float*>(ws + pl.sinks_off);
+  kp.sink_tiles = pl.sink_tiles; kp.far_slots = pl.far_slots;
+  kp.n_far_ctas = pl.sink_tiles * p.h_k * pl.far_slots * p.b;
+  auto kern = window.keys ? bwd256_kernel<kBf16, true> : bwd256_kernel<kBf16, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem256::kAlloc);
   if (e != cudaSuccess) return static_cast<int>(e);
-  const int64_t kv = static_cast<int64_t>((p.seqlen_k + kBN - 1) / kBN) * pl.nsplit * p.h_k * p.b;
+  const int64_t kv = static_cast<int64_t>((p.seqlen_k + kBN - 1) / kBN) * pl.nsplit * p.h_k * p.b +
+                     static_cast<int64_t>(pl.sink_tiles) * p.h_k * pl.far_slots * p.b;
   const int64_t ctas = 2 * kv + static_cast<int64_t>((p.seqlen_q + kBN - 1) / kBN) * p.h * p.b;
   if (ctas > 0x7FFFFFFF) return FDMA_ERR_TOO_LARGE;
   kp.n_kv_ctas = static_cast<int>(kv);
@@ -744,6 +841,12 @@ int launch256(const fdma_bwd_params& bp, const Plan256& pl, cudaStream_t stream)
   if (ev1) cudaEventRecord(ev1, stream);
   e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
+  if (window.keys) {
+    if (!pl.sink_tiles) return 0;
+    const int64_t rows = static_cast<int64_t>(p.b) * p.h_k * pl.sink_tiles * kBN;
+    sinks256_kernel<kBf16><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(kp);
+    return static_cast<int>(cudaGetLastError());
+  }
 
   BwdFinishArgs f = {};
   f.b = p.b; f.h = p.h; f.sq = p.seqlen_q; f.sq_r = pl.sq_r; f.d = p.d; f.D = kD;
@@ -796,11 +899,11 @@ bool tc_bwd256_supported(const fdma_bwd_params& bp) {
   return true;
 }
 
-size_t tc_bwd256_workspace_bytes(const fdma_bwd_params& bp) { return plan256(bp).total; }
+size_t tc_bwd256_workspace_bytes(const fdma_bwd_params& bp, const Window& window) { return plan256(bp, window).total; }
 
-int tc_bwd256(const fdma_bwd_params& bp, cudaStream_t stream) {
-  const Plan256 pl = plan256(bp);
-  return bp.f.dtype == FDMA_BF16 ? launch256<true>(bp, pl, stream) : launch256<false>(bp, pl, stream);
+int tc_bwd256(const fdma_bwd_params& bp, cudaStream_t stream, const Window& window) {
+  const Plan256 pl = plan256(bp, window);
+  return bp.f.dtype == FDMA_BF16 ? launch256<true>(bp, pl, window, stream) : launch256<false>(bp, pl, window, stream);
 }
 
 }  // namespace fdma

@@ -54,6 +54,9 @@ constexpr int kFlush = 2;
 constexpr int kKeyFlush = 48;
 constexpr int kMaxBits = 4096;   // 64-key tiles the activity bits of a row-pass item can hold
 constexpr int kMaxHeads = 4096;  // query heads of a group whose activity differs from head to head
+// Sliding windows: queries beyond the window that a CTA works on for a tile of sink keys. Such a tile is seen by all queries behind it, the
+// others by window + 128 of them.
+constexpr int kFarRows = 2048;
 constexpr int kDbHeads = 16;    // query heads of a group whose dBias sums have room in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -92,6 +95,12 @@ struct BwdRowsParams {
   int64_t pos_batch_stride, pos_head_stride;
   int h_pos, causal_shift;
   PackedSeqs seqs;   // packed sequences, each with tiles of its own; streamed query tiles are cut at fixed rows
+  // Sliding window (kWindow). A key tile's CTA takes the queries whose window reaches it (near); those beyond, which see the sinks alone,
+  // come from CTAs of their own (far), kFarRows queries each. Tiles with sinks leave fp32 sums, which sinks_kernel adds up:
+  // [2: dV, dK][near of each sequence or batch element, then a place for each part of kFarRows queries][h_k][sink_tiles * 128][D]
+  Window window;
+  float* sink_sums;
+  int sink_tiles, near_units, far_slots, n_far_ctas;
   int n_tiles;       // key tiles (packed: places for them)
   int q_tiles;       // row-pass tiles (packed: places for them)
   int nsplit;        // query-range splits per key tile
@@ -223,12 +232,21 @@ __device__ __forceinline__ float softmax_step(const uint32_t (&x)[32], const uin
   return (part[0].x + part[0].y) + (part[1].x + part[1].y);
 }
 
+// Whether the queries [q_lo, q_hi) hold one that sees the tile from key0 on as sinks alone, beyond its window. query + coff: its position
+__device__ __forceinline__ bool far_part(int key0, int key_end, int q_lo, int q_hi, int coff, const Window& window) {
+  return key0 < key_end && q_lo < q_hi && q_hi - 1 >= key0 + window.keys - coff;
+}
+// Where the far CTAs' rows begin in dkv_sums, behind the near ones' (half: dV, dK)
+__device__ __forceinline__ int64_t far_rows_at(const BwdRowsParams& p, int half, int key_tiles) {
+  return static_cast<int64_t>(2) * p.b * p.h_k * key_tiles * kBN + static_cast<int64_t>(half) * p.n_far_ctas * kBN;
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // Key pass: one tile of 128 keys of one (batch, kv head), every 64-row query tile of its range x every query head of the
 // group, so that dK, dV and dBias leave the CTA already summed over the group (the reference writes per-query-head temporaries
 // and reduces them on the host with at::sum_out, flash_api.cpp:970-983, :1027-1047).
 // ---------------------------------------------------------------------------------------------------------------------
-template <int D, bool kBf16, bool packed>
+template <int D, bool kBf16, bool packed, bool kWindow>
 __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* smem, uint32_t tmem_base, const Bars& bar,
                                          const WaitCtl& ctl) {
   using L = SmemR<D>;
@@ -247,8 +265,27 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
   // (query-range split, key tile), then kv head, then batch element. With more than one split the CTA covers the query tiles
   // [m_lo, M64) and leaves fp32 partials. The last query ranges, which causal masking never empties, run first.
   const int per = p.n_tiles * p.nsplit;
-  const int item = blockIdx.x % per, n = item % p.n_tiles, split = p.nsplit - 1 - item / p.n_tiles;
-  const int hk = blockIdx.x / per % p.h_k, b = blockIdx.x / per / p.h_k;
+  int item = blockIdx.x % per, n = item % p.n_tiles, split = p.nsplit - 1 - item / p.n_tiles;
+  int hk = blockIdx.x / per % p.h_k, b = blockIdx.x / per / p.h_k;
+  // Sliding window: the far CTAs run first (the longest ones where there are several query heads). n: the tile of the sequence
+  const bool far = kWindow && static_cast<int>(blockIdx.x) < p.n_far_ctas;
+  int slot = 0, sink_unit = -1;
+  if (kWindow) {
+    split = 0;
+    if (far) {
+      item = blockIdx.x;
+      n = item % p.sink_tiles;
+      hk = item / p.sink_tiles % p.h_k;
+      slot = item / (p.sink_tiles * p.h_k) % p.far_slots;
+      b = item / (p.sink_tiles * p.h_k * p.far_slots);
+      sink_unit = p.near_units + b * p.far_slots + slot;
+    } else {
+      item = blockIdx.x - p.n_far_ctas;
+      n = item % p.n_tiles;
+      hk = item / p.n_tiles % p.h_k;
+      b = item / p.n_tiles / p.h_k;
+    }
+  }
   const int M64_all = (Sq + kBM - 1) / kBM;
   const int m_chunk = (M64_all + p.nsplit - 1) / p.nsplit;
   const int m_lo = split * m_chunk;
@@ -265,7 +302,8 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
   } else if (causal) {
     m_start = max(0, (n * kBN - coff) / kBM);  // first query tile with a row that sees key n*128
   }
-  if (packed) {
+  int n_in_seq = n;  // tile of its sequence
+  if (packed && !far) {
     const PackedTile t = packed_tile(p.seqs.cu_k, p.seqs.n, Sk, kBN, n);
     const int2 q = packed_range(p.seqs.cu_q, p.seqs.n, Sq, t.seq);
     key0 = t.begin + t.tile * kBN;
@@ -275,6 +313,35 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
     coff = key_end - q_hi;              // the last query sees the last key
     m_start = (causal ? max(q_lo, key0 - coff) : q_lo) / kBM;
     M64 = warp_uniform(q_lo < q_hi ? min(M64, (q_hi + kBM - 1) / kBM) : 0);
+    n_in_seq = t.tile;
+    if (kWindow && t.seq >= 0 && t.seq < p.seqs.n && t.tile < p.sink_tiles) sink_unit = t.seq;
+  } else if (kWindow && !far && n < p.sink_tiles) {
+    sink_unit = b;
+  }
+  int beyond = 0;  // far: what is added to a key's first query that sees it; near: as many queries see it
+  if (kWindow) {
+    beyond = p.window.keys;
+    if (far) {
+      if (packed) {
+        const PackedTile t = packed_tile(p.seqs.cu_q, p.seqs.n, Sq, kFarRows, slot);
+        const int2 keys = packed_range(p.seqs.cu_k, p.seqs.n, Sk, t.seq);
+        key0 = keys.x + n * kBN;
+        key_end = min(keys.y, keys.x + p.window.sinks);
+        q_lo = t.begin + t.tile * kFarRows;
+        q_hi = min(t.end, q_lo + kFarRows);
+        coff = keys.y - t.end;
+      } else {
+        key_end = min(Sk, p.window.sinks);
+        q_lo = slot * kFarRows;
+        q_hi = min(Sq, q_lo + kFarRows);
+      }
+      if (!far_part(key0, key_end, q_lo, q_hi, coff, p.window)) return;  // (the whole CTA agrees)
+      m_start = max(q_lo, key0 + beyond - coff) / kBM;
+      M64 = (q_hi + kBM - 1) / kBM;
+    } else {
+      M64 = max(0, min(M64, (min(key0 + kBN, key_end) - 1 + beyond - coff + kBM - 1) / kBM));
+    }
+    M64 = warp_uniform(M64);
   }
   m_start = warp_uniform(max(m_start, m_lo));
   // The query heads for which the tile holds a kept key: all, none, or (a mask per query head) those in the list s_heads.
@@ -461,6 +528,16 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
       qlo_max = max(qlo_max, q_lo);
       qhi = qhi_min = q_hi;
     }
+    if (kWindow) {
+      if (far) {
+        qlo = max(q_lo, key + beyond - coff);
+        qlo_max = max(q_lo, ckey_wmax + beyond - coff);
+        qhi = qhi_min = q_hi;
+      } else {
+        qhi = min(qhi, key + beyond - coff);
+        qhi_min = min(qhi_min, key0 + (warp & 3) * 32 + beyond - coff);
+      }
+    }
     // addend of this key for query head h: bias in log2 units, -inf when the key is masked out (P = exp2(-inf) = 0 without any
     // per-element select). One value per thread for the whole CTA unless mask or bias differ between the heads of the group.
     auto addend = [&](int h) {
@@ -473,7 +550,8 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
     const uint32_t acc_addr = tmem_base + lane_addr + (half == 0 ? C::kAcc : kAcc2);
     const int rows = min(kBN, key_end - key0);
     float4* const sums = reinterpret_cast<float4*>(p.dkv_sums) +
-                         ((((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key0) * (D / 4) + krow;
+                         (far ? far_rows_at(p, half, NT) + (blockIdx.x * kBN)
+                              : (((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key0) * (D / 4) + krow;
     int moved = 0;  // how often
     auto move_sums = [&]() {
 #pragma unroll 1  // (little code: it lies in the loop over the steps)
@@ -619,10 +697,12 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = 0u;
         }
-        if (p.dkv_part) {
+        if (kWindow ? sink_unit >= 0 : p.dkv_part != nullptr) {
           // fp32 partial: part[dv|dk][split][b][hk][key][d]
-          if (packed && !key_ok) continue;  // (after the warp-wide load)
-          float* part = p.dkv_part + ((((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key) * D + c * 32;
+          if ((packed || kWindow) && !key_ok) continue;  // (after the warp-wide load)
+          float* part = kWindow ? p.sink_sums + (((static_cast<int64_t>(half) * (p.near_units + p.b * p.far_slots) + sink_unit) * p.h_k + hk) *
+                                                     (p.sink_tiles * kBN) + (n_in_seq * kBN + krow)) * D + c * 32
+                                : p.dkv_part + ((((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key) * D + c * 32;
 #pragma unroll
           for (int v4 = 0; v4 < 8; ++v4)
             *reinterpret_cast<float4*>(part + v4 * 4) =
@@ -650,14 +730,14 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
 // positions carry over; the next item's Q and dO wait in shared memory when an item ends, its first score products are issued
 // before the softmax teams store the item's dQ.
 // ---------------------------------------------------------------------------------------------------------------------
-template <int D, bool kBf16, bool packed>
+template <int D, bool kBf16, bool packed, bool kWindow>
 __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* smem, uint32_t tmem_base, const Bars& bar,
                                          const WaitCtl& ctl) {
   using L = SmemR<D>;
   using C = Cols<D, false>;
   float* s_vec = reinterpret_cast<float*>(smem + L::kVecOff);
   uint32_t* s_bits_all = reinterpret_cast<uint32_t*>(smem + L::kBitsOff);
-  volatile int* s_item = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 16);  // [2][4]: first 64-key tile, end of them, steps
+  volatile int* s_item = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 16);  // [2][4]: first 64-key tile, end of them, steps, gap
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.h / p.h_k;
   const bool causal = p.is_causal != 0;
@@ -690,6 +770,9 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
     return p.mask ? p.mask + b * p.mask_batch_stride + (p.h_mask == p.h ? h : (p.h_mask == p.h_k ? h / G : 0)) * p.mask_head_stride : nullptr;
   };
   const bool use_bits = p.mask != nullptr;
+  // Sliding window: the tiles of the sinks and those of the window, numbered without the gap between
+  const int sink_subs = kWindow ? (min(p.window.sinks, sk) + kBM - 1) / kBM : 0;
+  auto tile_of = [&](int m, int gap) { return kWindow && m >= sink_subs ? m + gap : m; };
   // Steps of an item: the 64-key tiles [first, end) that hold a kept key
   auto next = [&](int m, int first, int end, const uint32_t* bits) {
     do ++m;
@@ -708,7 +791,7 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
           const int h = h0 + ic, buf = ic & 1;
           ok = mbar_wait(bar.item_full + buf, (ic >> 1) & 1, ctl, kWaitItemFull);
           if (!ok) break;
-          const int first = s_item[buf * 4], end = s_item[buf * 4 + 1], n_steps = s_item[buf * 4 + 2];
+          const int first = s_item[buf * 4], end = s_item[buf * 4 + 1], n_steps = s_item[buf * 4 + 2], gap = s_item[buf * 4 + 3];
           const uint32_t* bits = s_bits_all + buf * (kMaxBits / 32);
           if (n_steps > 0) {
             ok = mbar_wait(bar.x_empty, (xc & 1) ^ 1, ctl, kWaitXEmpty);
@@ -732,8 +815,8 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
             unsigned char* dst = smem + L::kStOff + stage * 2 * L::kStep;
 #pragma unroll
             for (int kb = 0; kb < D / 64; ++kb) {
-              tma_load_4d(dst + kb * (kBM * 128), &p.tm_k, bar.st_full + stage, kb * 64, h / G, k0 + m * kBM, b);
-              tma_load_4d(dst + L::kStep + kb * (kBM * 128), &p.tm_v, bar.st_full + stage, kb * 64, h / G, k0 + m * kBM, b);
+              tma_load_4d(dst + kb * (kBM * 128), &p.tm_k, bar.st_full + stage, kb * 64, h / G, k0 + tile_of(m, gap) * kBM, b);
+              tma_load_4d(dst + L::kStep + kb * (kBM * 128), &p.tm_v, bar.st_full + stage, kb * 64, h / G, k0 + tile_of(m, gap) * kBM, b);
             }
           }
           mbar_arrive(bar.item_empty + buf);
@@ -761,14 +844,15 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
         ok = wait(bar.item_full + buf, ic >> 1, kWaitItemFull);
         if (!ok) break;
         const int end = warp_uniform(s_item[buf * 4 + 1]), n_steps = warp_uniform(s_item[buf * 4 + 2]);
+        const int left = sk - tile_of(end - 1, kWindow ? warp_uniform(s_item[buf * 4 + 3]) : 0) * kBM;  // keys in the last tile
         // Packed sequences: K and V rows beyond the sequence, in its last tile, become zeros, as TMA fills them in at the end of a
         // tensor (zero probabilities alone would pass a NaN on).
         auto stage_ready = [&](int i) {
           const int stage = (g0 + i) % kStages;
           if (!wait(bar.st_full + stage, (g0 + i) / kStages, kWaitStFull)) return false;
-          if (packed && i == n_steps - 1 && sk - (end - 1) * kBM < kBM) {
+          if (packed && i == n_steps - 1 && left < kBM) {
             unsigned char* st = smem + L::kStOff + stage * 2 * L::kStep;
-            for (int t = 0; t < 2; ++t) zero_tile_rows(st + t * L::kStep, D / 64, kBM * 128, sk - (end - 1) * kBM, kBM);
+            for (int t = 0; t < 2; ++t) zero_tile_rows(st + t * L::kStep, D / 64, kBM * 128, left, kBM);
             fence_proxy_async_smem();
             __syncwarp();
           }
@@ -819,14 +903,14 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
         const int h = h0 + ic, buf = ic & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(bar.item_full + buf, (ic >> 1) & 1, ctl, kWaitItemFull));
         if (!ok) break;
-        const int first = s_item[buf * 4], end = s_item[buf * 4 + 1], n_steps = s_item[buf * 4 + 2];
+        const int first = s_item[buf * 4], end = s_item[buf * 4 + 1], n_steps = s_item[buf * 4 + 2], gap = s_item[buf * 4 + 3];
         const uint32_t* bits = s_bits_all + buf * (kMaxBits / 32);
         const uint8_t* mrow = mask_of(h);
         const uint16_t* brow = p.bias ? reinterpret_cast<const uint16_t*>(p.bias) + b * p.bias_batch_stride +
                                             (p.h_bias == p.h ? h : (p.h_bias == p.h_k ? h / G : 0)) * p.bias_head_stride : nullptr;
         const int32_t* pos_row = pos_of(h);
         for (int i = 0, m = next(first - 1, first, end, bits); i < n_steps; ++i, m = next(m, first, end, bits), ++vi) {
-          const int k = m * kBM + lane * 2;
+          const int k = tile_of(m, gap) * kBM + lane * 2;
           const uint32_t mb = mrow ? *reinterpret_cast<const uint16_t*>(mrow + k) : 0x0101u;
           const uint32_t bb = brow ? *reinterpret_cast<const uint32_t*>(brow + k) : 0u;
           const float2 add = make_float2(k < sk && (mb & 0xFFu) ? raw16_to_f<kBf16>(static_cast<uint16_t>(bb & 0xFFFFu)) * kLog2e : -CUDART_INF_F,
@@ -870,7 +954,12 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
         } else if (causal) {
           vis = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(sk), static_cast<int64_t>(q_last) + coff + 1)));
         }
-        const int n_sub = (vis + kBM - 1) / kBM, chunk = (n_sub + p.ranges - 1) / p.ranges;
+        int n_sub = (vis + kBM - 1) / kBM, gap = 0;
+        if (kWindow) {
+          gap = max(0, min(max(0, n * kBN + coff - p.window.keys + 1) / kBM, n_sub) - sink_subs);
+          n_sub -= gap;
+        }
+        const int chunk = (n_sub + p.ranges - 1) / p.ranges;
         const int first = min(range * chunk, n_sub), end = min(first + chunk, n_sub);
         int n_steps = end - first;
         if (use_bits) {
@@ -883,12 +972,13 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
             if (m < end) {
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
-                const uint4 v = *reinterpret_cast<const uint4*>(mrow + m * kBM + c * 16);
+                const int k = tile_of(m, gap) * kBM + c * 16;
+                const uint4 v = *reinterpret_cast<const uint4*>(mrow + k);
                 uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                if (m * kBM + c * 16 + 16 > sk) {  // ragged end: drop keys beyond the last
+                if (k + 16 > sk) {  // ragged end: drop keys beyond the last
 #pragma unroll
                   for (int e = 0; e < 16; ++e)
-                    if (m * kBM + c * 16 + e >= sk) x[e >> 2] &= ~(0xFFu << ((e & 3) * 8));
+                    if (k + e >= sk) x[e >> 2] &= ~(0xFFu << ((e & 3) * 8));
                 }
                 any |= x[0] | x[1] | x[2] | x[3];
               }
@@ -902,6 +992,7 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
           s_item[buf * 4] = first;
           s_item[buf * 4 + 1] = end;
           s_item[buf * 4 + 2] = n_steps;
+          s_item[buf * 4 + 3] = gap;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar.item_full + buf);
@@ -919,6 +1010,8 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
     auto clamp = [](int64_t x) { return static_cast<int>(max(static_cast<int64_t>(-1), min(x, static_cast<int64_t>(0x7FFFFFFE)))); };
     const int qlim = causal ? clamp(static_cast<int64_t>(row) + coff) : 0x7FFFFFFE;
     const int qlim_wmin = causal ? clamp(static_cast<int64_t>(warp_row) + coff) : 0x7FFFFFFE;
+    // first key this row (and the warp's last row) sees in its window
+    const int qfirst = kWindow ? row + coff - p.window.keys + 1 : 0, qfirst_wmax = kWindow ? warp_row + 31 + coff - p.window.keys + 1 : 0;
     const int row_g = q0 + min(row, sq - 1);  // row in the tensors
     constexpr int kHalfCols = D / 2;          // columns of dQ each team takes out
     int g0 = 0, xc = 0, sums = 0;  // steps, items with steps, sums received so far
@@ -1048,11 +1141,13 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
           return __fadd2_rn((j & 1) ? make_float2(x.z, x.w) : make_float2(x.x, x.y), nlse2);
         };
         auto d2 = [&](int) { return dsum2; };
-        if (causal && pos[31] > qlim_wmin) {  // warp-uniform: some (row, key) of the warp is out of sight
+        // warp-uniform: some (row, key) of the warp is out of sight
+        if ((causal && pos[31] > qlim_wmin) || (kWindow && pos[0] < qfirst_wmax && pos[31] >= p.window.sinks)) {
           softmax_step<kBf16, false>(rs, rp, p.scale_log2, [&](int j) {
             float2 add = pair(j);
-            if (pos[2 * j] > qlim) add.x = -CUDART_INF_F;
-            if (pos[2 * j + 1] > qlim) add.y = -CUDART_INF_F;
+            const int x = pos[2 * j], y = pos[2 * j + 1];
+            if (x > qlim || (kWindow && x < qfirst && x >= p.window.sinks)) add.x = -CUDART_INF_F;
+            if (y > qlim || (kWindow && y < qfirst && y >= p.window.sinks)) add.y = -CUDART_INF_F;
             return add;
           }, d2, dsk, dsk);
         } else {
@@ -1073,7 +1168,7 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
   }
 }
 
-template <int D, bool kBf16, bool packed>
+template <int D, bool kBf16, bool packed, bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1) bwd_rows_kernel(const __grid_constant__ BwdRowsParams p) {
   using L = SmemR<D>;
   extern __shared__ unsigned char smem_dyn[];
@@ -1121,13 +1216,52 @@ __global__ void __launch_bounds__(kThreads, 1) bwd_rows_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = warp_uniform(*s_tmem);
-  if (blockIdx.x < static_cast<unsigned>(p.n_key_ctas)) key_pass<D, kBf16, packed>(p, smem, tmem_base, bar, ctl);
-  else row_pass<D, kBf16, packed>(p, smem, tmem_base, bar, ctl);
+  if (blockIdx.x < static_cast<unsigned>(p.n_key_ctas)) key_pass<D, kBf16, packed, kWindow>(p, smem, tmem_base, bar, ctl);
+  else row_pass<D, kBf16, packed, kWindow>(p, smem, tmem_base, bar, ctl);
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Sliding window, tiles that hold sinks: dV and dK as the sum of what the CTAs of the queries near them and of those beyond have left, in
+// the order of the queries. A warp per key row.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256) sinks_kernel(const __grid_constant__ BwdRowsParams p) {
+  const int lane = threadIdx.x & 31, rows = p.sink_tiles * kBN;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int unit = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * rows)), hk = static_cast<int>(w / rows % p.h_k), row = static_cast<int>(w % rows);
+  if (unit >= p.near_units) return;
+  const bool packed = p.seqs.cu_q != nullptr;
+  int2 keys = make_int2(0, p.seqlen_k), queries = make_int2(0, p.seqlen_q);
+  int first = p.near_units + unit * p.far_slots;
+  if (packed) {
+    keys = packed_range(p.seqs.cu_k, p.seqs.n, p.seqlen_k, unit);
+    queries = packed_range(p.seqs.cu_q, p.seqs.n, p.seqlen_q, unit);
+    first = p.near_units + queries.x / kFarRows + unit + 1;  // the sequence's first place
+  }
+  if (keys.x + row >= keys.y) return;
+  const int key0 = keys.x + row / kBN * kBN, coff = keys.y - queries.y;
+  const int64_t units = p.near_units + static_cast<int64_t>(p.b) * p.far_slots;
+  const int b = packed ? 0 : unit;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {  // dV, dK
+    float acc[D / 32];
+    auto add = [&](int64_t u, bool fresh) {
+      const float* src = p.sink_sums + (((x * units + u) * p.h_k + hk) * rows + row) * D + lane * (D / 32);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] = src[i] + (fresh ? 0.f : acc[i]);
+    };
+    add(unit, true);
+    for (int c = 0, q = queries.x; row < p.window.sinks && q < queries.y; ++c, q += kFarRows)
+      if (far_part(key0, key0 + 1, q, min(q + kFarRows, queries.y), coff, p.window)) add(first + c, false);
+    uint16_t* dst = x == 0 ? reinterpret_cast<uint16_t*>(p.dv) + b * p.dv_batch_stride + hk * p.dv_head_stride + static_cast<int64_t>(keys.x + row) * p.dv_row_stride
+                           : reinterpret_cast<uint16_t*>(p.dk) + b * p.dk_batch_stride + hk * p.dk_head_stride + static_cast<int64_t>(keys.x + row) * p.dk_row_stride;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      if (lane * (D / 32) + i < p.d) dst[lane * (D / 32) + i] = f_to_raw16<kBf16>(acc[i]);
   }
 }
 
@@ -1138,7 +1272,8 @@ struct RowsPlan {
   int D, sq_r, nsplit, dbias_mode;
   int ranges;  // key ranges per row-pass tile
   bool part;  // dK, dV (and column sums) leave the kernel as fp32 partials
-  size_t lse2_off, dsum_off, dq_off, dbias_off, sums_off, part_off, dbpart_off, total;
+  size_t lse2_off, dsum_off, dq_off, dbias_off, sums_off, part_off, dbpart_off, sinks_off, total;
+  int sink_tiles, near_units, far_slots;  // sliding window
 };
 
 // Query-range splits per key tile: one CTA per SM, as long as a split keeps 32 steps, and on to two per SM while it keeps 160. The row pass,
@@ -1175,7 +1310,7 @@ int pick_heads_per_cta(int64_t tiles, int h) {
 // Keys of the fp32 buffer of the atomic dBias mode: those of the tensor, or with gathered keys the gathered ones.
 int atomic_keys(const fdma_bwd_params& bp) { return bp.scatter_pos ? bp.f.seqlen_k : bp.dbias_keys; }
 
-RowsPlan plan(const fdma_bwd_params& bp) {
+RowsPlan plan(const fdma_bwd_params& bp, const Window& window, int sequences) {
   const fdma_fwd_params& p = bp.f;
   RowsPlan pl;
   pl.D = tile_head_dim(p.d);
@@ -1187,16 +1322,25 @@ RowsPlan plan(const fdma_bwd_params& bp) {
   const size_t rows = static_cast<size_t>(p.b) * p.h * pl.sq_r;
   pl.lse2_off = o; o += align256(rows * 4);
   pl.dsum_off = o; o += align256(rows * 4);
-  pl.ranges = pick_ranges(p);
+  pl.ranges = window.keys ? 1 : pick_ranges(p);
   pl.dq_off = o;
   if (pl.ranges > 1) o += align256(static_cast<size_t>(pl.ranges) * p.b * p.h * p.seqlen_q * pl.D * 4);
   pl.dbias_off = o;
   if (pl.dbias_mode == kDbAtomic) o += align256(static_cast<size_t>(bp.dbias_b) * bp.dbias_h * atomic_keys(bp) * 4);
-  pl.nsplit = pick_nsplit(p);
+  pl.nsplit = window.keys ? 1 : pick_nsplit(p);
+  pl.sink_tiles = pl.near_units = pl.far_slots = 0;
+  if (window.keys && window.sinks) {
+    pl.sink_tiles = (std::min(window.sinks, p.seqlen_k) + kBN - 1) / kBN;
+    pl.near_units = sequences ? sequences : p.b;
+    pl.far_slots = sequences ? packed_slots(p.seqlen_q, sequences, kFarRows) : (p.seqlen_q + kFarRows - 1) / kFarRows;
+  }
   pl.sums_off = o;
   const int64_t m_tiles = (p.seqlen_q + kBM - 1) / kBM;
   if ((m_tiles + pl.nsplit - 1) / pl.nsplit * (p.h / p.h_k) > kKeyFlush)
-    o += align256(static_cast<size_t>(2) * pl.nsplit * p.b * p.h_k * round_up(p.seqlen_k, kBN) * pl.D * 4);
+    o += align256((static_cast<size_t>(2) * pl.nsplit * p.b * p.h_k * round_up(p.seqlen_k, kBN) +
+                   static_cast<size_t>(2) * p.b * pl.far_slots * p.h_k * pl.sink_tiles * kBN) * pl.D * 4);
+  pl.sinks_off = o;
+  o += align256(static_cast<size_t>(2) * (pl.near_units + p.b * pl.far_slots) * p.h_k * pl.sink_tiles * kBN * pl.D * 4);
   pl.part = pl.nsplit > 1 || bp.scatter_pos != nullptr;
   pl.part_off = pl.dbpart_off = o;
   if (pl.part) {
@@ -1210,7 +1354,7 @@ RowsPlan plan(const fdma_bwd_params& bp) {
 }
 
 template <int D, bool kBf16>
-int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs, cudaStream_t stream) {
+int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs, const Window& window, cudaStream_t stream) {
   using L = SmemR<D>;
   const fdma_fwd_params& p = bp.f;
   if (!p.workspace || p.workspace_bytes < pl.total) return FDMA_ERR_WORKSPACE;
@@ -1288,16 +1432,22 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   kp.seqs = seqs;
   kp.n_tiles = seqs.cu_q ? packed_slots(p.seqlen_k, seqs.n, kBN) : (p.seqlen_k + kBN - 1) / kBN;
   kp.q_tiles = seqs.cu_q ? packed_slots(p.seqlen_q, seqs.n, kBN) : (p.seqlen_q + kBN - 1) / kBN;
+  kp.window = window;
+  kp.sink_sums = reinterpret_cast<float*>(ws + pl.sinks_off);
+  kp.sink_tiles = pl.sink_tiles; kp.near_units = pl.near_units; kp.far_slots = pl.far_slots;
+  kp.n_far_ctas = pl.sink_tiles * p.h_k * pl.far_slots * p.b;
   kp.nsplit = pl.nsplit;
   kp.ranges = seqs.cu_q ? 1 : pl.ranges;
   kp.heads_per_cta = pick_heads_per_cta(static_cast<int64_t>(kp.q_tiles) * p.b * kp.ranges, p.h);
   kp.scale_log2 = p.softmax_scale * kLog2e;
   kp.scale = p.softmax_scale;
 
-  auto kern = seqs.cu_q ? bwd_rows_kernel<D, kBf16, true> : bwd_rows_kernel<D, kBf16, false>;
+  auto kern = window.keys ? (seqs.cu_q ? bwd_rows_kernel<D, kBf16, true, true> : bwd_rows_kernel<D, kBf16, false, true>)
+                          : (seqs.cu_q ? bwd_rows_kernel<D, kBf16, true, false> : bwd_rows_kernel<D, kBf16, false, false>);
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
   if (e != cudaSuccess) return static_cast<int>(e);
-  const int64_t key_ctas = static_cast<int64_t>(kp.n_tiles) * pl.nsplit * p.h_k * p.b;
+  const int64_t far_ctas = static_cast<int64_t>(pl.sink_tiles) * p.h_k * pl.far_slots * p.b;
+  const int64_t key_ctas = static_cast<int64_t>(kp.n_tiles) * pl.nsplit * p.h_k * p.b + far_ctas;
   const int64_t ctas = key_ctas + static_cast<int64_t>(kp.q_tiles) * p.b * kp.ranges * ((p.h + kp.heads_per_cta - 1) / kp.heads_per_cta);
   if (ctas > 0x7FFFFFFF) return FDMA_ERR_TOO_LARGE;
   kp.n_key_ctas = static_cast<int>(key_ctas);
@@ -1308,6 +1458,12 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   if (ev1) cudaEventRecord(ev1, stream);
   e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
+  if (window.keys) {
+    if (!pl.sink_tiles) return 0;
+    const int64_t rows = static_cast<int64_t>(pl.near_units) * p.h_k * pl.sink_tiles * kBN;
+    sinks_kernel<D, kBf16><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(kp);
+    return static_cast<int>(cudaGetLastError());
+  }
 
   BwdFinishArgs f = {};
   f.b = p.b; f.h = p.h; f.sq = p.seqlen_q; f.sq_r = pl.sq_r; f.d = p.d; f.D = D;
@@ -1373,13 +1529,28 @@ bool bwd_rows_taken(const fdma_bwd_params& bp) {
 // 16384 875 / 706, 4 x 512 over 4 x 2048 170 / 163, 4 x 256 over 4 x 1024 71 / 72; MHA at head dim 64, 2 x 256 over 2 x 4096 182 / 195.
 bool bwd_rows_taken_packed(const fdma_bwd_params& bp) { return bp.f.seqlen_k < 4096 || bp.f.seqlen_k < 4ll * bp.f.seqlen_q; }
 
-size_t bwd_rows_workspace_bytes(const fdma_bwd_params& bp) { return plan(bp).total; }
+size_t bwd_rows_workspace_bytes(const fdma_bwd_params& bp, const Window& window, int sequences) { return plan(bp, window, sequences).total; }
 
-int bwd_rows(const fdma_bwd_params& bp, cudaStream_t stream, const PackedSeqs& seqs) {
-  const RowsPlan pl = plan(bp);
+bool tc_bwd_window_supported(const fdma_bwd_params& bp, const Window& window, int sequences) {
+  const fdma_fwd_params& p = bp.f;
+  if (bp.dbias || bp.scatter_pos || !tc_bwd_supported(bp)) return false;
+  if (tile_head_dim(p.d) == 256) return !sequences;
+  // the 64-key tiles that a query tile sees have to find room in the table of those with a kept key
+  const int64_t seen = (std::min(window.sinks, p.seqlen_k) + kBM - 1) / kBM + (std::min(window.keys, p.seqlen_k) + kBN) / kBM + 2;
+  return !p.mask || std::min<int64_t>(seen, (p.seqlen_k + kBM - 1) / kBM) <= kMaxBits;
+}
+size_t tc_bwd_window_workspace_bytes(const fdma_bwd_params& bp, const Window& window, int sequences) {
+  return tile_head_dim(bp.f.d) == 256 ? tc_bwd256_workspace_bytes(bp, window) : bwd_rows_workspace_bytes(bp, window, sequences);
+}
+int tc_bwd_window(const fdma_bwd_params& bp, cudaStream_t stream, const PackedSeqs& seqs, const Window& window) {
+  return tile_head_dim(bp.f.d) == 256 ? tc_bwd256(bp, stream, window) : bwd_rows(bp, stream, seqs, window);
+}
+
+int bwd_rows(const fdma_bwd_params& bp, cudaStream_t stream, const PackedSeqs& seqs, const Window& window) {
+  const RowsPlan pl = plan(bp, window, seqs.n);
   const bool bf16 = bp.f.dtype == FDMA_BF16;
-  if (pl.D == 64) return bf16 ? launch<64, true>(bp, pl, seqs, stream) : launch<64, false>(bp, pl, seqs, stream);
-  return bf16 ? launch<128, true>(bp, pl, seqs, stream) : launch<128, false>(bp, pl, seqs, stream);
+  if (pl.D == 64) return bf16 ? launch<64, true>(bp, pl, seqs, window, stream) : launch<64, false>(bp, pl, seqs, window, stream);
+  return bf16 ? launch<128, true>(bp, pl, seqs, window, stream) : launch<128, false>(bp, pl, seqs, window, stream);
 }
 
 }  // namespace fdma

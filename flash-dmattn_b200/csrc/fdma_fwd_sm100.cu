@@ -72,6 +72,7 @@ struct FwdKernelParams {
   int d;             // head dim, at most D: columns beyond it are zeros filled in by TMA and are not stored
   int is_causal;
   PackedSeqs seqs;   // packed sequences, each with query blocks and key tiles of its own
+  Window window;     // sliding window (kWindow)
   int n_mblk;        // query blocks (of kNQ tiles) per (batch, head); packed: places for them
   int n_items;       // work items = n_mblk * h * b
   float scale_log2;  // softmax_scale * log2(e)
@@ -182,9 +183,10 @@ __device__ __forceinline__ FwdItem fwd_item(const FwdKernelParams& p, int item, 
 
 // kVariant, per-query kernel: the mask holds one bit per key instead of one byte. Row-broadcast kernel: packed sequences, whose
 // items are the blocks of each (an instantiation of its own: the ordinary kernel's softmax threads have no registers to spare
-// for an item's extents). One launch instead of one per sequence: 8192 tokens in 5 sequences, 16 heads, d = 128: forward 258 ->
+// for an item's extents). kWindow: a sliding window with sinks; a block's key tiles are those of the sinks and, from the first one that
+// its first row sees, those up to the causal limit, numbered without the gap between (KeyTiles). One launch instead of one per sequence: 8192 tokens in 5 sequences, 16 heads, d = 128: forward 258 ->
 // 182 us, backward 617 -> 520 us, the call, with the fills, copies and adds of the sequences' gradients gone, 1510 -> 815 us.
-template <int D, bool kBf16, bool kBcast, bool kVariant = false>
+template <int D, bool kBf16, bool kBcast, bool kVariant = false, bool kWindow = false>
 __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_constant__ FwdKernelParams p) {
   using L = Smem<D>;
   constexpr int kNQ = L::kNQ, kStages = L::kStages;
@@ -224,7 +226,12 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool causal = p.is_causal != 0;
   const WaitCtl ctl{s_abort, p.status};
-  // Per item: number of key tiles each query tile can see at most (causal / length limit), and their maximum.
+  // Per item: number of key tiles each query tile can see at most (causal / length limit), and how many there are to look at: their
+  // maximum, less those between the sinks and the window, which tile_of leaves out.
+  auto gap_of = [&](const FwdItem& w, int nT) {  // of tile numbers from `first` on
+    const int first = (min(p.window.sinks, w.sk) + kBN - 1) / kBN, lo = max(0, w.mblk * kNQ * kBM + w.sk - w.sq - p.window.keys + 1) / kBN;
+    return make_int2(first, max(0, min(lo, nT) - first));
+  };
   auto tile_limits = [&](const FwdItem& w, int (&n_end)[kNQ], const int32_t*& pos_row) {
     pos_row = nullptr;
     if (kBcast && causal && p.key_pos)  // compacted keys: the causal limit is tested on the keys' positions
@@ -240,7 +247,16 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
       n_end[t] = ne;
       nT = max(nT, ne);
     }
-    return nT;
+    return kWindow ? nT - gap_of(w, nT).y : nT;
+  };
+  // number of the key tile at place j
+  auto tile_of = [&](int j, const int2& gap) { return kWindow && j >= gap.x ? j + gap.y : j; };
+  auto item_gap = [&](const FwdItem& w, const int (&n_end)[kNQ]) {
+    if (!kWindow) return make_int2(0, 0);
+    int nT = 0;
+#pragma unroll
+    for (int t = 0; t < kNQ; ++t) nT = max(nT, n_end[t]);
+    return gap_of(w, nT);
   };
 
   // ---------------- set-up: barriers, TMEM ----------------
@@ -301,6 +317,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
         int n_end[kNQ];
         const int32_t* pos_row;
         const int nT = tile_limits(w, n_end, pos_row);
+        const int2 gap = item_gap(w, n_end);
         const uint8_t* s_flags = s_flags_all + (ic & 1) * kMaxTiles;
         ok = mbar_wait(bar_q_empty, (ic & 1) ^ 1, ctl, kWaitQEmpty);
         if (!ok) break;
@@ -324,8 +341,8 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
             const int col = (kv % L::kHalves) * (D / L::kHalves);
 #pragma unroll
             for (int kb = 0; kb < D / L::kHalves / 64; ++kb)
-              tma_load_4d(s_kv + slot * L::kKvBytes + kb * (kBN * 128), tm, bar_kv_full + slot, col + kb * 64, w.hk, w.k0 + j * kBN,
-                          w.b);
+              tma_load_4d(s_kv + slot * L::kKvBytes + kb * (kBN * 128), tm, bar_kv_full + slot, col + kb * 64, w.hk,
+                          w.k0 + tile_of(j, gap) * kBN, w.b);
             ++it;
           }
         }
@@ -358,6 +375,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
       int n_end[kNQ];
       const int32_t* pos_row;
       const int nT = tile_limits(w, n_end, pos_row);
+      const int2 gap = item_gap(w, n_end);
       const uint8_t* s_flags = s_flags_all + (ic & 1) * kMaxTiles;
       ok = __all_sync(0xffffffffu, FDMA_PROF_WAIT(0, mbar_wait(bar_q, ic & 1, ctl, kWaitQ)));
       if (!ok) break;
@@ -367,8 +385,10 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
       // packed sequences: V rows beyond the sequence, in its last tile, become zeros, as TMA fills them in at the end of a
       // tensor (zero probabilities alone would pass a NaN on)
       auto end_v = [&](int slot) {
-        if (!packed || w.sk - prev_j * kBN >= kBN) return;
-        zero_tile_rows(s_kv + slot * L::kKvBytes, D / L::kHalves / 64, kBN * 128, w.sk - prev_j * kBN, kBN);
+        if (!packed) return;
+        const int left = w.sk - tile_of(prev_j, gap) * kBN;
+        if (left >= kBN) return;
+        zero_tile_rows(s_kv + slot * L::kKvBytes, D / L::kHalves / 64, kBN * 128, left, kBN);
         fence_proxy_async_smem();
         __syncwarp();
       };
@@ -515,6 +535,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
       int n_end[kNQ];
       const int32_t* pos_row;
       const int nT = tile_limits(w, n_end, pos_row);
+      const int2 gap = item_gap(w, n_end);
       const uint8_t* s_flags = s_flags_all + (ic & 1) * kMaxTiles;
       if (kBcast) {
         const uint8_t* mrow = p.mask ? p.mask + w.b * p.mask_batch_stride + w.hm * p.mask_head_stride : nullptr;
@@ -526,7 +547,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
           const int slot = bi % kBmSlots;
           ok = __all_sync(0xffffffffu, mbar_wait(bar_bm_empty + slot, ((bi / kBmSlots) & 1) ^ 1, ctl, kWaitBmEmpty));
           if (!ok) break;
-          const int k0 = j * kBN + lane * 4;
+          const int k0 = tile_of(j, gap) * kBN + lane * 4;
           float v[4];
           uint32_t mbits = 0x01010101u;
           if (mrow) mbits = *reinterpret_cast<const uint32_t*>(mrow + k0);
@@ -611,8 +632,10 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
       int n_end[kNQ];
       const int32_t* pos_row;
       const int nT = tile_limits(w, n_end, pos_row);
+      const int2 gap = item_gap(w, n_end);
       uint8_t* s_flags = s_flags_all + (ic & 1) * kMaxTiles;
-      for (int j = lane; j < nT; j += 32) {
+      for (int place = lane; place < nT; place += 32) {
+        const int j = tile_of(place, gap);
         uint8_t f = 0;
         if (kBcast) {
           bool any = true;
@@ -635,7 +658,9 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
           if (any) {
 #pragma unroll
             for (int t = 0; t < kNQ; ++t)
-              if (j < n_end[t]) f |= (1 << t);
+              if (j < n_end[t] && (!kWindow || j * kBN < p.window.sinks ||
+                                   j * kBN + kBN > (w.mblk * kNQ + t) * kBM + w.sk - w.sq - p.window.keys + 1))
+                f |= (1 << t);
             if (pos_row) {  // the tile's smallest position against the last row of each query tile
               const int64_t pmin = pos_row[j * kBN];
 #pragma unroll
@@ -658,7 +683,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
             }
           }
         }
-        s_flags[j] = f;
+        s_flags[place] = f;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_flags_full + (ic & 1));
@@ -696,6 +721,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
     int n_end[kNQ];
     const int32_t* pos_row;
     const int nT = tile_limits(w, n_end, pos_row);
+    const int2 gap = item_gap(w, n_end);
     const uint8_t* s_flags = s_flags_all + (ic & 1) * kMaxTiles;
     const int m0 = (w.mblk * kNQ + t) * kBM;
     const int qrow = m0 + row;
@@ -730,7 +756,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
         if (!ok) break;
       }
       if (fl & (1 << t)) {
-        const int kbase = j * kBN;
+        const int kbase = tile_of(j, gap) * kBN;
         const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
         // Per-query bias / mask: this row's 128 + 256 bytes of the tile are requested BEFORE the wait for the score
         // tile, so the load latency overlaps the wait; the scores then leave TMEM 32 columns at a time and take the
@@ -870,6 +896,15 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
             for (int i = 0; i < kBN / 2; ++i) {
               if (kbase + 2 * i >= klim) s2[i].x = -CUDART_INF_F;
               if (kbase + 2 * i + 1 >= klim) s2[i].y = -CUDART_INF_F;
+            }
+          }
+          // the window's other end: keys from the sinks up to this row's first one
+          if (kWindow && kbase < warp_q0 + 31 + w.sk - w.sq - p.window.keys + 1 && kbase + kBN > p.window.sinks) {
+            const int from = p.window.sinks - kbase, to = qrow + w.sk - w.sq - p.window.keys + 1 - kbase;
+#pragma unroll
+            for (int i = 0; i < kBN / 2; ++i) {
+              if (2 * i >= from && 2 * i < to) s2[i].x = -CUDART_INF_F;
+              if (2 * i + 1 >= from && 2 * i + 1 < to) s2[i].y = -CUDART_INF_F;
             }
           }
         }
@@ -1044,8 +1079,8 @@ FwdPlan plan(const fdma_fwd_params& p) {
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
-template <int D, bool kBf16, bool kBcast, bool kVariant = false>
-int launch(const fdma_fwd_params& p, const FwdPlan& pl, const PackedSeqs& seqs, cudaStream_t stream) {
+template <int D, bool kBf16, bool kBcast, bool kVariant = false, bool kWindow = false>
+int launch(const fdma_fwd_params& p, const FwdPlan& pl, const PackedSeqs& seqs, cudaStream_t stream, const Window& window = {}) {
   using L = Smem<D>;
   constexpr int kNQ = L::kNQ;
   FwdKernelParams kp;
@@ -1084,6 +1119,7 @@ int launch(const fdma_fwd_params& p, const FwdPlan& pl, const PackedSeqs& seqs, 
   kp.h_mask = p.h_mask; kp.h_bias = p.h_bias;
   kp.is_causal = p.is_causal;
   kp.seqs = seqs;
+  kp.window = window;
   kp.key_pos = p.key_pos;
   kp.pos_batch_stride = p.key_pos_batch_stride; kp.pos_head_stride = p.key_pos_head_stride;
   kp.h_pos = p.h_pos; kp.causal_shift = p.causal_shift;
@@ -1099,7 +1135,7 @@ int launch(const fdma_fwd_params& p, const FwdPlan& pl, const PackedSeqs& seqs, 
     kp.act = act;
   }
 
-  auto kern = fwd_kernel<D, kBf16, kBcast, kVariant>;
+  auto kern = fwd_kernel<D, kBf16, kBcast, kVariant, kWindow>;
   // The attribute belongs to the (function, device) pair: set it on every call, whichever device is current.
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -1124,6 +1160,11 @@ int launch_d(const fdma_fwd_params& p, const FwdPlan& pl, const PackedSeqs& seqs
   }
   if (pl.bcast) return seqs.cu_q ? launch<D, false, true, true>(p, pl, seqs, stream) : launch<D, false, true>(p, pl, seqs, stream);
   return (p.mask && p.mask_bits) ? launch<D, false, false, true>(p, pl, seqs, stream) : launch<D, false, false>(p, pl, seqs, stream);
+}
+
+template <int D, bool kBf16>
+int launch_window(const fdma_fwd_params& p, const FwdPlan& pl, const PackedSeqs& seqs, cudaStream_t stream, const Window& window) {
+  return seqs.cu_q ? launch<D, kBf16, true, true, true>(p, pl, seqs, stream, window) : launch<D, kBf16, true, false, true>(p, pl, seqs, stream, window);
 }
 
 }  // namespace
@@ -1178,8 +1219,16 @@ bool tc_fwd_supported(const fdma_fwd_params& p) {
 
 size_t tc_fwd_workspace_bytes(const fdma_fwd_params& p) { return plan(p).act_bytes; }
 
-int tc_fwd(const fdma_fwd_params& p, cudaStream_t stream, const PackedSeqs& seqs) {
+int tc_fwd(const fdma_fwd_params& p, cudaStream_t stream, const PackedSeqs& seqs, const Window& window) {
   const FwdPlan pl = plan(p);
+  if (window.keys > 0) {
+    const bool bf16 = p.dtype == FDMA_BF16;
+    switch (tile_head_dim(p.d)) {
+      case 64: return bf16 ? launch_window<64, true>(p, pl, seqs, stream, window) : launch_window<64, false>(p, pl, seqs, stream, window);
+      case 128: return bf16 ? launch_window<128, true>(p, pl, seqs, stream, window) : launch_window<128, false>(p, pl, seqs, stream, window);
+      default: return bf16 ? launch_window<256, true>(p, pl, seqs, stream, window) : launch_window<256, false>(p, pl, seqs, stream, window);
+    }
+  }
   switch (tile_head_dim(p.d)) {
     case 64: return launch_d<64>(p, pl, seqs, stream);
     case 128: return launch_d<128>(p, pl, seqs, stream);

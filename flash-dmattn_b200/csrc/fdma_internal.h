@@ -25,28 +25,36 @@ struct PackedSeqs {
   const int32_t *cu_q = nullptr, *cu_k = nullptr;
   int n = 0;
 };
+// A sliding window: besides the causal limit, key k is seen by the query at position t only if t - k < keys or k < sinks. keys = 0: none.
+struct Window {
+  int keys = 0, sinks = 0;
+};
 bool tc_fwd_supported(const fdma_fwd_params& p);
 size_t tc_fwd_workspace_bytes(const fdma_fwd_params& p);
-// seqs: packed sequences, see fdma_fwd_varlen
-int tc_fwd(const fdma_fwd_params& p, cudaStream_t stream, const PackedSeqs& seqs = {});
+// seqs: packed sequences, see fdma_fwd_varlen; window: mask broadcast over the queries or absent, no bias, no key positions
+int tc_fwd(const fdma_fwd_params& p, cudaStream_t stream, const PackedSeqs& seqs = {}, const Window& window = {});
 
 // Per-tile mask activity map for per-query masks: act[b][h_mask][ceil(Sq/128)][ceil(Sk/128)] bytes.
 int launch_tile_activity(const fdma_fwd_params& p, uint8_t* act, cudaStream_t stream);
 
 // head dim 256, row-broadcast mask / bias (fdma_bwd256_sm100.cu); reached through the three tc_bwd entry points
 bool tc_bwd256_supported(const fdma_bwd_params& p);
-size_t tc_bwd256_workspace_bytes(const fdma_bwd_params& p);
-int tc_bwd256(const fdma_bwd_params& p, cudaStream_t stream);
+size_t tc_bwd256_workspace_bytes(const fdma_bwd_params& p, const Window& window = {});
+int tc_bwd256(const fdma_bwd_params& p, cudaStream_t stream, const Window& window = {});
 
 // head dims up to 128, row-broadcast mask / bias, packed sequences (fdma_bwd_rows_sm100.cu); also reached through tc_bwd
 bool bwd_rows_taken(const fdma_bwd_params& p);
 bool bwd_rows_taken_packed(const fdma_bwd_params& p);  // the same call, about packed sequences
-size_t bwd_rows_workspace_bytes(const fdma_bwd_params& p);
-int bwd_rows(const fdma_bwd_params& p, cudaStream_t stream, const PackedSeqs& seqs);
+size_t bwd_rows_workspace_bytes(const fdma_bwd_params& p, const Window& window = {}, int sequences = 0);
+int bwd_rows(const fdma_bwd_params& p, cudaStream_t stream, const PackedSeqs& seqs, const Window& window = {});
 
 bool tc_bwd_supported(const fdma_bwd_params& p);
 size_t tc_bwd_workspace_bytes(const fdma_bwd_params& p);
 int tc_bwd(const fdma_bwd_params& p, cudaStream_t stream, const PackedSeqs& seqs = {});  // seqs: head dims up to 128
+// The same with a sliding window; sequences: 0, or the number of packed ones
+bool tc_bwd_window_supported(const fdma_bwd_params& p, const Window& window, int sequences);
+size_t tc_bwd_window_workspace_bytes(const fdma_bwd_params& p, const Window& window, int sequences);
+int tc_bwd_window(const fdma_bwd_params& p, cudaStream_t stream, const PackedSeqs& seqs, const Window& window);
 
 // ---- the kernels before and after every tensor-core backward (fdma_bwd_common.cu) ---------------
 constexpr int kDetFracBits = 40;  // deterministic dQ accumulator: fixed point, |dQ / scale| < 2^23, resolution 2^-40

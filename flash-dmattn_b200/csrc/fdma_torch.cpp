@@ -52,6 +52,9 @@ struct Api {
   decltype(&fdma_bwd) bwd;
   decltype(&fdma_fwd_varlen) fwd_varlen;
   decltype(&fdma_bwd_varlen) bwd_varlen;
+  decltype(&fdma_fwd_window) fwd_window;
+  decltype(&fdma_bwd_window_workspace_bytes) bwd_window_workspace_bytes;
+  decltype(&fdma_bwd_window) bwd_window;
   decltype(&fdma_create_mask) create_mask;
   decltype(&fdma_gather_kept) gather_kept;
   decltype(&fdma_decode_kept) decode_kept;
@@ -74,6 +77,9 @@ void init(const std::string& path) {
   get(api.bwd, "fdma_bwd");
   get(api.fwd_varlen, "fdma_fwd_varlen");
   get(api.bwd_varlen, "fdma_bwd_varlen");
+  get(api.fwd_window, "fdma_fwd_window");
+  get(api.bwd_window_workspace_bytes, "fdma_bwd_window_workspace_bytes");
+  get(api.bwd_window, "fdma_bwd_window");
   get(api.create_mask, "fdma_create_mask");
   get(api.gather_kept, "fdma_gather_kept");
   get(api.decode_kept, "fdma_decode_kept");
@@ -152,6 +158,7 @@ struct Call {
   float scale = 0.f;
   bool causal = false, deterministic = false, bits = false, gathered = false, packed = false;
   int path = FDMA_PATH_AUTO;
+  int64_t window = 0, sinks = 0;  // sliding window: keys that a query sees, first keys that stay visible; 0: none
   int64_t seqlen_k = 0;      // keys of the caller's K
   int64_t bias_keys = 0;     // key extent of the caller's bias
   std::vector<int64_t> bias_c;  // gathered: shape of the gathered bias (empty: no bias)
@@ -259,7 +266,7 @@ struct Meta {
   bool want_bias = false;
 
   std::vector<int64_t> pack() const {
-    std::vector<int64_t> x = {c.causal, c.deterministic, c.bits, c.gathered, c.packed, c.path, c.seqlen_k, c.bias_keys, want_bias};
+    std::vector<int64_t> x = {c.causal, c.deterministic, c.bits, c.gathered, c.packed, c.path, c.window, c.sinks, c.seqlen_k, c.bias_keys, want_bias};
     for (const auto* v : {&c.bias_c, &k_sizes, &bias_sizes}) {
       x.push_back(static_cast<int64_t>(v->size()));
       x.insert(x.end(), v->begin(), v->end());
@@ -273,6 +280,7 @@ struct Meta {
     m.c.scale = static_cast<float>(scale);
     m.c.causal = next(); m.c.deterministic = next(); m.c.bits = next(); m.c.gathered = next(); m.c.packed = next();
     m.c.path = static_cast<int>(next());
+    m.c.window = next(); m.c.sinks = next();
     m.c.seqlen_k = next(); m.c.bias_keys = next(); m.want_bias = next();
     for (auto* v : {&m.c.bias_c, &m.k_sizes, &m.bias_sizes}) {
       v->resize(next());
@@ -365,15 +373,18 @@ variable_list packed_backward(const SavedTensors& t, const Call& c, const Tensor
   bp.dk_row_stride = bp.dv_row_stride = sk.r;
   bp.dk_head_stride = bp.dv_head_stride = sk.h;
   bp.deterministic = c.deterministic ? 1 : 0;
-  const size_t bytes = api.bwd_workspace_bytes(&bp);
+  const int32_t* cu_q = cu.data_ptr<int32_t>();
+  const int32_t *cu_k = cu_q + cu.stride(0), n = static_cast<int32_t>(cu.size(1) - 1);
+  const int32_t window = static_cast<int32_t>(c.window), sinks = static_cast<int32_t>(c.sinks);
+  const size_t bytes = window ? api.bwd_window_workspace_bytes(&bp, window, sinks, n) : api.bwd_workspace_bytes(&bp);
   Tensor ws;
   if (bytes) {
     ws = empty({static_cast<int64_t>(bytes)}, at::kByte, tq);
     bp.f.workspace = ws.data_ptr();
     bp.f.workspace_bytes = bytes;
   }
-  const int32_t* cu_q = cu.data_ptr<int32_t>();
-  check(api.bwd_varlen(&bp, cu_q, cu_q + cu.stride(0), static_cast<int32_t>(cu.size(1) - 1), stream), "fdma_bwd_varlen");
+  if (window) check(api.bwd_window(&bp, window, sinks, cu_q, cu_k, n, stream), "fdma_bwd_window");
+  else check(api.bwd_varlen(&bp, cu_q, cu_k, n, stream), "fdma_bwd_varlen");
   res[0] = dq; res[1] = dk; res[2] = dv;
   return res;
 }
@@ -388,7 +399,7 @@ variable_list backward(const Tensor& grad, const SavedTensors& t, const Meta& me
   const cudaStream_t stream = stream_of(tq);
   raise_if_timed_out(stream);
   if (c.packed) return packed_backward(t, c, kernel_layout(grad), stream);
-  const Tensor dout = c.gathered || c.bits ? kernel_layout(grad) : inner_contiguous(grad);
+  const Tensor dout = c.gathered || c.bits || c.window ? kernel_layout(grad) : inner_contiguous(grad);
 
   fdma_bwd_params bp = {};
   Tensor dq = empty_as(tq), dk, dv, dbias;
@@ -429,14 +440,16 @@ variable_list backward(const Tensor& grad, const SavedTensors& t, const Meta& me
     bp.dbias_keys = static_cast<int32_t>(dbias.size(3));
   }
   bp.deterministic = c.deterministic ? 1 : 0;
-  const size_t bytes = api.bwd_workspace_bytes(&bp);
+  const int32_t window = static_cast<int32_t>(c.window), sinks = static_cast<int32_t>(c.sinks);
+  const size_t bytes = window ? api.bwd_window_workspace_bytes(&bp, window, sinks, 0) : api.bwd_workspace_bytes(&bp);
   Tensor ws;
   if (bytes) {
     ws = empty({static_cast<int64_t>(bytes)}, at::kByte, tq);
     bp.f.workspace = ws.data_ptr();
     bp.f.workspace_bytes = bytes;
   }
-  check(api.bwd(&bp, stream), "fdma_bwd");
+  if (window) check(api.bwd_window(&bp, window, sinks, nullptr, nullptr, 0, stream), "fdma_bwd_window");
+  else check(api.bwd(&bp, stream), "fdma_bwd");
   if (dbias.defined() && !c.gathered && c.bias_keys != dbias.size(3)) {
     dbias = dbias.narrow(3, 0, c.seqlen_k);
     if (c.bias_keys == 1) dbias = dbias.sum({3}, /*keepdim=*/true);
@@ -501,7 +514,8 @@ std::optional<Tensor> decode(const Tensor& q0, const Tensor& k, const Tensor& v,
 // the position list of the kept keys (key_pos, slot_mask), bits with their tile activity, or none.
 std::optional<Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, const OptTensor& mask_, const OptTensor& bias_,
                                 const OptTensor& key_pos_, const OptTensor& slot_mask_, const OptTensor& bits_,
-                                const OptTensor& activity_, double scale, bool causal, bool deterministic, int path) {
+                                const OptTensor& activity_, double scale, bool causal, bool deterministic, int path, int64_t window,
+                                int64_t sinks) {
   const Tensor &mask0 = get(mask_), &bias0 = get(bias_), &key_pos = get(key_pos_), &slot_mask = get(slot_mask_),
                &bits = get(bits_), &activity = get(activity_);
   if (!plain(q0) || !plain(k0) || !plain(v0)) return std::nullopt;
@@ -522,6 +536,11 @@ std::optional<Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor
   c.causal = causal;
   c.deterministic = deterministic;
   c.path = path;
+  if (window) {  // (the caller has checked the rest)
+    if (bias0.defined() || key_pos.defined() || bits.defined() || (mask0.defined() && mask0.size(2) != 1 && Sq != 1)) return std::nullopt;
+    c.window = std::min(window, Sk);
+    c.sinks = std::min(sinks, Sk);
+  }
   c.seqlen_k = Sk;
   c.bias_keys = bias0.defined() ? bias0.size(3) : 0;
   if (key_pos.defined() && Sq == 1) {
@@ -567,7 +586,7 @@ std::optional<Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor
     const c10::cuda::CUDAGuard device(q0.device());
     const cudaStream_t stream = stream_of(q0);
     raise_if_timed_out(stream);
-    const auto layout = c.gathered || c.bits ? kernel_layout : inner_contiguous;
+    const auto layout = c.gathered || c.bits || c.window ? kernel_layout : inner_contiguous;
     q = layout(q0);
     out = empty_as(q);
     lse = empty({B, H, Sq}, at::kFloat, q);
@@ -605,6 +624,11 @@ std::optional<Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor
       v = layout(v0);
       if (c.bits) mask = bits;
       else if (mask0.defined()) mask = inner_contiguous(fit_keys(mask0, Sk_r));
+      if (c.window && mask.defined()) {  // 16-byte loads
+        bool ok = (reinterpret_cast<uintptr_t>(mask.data_ptr()) & 15) == 0;
+        for (int i = 0; i < 2; ++i) ok = ok && bcast_stride(mask, i) % 16 == 0;
+        if (!ok) mask = mask.clone(at::MemoryFormat::Contiguous);
+      }
       if (bias0.defined()) bias = inner_contiguous(fit_keys(bias0, Sk_r));
       if (c.bits && bias0.defined()) {  // 16-byte loads; expanded dimensions are fine
         bool ok = (reinterpret_cast<uintptr_t>(bias.data_ptr()) & 15) == 0;
@@ -616,14 +640,18 @@ std::optional<Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor
       fill_mask_bias(p, mask, bias, activity, c);
     }
     fill_out(p, out, lse);
-    const size_t bytes = api.fwd_workspace_bytes(&p);
-    Tensor ws;
-    if (bytes) {
-      ws = empty({static_cast<int64_t>(bytes)}, at::kByte, q);
-      p.workspace = ws.data_ptr();
-      p.workspace_bytes = bytes;
+    if (c.window) {
+      check(api.fwd_window(&p, static_cast<int32_t>(c.window), static_cast<int32_t>(c.sinks), nullptr, nullptr, 0, stream), "fdma_fwd_window");
+    } else {
+      const size_t bytes = api.fwd_workspace_bytes(&p);
+      Tensor ws;
+      if (bytes) {
+        ws = empty({static_cast<int64_t>(bytes)}, at::kByte, q);
+        p.workspace = ws.data_ptr();
+        p.workspace_bytes = bytes;
+      }
+      check(api.fwd(&p, stream), "fdma_fwd");
     }
-    check(api.fwd(&p, stream), "fdma_fwd");
   }
   if (grad) {
     auto node = std::shared_ptr<AttnBackward>(new AttnBackward(), torch::autograd::deleteNode);
@@ -655,7 +683,7 @@ std::optional<Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor
 // Packed sequences in one launch: q (Tq, H, d), k and v (Tk, Hk, d), cu_q / cu_k (n + 1) int32 on the device, ascending from 0
 // to Tq / Tk (the caller has looked). Returns (out, lse (1, H, Tq)); empty for inputs this path does not take.
 std::vector<Tensor> packed_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& cu_q, const Tensor& cu_k,
-                                     double scale, bool causal, bool deterministic) {
+                                     double scale, bool causal, bool deterministic, int64_t window, int64_t sinks) {
   for (const Tensor* t : {&q0, &k0, &v0})
     if (!t->defined() || !t->is_cuda() || t->layout() != at::kStrided || t->dim() != 3 || t->device() != q0.device()) return {};
   const auto type = q0.scalar_type();
@@ -678,6 +706,8 @@ std::vector<Tensor> packed_attention(const Tensor& q0, const Tensor& k0, const T
   c.causal = causal;
   c.deterministic = deterministic;
   c.packed = true;
+  c.window = std::min(window, Tk);
+  c.sinks = window ? std::min(sinks, Tk) : 0;
   c.seqlen_k = Tk;
   Tensor out, lse, cu;
   {
@@ -696,7 +726,9 @@ std::vector<Tensor> packed_attention(const Tensor& q0, const Tensor& k0, const T
     fill_geometry(p, q4, Tk, Hk, c);
     fill_kv(p, k4, v0.unsqueeze(0));
     fill_out(p, out.unsqueeze(0), lse);
-    check(api.fwd_varlen(&p, pq, pk, static_cast<int32_t>(cu_q.size(0) - 1), stream), "fdma_fwd_varlen");
+    const int32_t n = static_cast<int32_t>(cu_q.size(0) - 1);
+    if (c.window) check(api.fwd_window(&p, static_cast<int32_t>(c.window), static_cast<int32_t>(c.sinks), pq, pk, n, stream), "fdma_fwd_window");
+    else check(api.fwd_varlen(&p, pq, pk, n, stream), "fdma_fwd_varlen");
   }
   if (grad) {
     auto node = std::shared_ptr<AttnBackward>(new AttnBackward(), torch::autograd::deleteNode);
@@ -806,7 +838,7 @@ bool as_tensor(const py::handle& o, OptTensor& t) {
 
 py::object py_attention(py::handle q, py::handle k, py::handle v, py::handle mask, py::handle bias, py::handle key_pos,
                         py::handle slot_mask, py::handle bits, py::handle activity, py::handle scale, bool causal,
-                        bool deterministic, int path) {
+                        bool deterministic, int path, int64_t window, int64_t sinks) {
   OptTensor t[9];
   const py::handle in[9] = {q, k, v, mask, bias, key_pos, slot_mask, bits, activity};
   for (int i = 0; i < 9; ++i)
@@ -822,14 +854,14 @@ py::object py_attention(py::handle q, py::handle k, py::handle v, py::handle mas
   std::optional<Tensor> out;
   {
     py::gil_scoped_release release;
-    out = attention(*t[0], *t[1], *t[2], t[3], t[4], t[5], t[6], t[7], t[8], s, causal, deterministic, path);
+    out = attention(*t[0], *t[1], *t[2], t[3], t[4], t[5], t[6], t[7], t[8], s, causal, deterministic, path, window, sinks);
   }
   if (!out) return py::none();
   return py::reinterpret_steal<py::object>(THPVariable_Wrap(*out));
 }
 
 py::object py_packed_attention(py::handle q, py::handle k, py::handle v, py::handle cu_q, py::handle cu_k, double scale, bool causal,
-                               bool deterministic) {
+                               bool deterministic, int64_t window, int64_t sinks) {
   OptTensor t[5];
   const py::handle in[5] = {q, k, v, cu_q, cu_k};
   for (int i = 0; i < 5; ++i)
@@ -838,7 +870,7 @@ py::object py_packed_attention(py::handle q, py::handle k, py::handle v, py::han
   std::vector<Tensor> res;
   {
     py::gil_scoped_release release;
-    res = packed_attention(*t[0], *t[1], *t[2], *t[3], *t[4], scale, causal, deterministic);
+    res = packed_attention(*t[0], *t[1], *t[2], *t[3], *t[4], scale, causal, deterministic, window, sinks);
   }
   if (res.empty()) return py::none();
   py::tuple out(res.size());
@@ -864,8 +896,11 @@ py::object py_topk_mask(py::handle bias, py::handle premask, int64_t window, dou
 
 PYBIND11_MODULE(_fdma_torch, m) {
   m.def("init", &init);
-  m.def("attention", &py_attention);
-  m.def("packed_attention", &py_packed_attention);
+  using py::arg;
+  m.def("attention", &py_attention, arg("query"), arg("key"), arg("value"), arg("mask"), arg("bias"), arg("key_pos"), arg("slot_mask"),
+        arg("bits"), arg("activity"), arg("scale"), arg("causal"), arg("deterministic"), arg("path"), arg("window") = 0, arg("sinks") = 0);
+  m.def("packed_attention", &py_packed_attention, arg("query"), arg("key"), arg("value"), arg("cu_q"), arg("cu_k"), arg("scale"),
+        arg("causal"), arg("deterministic"), arg("window") = 0, arg("sinks") = 0);
   m.def("topk_mask", &py_topk_mask);
   bind_cache_ops(m);
 }

@@ -68,6 +68,9 @@ EXPORTED_SYMBOLS = (
     "fdma_bwd",
     "fdma_fwd_varlen",
     "fdma_bwd_varlen",
+    "fdma_fwd_window",
+    "fdma_bwd_window_workspace_bytes",
+    "fdma_bwd_window",
     "fdma_create_mask",
     "fdma_last_kernel_status",
     "fdma_poll_kernel_status",
@@ -174,6 +177,12 @@ def load():
     lib.fdma_bwd_workspace_bytes.argtypes = [POINTER(BwdParams)]
     lib.fdma_bwd.restype = c_int
     lib.fdma_bwd.argtypes = [POINTER(BwdParams), c_void_p]
+    lib.fdma_fwd_window.restype = c_int
+    lib.fdma_fwd_window.argtypes = [POINTER(FwdParams), c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p]
+    lib.fdma_bwd_window_workspace_bytes.restype = c_size_t
+    lib.fdma_bwd_window_workspace_bytes.argtypes = [POINTER(BwdParams), c_int32, c_int32, c_int32]
+    lib.fdma_bwd_window.restype = c_int
+    lib.fdma_bwd_window.argtypes = [POINTER(BwdParams), c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p]
     lib.fdma_create_mask.restype = c_int
     lib.fdma_create_mask.argtypes = [POINTER(MaskParams), c_void_p]
     lib.fdma_last_kernel_status.restype = c_int

@@ -533,7 +533,7 @@ def flash_sparse_attn_func(
     )
 
 
-def _one_launch(query, key, value, cu_q, cu_k, cq, ck, max_q, max_k, softmax_scale, is_causal, deterministic):
+def _one_launch(query, key, value, cu_q, cu_k, cq, ck, max_q, max_k, softmax_scale, is_causal, deterministic, window, sinks):
     """Packed sequences in one launch: (out, lse (1, H, total_q)), or None for calls that go sequence by sequence -- lengths
     that leave tokens out, decrease or exceed the given maxima (the loop raises the right error), tracing, forced kernel
     families, and the layouts the native path declines."""
@@ -545,7 +545,8 @@ def _one_launch(query, key, value, cu_q, cu_k, cq, ck, max_q, max_k, softmax_sca
         if not (0 <= cq[i + 1] - cq[i] <= max_q and 0 <= ck[i + 1] - ck[i] <= max_k):
             return None
     scale = query.shape[-1] ** (-0.5) if softmax_scale is None else float(softmax_scale)
-    return _native.load().packed_attention(query, key, value, cu_q, cu_k, scale, bool(is_causal), bool(deterministic))
+    return _native.load().packed_attention(query, key, value, cu_q, cu_k, scale, bool(is_causal), bool(deterministic), window,
+                                           sinks)
 
 
 def flash_sparse_attn_varlen_func(
@@ -580,6 +581,13 @@ def flash_sparse_attn_varlen_func(
     built and raises NotImplementedError."""
     if block_table is not None:
         raise NotImplementedError("paged KV (block_table) is not built into the B200 kernels")
+    return _varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal, softcap,
+                   deterministic, return_attn_probs)
+
+
+def _varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal, softcap, deterministic,
+            return_attn_probs, window=0, sinks=0):
+    """`flash_sparse_attn_varlen_func`, with a sliding window (0: none)."""
     if query.dim() != 3 or key.dim() != 3 or value.dim() != 3:
         raise RuntimeError("query, key and value must be (total_tokens, nheads, headdim)")
     if cu_seqlens_q.numel() != cu_seqlens_k.numel() or cu_seqlens_q.numel() < 2:
@@ -592,7 +600,7 @@ def flash_sparse_attn_varlen_func(
     res = None
     if not softcap and len(cq) > 2:
         res = _one_launch(query, key, value, cu_seqlens_q, cu_seqlens_k, cq, ck, max_seqlen_q, max_seqlen_k, softmax_scale,
-                          is_causal, deterministic)
+                          is_causal, deterministic, window, sinks)
     if res is not None:
         if not return_attn_probs:
             return res[0]
@@ -612,8 +620,13 @@ def flash_sparse_attn_varlen_func(
             outs.append((q_i * 0)[0])
             lses.append(torch.full((H, lq), float("inf"), dtype=torch.float32, device=query.device))
             continue
-        res = flash_sparse_attn_func(q_i, key[ck[i]:ck[i + 1]].unsqueeze(0), value[ck[i]:ck[i + 1]].unsqueeze(0),
-                                     None, None, softmax_scale, is_causal, softcap, deterministic, return_attn_probs)
+        k_i, v_i = key[ck[i]:ck[i + 1]].unsqueeze(0), value[ck[i]:ck[i + 1]].unsqueeze(0)
+        if window:
+            from .window import flash_sparse_attn_window_func
+
+            res = flash_sparse_attn_window_func(q_i, k_i, v_i, window, sinks, None, softmax_scale, deterministic, return_attn_probs)
+        else:
+            res = flash_sparse_attn_func(q_i, k_i, v_i, None, None, softmax_scale, is_causal, softcap, deterministic, return_attn_probs)
         if return_attn_probs:
             outs.append(res[0][0])
             lses.append(res[1][0])

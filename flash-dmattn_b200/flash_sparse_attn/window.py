@@ -1,0 +1,178 @@
+"""Attention with a sliding window and sink tokens, dense and on packed sequences. No counterpart in the reference, whose window is the
+number of keys that a dynamic mask keeps. Over the paged 8-bit cache: `flash_sparse_attn_cache_func(..., sliding_window, sink_tokens)`.
+
+    the query at position t sees the key at position k:  k <= t  and  (t - k < sliding_window or k < sink_tokens)  and  mask(k)
+
+Key tiles that no query of a tile sees are neither loaded nor multiplied (csrc/fdma_fwd_sm100.cu, fdma_bwd_rows_sm100.cu,
+fdma_bwd256_sm100.cu); the mask is one of the keys, for all queries.
+"""
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib, _native
+from . import flash_sparse_attn_interface as _interface
+
+__all__ = ["flash_sparse_attn_window_func", "flash_sparse_attn_window_varlen_func"]
+
+
+def check_window(sliding_window, sink_tokens) -> None:
+    for name, x in (("sliding_window", sliding_window), ("sink_tokens", sink_tokens)):
+        if not isinstance(x, (int, torch.SymInt)) or isinstance(x, bool):
+            raise TypeError(f"{name} must be an int, got {type(x).__name__}")
+    if not 1 <= sliding_window < 2 ** 31 or not 0 <= sink_tokens < 2 ** 31:
+        raise ValueError("sliding_window must be at least 1 and sink_tokens at least 0, both below 2^31")
+
+
+def flash_sparse_attn_window_func(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    sliding_window: int,
+    sink_tokens: int = 0,
+    attn_mask: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    deterministic: Optional[bool] = None,
+    return_attn_probs: Optional[bool] = None,
+):
+    """Causal attention in which a query sees the last `sliding_window` keys, its own among them, and the first `sink_tokens`.
+
+    query (B, Sq, H, d); key, value (B, Sk, Hk, d) with H % Hk == 0; fp16 or bf16, head dims up to 256. Query i is at position
+    i + Sk - Sq, as under `flash_sparse_attn_func(is_causal=True)`, which this equals where the window is as long as the keys.
+    attn_mask: bool ({B|1}, {H|Hk|1}, 1, {Sk|1}), False = masked out, such as padding; masks per query are not built. Rows that see no key
+    return 0. Keys and values are expected to be finite, also where the mask hides them. softmax_scale defaults to d ** -0.5.
+    return_attn_probs=True returns (out, softmax_lse (B, H, Sq) fp32, empty tensor).
+
+    Time and traffic go with the window, not with Sk. Returns out (B, Sq, H, d); gradients flow to query, key and value, each a sum in
+    a fixed order, with `deterministic` or without. Head dims above 128 take gradients of masks that are shared by the query heads of a
+    kv head. Nothing synchronises: a step can be captured into a CUDA graph."""
+    check_window(sliding_window, sink_tokens)
+    if attn_mask is not None:
+        if not isinstance(attn_mask, torch.Tensor) or attn_mask.dtype != torch.bool or attn_mask.dim() != 4:
+            raise RuntimeError("attn_mask must be a bool tensor ({B|1}, {H|Hk|1}, 1, {Sk|1})")
+        if attn_mask.shape[2] != 1:
+            raise NotImplementedError("masks per query are not built with a sliding window: attn_mask must be ({B|1}, {H|Hk|1}, 1, {Sk|1})")
+    elif key.dim() == 4 and sliding_window + sink_tokens >= key.shape[1]:  # every query sees all keys up to its own
+        return _interface.flash_sparse_attn_func(query, key, value, None, None, softmax_scale, True, None, deterministic,
+                                                 return_attn_probs)
+    if not return_attn_probs and not torch.compiler.is_compiling() and _interface._kernel_path in (_lib.PATH_AUTO, _lib.PATH_TCGEN05):
+        out = _native.load().attention(query, key, value, attn_mask, None, None, None, None, None, softmax_scale, True, bool(deterministic),
+                                       _interface._kernel_path, sliding_window, sink_tokens)
+        if out is not None:
+            return out
+    d = query.shape[-1]
+    softmax_scale = d ** -0.5 if softmax_scale is None else softmax_scale
+    if d % 8:  # 16-bit rows are kept 16-byte aligned
+        query, key, value = (torch.nn.functional.pad(t, [0, 8 - d % 8]) for t in (query, key, value))
+    if attn_mask is not None and key.dim() == 4:
+        keys = _interface.round_multiple(key.shape[1], _interface._KEY_PAD)
+        if attn_mask.shape[-1] == 1:
+            attn_mask = attn_mask.expand(*attn_mask.shape[:-1], keys)
+        elif attn_mask.shape[-1] != keys:
+            attn_mask = torch.nn.functional.pad(attn_mask, [0, keys - attn_mask.shape[-1]])
+    out, lse = _WindowAttnFunc.apply(query, key, value, attn_mask, softmax_scale, sliding_window, sink_tokens)
+    out = out[..., :d]
+    return (out, lse, torch.empty((0,), dtype=query.dtype, device=query.device)) if return_attn_probs else out
+
+
+def flash_sparse_attn_window_varlen_func(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: torch.Tensor,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    sliding_window: int,
+    sink_tokens: int = 0,
+    softmax_scale: Optional[float] = None,
+    deterministic: Optional[bool] = None,
+    return_attn_probs: Optional[bool] = None,
+):
+    """`flash_sparse_attn_window_func` on packed sequences: arguments and results as of `flash_sparse_attn_varlen_func`, positions,
+    window and sinks in each sequence. Sequences that cover the tokens run in one launch per direction up to head dim 128; the
+    boundaries are read on the host (one device synchronisation per call)."""
+    check_window(sliding_window, sink_tokens)
+    if sliding_window + sink_tokens >= max_seqlen_k:  # every query sees all keys up to its own
+        sliding_window = sink_tokens = 0
+    return _interface._varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, True, None,
+                              deterministic, return_attn_probs, sliding_window, sink_tokens)
+
+
+class _WindowAttnFunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, scale, window, sinks):
+        out, lse = torch.ops.flash_sparse_attn._window_forward(q, k, v, mask, scale, window, sinks)
+        ctx.save_for_backward(q, k, v, mask, out, lse)
+        ctx.args = (scale, window, sinks)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    def backward(ctx, dout, *_):
+        q, k, v, mask, out, lse = ctx.saved_tensors
+        return (*torch.ops.flash_sparse_attn._window_backward(dout, q, k, v, mask, out, lse, *ctx.args), None, None, None, None)
+
+
+def _aligned(t: Optional[torch.Tensor], unit: int) -> Optional[torch.Tensor]:
+    """The tensor as the kernels load it: 16-byte aligned base and strides, innermost dimension dense."""
+    if t is None:
+        return None
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    ok = ok and all(t.stride(i) % unit == 0 and (t.stride(i) > 0 or unit == 16) for i in range(t.dim() - 1) if t.shape[i] > 1)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _prepare(q, k, v, mask):
+    q, k, v, mask = _aligned(q, 8), _aligned(k, 8), _aligned(v, 8), _aligned(mask, 16)
+    _interface._check_inputs(q, k, v, mask, None)
+    return q, k, v, mask
+
+
+@torch.library.custom_op("flash_sparse_attn::_window_forward", mutates_args=(), device_types="cuda")
+def _window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor], softmax_scale: float, window: int,
+                    sinks: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    q, k, v, mask = _prepare(q, k, v, mask)
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        _interface._raise_if_kernel_timed_out(lib)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+        p = _lib.FwdParams()
+        _interface._fill_fwd(p, q, k, v, mask, None, out, lse, softmax_scale, True)
+        _lib.check(lib.fdma_fwd_window(ctypes.byref(p), window, sinks, None, None, 0, _interface._stream_ptr(q.device)), "fdma_fwd_window")
+    return out, lse
+
+
+@torch.library.register_fake("flash_sparse_attn::_window_forward")
+def _window_forward_fake(q, k, v, mask, softmax_scale, window, sinks):
+    B, Sq, H, _ = q.shape
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
+
+
+@torch.library.custom_op("flash_sparse_attn::_window_backward", mutates_args=(), device_types="cuda")
+def _window_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor], out: torch.Tensor,
+                     softmax_lse: torch.Tensor, softmax_scale: float, window: int, sinks: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    q, k, v, mask = _prepare(q, k, v, mask)
+    dout, out, lse = _aligned(dout, 8), _aligned(out, 8), softmax_lse.contiguous()
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        _interface._raise_if_kernel_timed_out(lib)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        bp = _lib.BwdParams()
+        _interface._fill_fwd(bp.f, q, k, v, mask, None, out, lse, softmax_scale, True)
+        for name, t in (("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+            setattr(bp, "dout" if name == "do" else name, t.data_ptr())
+            for s, x in zip(("batch", "row", "head"), _interface._bsh(t)):
+                setattr(bp, f"{name}_{s}_stride", x)
+        size = lib.fdma_bwd_window_workspace_bytes(ctypes.byref(bp), window, sinks, 0)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        bp.f.workspace, bp.f.workspace_bytes = ws.data_ptr(), size
+        _lib.check(lib.fdma_bwd_window(ctypes.byref(bp), window, sinks, None, None, 0, _interface._stream_ptr(q.device)), "fdma_bwd_window")
+    return dq, dk, dv
+
+
+@torch.library.register_fake("flash_sparse_attn::_window_backward")
+def _window_backward_fake(dout, q, k, v, mask, out, softmax_lse, softmax_scale, window, sinks):
+    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
