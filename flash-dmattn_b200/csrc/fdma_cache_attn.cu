@@ -55,6 +55,8 @@ struct AttnArgs {
   const int32_t* prompts;  // not null: rows of no request are written already, and if it points to 0, those of requests with
                            // kPromptTokens or more as well (one word: look-ups that read three more took 10 us of 340)
   int cluster, tiles;      // CTAs that share a unit, and tiles of a request, where there are few units (kCluster)
+  // Sliding window: first chunks with sinks; most chunks that a unit has, all others lying between the sinks and the window (see gap_of)
+  int sink_chunks, unit_chunks;
   bool merge_requests;     // CTAs of the second kernel: kPromptTokens - 1 for each request, not one for every token
   float* partial;          // [cta][2][rows][D + 4]: sums over the values, then maximum, sum and the maximum's exponent
   int* status;
@@ -183,7 +185,7 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
   q.chunks = max(0, chunk1 - chunk0);
   q.rows = q.chunks ? min(q.n, a.p.max_seqlen_q) * a.group : 0;  // no chunks: refused
   if (a.prompts && q.n >= kPromptTokens && *a.prompts == 0) q.rows = -1;
-  if (a.list_chunks) q.chunks = a.list_chunks;
+  q.chunks = a.list_chunks ? a.list_chunks : min(q.chunks, a.unit_chunks);
   return q;
 }
 
@@ -203,6 +205,16 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, int rows) { return rows > 0 ? (rows + (1 << a.row_shift) - 1) >> a.row_shift : 0; }
 // (token, head) of a request's row
 __device__ __forceinline__ uint2 token_head(const AttnArgs& a, int row) { return divide(row, a.group, a.group_inverse); }
+// Sliding window: first key in the window of a request's row
+__device__ __forceinline__ int first_key(const AttnArgs& a, const Request& q, int row) {
+  return q.length - q.n + static_cast<int>(token_head(a, row).x) - a.p.window + 1;
+}
+// Chunks between those of the sinks and the first one in the window of the tile whose first row is `row0`: unit_chunks from there reach
+// beyond the last key that a row of the tile sees. Chunk i of a unit lies at i, from sink_chunks on at i + gap.
+__device__ __forceinline__ int gap_of(const AttnArgs& a, const Request& q, int row0) {
+  return !a.list_chunks ? max(0, (max(0, first_key(a, q, row0)) >> 6) - a.sink_chunks) : 0;
+}
+__device__ __forceinline__ int chunk_at(const AttnArgs& a, int i, int gap) { return i < a.sink_chunks ? i : i + gap; }
 
 // The units in the order of their chunks. Up to kHeld requests: their data and the sums of their chunks x tiles are held in shared
 // memory. More: the sums are in global memory, and the data is read where it is needed.
@@ -359,7 +371,8 @@ struct Layout {
 
 // kBias: with a bias, dense (without one the loop is shorter by its loads: 14.2 us instead of 14.7 for 16 requests of drafts). With a list
 // of kept keys the bias is looked for when it runs.
-template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster, bool kBias>
+// kWindow: a sliding window with sinks, an instantiation of its own: the first keys of rows' windows take registers.
+template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster, bool kBias, bool kWindow>
 __global__ void __launch_bounds__(Layout<D, ROWS, kGather>::kThreads, Layout<D, ROWS, kGather>::kCtas)
 cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using L = Layout<D, ROWS, kGather>;
@@ -434,7 +447,9 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
         hk = u.hk;
         used = lane_q.rows > u.tile * ROWS;
-        const int pos = static_cast<int>(w - u.start) * kChunk + (lane & 3) * kSlice;
+        int chunk = static_cast<int>(w - u.start);
+        if (kWindow) chunk = chunk_at(a, chunk, gap_of(a, lane_q, u.tile * ROWS));
+        const int pos = chunk * kChunk + (lane & 3) * kSlice;
         if (used && pos < min(lane_q.length, p.max_seqlen_k) && (pos >> a.shift) < c.width) {
           block = c.table[static_cast<int64_t>(u.r) * c.width + (pos >> a.shift)];
           row = pos & ((1 << a.shift) - 1);
@@ -539,6 +554,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const int length = min(q.length, p.max_seqlen_k);
     // oldest key that not every row sees
     const int sure = p.is_causal ? min(length, q.length - q.n + static_cast<int>(token_head(a, row0).x) + 1) : length;
+    // sliding window: the key from which on every row sees it
+    const int gap = kWindow ? gap_of(a, q, row0) : 0, all_from = kWindow ? first_key(a, q, row0 + nrows - 1) : 0;
 
     // queries: eight threads a row, to fp16 in the order of the fragments
     consumers_sync();
@@ -605,7 +622,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     // share of the softmax's sum, factor of the scores, newest position seen
     float o[kTiles][D / 32][2][4], l[kTiles][2], row_scale[kTiles][2];
     Peak top[kTiles][2];
-    int newest[kTiles][2];
+    int newest[kTiles][2], oldest[kTiles][2];  // (oldest: of the window)
     const uint16_t* bias_row[kTiles][2];
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
@@ -617,6 +634,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         row_scale[nt][e] = s_row_scale[rr];
         const uint2 th = token_head(a, row);
         newest[nt][e] = p.is_causal ? min(length - 1, q.length - q.n + static_cast<int>(th.x)) : length - 1;
+        oldest[nt][e] = kWindow ? first_key(a, q, row) : 0;
         const int head = u.hk * a.group + th.y;
         bias_row[nt][e] = biased ? static_cast<const uint16_t*>(p.bias) + u.r * p.bias_batch_stride +
                                        (p.h_bias == p.h ? head : p.h_bias == c.h_k ? u.hk : 0) * p.bias_head_stride
@@ -701,7 +719,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
 
     for (int chunk = first; chunk < last; ++chunk) {
-      const int pos0 = chunk * kChunk + warp * kSlice;
+      const int pos0 = (kWindow ? chunk_at(a, chunk, gap) : chunk) * kChunk + warp * kSlice;
       if (kGather) gather(chunk);
       const int key = key_row(g);  // this lane's scores: keys pos0 + key, + 8
       uint16_t raw_bias[kTiles][2][2];
@@ -750,7 +768,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
       }
       // all 16 keys are there and seen by every row
-      const bool clean = !kGather && pos0 + kSlice <= sure && meta.x != 0.f;
+      const bool clean = !kGather && pos0 + kSlice <= sure && (!kWindow || pos0 >= all_from || pos0 + kSlice <= p.sinks) && meta.x != 0.f;
+      auto behind = [&](int pos, int nt, int k) { return kWindow && pos < oldest[nt][k & 1] && pos >= p.sinks; };
       float x[kTiles][4];
       auto z_of = [&](int k) { return kGather ? key_meta[k >> 1].z : meta.z; };  // exponent of the V scale of score k
       // log2 of its ratio to the maximum
@@ -771,14 +790,15 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             float add = km.x;
             if (head_bias && pos >= 0 && pos < p.bias_keys) add = bias_log2(raw_to_f<kBf16>(__ldg(bias_row[nt][k & 1] + pos)));
             v = fmaf(s[nt][k], row_scale[nt][k & 1] * km.y, add);
-            if (add == -CUDART_INF_F || pos > newest[nt][k & 1]) v = -CUDART_INF_F;  // even where the key is NaN
+            if (add == -CUDART_INF_F || pos > newest[nt][k & 1] || behind(pos, nt, k)) v = -CUDART_INF_F;  // even where the key is NaN
           } else {
             v = s[nt][k] * (row_scale[nt][k & 1] * meta.y);
             if (with_bias) {
               const float add = bias_log2(raw_to_f<kBf16>(raw_bias[nt][k >> 1][k & 1]));
               v = add == -CUDART_INF_F ? add : v + add;
             }
-            if (!clean && (pos0 + (k >> 1) * 8 + key > newest[nt][k & 1] || meta.x == 0.f)) v = -CUDART_INF_F;
+            const int pos = pos0 + (k >> 1) * 8 + key;
+            if (!clean && (pos > newest[nt][k & 1] || behind(pos, nt, k) || meta.x == 0.f)) v = -CUDART_INF_F;
           }
           d[nt][k] = ratio(nt, k);
           grows |= d[nt][k] > 0.f;
@@ -1205,7 +1225,7 @@ __global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const
 int tile_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 struct Plan {
-  int D, rows, ctas, list_chunks;
+  int D, rows, ctas, list_chunks, sink_chunks, unit_chunks;
   bool sums;  // by a kernel of their own: many requests, and not one tile of cu_chunks' chunks for each
   int64_t most_chunks;
   bool prompts;
@@ -1222,12 +1242,20 @@ Plan plan_of(const fdma_cache_attention_params& p) {
   pl.rows = most <= 8 || pl.D == 256 ? 8 : 16;
   pl.ctas = (pl.D == 256 || pl.rows > 8 ? 2 : 3) * sm_count();
   pl.list_chunks = p.kept_pos ? (p.kept_capacity + kChunk - 1) / kChunk : 0;
-  pl.sums = p.c.requests > kHeld && (pl.list_chunks || most > pl.rows);
+  pl.sink_chunks = (p.sinks + kChunk - 1) / kChunk;
+  pl.unit_chunks = 0x7FFFFFFF;
+  if (p.window) {
+    // the tokens of a tile see window + tokens - 1 keys in a row
+    const int group = p.h / p.c.h_k;
+    const int64_t tokens = std::min<int64_t>(std::max(std::min(p.max_seqlen_q, p.c.tokens), 1), (pl.rows - 1) / group + 2), keys = p.window + tokens - 1;
+    pl.unit_chunks = static_cast<int>(std::min<int64_t>(pl.unit_chunks, pl.sink_chunks + (keys + kChunk - 2) / kChunk + 1));
+  }
+  pl.sums = p.c.requests > kHeld && (pl.list_chunks || most > pl.rows || p.window);
   const int64_t tiles = static_cast<int64_t>(p.c.tokens) * (p.h / p.c.h_k) / pl.rows + p.c.requests;
-  pl.most_chunks = tiles * (pl.list_chunks ? pl.list_chunks : (static_cast<int64_t>(p.c.width) * p.c.block_size + kChunk - 1) / kChunk);
+  pl.most_chunks = tiles * (pl.list_chunks ? pl.list_chunks : std::min<int64_t>((static_cast<int64_t>(p.c.width) * p.c.block_size + kChunk - 1) / kChunk, pl.unit_chunks));
   pl.tiles = static_cast<int>((most + pl.rows - 1) / pl.rows);
   const int64_t units = static_cast<int64_t>(p.c.requests) * p.c.h_k * pl.tiles;
-  const int64_t chunks = pl.list_chunks ? pl.list_chunks : (std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size) + kChunk - 1) / kChunk;
+  const int64_t chunks = pl.list_chunks ? pl.list_chunks : std::min<int64_t>((std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size) + kChunk - 1) / kChunk, pl.unit_chunks);
   pl.units = static_cast<int>(std::min<int64_t>(units, 1 << 20));
   pl.cluster = 0;
   // Few and short enough units get a cluster each: as many CTAs as run at once (clusters leave places of a GPU's parts empty, 16 a
@@ -1254,7 +1282,7 @@ int allow_wide_clusters_once(const void* kernel, std::atomic<uint64_t>& prepared
   return 0;
 }
 
-template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster, bool kBias>
+template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster, bool kBias, bool kWindow>
 int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
   using L = Layout<D, ROWS, kGather>;
   const fdma_cache& c = a.p.c;
@@ -1267,7 +1295,7 @@ int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
     if (!st) st = encode_tmap_4d(&map_v, c.v, 1, dims, strides, box);
     if (st) return st;
   }
-  auto kern = cache_attend_kernel<D, ROWS, kGather, kBf16, kCluster, kBias>;
+  auto kern = cache_attend_kernel<D, ROWS, kGather, kBf16, kCluster, kBias, kWindow>;
   static std::atomic<uint64_t> prepared{0}, wide{0};
   const int st_smem = allow_smem_once(reinterpret_cast<const void*>(kern), L::kTotal, prepared);
   if (st_smem) return st_smem;
@@ -1306,15 +1334,19 @@ int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
   cfg.numAttrs = 1;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, cache_merge_kernel<D, kBf16>, a));
 }
-template <int D, int ROWS, bool kCluster, bool kBf16>
+template <int D, int ROWS, bool kCluster, bool kBf16, bool kWindow>
 int launch_c(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
-  if (a.list_chunks) return launch<D, ROWS, true, kBf16, kCluster, false>(a, pl, stream);
-  return a.p.bias ? launch<D, ROWS, false, kBf16, kCluster, true>(a, pl, stream) : launch<D, ROWS, false, kBf16, kCluster, false>(a, pl, stream);
+  if (a.list_chunks) return launch<D, ROWS, true, kBf16, kCluster, false, kWindow>(a, pl, stream);
+  return a.p.bias ? launch<D, ROWS, false, kBf16, kCluster, true, kWindow>(a, pl, stream) : launch<D, ROWS, false, kBf16, kCluster, false, kWindow>(a, pl, stream);
+}
+template <int D, int ROWS, bool kWindow>
+int launch_w(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
+  if (a.p.dtype == FDMA_BF16) return pl.cluster ? launch_c<D, ROWS, true, true, kWindow>(a, pl, stream) : launch_c<D, ROWS, false, true, kWindow>(a, pl, stream);
+  return pl.cluster ? launch_c<D, ROWS, true, false, kWindow>(a, pl, stream) : launch_c<D, ROWS, false, false, kWindow>(a, pl, stream);
 }
 template <int D, int ROWS>
 int launch_t(const AttnArgs& a, const Plan& pl, cudaStream_t stream) {
-  if (a.p.dtype == FDMA_BF16) return pl.cluster ? launch_c<D, ROWS, true, true>(a, pl, stream) : launch_c<D, ROWS, false, true>(a, pl, stream);
-  return pl.cluster ? launch_c<D, ROWS, true, false>(a, pl, stream) : launch_c<D, ROWS, false, false>(a, pl, stream);
+  return a.p.window ? launch_w<D, ROWS, true>(a, pl, stream) : launch_w<D, ROWS, false>(a, pl, stream);
 }
 
 int check_attention(const fdma_cache_attention_params* pp) {
@@ -1325,6 +1357,7 @@ int check_attention(const fdma_cache_attention_params* pp) {
   if (p.h <= 0 || p.h % p.c.h_k || p.max_seqlen_q < 0 || p.max_seqlen_k < 0) return FDMA_ERR_BAD_ARG;
   if (p.bias && ((p.h_bias != 1 && p.h_bias != p.c.h_k && p.h_bias != p.h) || p.bias_keys <= 0)) return FDMA_ERR_BAD_ARG;
   if (p.kept_pos && p.kept_capacity <= 0) return FDMA_ERR_BAD_ARG;
+  if (p.window < 0 || p.sinks < 0 || (p.window && !p.is_causal) || (p.sinks && !p.window)) return FDMA_ERR_BAD_ARG;
   if (p.dtype != FDMA_BF16 && p.dtype != FDMA_FP16) return FDMA_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(p.c.num_blocks) * p.c.h_k > 0x7FFFFFFF || static_cast<int64_t>(p.c.tokens) * p.h > 0x7FFFFFFF) return FDMA_ERR_UNSUPPORTED;
   return 0;
@@ -1335,15 +1368,28 @@ int check_attention(const fdma_cache_attention_params* pp) {
 
 using namespace fdma;
 
+namespace fdma {
+namespace {
+// More than a request can hold makes no difference.
+fdma_cache_attention_params with_window(const fdma_cache_attention_params& in) {
+  fdma_cache_attention_params p = in;
+  const int most = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.c.width) * p.c.block_size, 0x3FFFFFFF));
+  p.window = std::min(p.window, most);
+  p.sinks = std::min(p.sinks, most);
+  return p;
+}
+}  // namespace
+}  // namespace fdma
+
 extern "C" size_t fdma_cache_attention_workspace_bytes(const fdma_cache_attention_params* p) {
   if (check_attention(p) || p->c.tokens == 0) return 0;
-  return plan_of(*p).bytes;
+  return plan_of(with_window(*p)).bytes;
 }
 
 extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void* stream_) {
   const int st = check_attention(pp);
   if (st) return st;
-  const fdma_cache_attention_params& p = *pp;
+  const fdma_cache_attention_params p = with_window(*pp);
   if (p.c.tokens == 0) return FDMA_OK;
   if (!p.query || !p.out) return FDMA_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uint64_t>(p.out_row_stride | p.out_head_stride) * 2) % 16) return FDMA_ERR_UNSUPPORTED;
@@ -1360,6 +1406,8 @@ extern "C" int fdma_cache_attention(const fdma_cache_attention_params* pp, void*
   a.h_k_inverse = inverse(p.c.h_k);
   a.p.max_seqlen_q = std::max(a.p.max_seqlen_q, 1);
   a.list_chunks = pl.list_chunks;
+  a.sink_chunks = pl.sink_chunks;
+  a.unit_chunks = pl.unit_chunks;
   a.ctas = pl.ctas;
   a.scale_log2 = p.softmax_scale * kLog2e;
   a.q_vec = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uint64_t>(p.query_row_stride | p.query_head_stride) * 2) % 16 == 0;

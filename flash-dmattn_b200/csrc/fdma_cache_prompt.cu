@@ -40,7 +40,14 @@ struct UnpackArgs {
   PromptFound* found;  // zeros before
   void *k, *v;  // (rows, h_k, d)
   int shift, max_keys, max_queries, rows, heads;
+  // Sliding window (0: none): of a request the chunks with sinks are converted and those from the first key on that one of its queries sees.
+  // Behind one another they are a sequence whose window and sinks leave the same keys visible.
+  int window, sink_chunks;
 };
+// Chunks that are left out, of a request of `length` tokens of which `queries` are new
+__device__ __forceinline__ int gap_of(const UnpackArgs& a, int length, int queries) {
+  return a.window ? max(0, max(0, length - queries - a.window + 1) / kChunk - a.sink_chunks) : 0;
+}
 
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack_scaled(uint16_t two, float scale) {
@@ -93,11 +100,11 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
     long long my_pairs = 0;
     int my_length = 0;
     if (r < R && c.cu_chunks[r + 1] > c.cu_chunks[r] && c.cu_seqlens[r + 1] - c.cu_seqlens[r] >= kPromptTokens) {
-      const int n = max(0, min(min(c.lengths[r], a.max_keys), c.width << a.shift));
+      const int queries = c.cu_seqlens[r + 1] - c.cu_seqlens[r], held = max(0, min(min(c.lengths[r], a.max_keys), c.width << a.shift));
+      const int n = held - min(held, gap_of(a, c.lengths[r], queries) * kChunk);
       x = (static_cast<long long>(n) << 32) | ((n + kChunk - 1) / kChunk);
-      my_length = n;
-      const int queries = c.cu_seqlens[r + 1] - c.cu_seqlens[r];
-      my_pairs = static_cast<long long>(n + kTileKeys) * queries;
+      my_length = a.window ? window_keys(n, a.window, a.sink_chunks * kChunk) : n;
+      my_pairs = static_cast<long long>(my_length + kTileKeys) * queries;
       if (c.lengths[r] > a.max_keys || queries > a.max_queries) s_beyond = true;
     }
     my_length = __reduce_max_sync(0xffffffffu, my_length);
@@ -146,7 +153,8 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
       if (pre_chunks[mid + 1] > w) hi = mid;
       else lo = mid + 1;
     }
-    const int pos0 = (w - pre_chunks[lo]) * kChunk, row0 = pre_rows[lo] + pos0, n = min(kChunk, pre_rows[lo + 1] - row0);
+    const int chunk = w - pre_chunks[lo], row0 = pre_rows[lo] + chunk * kChunk, n = min(kChunk, pre_rows[lo + 1] - row0);
+    const int gap = gap_of(a, c.lengths[lo], c.cu_seqlens[lo + 1] - c.cu_seqlens[lo]), pos0 = (chunk < a.sink_chunks ? chunk : chunk + gap) * kChunk;
     if (tid < 4) {
       const int pos = pos0 + tid * 16;
       int block = tid * 16 < n ? c.table[static_cast<int64_t>(lo) * c.width + (pos >> a.shift)] : -1;
@@ -205,7 +213,9 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const __grid_constant_
 // At most so many keys: requests that have kPromptTokens new ones each, of the longest length.
 int64_t most_rows(const fdma_cache_attention_params& p) {
   const int64_t requests = std::min<int64_t>(p.c.requests, p.c.tokens / kPromptTokens);
-  return requests * std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size);
+  int64_t keys = std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size);
+  if (p.window) keys = std::min<int64_t>(keys, static_cast<int64_t>(p.window) + std::min(p.max_seqlen_q, p.c.tokens) + p.sinks + 2 * kChunk);
+  return requests * keys;
 }
 struct Scratch {
   size_t v, lse, found, cu_k, total;
@@ -246,7 +256,8 @@ fdma_fwd_params forward_params(const fdma_cache_attention_params& p, char* ws) {
 
 bool cache_prompt_taken(const fdma_cache_attention_params& p) {
   if (std::min(p.max_seqlen_q, p.c.tokens) < kPromptTokens || p.bias || p.kept_pos || p.c.requests > kMostRequests) return false;
-  const int64_t keys = std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size);
+  int64_t keys = std::min<int64_t>(p.max_seqlen_k, static_cast<int64_t>(p.c.width) * p.c.block_size);
+  if (p.window) keys = window_keys(keys, p.window, p.sinks);
   if (!prompt_pays(static_cast<int64_t>(p.c.tokens) * p.h * (keys + kTileKeys), keys, p.c.d)) return false;
   const int64_t rows = most_rows(p);
   if (rows <= 0 || rows > kMostRows || scratch(p).total > static_cast<size_t>(kMostBytes)) return false;
@@ -271,6 +282,8 @@ int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspac
   a.max_queries = p.max_seqlen_q;
   a.rows = static_cast<int>(most_rows(p));
   a.heads = p.h;
+  a.window = p.window;
+  a.sink_chunks = (p.sinks + kChunk - 1) / kChunk;
   const size_t smem = (static_cast<size_t>(p.c.requests) + 1) * 8;
   const bool bf16 = p.dtype == FDMA_BF16;
   if (smem > 40 * 1024) {
@@ -287,7 +300,8 @@ int cache_prompt(const fdma_cache_attention_params& p, int shift, void* workspac
   else unpack_kernel<false><<<ctas, kThreads, smem, stream>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
-  return tc_fwd(forward_params(p, ws), stream, PackedSeqs{p.c.cu_seqlens, a.cu_k, p.c.requests});
+  const fdma_fwd_params f = forward_params(p, ws);
+  return tc_fwd(f, stream, PackedSeqs{p.c.cu_seqlens, a.cu_k, p.c.requests}, Window{std::min(p.window, f.seqlen_k), std::min(p.sinks, f.seqlen_k)});
 }
 
 }  // namespace fdma

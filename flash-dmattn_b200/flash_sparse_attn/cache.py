@@ -20,6 +20,7 @@ import torch
 from . import _native
 from .rotary import RotaryFrequencies
 from .utils.mask import KeptKeys
+from .window import check_window
 
 __all__ = ["BlockTables", "CacheStep", "QuantizedCache", "block_tables", "quantized_cache", "cache_append",
            "flash_sparse_attn_cache_func"]
@@ -159,6 +160,8 @@ def flash_sparse_attn_cache_func(
     is_causal: bool = True,
     max_seqlen_q: Optional[int] = None,
     max_seqlen_k: Optional[int] = None,
+    sliding_window: Optional[int] = None,
+    sink_tokens: int = 0,
 ) -> torch.Tensor:
     """Attention of the step's queries over the cache, after `cache_append` has written the step's keys and values.
 
@@ -170,6 +173,9 @@ def flash_sparse_attn_cache_func(
     host knows them (default: the step's tokens, the tables' width). They choose how the work is split and how much scratch a call
     takes: pass them where you can. Where a request goes beyond them, its queries from max_seqlen_q on are 0 (the first always counts), and
     keys from max_seqlen_k on are not seen; queries' positions stay those in the whole request.
+    sliding_window, sink_tokens: as in `flash_sparse_attn_window_func`, of the keys seen so far a query sees the last sliding_window, its own
+    among them, and those at positions below sink_tokens. Blocks that nobody sees are not read, so that a step's time goes with the window
+    (with attn_mask: with the mask); the requests keep them.
 
     Returns (tokens, H, d). Rows of tokens behind the last request, of refused requests and of queries that see no key are 0. A key or
     value that is NaN reaches the queries that see it and no others.
@@ -180,6 +186,14 @@ def flash_sparse_attn_cache_func(
     of scratch: a call whose bounds allow for more reads the 8 bits, as one does that comes upon NaN in a value or numbers that 16 bits do not hold.
     There are no gradients: a call that would need them raises."""
     args = _cache_args(cache, tables, step)
+    window = 0
+    if sliding_window is not None:
+        check_window(sliding_window, sink_tokens)
+        if not is_causal:
+            raise ValueError("sliding_window needs is_causal=True")
+        window = sliding_window
+    elif sink_tokens:
+        raise ValueError("sink_tokens needs a sliding_window")
     key_pos = count = None
     if isinstance(attn_mask, KeptKeys):
         key_pos, count = attn_mask.key_pos, attn_mask.count
@@ -198,10 +212,10 @@ def flash_sparse_attn_cache_func(
     max_k = tables.table.shape[-1] * tables.block_size if max_seqlen_k is None else max_seqlen_k
     args = args + (query, key_pos, count, attn_bias)
     if not torch.compiler.is_compiling():
-        out = _native.load().cache_attention(args, softmax_scale, is_causal, max_q, max_k)
+        out = _native.load().cache_attention(args, softmax_scale, is_causal, max_q, max_k, window, sink_tokens)
         if out is not None:
             return out
-    return torch.ops.flash_sparse_attn._cache_attention(*args, softmax_scale, is_causal, max_q, max_k)
+    return torch.ops.flash_sparse_attn._cache_attention(*args, softmax_scale, is_causal, max_q, max_k, window, sink_tokens)
 
 
 # ---- the same as custom operators, for tracing -------------------------------------------------------------------------
@@ -264,13 +278,14 @@ def _cache_attention(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_
                      cu_seqlens: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor, cu_blocks: torch.Tensor,
                      cu_chunks: torch.Tensor, query: torch.Tensor, key_pos: Optional[torch.Tensor], count: Optional[torch.Tensor],
                      bias: Optional[torch.Tensor], softmax_scale: Optional[float], is_causal: bool, max_seqlen_q: int,
-                     max_seqlen_k: int) -> torch.Tensor:
+                     max_seqlen_k: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
     return _plain(_native.load().cache_attention((k, v, k_scale, v_scale, table, cu_seqlens, positions, lengths, cu_blocks, cu_chunks,
-                                                  query, key_pos, count, bias), softmax_scale, is_causal, max_seqlen_q, max_seqlen_k),
+                                                  query, key_pos, count, bias), softmax_scale, is_causal, max_seqlen_q, max_seqlen_k,
+                                                 window, sinks),
                   "flash_sparse_attn_cache_func")
 
 
 @torch.library.register_fake("flash_sparse_attn::_cache_attention")
 def _cache_attention_fake(k, v, k_scale, v_scale, table, cu_seqlens, positions, lengths, cu_blocks, cu_chunks, query, key_pos, count,
-                          bias, softmax_scale, is_causal, max_seqlen_q, max_seqlen_k):
+                          bias, softmax_scale, is_causal, max_seqlen_q, max_seqlen_k, window=0, sinks=0):
     return torch.empty(query.shape, dtype=query.dtype, device=query.device)
