@@ -1,5 +1,5 @@
-// Native host path of the rotary positions, the block tables and the 8-bit cache: argument checks, allocations, the autograd
-// node and the launches of flash_sparse_attn/rotary.py and cache.py, on top of the C ABI (include/fdma.h). Wrong arguments raise
+// Native host path of the rotary positions, the block tables, the 8-bit cache and the verification of drafts: argument checks,
+// allocations, the autograd node and the launches of flash_sparse_attn/rotary.py, cache.py and drafts.py, on top of the C ABI (include/fdma.h). Wrong arguments raise
 // RuntimeError here. Tensors that stand for something else (tracing, subclasses, functorch) get None: the Python layer then goes
 // through its custom operators, which come back here with plain tensors.
 #include <ATen/ATen.h>
@@ -35,6 +35,7 @@ struct Api {
   decltype(&fdma_cache_append) cache_append;
   decltype(&fdma_cache_attention) cache_attention;
   decltype(&fdma_cache_attention_workspace_bytes) cache_attention_workspace_bytes;
+  decltype(&fdma_verify_drafts) verify_drafts;
   decltype(&fdma_strerror) strerror;
   decltype(&fdma_poll_kernel_status) poll_kernel_status;
   decltype(&fdma_last_kernel_status) last_kernel_status;
@@ -375,11 +376,13 @@ std::optional<Tensor> append(const Cache& t, const Tensor& key0, const Tensor& v
 }
 
 Tensor attend(const Cache& t, const Tensor& query0, const Tensor& key_pos, const Tensor& count, const Tensor& bias0, std::optional<double> scale,
-              bool causal, int64_t max_q, int64_t max_k) {
+              bool causal, int64_t max_q, int64_t max_k, int64_t window, int64_t sinks) {
   check_tokens(query0, t, "query must be a bf16 or fp16 tensor (tokens, heads, headdim) on the cache's device");
   const int64_t T = query0.size(0), H = query0.size(1), d = query0.size(2), Hk = t.k.size(1), R = t.table.size(0);
   need(H > 0 && H % Hk == 0, "Number of heads in key/value must divide number of heads in query");
   need(max_q >= 0 && max_k >= 0, "max_seqlen_q and max_seqlen_k must not be negative");
+  need(window >= 0 && sinks >= 0 && (!sinks || window), "sliding_window must be positive, and sink_tokens need one");
+  need(!window || causal, "a sliding window is causal");
   fdma_cache_attention_params p = {};
   p.c = cache_params(t, T);
   at::AutoDispatchBelowADInplaceOrView guard;
@@ -394,6 +397,8 @@ Tensor attend(const Cache& t, const Tensor& query0, const Tensor& key_pos, const
   p.h = static_cast<int32_t>(H);
   p.dtype = dtype_code(query);
   p.is_causal = causal;
+  p.window = static_cast<int32_t>(std::min<int64_t>(window, 0x7FFFFFFF));
+  p.sinks = static_cast<int32_t>(std::min<int64_t>(sinks, 0x7FFFFFFF));
   p.softmax_scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d)));
   p.max_seqlen_q = static_cast<int32_t>(std::min<int64_t>(max_q, T));
   p.max_seqlen_k = static_cast<int32_t>(std::min<int64_t>(max_k, static_cast<int64_t>(p.c.width) * p.c.block_size));
@@ -430,6 +435,63 @@ Tensor attend(const Cache& t, const Tensor& query0, const Tensor& key_pos, const
   }
   check(api.cache_attention(&p, stream), "fdma_cache_attention");
   return out;
+}
+
+// ---- drafts -----------------------------------------------------------------------------------------------------------
+// temperatures: undefined, or one for each request; then `temperature` is not used
+std::vector<Tensor> verify(const Tensor& cu_seqlens, const Tensor& lengths, const Tensor& granted, const Tensor& ids, const Tensor& logits0,
+                           const Tensor& uniforms, const Tensor& probs0, const Tensor& temperatures, double temperature) {
+  need(logits0.is_cuda(), "Input tensor must be on CUDA device");
+  need(dtype_code(logits0) >= 0 && logits0.dim() == 2 && logits0.size(1) > 0 && logits0.size(0) <= 0x7FFFFFFF && logits0.size(1) <= 0x7FFFFFFF,
+       "logits must be a bf16, fp16 or fp32 tensor (tokens, vocabulary)");
+  const int64_t T = logits0.size(0), V = logits0.size(1), R = lengths.dim() == 1 ? lengths.size(0) : -1;
+  check_int(cu_seqlens, logits0, 1, "the step's tensors must be contiguous int32 tensors on the logits' device");
+  check_int(lengths, logits0, 1, "the step's tensors must be contiguous int32 tensors on the logits' device");
+  need(granted.device() == logits0.device() && granted.scalar_type() == at::kBool && granted.dim() == 1 && granted.is_contiguous(),
+       "step.granted must be a contiguous bool tensor on the logits' device");
+  need(cu_seqlens.size(0) == R + 1 && granted.size(0) == R, "the step's tensors are of different numbers of requests");
+  need(ids.device() == logits0.device() && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong) && ids.dim() == 1 && ids.size(0) == T && ids.is_contiguous(),
+       "token_ids must be a contiguous int32 or int64 tensor (tokens) on the logits' device");
+  need(uniforms.device() == logits0.device() && uniforms.scalar_type() == at::kFloat && uniforms.dim() == 1 && uniforms.size(0) == T && uniforms.is_contiguous(),
+       "uniforms must be a contiguous float32 tensor (tokens) on the logits' device");
+  if (probs0.defined())
+    need(probs0.device() == logits0.device() && dtype_code(probs0) >= 0 && probs0.sizes() == logits0.sizes(),
+         "draft_probs must be a bf16, fp16 or fp32 tensor of the logits' shape and device");
+  if (temperatures.defined())
+    need(temperatures.device() == logits0.device() && temperatures.scalar_type() == at::kFloat && temperatures.dim() == 1 && temperatures.size(0) == R &&
+             temperatures.is_contiguous(),
+         "temperature must be a number or a contiguous float32 tensor (requests) on the logits' device");
+  for (const Tensor* t : {&logits0, &uniforms, &probs0, &temperatures})
+    need(!(at::GradMode::is_enabled() && t->defined() && t->requires_grad()), "the verification of drafts has no gradients: call it under torch.no_grad()");
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const c10::cuda::CUDAGuard device(logits0.device());
+  const Tensor logits = inner_contiguous(logits0), probs = probs0.defined() ? inner_contiguous(probs0) : probs0;
+  Tensor accepted = empty({R}, at::kInt, logits), next = empty({R}, at::kLong, logits), after = empty({R}, at::kInt, logits);
+  fdma_verify_params p = {};
+  p.logits = logits.data_ptr();
+  p.logits_row_stride = stride_of(logits, 0);
+  p.dtype = dtype_code(logits);
+  if (probs.defined()) {
+    p.draft_probs = probs.data_ptr();
+    p.probs_row_stride = stride_of(probs, 0);
+    p.probs_dtype = dtype_code(probs);
+  }
+  p.token_ids = ids.data_ptr();
+  p.id_bits = ids.scalar_type() == at::kLong ? 64 : 32;
+  p.uniforms = uniforms.data_ptr<float>();
+  p.temperatures = temperatures.defined() ? temperatures.data_ptr<float>() : nullptr;
+  p.temperature = static_cast<float>(temperature);
+  p.cu_seqlens = cu_seqlens.data_ptr<int32_t>();
+  p.lengths = lengths.data_ptr<int32_t>();
+  p.granted = static_cast<const uint8_t*>(granted.data_ptr());
+  p.accepted = accepted.data_ptr<int32_t>();
+  p.next_tokens = next.data_ptr<int64_t>();
+  p.lengths_out = after.data_ptr<int32_t>();
+  p.requests = static_cast<int32_t>(R);
+  p.tokens = static_cast<int32_t>(T);
+  p.vocab = static_cast<int32_t>(V);
+  check(api.verify_drafts(&p, stream_of(logits)), "fdma_verify_drafts");
+  return {accepted, next, after};
 }
 
 // ---- Python -----------------------------------------------------------------------------------------------------------
@@ -508,16 +570,27 @@ py::object py_append(const py::tuple& tensors, bool interleaved, double amplitud
 }
 
 // tensors: the same ten; query, key_pos, count, bias
-py::object py_attend(const py::tuple& tensors, const py::object& scale, bool causal, int64_t max_q, int64_t max_k) {
+py::object py_attend(const py::tuple& tensors, const py::object& scale, bool causal, int64_t max_q, int64_t max_k, int64_t window, int64_t sinks) {
   std::vector<Tensor> t;
   if (!unpack(tensors, t)) return py::none();
   const std::optional<double> s = scale.is_none() ? std::nullopt : std::optional<double>(py::cast<double>(scale));
   Tensor out;
   {
     py::gil_scoped_release release;
-    out = attend(cache_of(t), t.at(10), t.at(11), t.at(12), t.at(13), s, causal, max_q, max_k);
+    out = attend(cache_of(t), t.at(10), t.at(11), t.at(12), t.at(13), s, causal, max_q, max_k, window, sinks);
   }
   return wrap(out);
+}
+
+// tensors: cu_seqlens, lengths, granted, token ids, logits, uniforms, draft probabilities or None, temperatures or None
+py::object py_verify(const py::tuple& tensors, double temperature) {
+  std::vector<Tensor> t, res;
+  if (!unpack(tensors, t)) return py::none();
+  {
+    py::gil_scoped_release release;
+    res = verify(t.at(0), t.at(1), t.at(2), t.at(3), t.at(4), t.at(5), t.at(6), t.at(7), temperature);
+  }
+  return wrap(res);
 }
 
 }  // namespace
@@ -533,6 +606,7 @@ void init_cache_ops(void* library) {
   get(api.cache_append, "fdma_cache_append");
   get(api.cache_attention, "fdma_cache_attention");
   get(api.cache_attention_workspace_bytes, "fdma_cache_attention_workspace_bytes");
+  get(api.verify_drafts, "fdma_verify_drafts");
   get(api.strerror, "fdma_strerror");
   get(api.poll_kernel_status, "fdma_poll_kernel_status");
   get(api.last_kernel_status, "fdma_last_kernel_status");
@@ -540,8 +614,10 @@ void init_cache_ops(void* library) {
 
 void bind_cache_ops(py::module& m) {
   m.def("rotary", &py_rotary);
+  m.def("verify_drafts", &py_verify);
   m.def("tables_extend", &py_extend);
   m.def("tables_truncate", &py_truncate);
   m.def("cache_append", &py_append);
-  m.def("cache_attention", &py_attend);
+  using py::arg;
+  m.def("cache_attention", &py_attend, arg("tensors"), arg("scale"), arg("causal"), arg("max_q"), arg("max_k"), arg("window") = 0, arg("sinks") = 0);
 }

@@ -14,6 +14,7 @@ from .packed import PackedMask, pack_mask  # noqa: F401
 from .rotary import RotaryFrequencies, apply_rotary, rotary_frequencies  # noqa: F401
 from .cache import (BlockTables, CacheStep, QuantizedCache, block_tables, cache_append,  # noqa: F401
                     flash_sparse_attn_cache_func, quantized_cache)
+from .drafts import VerifiedDrafts, verify_drafts  # noqa: F401
 from .window import (flash_sparse_attn_window_func,  # noqa: F401
                      flash_sparse_attn_window_varlen_func)
 from .utils.mask import KeptKeys  # noqa: F401

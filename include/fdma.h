@@ -506,9 +506,38 @@ typedef struct fdma_cache_attention_params {
   int32_t reserved;
   void* workspace;
   size_t workspace_bytes;
+  int32_t window, sinks; /* sliding window, 0: none. With is_causal: the key at position k is seen by the query at position t only if
+                            t - k < window or k < sinks too. Blocks that nobody sees are not read */
 } fdma_cache_attention_params;
 size_t fdma_cache_attention_workspace_bytes(const fdma_cache_attention_params* p);
 int fdma_cache_attention(const fdma_cache_attention_params* p, void* stream);
+
+/*
+ * Verification of drafted tokens. The step's token j of request r is followed by its token j + 1, a draft, for all but the request's
+ * last; row cu_seqlens[r] + j of logits (tokens, vocab) is the target's for what follows. With p = softmax(logits / T) a draft x is
+ * accepted if uniforms[row] q(x) < p(x), q = draft_probs[row] (tokens, vocab; each row the probabilities that the draft behind it was
+ * drawn from), or 1 without them; the first one that is not ends the request's. accepted[r]: how many are; lengths_out[r] = lengths[r] less those that are not, as
+ * fdma_tables_truncate takes them; next_tokens[r]: drawn from max(p - q, 0) of the first rejected row (without draft_probs: p without
+ * the draft), or from p of the last row, by uniforms[last row of the request]: the first token whose running sum is above that number times
+ * the total. What nothing is left of is drawn from p. T not above 0: the largest logit (of equal ones the first) is what is accepted
+ * and comes next. temperatures (requests), or NULL: temperature for all. NaN logits count as -inf, +inf as the largest finite number, probabilities that are negative or NaN as 0. Requests
+ * without tokens or not granted (granted may be NULL): 0 accepted, next token -1, lengths as they are; -1 also where a row is -inf
+ * throughout. Drafts outside the vocabulary are rejected. dtype, probs_dtype: fdma_dtype; id_bits: 32 or 64. Row strides in elements.
+ */
+typedef struct fdma_verify_params {
+  const void *logits, *draft_probs, *token_ids;
+  const float *uniforms, *temperatures;
+  const int32_t *cu_seqlens, *lengths;
+  const uint8_t* granted;
+  int32_t* accepted;
+  int64_t* next_tokens;
+  int32_t* lengths_out;
+  int64_t logits_row_stride, probs_row_stride;
+  int32_t requests, tokens, vocab, dtype, probs_dtype, id_bits;
+  float temperature;
+  int32_t reserved;
+} fdma_verify_params;
+int fdma_verify_drafts(const fdma_verify_params* p, void* stream);
 
 /*
  * Measurement hook (no counterpart in the reference, which is timed from Python with wall clocks,
