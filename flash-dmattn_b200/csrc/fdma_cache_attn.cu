@@ -1270,18 +1270,6 @@ Plan plan_of(const fdma_cache_attention_params& p) {
   return pl;
 }
 
-int allow_wide_clusters_once(const void* kernel, std::atomic<uint64_t>& prepared) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (prepared.load(std::memory_order_acquire) & bit)) return 0;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (dev < 64) prepared.fetch_or(bit, std::memory_order_release);
-  return 0;
-}
-
 template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster, bool kBias, bool kWindow>
 int launch(AttnArgs a, const Plan& pl, cudaStream_t stream) {
   using L = Layout<D, ROWS, kGather>;

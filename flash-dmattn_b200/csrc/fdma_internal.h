@@ -166,6 +166,19 @@ inline int allow_smem_once(const void* kernel, int bytes, std::atomic<uint64_t>&
   return 0;
 }
 
+// Allows a kernel clusters of more than 8 CTAs on the current device, once per device.
+inline int allow_wide_clusters_once(const void* kernel, std::atomic<uint64_t>& prepared) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (prepared.load(std::memory_order_acquire) & bit)) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 64) prepared.fetch_or(bit, std::memory_order_release);
+  return 0;
+}
+
 // Events registered by fdma_time_next_kernel for this host thread (both null when none); take_* clears them.
 void take_timing_events(cudaEvent_t* start, cudaEvent_t* stop);
 

@@ -36,6 +36,7 @@ struct Api {
   decltype(&fdma_cache_attention) cache_attention;
   decltype(&fdma_cache_attention_workspace_bytes) cache_attention_workspace_bytes;
   decltype(&fdma_verify_drafts) verify_drafts;
+  decltype(&fdma_verify_drafts_workspace_bytes) verify_drafts_workspace_bytes;
   decltype(&fdma_strerror) strerror;
   decltype(&fdma_poll_kernel_status) poll_kernel_status;
   decltype(&fdma_last_kernel_status) last_kernel_status;
@@ -490,6 +491,13 @@ std::vector<Tensor> verify(const Tensor& cu_seqlens, const Tensor& lengths, cons
   p.requests = static_cast<int32_t>(R);
   p.tokens = static_cast<int32_t>(T);
   p.vocab = static_cast<int32_t>(V);
+  const size_t bytes = api.verify_drafts_workspace_bytes(&p);
+  Tensor ws;
+  if (bytes) {
+    ws = empty({static_cast<int64_t>(bytes)}, at::kByte, logits);
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = bytes;
+  }
   check(api.verify_drafts(&p, stream_of(logits)), "fdma_verify_drafts");
   return {accepted, next, after};
 }
@@ -607,6 +615,7 @@ void init_cache_ops(void* library) {
   get(api.cache_attention, "fdma_cache_attention");
   get(api.cache_attention_workspace_bytes, "fdma_cache_attention_workspace_bytes");
   get(api.verify_drafts, "fdma_verify_drafts");
+  get(api.verify_drafts_workspace_bytes, "fdma_verify_drafts_workspace_bytes");
   get(api.strerror, "fdma_strerror");
   get(api.poll_kernel_status, "fdma_poll_kernel_status");
   get(api.last_kernel_status, "fdma_last_kernel_status");

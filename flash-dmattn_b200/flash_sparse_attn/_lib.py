@@ -89,6 +89,7 @@ EXPORTED_SYMBOLS = (
     "fdma_cache_append",
     "fdma_cache_attention_workspace_bytes",
     "fdma_cache_attention",
+    "fdma_verify_drafts_workspace_bytes",
     "fdma_verify_drafts",
 )
 

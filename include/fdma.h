@@ -536,7 +536,10 @@ typedef struct fdma_verify_params {
   int32_t requests, tokens, vocab, dtype, probs_dtype, id_bits;
   float temperature;
   int32_t reserved;
+  void* workspace; /* 16-byte aligned */
+  size_t workspace_bytes;
 } fdma_verify_params;
+size_t fdma_verify_drafts_workspace_bytes(const fdma_verify_params* p);
 int fdma_verify_drafts(const fdma_verify_params* p, void* stream);
 
 /*
