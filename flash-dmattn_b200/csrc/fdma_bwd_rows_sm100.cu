@@ -96,7 +96,7 @@ struct BwdRowsParams {
   int h_pos, causal_shift;
   PackedSeqs seqs;   // packed sequences, each with tiles of its own; streamed query tiles are cut at fixed rows
   // Sliding window (kWindow). A key tile's CTA takes the queries whose window reaches it (near); those beyond, which see the sinks alone,
-  // come from CTAs of their own (far), kFarRows queries each. Tiles with sinks leave fp32 sums, which sinks_kernel adds up:
+  // come from CTAs of their own (far), kFarRows queries each. Both leave fp32 sums of the sinks' rows, which sinks_kernel adds up:
   // [2: dV, dK][near of each sequence or batch element, then a place for each part of kFarRows queries][h_k][sink_tiles * 128][D]
   Window window;
   float* sink_sums;
@@ -321,6 +321,7 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
   int beyond = 0;  // far: what is added to a key's first query that sees it; near: as many queries see it
   if (kWindow) {
     beyond = p.window.keys;
+    if (!far && sink_unit >= 0 && !far_part(key0, key_end, q_lo, q_hi, coff, p.window)) sink_unit = -1;  // nobody is beyond
     if (far) {
       if (packed) {
         const PackedTile t = packed_tile(p.seqs.cu_q, p.seqs.n, Sq, kFarRows, slot);
@@ -697,7 +698,7 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = 0u;
         }
-        if (kWindow ? sink_unit >= 0 : p.dkv_part != nullptr) {
+        if (kWindow ? sink_unit >= 0 && n_in_seq * kBN + krow < p.window.sinks : p.dkv_part != nullptr) {
           // fp32 partial: part[dv|dk][split][b][hk][key][d]
           if ((packed || kWindow) && !key_ok) continue;  // (after the warp-wide load)
           float* part = kWindow ? p.sink_sums + (((static_cast<int64_t>(half) * (p.near_units + p.b * p.far_slots) + sink_unit) * p.h_k + hk) *
@@ -1226,13 +1227,13 @@ __global__ void __launch_bounds__(kThreads, 1) bwd_rows_kernel(const __grid_cons
   }
 }
 
-// Sliding window, tiles that hold sinks: dV and dK as the sum of what the CTAs of the queries near them and of those beyond have left, in
-// the order of the queries. A warp per key row.
+// Sliding window, sinks that queries beyond the window see: dV and dK as the sum of what the CTAs of the queries near them and of those beyond
+// have left, in the order of the queries. A warp per key row.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) sinks_kernel(const __grid_constant__ BwdRowsParams p) {
-  const int lane = threadIdx.x & 31, rows = p.sink_tiles * kBN;
+  const int lane = threadIdx.x & 31, rows = p.sink_tiles * kBN, sinks = min(p.window.sinks, rows);
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int unit = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * rows)), hk = static_cast<int>(w / rows % p.h_k), row = static_cast<int>(w % rows);
+  const int unit = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * sinks)), hk = static_cast<int>(w / sinks % p.h_k), row = static_cast<int>(w % sinks);
   if (unit >= p.near_units) return;
   const bool packed = p.seqs.cu_q != nullptr;
   int2 keys = make_int2(0, p.seqlen_k), queries = make_int2(0, p.seqlen_q);
@@ -1244,19 +1245,30 @@ __global__ void __launch_bounds__(256) sinks_kernel(const __grid_constant__ BwdR
   }
   if (keys.x + row >= keys.y) return;
   const int key0 = keys.x + row / kBN * kBN, coff = keys.y - queries.y;
+  if (!far_part(key0, key0 + 1, queries.x, queries.y, coff, p.window)) return;  // written by the CTA of the tile
   const int64_t units = p.near_units + static_cast<int64_t>(p.b) * p.far_slots;
   const int b = packed ? 0 : unit;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {  // dV, dK
     float acc[D / 32];
-    auto add = [&](int64_t u, bool fresh) {
-      const float* src = p.sink_sums + (((x * units + u) * p.h_k + hk) * rows + row) * D + lane * (D / 32);
+    auto at = [&](int64_t u) { return p.sink_sums + (((x * units + u) * p.h_k + hk) * rows + row) * D + lane * (D / 32); };
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = src[i] + (fresh ? 0.f : acc[i]);
-    };
-    add(unit, true);
-    for (int c = 0, q = queries.x; row < p.window.sinks && q < queries.y; ++c, q += kFarRows)
-      if (far_part(key0, key0 + 1, q, min(q + kFarRows, queries.y), coff, p.window)) add(first + c, false);
+    for (int i = 0; i < D / 32; ++i) acc[i] = at(unit)[i];
+    // parts that reach beyond the window: those from this one on. Eight are asked for at a time.
+    const int parts = (queries.y - queries.x + kFarRows - 1) / kFarRows;
+    int c0 = 0;
+    while (!far_part(key0, key0 + 1, queries.x + c0 * kFarRows, min(queries.x + (c0 + 1) * kFarRows, queries.y), coff, p.window)) ++c0;
+    for (; c0 < parts; c0 += 8) {
+      float y[8][D / 32];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) y[j][i] = c0 + j < parts ? at(first + c0 + j)[i] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] += y[j][i];
+    }
     uint16_t* dst = x == 0 ? reinterpret_cast<uint16_t*>(p.dv) + b * p.dv_batch_stride + hk * p.dv_head_stride + static_cast<int64_t>(keys.x + row) * p.dv_row_stride
                            : reinterpret_cast<uint16_t*>(p.dk) + b * p.dk_batch_stride + hk * p.dk_head_stride + static_cast<int64_t>(keys.x + row) * p.dk_row_stride;
 #pragma unroll
@@ -1303,7 +1315,10 @@ int pick_ranges(const fdma_fwd_params& p) {
 // of a CTA are paid once for several items and the last ones still even out. 32768 queries, 32 heads, backward in us with one head / 12 / 6 / 3
 // CTAs per SM: 2048 gathered keys 2265 / 2077 / 2057 / 2058, 128 keys 808 / 654 / 651 / 656; three per SM also 4 x 2048 at head dim 64 265 -> 251,
 // but 16384 x 8 heads at head dim 64 2523 -> 2690.
-int pick_heads_per_cta(int64_t tiles, int h) {
+// Sliding windows, whose items are short: as many as leave three, up to four. 8192 queries, 32 heads, d = 128, a window of 128 keys: 1 / 2 / 4 / 8
+// heads 314 / 295 / 282 / 281; 32768, 2048 keys: 1 / 3 / 4 / 8 4552 / 4339 / 4313 / 4450.
+int pick_heads_per_cta(int64_t tiles, int h, bool window) {
+  if (window) return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(h, 4), tiles * h / (3 * sm_count()))));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(h, 16), tiles * h / (6 * sm_count()))));
 }
 
@@ -1438,7 +1453,7 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   kp.n_far_ctas = pl.sink_tiles * p.h_k * pl.far_slots * p.b;
   kp.nsplit = pl.nsplit;
   kp.ranges = seqs.cu_q ? 1 : pl.ranges;
-  kp.heads_per_cta = pick_heads_per_cta(static_cast<int64_t>(kp.q_tiles) * p.b * kp.ranges, p.h);
+  kp.heads_per_cta = pick_heads_per_cta(static_cast<int64_t>(kp.q_tiles) * p.b * kp.ranges, p.h, window.keys > 0);
   kp.scale_log2 = p.softmax_scale * kLog2e;
   kp.scale = p.softmax_scale;
 
@@ -1460,7 +1475,7 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   if (e != cudaSuccess) return static_cast<int>(e);
   if (window.keys) {
     if (!pl.sink_tiles) return 0;
-    const int64_t rows = static_cast<int64_t>(pl.near_units) * p.h_k * pl.sink_tiles * kBN;
+    const int64_t rows = static_cast<int64_t>(pl.near_units) * p.h_k * std::min(window.sinks, pl.sink_tiles * kBN);
     sinks_kernel<D, kBf16><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(kp);
     return static_cast<int>(cudaGetLastError());
   }

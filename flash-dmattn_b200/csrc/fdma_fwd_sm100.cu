@@ -73,6 +73,9 @@ struct FwdKernelParams {
   int is_causal;
   PackedSeqs seqs;   // packed sequences, each with query blocks and key tiles of its own
   Window window;     // sliding window (kWindow)
+  // kWindow: the two query tiles of an item are those of two heads that share a kv head, at the same rows, and not two tiles of one head. Then
+  // they see the same key tiles: one fewer, and none that only one of them works on.
+  bool pair;
   int n_mblk;        // query blocks (of kNQ tiles) per (batch, head); packed: places for them
   int n_items;       // work items = n_mblk * h * b
   float scale_log2;  // softmax_scale * log2(e)
@@ -157,14 +160,15 @@ struct FwdItem {
 };
 
 // `seq`: packed sequences, what warp 3 has found for the item: block and sequence (see packed_tile)
-template <bool packed>
+template <bool packed, bool kWindow>
 __device__ __forceinline__ FwdItem fwd_item(const FwdKernelParams& p, int item, const volatile int* seq) {
   FwdItem w;
-  const int per_block = p.h * p.b;
+  const int heads = kWindow && p.pair ? p.h / 2 : p.h, per_block = heads * p.b;
   const int rem = item % per_block;
   w.mblk = p.n_mblk - 1 - item / per_block;
-  w.h = rem % p.h;  // heads of one kv group are neighbours in the list: they meet their shared tiles in L2
-  w.b = rem / p.h;
+  w.h = rem % heads;  // heads of one kv group are neighbours in the list: they meet their shared tiles in L2
+  w.b = rem / heads;
+  if (kWindow && p.pair) w.h *= 2;
   w.hk = w.h / (p.h / p.h_k);
   w.hm = w.h / (p.h / p.h_mask);
   w.hb = w.h / (p.h / p.h_bias);
@@ -226,10 +230,14 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool causal = p.is_causal != 0;
   const WaitCtl ctl{s_abort, p.status};
+  // the block's query tile t: its number, and its head
+  const bool pair = kWindow && p.pair;
+  auto q_tile = [&](const FwdItem& w, int t) { return pair ? w.mblk : w.mblk * kNQ + t; };
+  auto head_of = [&](const FwdItem& w, int t) { return pair ? w.h + t : w.h; };
   // Per item: number of key tiles each query tile can see at most (causal / length limit), and how many there are to look at: their
   // maximum, less those between the sinks and the window, which tile_of leaves out.
   auto gap_of = [&](const FwdItem& w, int nT) {  // of tile numbers from `first` on
-    const int first = (min(p.window.sinks, w.sk) + kBN - 1) / kBN, lo = max(0, w.mblk * kNQ * kBM + w.sk - w.sq - p.window.keys + 1) / kBN;
+    const int first = (min(p.window.sinks, w.sk) + kBN - 1) / kBN, lo = max(0, q_tile(w, 0) * kBM + w.sk - w.sq - p.window.keys + 1) / kBN;
     return make_int2(first, max(0, min(lo, nT) - first));
   };
   auto tile_limits = [&](const FwdItem& w, int (&n_end)[kNQ], const int32_t*& pos_row) {
@@ -240,7 +248,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
     int nT = 0;
 #pragma unroll
     for (int t = 0; t < kNQ; ++t) {
-      const int m0 = (w.mblk * kNQ + t) * kBM;
+      const int m0 = q_tile(w, t) * kBM;
       int ne = (w.sk + kBN - 1) / kBN;
       if (causal && !pos_row) ne = min(ne, max(0, (m0 + kBM + w.sk - w.sq + kBN - 1) / kBN));
       if (m0 >= w.sq) ne = 0;
@@ -313,7 +321,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
         if (!ok) break;
         const int item = s_item[ic & 1];
         if (item >= p.n_items) break;
-        const FwdItem w = fwd_item<packed>(p, item, s_seq + (ic & 1) * 8);
+        const FwdItem w = fwd_item<packed, kWindow>(p, item, s_seq + (ic & 1) * 8);
         int n_end[kNQ];
         const int32_t* pos_row;
         const int nT = tile_limits(w, n_end, pos_row);
@@ -327,8 +335,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
         for (int t = 0; t < kNQ; ++t)
 #pragma unroll
           for (int kb = 0; kb < D / 64; ++kb)
-            tma_load_4d(s_q + t * L::kQBytes + kb * (kBM * 128), &p.tm_q, bar_q, kb * 64, w.h,
-                        w.q0 + (w.mblk * kNQ + t) * kBM, w.b);
+            tma_load_4d(s_q + t * L::kQBytes + kb * (kBM * 128), &p.tm_q, bar_q, kb * 64, head_of(w, t), w.q0 + q_tile(w, t) * kBM, w.b);
         for (int j = 0; j < nT && ok; ++j) {
           if (s_flags[j] == 0) continue;
 #pragma unroll
@@ -366,7 +373,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
       if (!ok) break;
       const int item = warp_uniform(s_item[ic & 1]);
       if (item >= p.n_items) break;
-      FwdItem w = fwd_item<packed>(p, item, s_seq + (ic & 1) * 8);
+      FwdItem w = fwd_item<packed, kWindow>(p, item, s_seq + (ic & 1) * 8);
       if (packed) {
         w.mblk = warp_uniform(w.mblk);
         w.sq = warp_uniform(w.sq);
@@ -531,7 +538,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
       if (!ok) break;
       const int item = s_item[ic & 1];
       if (item >= p.n_items) break;
-      const FwdItem w = fwd_item<packed>(p, item, s_seq + (ic & 1) * 8);
+      const FwdItem w = fwd_item<packed, kWindow>(p, item, s_seq + (ic & 1) * 8);
       int n_end[kNQ];
       const int32_t* pos_row;
       const int nT = tile_limits(w, n_end, pos_row);
@@ -616,7 +623,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
         break;
       }
       if (packed) {
-        const PackedTile t = packed_tile(p.seqs.cu_q, p.seqs.n, p.seqlen_q, kNQ * kBM, p.n_mblk - 1 - item / (p.h * p.b));
+        const PackedTile t = packed_tile(p.seqs.cu_q, p.seqs.n, p.seqlen_q, pair ? kBM : kNQ * kBM, p.n_mblk - 1 - item / ((pair ? p.h / 2 : p.h) * p.b));
         const int2 keys = packed_range(p.seqs.cu_k, p.seqs.n, p.seqlen_k, t.seq);
         if (lane == 0) {
           volatile int* seq = s_seq + (ic & 1) * 8;
@@ -628,7 +635,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
         }
         __syncwarp();
       }
-      const FwdItem w = fwd_item<packed>(p, item, s_seq + (ic & 1) * 8);
+      const FwdItem w = fwd_item<packed, kWindow>(p, item, s_seq + (ic & 1) * 8);
       int n_end[kNQ];
       const int32_t* pos_row;
       const int nT = tile_limits(w, n_end, pos_row);
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
 #pragma unroll
             for (int t = 0; t < kNQ; ++t)
               if (j < n_end[t] && (!kWindow || j * kBN < p.window.sinks ||
-                                   j * kBN + kBN > (w.mblk * kNQ + t) * kBM + w.sk - w.sq - p.window.keys + 1))
+                                   j * kBN + kBN > q_tile(w, t) * kBM + w.sk - w.sq - p.window.keys + 1))
                 f |= (1 << t);
             if (pos_row) {  // the tile's smallest position against the last row of each query tile
               const int64_t pmin = pos_row[j * kBN];
@@ -716,14 +723,14 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
     if (!ok) break;
     const int item = s_item[ic & 1];
     if (item >= p.n_items) break;
-    const FwdItem w = fwd_item<packed>(p, item, s_seq + (ic & 1) * 8);
-    const int h = w.h, b = w.b;
+    const FwdItem w = fwd_item<packed, kWindow>(p, item, s_seq + (ic & 1) * 8);
+    const int h = head_of(w, t), b = w.b;
     int n_end[kNQ];
     const int32_t* pos_row;
     const int nT = tile_limits(w, n_end, pos_row);
     const int2 gap = item_gap(w, n_end);
     const uint8_t* s_flags = s_flags_all + (ic & 1) * kMaxTiles;
-    const int m0 = (w.mblk * kNQ + t) * kBM;
+    const int m0 = q_tile(w, t) * kBM;
     const int qrow = m0 + row;
     const int qclamp = min(qrow, w.sq - 1);
     const uint8_t* mrow = nullptr;
@@ -1139,8 +1146,11 @@ int launch(const fdma_fwd_params& p, const FwdPlan& pl, const PackedSeqs& seqs, 
   // The attribute belongs to the (function, device) pair: set it on every call, whichever device is current.
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
   if (e != cudaSuccess) return static_cast<int>(e);
-  kp.n_mblk = seqs.cu_q ? packed_slots(p.seqlen_q, seqs.n, kNQ * kBM) : (p.seqlen_q + kNQ * kBM - 1) / (kNQ * kBM);
-  const int64_t n_items = static_cast<int64_t>(kp.n_mblk) * p.h * p.b;
+  // (a mask per query head is one for both tiles)
+  kp.pair = kWindow && kNQ == 2 && p.h / p.h_k % 2 == 0 && !(p.mask && p.h_mask == p.h);
+  const int rows = kp.pair ? kBM : kNQ * kBM;
+  kp.n_mblk = seqs.cu_q ? packed_slots(p.seqlen_q, seqs.n, rows) : (p.seqlen_q + rows - 1) / rows;
+  const int64_t n_items = static_cast<int64_t>(kp.n_mblk) * (kp.pair ? p.h / 2 : p.h) * p.b;
   if (n_items > 0x7FFFFFFF) return FDMA_ERR_TOO_LARGE;
   kp.n_items = static_cast<int>(n_items);
   const dim3 grid(static_cast<unsigned>(n_items));

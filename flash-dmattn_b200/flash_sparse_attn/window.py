@@ -91,11 +91,16 @@ def flash_sparse_attn_window_varlen_func(
     return_attn_probs: Optional[bool] = None,
 ):
     """`flash_sparse_attn_window_func` on packed sequences: arguments and results as of `flash_sparse_attn_varlen_func`, positions,
-    window and sinks in each sequence. Sequences that cover the tokens run in one launch per direction up to head dim 128; the
-    boundaries are read on the host (one device synchronisation per call)."""
+    window and sinks in each sequence. Up to head dim 128 the sequences run in one launch per direction and nothing synchronises: the boundaries stay
+    on the GPU, where they must ascend from 0 or more; what they leave out, or what lies beyond the tensors, belongs to no sequence, whose
+    rows are 0, gradients too. Other calls go sequence by sequence, their boundaries read on the host."""
     check_window(sliding_window, sink_tokens)
-    if sliding_window + sink_tokens >= max_seqlen_k:  # every query sees all keys up to its own
-        sliding_window = sink_tokens = 0
+    if not return_attn_probs and not torch.compiler.is_compiling() and _interface._kernel_path == _lib.PATH_AUTO and query.is_cuda:
+        scale = query.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
+        res = _native.load().packed_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, scale, True, bool(deterministic), sliding_window,
+                                              sink_tokens)
+        if res is not None:
+            return res[0]
     return _interface._varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, True, None,
                               deterministic, return_attn_probs, sliding_window, sink_tokens)
 

@@ -165,3 +165,36 @@ def test_packed_sequences(lengths_q, lengths_k, window, sinks, d):
     cu = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (cu_q, cu_k)]
     out = fsa.flash_sparse_attn_window_varlen_func(q, k, v, *cu, max(lengths_q), max(lengths_k), window, sinks)
     check([out, *torch.autograd.grad(out, (q, k, v), dout)], *packed_reference(q, k, v, cu_q, cu_k, window, sinks, dout))
+
+
+def test_packed_rows_outside_every_sequence_and_no_synchronisation():
+    """Tokens before the first boundary and behind the last one, a boundary beyond the tensors; the call is captured, which a synchronisation
+    would end."""
+    T, window, sinks, lengths = 700, 40, 3, [200, 0, 1, 300]
+    q, k, v, dout = (x[0].detach() for x in tensors(1, T, T, 4, 2, 64, torch.bfloat16))
+    cu = [50 + sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    bounds = torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+    def run(q, k, v):
+        q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+        out = fsa.flash_sparse_attn_window_varlen_func(q, k, v, bounds, bounds, max(lengths), max(lengths), window, sinks)
+        return [out, *torch.autograd.grad(out, (q, k, v), dout)]
+
+    run(q, k, v)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        run(q, k, v)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            got = run(q, k, v)
+    graph.replay()
+    torch.cuda.synchronize()
+    a, b = cu[0], cu[-1]
+    inside = [x - a for x in cu]
+    check([x[a:b] for x in got], *packed_reference(q[a:b], k[a:b], v[a:b], inside, inside, window, sinks, dout[a:b]))
+    for x in got:
+        assert not bool(x[:a].any()) and not bool(x[b:].any())
+    bounds.copy_(torch.tensor([0, 100, 100, 400, 2 ** 30]))  # the last sequence ends where the tensors do
+    graph.replay()
+    torch.cuda.synchronize()
+    check(got, *packed_reference(q, k, v, [0, 100, 100, 400, T], [0, 100, 100, 400, T], window, sinks, dout))
