@@ -914,8 +914,10 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
           const int k = tile_of(m, gap) * kBM + lane * 2;
           const uint32_t mb = mrow ? *reinterpret_cast<const uint16_t*>(mrow + k) : 0x0101u;
           const uint32_t bb = brow ? *reinterpret_cast<const uint32_t*>(brow + k) : 0u;
-          const float2 add = make_float2(k < sk && (mb & 0xFFu) ? raw16_to_f<kBf16>(static_cast<uint16_t>(bb & 0xFFFFu)) * kLog2e : -CUDART_INF_F,
-                                         k + 1 < sk && (mb >> 8) ? raw16_to_f<kBf16>(static_cast<uint16_t>(bb >> 16)) * kLog2e : -CUDART_INF_F);
+          // (tiles in front of a gap are seen as sinks alone)
+          const int end_k = kWindow && gap > 0 && m < sink_subs ? p.window.sinks : sk;
+          const float2 add = make_float2(k < end_k && (mb & 0xFFu) ? raw16_to_f<kBf16>(static_cast<uint16_t>(bb & 0xFFFFu)) * kLog2e : -CUDART_INF_F,
+                                         k + 1 < end_k && (mb >> 8) ? raw16_to_f<kBf16>(static_cast<uint16_t>(bb >> 16)) * kLog2e : -CUDART_INF_F);
           int2 pos = make_int2(k, k + 1);
           if (pos_row) pos = make_int2(k < sk ? pos_row[k] : 0x7FFFFFFF, k + 1 < sk ? pos_row[k + 1] : 0x7FFFFFFF);
           const int slot = vi % kVecSlots;
@@ -1013,6 +1015,7 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
     const int qlim_wmin = causal ? clamp(static_cast<int64_t>(warp_row) + coff) : 0x7FFFFFFE;
     // first key this row (and the warp's last row) sees in its window
     const int qfirst = kWindow ? row + coff - p.window.keys + 1 : 0, qfirst_wmax = kWindow ? warp_row + 31 + coff - p.window.keys + 1 : 0;
+    const uint32_t hidden = kWindow ? max(0, qfirst - p.window.sinks) : 0;  // keys between the sinks and that one
     const int row_g = q0 + min(row, sq - 1);  // row in the tensors
     constexpr int kHalfCols = D / 2;          // columns of dQ each team takes out
     int g0 = 0, xc = 0, sums = 0;  // steps, items with steps, sums received so far
@@ -1075,7 +1078,7 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
     };
     for (int ic = 0; ok; ++ic) {
       const int h = h0 + ic, buf = ic & 1;
-      int n_steps = 0;
+      int n_steps = 0, first_hidden = 0;
       float lse = CUDART_INF_F, dsum = 0.f;
       if (h < h1) {
         if (row_ok) {
@@ -1086,6 +1089,8 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
         ok = __all_sync(0xffffffffu, mbar_wait(bar.item_full + buf, (ic >> 1) & 1, ctl, kWaitItemFull));
         if (!ok) break;
         n_steps = s_item[buf * 4 + 2];
+        // keys that a row may not see in its window, beside the tiles that hold nothing but sinks for all rows
+        if (kWindow) first_hidden = s_item[buf * 4 + 3] > 0 ? max(p.window.sinks, sink_subs * kBM) : p.window.sinks;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar.item_empty + buf);
         if (n_steps > 0) {
@@ -1143,12 +1148,12 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
         };
         auto d2 = [&](int) { return dsum2; };
         // warp-uniform: some (row, key) of the warp is out of sight
-        if ((causal && pos[31] > qlim_wmin) || (kWindow && pos[0] < qfirst_wmax && pos[31] >= p.window.sinks)) {
+        if ((causal && pos[31] > qlim_wmin) || (kWindow && pos[0] < qfirst_wmax && pos[31] >= first_hidden)) {
           softmax_step<kBf16, false>(rs, rp, p.scale_log2, [&](int j) {
             float2 add = pair(j);
             const int x = pos[2 * j], y = pos[2 * j + 1];
-            if (x > qlim || (kWindow && x < qfirst && x >= p.window.sinks)) add.x = -CUDART_INF_F;
-            if (y > qlim || (kWindow && y < qfirst && y >= p.window.sinks)) add.y = -CUDART_INF_F;
+            if (x > qlim || (kWindow && static_cast<uint32_t>(x - p.window.sinks) < hidden)) add.x = -CUDART_INF_F;
+            if (y > qlim || (kWindow && static_cast<uint32_t>(y - p.window.sinks) < hidden)) add.y = -CUDART_INF_F;
             return add;
           }, d2, dsk, dsk);
         } else {
