@@ -44,7 +44,7 @@ constexpr int kBN = 128;  // stationary rows per CTA
 constexpr int kBM = 64;   // streamed rows per step
 constexpr int kThreads = 384;
 constexpr int kFlush = 64;  // 64-key steps whose dQ the tensor core sums up (4096 keys)
-constexpr int kFarRows = 2048;  // sliding windows: queries beyond the window that a CTA works on for a tile of sink keys
+constexpr int kFarRows = 2048, kFarCtas = 4096;  // sliding windows: as in fdma_bwd_rows_sm100.cu
 constexpr int kMaxBits = 4096;  // 64-key tiles the activity bits of a dQ pass can hold; beyond, every tile is worked on
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -80,10 +80,10 @@ struct Bwd256Params {
   int64_t pos_batch_stride, pos_head_stride;
   int h_pos, causal_shift;
   // Sliding window (kWindow): as in fdma_bwd_rows_sm100.cu, near and far CTAs of the tiles that hold sinks leave fp32 sums,
-  // [2: dV, dK][near of each batch element, then its parts of kFarRows queries][h_k][sink_tiles * 128][256]
+  // [2: dV, dK][near of each batch element, then its parts of far_rows queries][h_k][sink_rows][256]
   Window window;
   float* sink_sums;
-  int sink_tiles, far_slots, n_far_ctas;  // far CTAs of a pass
+  int sink_rows, sink_tiles, far_slots, far_rows, n_far_ctas;  // far CTAs of a pass
   float scale_log2, scale;
 };
 
@@ -201,7 +201,7 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
     m_start = max(m_start, split * m_chunk);
     if (kWindow) {
       if (far) {
-        const int q_lo = slot * kFarRows, q_hi = min(Sq, q_lo + kFarRows);
+        const int q_lo = slot * p.far_rows, q_hi = min(Sq, q_lo + p.far_rows);
         if (!far_part(n * kBN, q_lo, q_hi, coff, p.window)) return;  // (the whole CTA agrees)
         m_start = max(q_lo, n * kBN + p.window.keys - coff) / kBM;
         M64 = (q_hi + kBM - 1) / kBM;
@@ -605,7 +605,7 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
       // partial: part[dv|dk][split][b][hk][key][256]
       const int64_t unit = far ? p.b + b * p.far_slots + slot : b;
       float* part = kWindow ? p.sink_sums + (((static_cast<int64_t>(kPass == kDk ? 1 : 0) * (p.b + p.b * p.far_slots) + unit) * p.h_k + hk) *
-                                                 (p.sink_tiles * kBN) + row) * kD
+                                                 p.sink_rows + row) * kD
                             : p.dkv_part + ((((static_cast<int64_t>(kPass == kDk ? 1 : 0) * p.nsplit + split) * p.b + b) * p.h_k + hk) *
                                                 (NT * kBN) + row) * kD;
 #pragma unroll
@@ -629,7 +629,7 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
             r[v4 * 4 + 3] = __float_as_uint(__uint_as_float(r[v4 * 4 + 3]) + y.w);
           }
         }
-        if (kKeys && (kWindow ? n < p.sink_tiles : p.dkv_part != nullptr)) {
+        if (kKeys && (kWindow ? row < p.sink_rows : p.dkv_part != nullptr)) {
           if (kWindow && !row_ok) continue;  // (after the warp-wide load)
 #pragma unroll
           for (int v4 = 0; v4 < 8; ++v4)
@@ -671,14 +671,14 @@ __global__ void __launch_bounds__(kThreads, 1) bwd256_kernel(const __grid_consta
   else pass256<kBf16, kDq, kWindow>(p, smem, item - 2 * p.n_kv_ctas);
 }
 
-// Sliding window, tiles that hold sinks: dV and dK as the sum of what the CTAs of the queries near them and of those beyond have left, in
+// Sliding window, sinks: dV and dK as the sum of what the CTAs of the queries near them and of those beyond have left, in
 // the order of the queries. A warp per key row.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) sinks256_kernel(const __grid_constant__ Bwd256Params p) {
-  const int lane = threadIdx.x & 31, rows = p.sink_tiles * kBN, coff = p.seqlen_k - p.seqlen_q;
+  const int lane = threadIdx.x & 31, rows = p.sink_rows, coff = p.seqlen_k - p.seqlen_q;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int b = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * rows)), hk = static_cast<int>(w / rows % p.h_k), row = static_cast<int>(w % rows);
-  if (b >= p.b || row >= p.seqlen_k) return;
+  if (b >= p.b) return;
   const int64_t units = p.b + static_cast<int64_t>(p.b) * p.far_slots;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {  // dV, dK
@@ -689,8 +689,8 @@ __global__ void __launch_bounds__(256) sinks256_kernel(const __grid_constant__ B
       for (int i = 0; i < kD / 32; ++i) acc[i] = src[i] + (fresh ? 0.f : acc[i]);
     };
     add(b, true);
-    for (int c = 0; row < p.window.sinks && c < p.far_slots; ++c)
-      if (far_part(row / kBN * kBN, c * kFarRows, min((c + 1) * kFarRows, p.seqlen_q), coff, p.window)) add(p.b + b * p.far_slots + c, false);
+    for (int c = 0; c < p.far_slots; ++c)
+      if (far_part(row / kBN * kBN, c * p.far_rows, min((c + 1) * p.far_rows, p.seqlen_q), coff, p.window)) add(p.b + b * p.far_slots + c, false);
     uint16_t* dst = x == 0 ? reinterpret_cast<uint16_t*>(p.dv) + b * p.dv_batch_stride + hk * p.dv_head_stride + row * p.dv_row_stride
                            : reinterpret_cast<uint16_t*>(p.dk) + b * p.dk_batch_stride + hk * p.dk_head_stride + row * p.dk_row_stride;
 #pragma unroll
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(256) sinks256_kernel(const __grid_constant__ B
 }
 
 struct Plan256 {
-  int sq_r, nsplit, sink_tiles, far_slots;
+  int sq_r, nsplit, sink_rows, sink_tiles, far_slots, far_rows;
   bool want_dbias;
   bool part;  // dK, dV and column sums leave the main kernel as fp32 partials
   size_t lse2_off, dsum_off, dq_off, part_off, dbpart_off, sinks_off, total;
@@ -723,8 +723,11 @@ Plan256 plan256(const fdma_bwd_params& bp, const Window& window) {
   Plan256 pl;
   pl.sq_r = static_cast<int>(round_up(p.seqlen_q, kBM));
   pl.nsplit = window.keys ? 1 : pick_nsplit256(p);
-  pl.sink_tiles = window.keys ? (std::min(window.sinks, p.seqlen_k) + kBN - 1) / kBN : 0;
-  pl.far_slots = pl.sink_tiles ? (p.seqlen_q + kFarRows - 1) / kFarRows : 0;
+  pl.sink_rows = window.keys ? std::min(window.sinks, p.seqlen_k) : 0;
+  pl.sink_tiles = (pl.sink_rows + kBN - 1) / kBN;
+  pl.far_rows = kFarRows;
+  while (pl.far_rows < p.seqlen_q / 2 && static_cast<int64_t>(pl.sink_tiles) * p.h_k * p.b * (p.seqlen_q / pl.far_rows) > kFarCtas) pl.far_rows *= 2;
+  pl.far_slots = pl.sink_tiles ? (p.seqlen_q + pl.far_rows - 1) / pl.far_rows : 0;
   pl.want_dbias = bp.dbias != nullptr;
   size_t o = 0;
   const size_t rows = static_cast<size_t>(p.b) * p.h * pl.sq_r;
@@ -741,7 +744,7 @@ Plan256 plan256(const fdma_bwd_params& bp, const Window& window) {
     if (pl.want_dbias) o += align256(static_cast<size_t>(pl.nsplit) * p.b * p.h_k * keys_r * 4);
   }
   pl.sinks_off = o;
-  o += align256(static_cast<size_t>(2) * p.b * (1 + pl.far_slots) * p.h_k * pl.sink_tiles * kBN * kD * 4);
+  o += align256(static_cast<size_t>(2) * p.b * (1 + pl.far_slots) * p.h_k * pl.sink_rows * kD * 4);
   pl.total = o;
   return pl;
 }
@@ -823,7 +826,7 @@ int launch256(const fdma_bwd_params& bp, const Plan256& pl, const Window& window
 
   kp.window = window;
   kp.sink_sums = reinterpret_cast<float*>(ws + pl.sinks_off);
-  kp.sink_tiles = pl.sink_tiles; kp.far_slots = pl.far_slots;
+  kp.sink_rows = pl.sink_rows; kp.sink_tiles = pl.sink_tiles; kp.far_rows = pl.far_rows; kp.far_slots = pl.far_slots;
   kp.n_far_ctas = pl.sink_tiles * p.h_k * pl.far_slots * p.b;
   auto kern = window.keys ? bwd256_kernel<kBf16, true> : bwd256_kernel<kBf16, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem256::kAlloc);
@@ -843,7 +846,7 @@ int launch256(const fdma_bwd_params& bp, const Plan256& pl, const Window& window
   if (e != cudaSuccess) return static_cast<int>(e);
   if (window.keys) {
     if (!pl.sink_tiles) return 0;
-    const int64_t rows = static_cast<int64_t>(p.b) * p.h_k * pl.sink_tiles * kBN;
+    const int64_t rows = static_cast<int64_t>(p.b) * p.h_k * pl.sink_rows;
     sinks256_kernel<kBf16><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(kp);
     return static_cast<int>(cudaGetLastError());
   }

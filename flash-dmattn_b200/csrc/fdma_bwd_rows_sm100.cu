@@ -54,9 +54,10 @@ constexpr int kFlush = 2;
 constexpr int kKeyFlush = 48;
 constexpr int kMaxBits = 4096;   // 64-key tiles the activity bits of a row-pass item can hold
 constexpr int kMaxHeads = 4096;  // query heads of a group whose activity differs from head to head
-// Sliding windows: queries beyond the window that a CTA works on for a tile of sink keys. Such a tile is seen by all queries behind it, the
-// others by window + 128 of them.
-constexpr int kFarRows = 2048;
+// Sliding windows: queries beyond the window that a CTA works on for a tile of sink keys (such a tile is seen by all queries behind it, the
+// others by window + 128 of them), or that times a power of two where the CTAs would be more than kFarCtas: by then every SM has many of
+// them, and each leaves an fp32 row per sink, head and 16-bit row.
+constexpr int kFarRows = 2048, kFarCtas = 4096;
 constexpr int kDbHeads = 16;    // query heads of a group whose dBias sums have room in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -96,11 +97,11 @@ struct BwdRowsParams {
   int h_pos, causal_shift;
   PackedSeqs seqs;   // packed sequences, each with tiles of its own; streamed query tiles are cut at fixed rows
   // Sliding window (kWindow). A key tile's CTA takes the queries whose window reaches it (near); those beyond, which see the sinks alone,
-  // come from CTAs of their own (far), kFarRows queries each. Both leave fp32 sums of the sinks' rows, which sinks_kernel adds up:
-  // [2: dV, dK][near of each sequence or batch element, then a place for each part of kFarRows queries][h_k][sink_tiles * 128][D]
+  // come from CTAs of their own (far), far_rows queries each. Both leave fp32 sums of the sinks' rows, which sinks_kernel adds up:
+  // [2: dV, dK][near of each sequence or batch element, then a place for each part of far_rows queries][h_k][sink_rows][D]
   Window window;
   float* sink_sums;
-  int sink_tiles, near_units, far_slots, n_far_ctas;
+  int sink_rows, sink_tiles, near_units, far_slots, far_rows, n_far_ctas;
   int n_tiles;       // key tiles (packed: places for them)
   int q_tiles;       // row-pass tiles (packed: places for them)
   int nsplit;        // query-range splits per key tile
@@ -324,17 +325,17 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
     if (!far && sink_unit >= 0 && !far_part(key0, key_end, q_lo, q_hi, coff, p.window)) sink_unit = -1;  // nobody is beyond
     if (far) {
       if (packed) {
-        const PackedTile t = packed_tile(p.seqs.cu_q, p.seqs.n, Sq, kFarRows, slot);
+        const PackedTile t = packed_tile(p.seqs.cu_q, p.seqs.n, Sq, p.far_rows, slot);
         const int2 keys = packed_range(p.seqs.cu_k, p.seqs.n, Sk, t.seq);
         key0 = keys.x + n * kBN;
         key_end = min(keys.y, keys.x + p.window.sinks);
-        q_lo = t.begin + t.tile * kFarRows;
-        q_hi = min(t.end, q_lo + kFarRows);
+        q_lo = t.begin + t.tile * p.far_rows;
+        q_hi = min(t.end, q_lo + p.far_rows);
         coff = keys.y - t.end;
       } else {
         key_end = min(Sk, p.window.sinks);
-        q_lo = slot * kFarRows;
-        q_hi = min(Sq, q_lo + kFarRows);
+        q_lo = slot * p.far_rows;
+        q_hi = min(Sq, q_lo + p.far_rows);
       }
       if (!far_part(key0, key_end, q_lo, q_hi, coff, p.window)) return;  // (the whole CTA agrees)
       m_start = max(q_lo, key0 + beyond - coff) / kBM;
@@ -702,7 +703,7 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
           // fp32 partial: part[dv|dk][split][b][hk][key][d]
           if ((packed || kWindow) && !key_ok) continue;  // (after the warp-wide load)
           float* part = kWindow ? p.sink_sums + (((static_cast<int64_t>(half) * (p.near_units + p.b * p.far_slots) + sink_unit) * p.h_k + hk) *
-                                                     (p.sink_tiles * kBN) + (n_in_seq * kBN + krow)) * D + c * 32
+                                                     p.sink_rows + (n_in_seq * kBN + krow)) * D + c * 32
                                 : p.dkv_part + ((((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key) * D + c * 32;
 #pragma unroll
           for (int v4 = 0; v4 < 8; ++v4)
@@ -1236,9 +1237,9 @@ __global__ void __launch_bounds__(kThreads, 1) bwd_rows_kernel(const __grid_cons
 // have left, in the order of the queries. A warp per key row.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) sinks_kernel(const __grid_constant__ BwdRowsParams p) {
-  const int lane = threadIdx.x & 31, rows = p.sink_tiles * kBN, sinks = min(p.window.sinks, rows);
+  const int lane = threadIdx.x & 31, rows = p.sink_rows;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int unit = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * sinks)), hk = static_cast<int>(w / sinks % p.h_k), row = static_cast<int>(w % sinks);
+  const int unit = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * rows)), hk = static_cast<int>(w / rows % p.h_k), row = static_cast<int>(w % rows);
   if (unit >= p.near_units) return;
   const bool packed = p.seqs.cu_q != nullptr;
   int2 keys = make_int2(0, p.seqlen_k), queries = make_int2(0, p.seqlen_q);
@@ -1246,7 +1247,7 @@ __global__ void __launch_bounds__(256) sinks_kernel(const __grid_constant__ BwdR
   if (packed) {
     keys = packed_range(p.seqs.cu_k, p.seqs.n, p.seqlen_k, unit);
     queries = packed_range(p.seqs.cu_q, p.seqs.n, p.seqlen_q, unit);
-    first = p.near_units + queries.x / kFarRows + unit + 1;  // the sequence's first place
+    first = p.near_units + queries.x / p.far_rows + unit + 1;  // the sequence's first place
   }
   if (keys.x + row >= keys.y) return;
   const int key0 = keys.x + row / kBN * kBN, coff = keys.y - queries.y;
@@ -1260,9 +1261,9 @@ __global__ void __launch_bounds__(256) sinks_kernel(const __grid_constant__ BwdR
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[i] = at(unit)[i];
     // parts that reach beyond the window: those from this one on. Eight are asked for at a time.
-    const int parts = (queries.y - queries.x + kFarRows - 1) / kFarRows;
+    const int parts = (queries.y - queries.x + p.far_rows - 1) / p.far_rows;
     int c0 = 0;
-    while (!far_part(key0, key0 + 1, queries.x + c0 * kFarRows, min(queries.x + (c0 + 1) * kFarRows, queries.y), coff, p.window)) ++c0;
+    while (!far_part(key0, key0 + 1, queries.x + c0 * p.far_rows, min(queries.x + (c0 + 1) * p.far_rows, queries.y), coff, p.window)) ++c0;
     for (; c0 < parts; c0 += 8) {
       float y[8][D / 32];
 #pragma unroll
@@ -1290,7 +1291,7 @@ struct RowsPlan {
   int ranges;  // key ranges per row-pass tile
   bool part;  // dK, dV (and column sums) leave the kernel as fp32 partials
   size_t lse2_off, dsum_off, dq_off, dbias_off, sums_off, part_off, dbpart_off, sinks_off, total;
-  int sink_tiles, near_units, far_slots;  // sliding window
+  int sink_rows, sink_tiles, near_units, far_slots, far_rows;  // sliding window
 };
 
 // Query-range splits per key tile: one CTA per SM, as long as a split keeps 32 steps, and on to two per SM while it keeps 160. The row pass,
@@ -1348,11 +1349,14 @@ RowsPlan plan(const fdma_bwd_params& bp, const Window& window, int sequences) {
   pl.dbias_off = o;
   if (pl.dbias_mode == kDbAtomic) o += align256(static_cast<size_t>(bp.dbias_b) * bp.dbias_h * atomic_keys(bp) * 4);
   pl.nsplit = window.keys ? 1 : pick_nsplit(p);
-  pl.sink_tiles = pl.near_units = pl.far_slots = 0;
+  pl.sink_rows = pl.sink_tiles = pl.near_units = pl.far_slots = 0;
+  pl.far_rows = kFarRows;
   if (window.keys && window.sinks) {
-    pl.sink_tiles = (std::min(window.sinks, p.seqlen_k) + kBN - 1) / kBN;
+    pl.sink_rows = std::min(window.sinks, p.seqlen_k);
+    pl.sink_tiles = (pl.sink_rows + kBN - 1) / kBN;
+    while (pl.far_rows < p.seqlen_q / 2 && static_cast<int64_t>(pl.sink_tiles) * p.h_k * p.b * (p.seqlen_q / pl.far_rows) > kFarCtas) pl.far_rows *= 2;
     pl.near_units = sequences ? sequences : p.b;
-    pl.far_slots = sequences ? packed_slots(p.seqlen_q, sequences, kFarRows) : (p.seqlen_q + kFarRows - 1) / kFarRows;
+    pl.far_slots = sequences ? packed_slots(p.seqlen_q, sequences, pl.far_rows) : (p.seqlen_q + pl.far_rows - 1) / pl.far_rows;
   }
   pl.sums_off = o;
   const int64_t m_tiles = (p.seqlen_q + kBM - 1) / kBM;
@@ -1360,7 +1364,7 @@ RowsPlan plan(const fdma_bwd_params& bp, const Window& window, int sequences) {
     o += align256((static_cast<size_t>(2) * pl.nsplit * p.b * p.h_k * round_up(p.seqlen_k, kBN) +
                    static_cast<size_t>(2) * p.b * pl.far_slots * p.h_k * pl.sink_tiles * kBN) * pl.D * 4);
   pl.sinks_off = o;
-  o += align256(static_cast<size_t>(2) * (pl.near_units + p.b * pl.far_slots) * p.h_k * pl.sink_tiles * kBN * pl.D * 4);
+  o += align256(static_cast<size_t>(2) * (pl.near_units + p.b * pl.far_slots) * p.h_k * pl.sink_rows * pl.D * 4);
   pl.part = pl.nsplit > 1 || bp.scatter_pos != nullptr;
   pl.part_off = pl.dbpart_off = o;
   if (pl.part) {
@@ -1454,7 +1458,7 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   kp.q_tiles = seqs.cu_q ? packed_slots(p.seqlen_q, seqs.n, kBN) : (p.seqlen_q + kBN - 1) / kBN;
   kp.window = window;
   kp.sink_sums = reinterpret_cast<float*>(ws + pl.sinks_off);
-  kp.sink_tiles = pl.sink_tiles; kp.near_units = pl.near_units; kp.far_slots = pl.far_slots;
+  kp.sink_rows = pl.sink_rows; kp.sink_tiles = pl.sink_tiles; kp.far_rows = pl.far_rows; kp.near_units = pl.near_units; kp.far_slots = pl.far_slots;
   kp.n_far_ctas = pl.sink_tiles * p.h_k * pl.far_slots * p.b;
   kp.nsplit = pl.nsplit;
   kp.ranges = seqs.cu_q ? 1 : pl.ranges;
@@ -1480,7 +1484,7 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   if (e != cudaSuccess) return static_cast<int>(e);
   if (window.keys) {
     if (!pl.sink_tiles) return 0;
-    const int64_t rows = static_cast<int64_t>(pl.near_units) * p.h_k * std::min(window.sinks, pl.sink_tiles * kBN);
+    const int64_t rows = static_cast<int64_t>(pl.near_units) * p.h_k * pl.sink_rows;
     sinks_kernel<D, kBf16><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(kp);
     return static_cast<int>(cudaGetLastError());
   }
