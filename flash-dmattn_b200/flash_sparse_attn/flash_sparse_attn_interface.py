@@ -215,6 +215,8 @@ def _check_inputs(q, k, v, mask, bias):
         raise RuntimeError("FlashSparseAttention only supports fp16 and bf16 data type")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise RuntimeError("query, key and value must have the same dtype")
+    if k.device != q.device or v.device != q.device:
+        raise RuntimeError("query, key and value must be on the same device")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise RuntimeError("query, key and value must be (batch, seqlen, nheads, headdim)")
     B, Sq, H, d = q.shape
@@ -636,7 +638,7 @@ def _varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seq
     if tail > 0:
         outs.append(query.new_zeros((tail, H, d)))
         lses.append(torch.full((H, tail), float("inf"), dtype=torch.float32, device=query.device))
-    out = torch.cat(outs, dim=0) if outs else query.new_zeros(query.shape)
+    out = torch.cat(outs, dim=0) if outs else query * 0
     if not return_attn_probs:
         return out
     return out, torch.cat(lses, dim=1), torch.empty((0,), dtype=query.dtype, device=query.device)

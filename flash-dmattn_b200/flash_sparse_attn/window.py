@@ -7,6 +7,7 @@ Key tiles that no query of a tile sees are neither loaded nor multiplied (csrc/f
 fdma_bwd256_sm100.cu); the mask is one of the keys, for all queries.
 """
 import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -15,6 +16,11 @@ from . import _lib, _native
 from . import flash_sparse_attn_interface as _interface
 
 __all__ = ["flash_sparse_attn_window_func", "flash_sparse_attn_window_varlen_func"]
+
+
+def _check_scale(softmax_scale) -> None:
+    if softmax_scale is not None and not 0 <= softmax_scale < math.inf:
+        raise ValueError(f"softmax_scale must be a finite number of at least 0, got {softmax_scale}")
 
 
 def check_window(sliding_window, sink_tokens) -> None:
@@ -41,18 +47,25 @@ def flash_sparse_attn_window_func(
     query (B, Sq, H, d); key, value (B, Sk, Hk, d) with H % Hk == 0; fp16 or bf16, head dims up to 256. Query i is at position
     i + Sk - Sq, as under `flash_sparse_attn_func(is_causal=True)`, which this equals where the window is as long as the keys.
     attn_mask: bool ({B|1}, {H|Hk|1}, 1, {Sk|1}), False = masked out, such as padding; masks per query are not built. Rows that see no key
-    return 0. Keys and values are expected to be finite, also where the mask hides them. softmax_scale defaults to d ** -0.5.
+    return 0. Keys and values are expected to be finite, also where the mask hides them. softmax_scale, 0 or above, defaults to d ** -0.5.
+    B, Sq and Sk are at least 1 (packed sequences may be empty).
     return_attn_probs=True returns (out, softmax_lse (B, H, Sq) fp32, empty tensor).
 
     Time and traffic go with the window, not with Sk. Returns out (B, Sq, H, d); gradients flow to query, key and value, each a sum in
-    a fixed order, with `deterministic` or without. Head dims above 128 take gradients of masks that are shared by the query heads of a
-    kv head. Nothing synchronises: a step can be captured into a CUDA graph."""
+    a fixed order, with `deterministic` or without. Head dims above 128 have none with a mask of its own for each query
+    head. Nothing synchronises: a step can be captured into a CUDA graph."""
     check_window(sliding_window, sink_tokens)
+    _check_scale(softmax_scale)
     if attn_mask is not None:
         if not isinstance(attn_mask, torch.Tensor) or attn_mask.dtype != torch.bool or attn_mask.dim() != 4:
             raise RuntimeError("attn_mask must be a bool tensor ({B|1}, {H|Hk|1}, 1, {Sk|1})")
         if attn_mask.shape[2] != 1:
             raise NotImplementedError("masks per query are not built with a sliding window: attn_mask must be ({B|1}, {H|Hk|1}, 1, {Sk|1})")
+        if key.dim() == 4 and attn_mask.shape[3] not in (1, key.shape[1], _interface.round_multiple(key.shape[1], _interface._KEY_PAD)):
+            raise RuntimeError("attn_mask must be a bool tensor ({B|1}, {H|Hk|1}, 1, {Sk|1})")
+        if query.dim() == key.dim() == 4 and query.shape[-1] > 128 and attn_mask.shape[1] not in (1, key.shape[2]) and torch.is_grad_enabled() \
+                and any(t.requires_grad for t in (query, key, value)):
+            raise NotImplementedError("head dims above 128 have no gradients with a mask of its own for each query head")
     elif key.dim() == 4 and sliding_window + sink_tokens >= key.shape[1]:  # every query sees all keys up to its own
         return _interface.flash_sparse_attn_func(query, key, value, None, None, softmax_scale, True, None, deterministic,
                                                  return_attn_probs)
@@ -95,6 +108,7 @@ def flash_sparse_attn_window_varlen_func(
     on the GPU, where they must ascend from 0 or more; what they leave out, or what lies beyond the tensors, belongs to no sequence, whose
     rows are 0, gradients too. Other calls go sequence by sequence, their boundaries read on the host."""
     check_window(sliding_window, sink_tokens)
+    _check_scale(softmax_scale)
     if not return_attn_probs and not torch.compiler.is_compiling() and _interface._kernel_path == _lib.PATH_AUTO and query.is_cuda:
         scale = query.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
         res = _native.load().packed_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, scale, True, bool(deterministic), sliding_window,
