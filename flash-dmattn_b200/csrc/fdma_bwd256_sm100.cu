@@ -114,9 +114,14 @@ __device__ __forceinline__ uint16_t f_to_raw16(float x) {
   return static_cast<uint16_t>(pack_16x2<kBf16>(x, 0.f) & 0xFFFFu);
 }
 
-// Whether the queries [q_lo, q_hi) hold one that sees the tile from key0 on as sinks alone, beyond its window. query + coff: its position
+// Sliding window: the end of the query tiles whose rows see the key tile from key0 on in their window; those behind see its sinks alone.
+// query + coff: its position
+__device__ __forceinline__ int near_end(int key0, int coff, const Window& window) {
+  return max(0, (key0 + kBN - 1 + window.keys - coff + kBM - 1) / kBM * kBM);
+}
+// Whether there are such among the queries [q_lo, q_hi)
 __device__ __forceinline__ bool far_part(int key0, int q_lo, int q_hi, int coff, const Window& window) {
-  return q_lo < q_hi && q_hi - 1 >= key0 + window.keys - coff;
+  return q_lo < q_hi && q_hi > near_end(key0, coff, window);
 }
 
 template <bool kBf16, int kPass, bool kWindow>
@@ -203,10 +208,10 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
       if (far) {
         const int q_lo = slot * p.far_rows, q_hi = min(Sq, q_lo + p.far_rows);
         if (!far_part(n * kBN, q_lo, q_hi, coff, p.window)) return;  // (the whole CTA agrees)
-        m_start = max(q_lo, n * kBN + p.window.keys - coff) / kBM;
+        m_start = max(q_lo, near_end(n * kBN, coff, p.window)) / kBM;
         M64 = (q_hi + kBM - 1) / kBM;
       } else {
-        M64 = max(0, min(M64, (min(n * kBN + kBN, Sk) - 1 + p.window.keys - coff + kBM - 1) / kBM));
+        M64 = min(M64, near_end(n * kBN, coff, p.window) / kBM);
       }
     }
   }
@@ -479,8 +484,9 @@ __device__ __forceinline__ void pass256(const Bwd256Params& p, unsigned char* sm
     }
     // Sliding window. Key passes: the queries [qlo, qhi) see this key, [qlo_max, qhi_min) all keys of the warp; dQ pass: the first key this
     // row (and the warp's last row) sees in its window
-    const int qlo = ckey - coff + (far ? p.window.keys : 0), qhi = far ? 0x7FFFFFFF : ckey - coff + p.window.keys;
-    const int qlo_max = ckey_wmax - coff + (far ? p.window.keys : 0), qhi_min = far ? 0x7FFFFFFF : warp_row - coff + p.window.keys;
+    const bool sink = kWindow && row < p.window.sinks, sinks = kWindow && warp_row + 31 < p.window.sinks;
+    const int qlo = far ? near_end(n * kBN, coff, p.window) : ckey - coff, qhi = sink ? 0x7FFFFFFF : ckey - coff + p.window.keys;
+    const int qlo_max = far ? qlo : ckey_wmax - coff, qhi_min = far || sinks ? 0x7FFFFFFF : warp_row - coff + p.window.keys;
     const int kfirst = row + coff - p.window.keys + 1, kfirst_wmax = warp_row + 31 + coff - p.window.keys + 1;
     float colsum = 0.f;
     bool ok = true;

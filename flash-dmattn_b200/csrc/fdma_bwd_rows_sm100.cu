@@ -96,7 +96,7 @@ struct BwdRowsParams {
   int64_t pos_batch_stride, pos_head_stride;
   int h_pos, causal_shift;
   PackedSeqs seqs;   // packed sequences, each with tiles of its own; streamed query tiles are cut at fixed rows
-  // Sliding window (kWindow). A key tile's CTA takes the queries whose window reaches it (near); those beyond, which see the sinks alone,
+  // Sliding window (kWindow). A key tile's CTA takes the query tiles whose windows reach it (near); those beyond, which see the sinks alone,
   // come from CTAs of their own (far), far_rows queries each. Both leave fp32 sums of the sinks' rows, which sinks_kernel adds up:
   // [2: dV, dK][near of each sequence or batch element, then a place for each part of far_rows queries][h_k][sink_rows][D]
   Window window;
@@ -233,9 +233,14 @@ __device__ __forceinline__ float softmax_step(const uint32_t (&x)[32], const uin
   return (part[0].x + part[0].y) + (part[1].x + part[1].y);
 }
 
-// Whether the queries [q_lo, q_hi) hold one that sees the tile from key0 on as sinks alone, beyond its window. query + coff: its position
+// Sliding window: the end of the query tiles whose rows see the key tile from key0 on in their window; those behind see its sinks alone.
+// query + coff: its position
+__device__ __forceinline__ int near_end(int key0, int coff, const Window& window) {
+  return max(0, (key0 + kBN - 1 + window.keys - coff + kBM - 1) / kBM * kBM);
+}
+// Whether there are such among the queries [q_lo, q_hi)
 __device__ __forceinline__ bool far_part(int key0, int key_end, int q_lo, int q_hi, int coff, const Window& window) {
-  return key0 < key_end && q_lo < q_hi && q_hi - 1 >= key0 + window.keys - coff;
+  return key0 < key_end && q_lo < q_hi && q_hi > near_end(key0, coff, window);
 }
 // Where the far CTAs' rows begin in dkv_sums, behind the near ones' (half: dV, dK)
 __device__ __forceinline__ int64_t far_rows_at(const BwdRowsParams& p, int half, int key_tiles) {
@@ -319,9 +324,8 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
   } else if (kWindow && !far && n < p.sink_tiles) {
     sink_unit = b;
   }
-  int beyond = 0;  // far: what is added to a key's first query that sees it; near: as many queries see it
+  int behind = 0;  // where the near queries end and the far ones begin
   if (kWindow) {
-    beyond = p.window.keys;
     if (!far && sink_unit >= 0 && !far_part(key0, key_end, q_lo, q_hi, coff, p.window)) sink_unit = -1;  // nobody is beyond
     if (far) {
       if (packed) {
@@ -338,10 +342,11 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
         q_hi = min(Sq, q_lo + p.far_rows);
       }
       if (!far_part(key0, key_end, q_lo, q_hi, coff, p.window)) return;  // (the whole CTA agrees)
-      m_start = max(q_lo, key0 + beyond - coff) / kBM;
+      behind = near_end(key0, coff, p.window);
+      m_start = max(q_lo, behind) / kBM;
       M64 = (q_hi + kBM - 1) / kBM;
     } else {
-      M64 = max(0, min(M64, (min(key0 + kBN, key_end) - 1 + beyond - coff + kBM - 1) / kBM));
+      M64 = min(M64, near_end(key0, coff, p.window) / kBM);
     }
     M64 = warp_uniform(M64);
   }
@@ -532,12 +537,11 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
     }
     if (kWindow) {
       if (far) {
-        qlo = max(q_lo, key + beyond - coff);
-        qlo_max = max(q_lo, ckey_wmax + beyond - coff);
+        qlo = qlo_max = max(q_lo, behind);
         qhi = qhi_min = q_hi;
       } else {
-        qhi = min(qhi, key + beyond - coff);
-        qhi_min = min(qhi_min, key0 + (warp & 3) * 32 + beyond - coff);
+        if (n_in_seq * kBN + krow >= p.window.sinks) qhi = min(qhi, key + p.window.keys - coff);
+        if (n_in_seq * kBN + (warp & 3) * 32 + 31 >= p.window.sinks) qhi_min = min(qhi_min, key0 + (warp & 3) * 32 + p.window.keys - coff);
       }
     }
     // addend of this key for query head h: bias in log2 units, -inf when the key is masked out (P = exp2(-inf) = 0 without any
