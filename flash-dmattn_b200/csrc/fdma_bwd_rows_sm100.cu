@@ -97,7 +97,11 @@ struct BwdRowsParams {
   int h_pos, causal_shift;
   PackedSeqs seqs;   // packed sequences, each with tiles of its own; streamed query tiles are cut at fixed rows
   // Sliding window (kWindow). A key tile's CTA takes the query tiles whose windows reach it (near); those beyond, which see the sinks alone,
-  // come from CTAs of their own (far), far_rows queries each. Both leave fp32 sums of the sinks' rows, which sinks_kernel adds up:
+  // come from CTAs of their own (far), far_rows queries each: one CTA for a sink tile and all queries would be the whole launch's tail. Row-pass
+  // items walk the sinks' and the window's key tiles, numbered without the gap between. 10 d products per pair that is seen and head, of which
+  // S and dP are formed twice; 32 heads over 8, d = 128, bf16: 32768 queries, 2048 keys + 4 sinks 4400 us (625 TFLOP/s counted once, 875 as
+  // issued), 8192 queries: 1024 keys 585 us, 128 + 4 sinks 282, 1 key 199. Bound by the softmax arithmetic, narrow windows by the CTAs' set-up.
+  // Where a sequence has far queries, near and far leave fp32 sums of the sinks' rows, which sinks_kernel adds up in their order:
   // [2: dV, dK][near of each sequence or batch element, then a place for each part of far_rows queries][h_k][sink_rows][D]
   Window window;
   float* sink_sums;

@@ -371,7 +371,9 @@ struct Layout {
 
 // kBias: with a bias, dense (without one the loop is shorter by its loads: 14.2 us instead of 14.7 for 16 requests of drafts). With a list
 // of kept keys the bias is looked for when it runs.
-// kWindow: a sliding window with sinks, an instantiation of its own: the first keys of rows' windows take registers.
+// kWindow: a sliding window with sinks, an instantiation of its own: the first keys of rows' windows take registers. A unit's chunks are
+// those of the sinks and those from its oldest row's window on, so that it reads and costs what a cache of as many keys does: 64 requests of
+// one token, 32 heads over 8, d = 128, 4096 keys of 40000: 105 us (5.2 TB/s), caches of 4096 without a window 103.
 template <int D, int ROWS, bool kGather, bool kBf16, bool kCluster, bool kBias, bool kWindow>
 __global__ void __launch_bounds__(Layout<D, ROWS, kGather>::kThreads, Layout<D, ROWS, kGather>::kCtas)
 cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {

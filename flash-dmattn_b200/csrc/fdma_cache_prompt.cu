@@ -41,7 +41,8 @@ struct UnpackArgs {
   void *k, *v;  // (rows, h_k, d)
   int shift, max_keys, max_queries, rows, heads;
   // Sliding window (0: none): of a request the chunks with sinks are converted and those from the first key on that one of its queries sees.
-  // Behind one another they are a sequence whose window and sinks leave the same keys visible.
+  // Behind one another they are a sequence whose window and sinks leave the same keys visible. (4 requests, 2048 new tokens over 14000, 32
+  // heads over 8, d = 128, a window of 2048 + 4 sinks: 434 us, the conversion 32 of them; the forward's floor is 165.)
   int window, sink_chunks;
 };
 // Chunks that are left out, of a request of `length` tokens of which `queries` are new

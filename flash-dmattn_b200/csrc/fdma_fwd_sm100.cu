@@ -74,7 +74,8 @@ struct FwdKernelParams {
   PackedSeqs seqs;   // packed sequences, each with query blocks and key tiles of its own
   Window window;     // sliding window (kWindow)
   // kWindow: the two query tiles of an item are those of two heads that share a kv head, at the same rows, and not two tiles of one head. Then
-  // they see the same key tiles: one fewer, and none that only one of them works on.
+  // they see the same key tiles: one fewer, and none that only one of them works on (8192 queries, 32 heads over 8, d = 128: a window of 128
+  // keys 118 -> 100 us, 1024 197 -> 186). Where the group is even and the mask, if any, the same for both.
   bool pair;
   int n_mblk;        // query blocks (of kNQ tiles) per (batch, head); packed: places for them
   int n_items;       // work items = n_mblk * h * b
@@ -187,9 +188,16 @@ __device__ __forceinline__ FwdItem fwd_item(const FwdKernelParams& p, int item, 
 
 // kVariant, per-query kernel: the mask holds one bit per key instead of one byte. Row-broadcast kernel: packed sequences, whose
 // items are the blocks of each (an instantiation of its own: the ordinary kernel's softmax threads have no registers to spare
-// for an item's extents). kWindow: a sliding window with sinks; a block's key tiles are those of the sinks and, from the first one that
-// its first row sees, those up to the causal limit, numbered without the gap between (KeyTiles). One launch instead of one per sequence: 8192 tokens in 5 sequences, 16 heads, d = 128: forward 258 ->
+// for an item's extents). One launch instead of one per sequence: 8192 tokens in 5 sequences, 16 heads, d = 128: forward 258 ->
 // 182 us, backward 617 -> 520 us, the call, with the fills, copies and adds of the sequences' gradients gone, 1510 -> 815 us.
+//
+// kWindow: a sliding window with sinks, key k for query position t:  k <= t and (t - k < window or k < sinks). A block's key tiles are those
+// of the sinks and, from the first one that its first row sees, those up to the causal limit, numbered without the gap between (gap_of), so
+// that producer, mask, MMA and softmax warps walk one row of tiles; per element only the tiles on the window's two ends are masked. What it
+// cannot do without is 4 d products per pair that is seen and head. 32 heads over 8, d = 128, bf16: 32768 queries, 2048 keys + 4 sinks 1180 us
+// (930 TFLOP/s; causal over all keys 8990), 8192 queries: 1024 keys 175 us (750 TFLOP/s; causal 527), 128 + 4 sinks 92, 1 key 63. Bound by the
+// softmax chain as without a window, and below some 1000 keys by what an item costs beside its tiles: about 8000 cycles for its queries' way
+// in, the first product and the results' way out (stalls for instructions, twice those of a window of 1024 keys at 128, are part of it).
 template <int D, bool kBf16, bool kBcast, bool kVariant = false, bool kWindow = false>
 __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_constant__ FwdKernelParams p) {
   using L = Smem<D>;
@@ -502,7 +510,7 @@ __global__ void __launch_bounds__(Smem<D>::kThreads, 1) fwd_kernel(const __grid_
             ++pcnt[t];
             ++pv_done[t];
             // Sliding window: the query tile's last product of the item. Its warps do not wait for those of the other one, half a period behind.
-            // (8192 queries, 32 heads, d = 128, a window of 1024 keys 186 -> 181 us; without a window, in longer items, no difference.)
+            // (8192 queries, 32 heads, d = 128, a window of 1024 keys 186 -> 181 us; without a window, in longer items, no difference, 528.)
             if (kWindow && prev_j == place_last[t]) {
               umma_commit(lead, bar_o_done + t);
               ++ocnt[t];

@@ -7,7 +7,9 @@
 // What it has to move is the logits, once: HBM-bound, 2 or 4 bytes a number. rows_kernel streams all rows, a part of one in each CTA, and
 // leaves its maximum and the sum of its exponentials, in 32 bits. In verify_kernel a cluster of CTAs has a request: they know from those
 // how many drafts pass, and read the row that the next token comes from again, from L2, with the drafter's, each a slice of the vocabulary.
-// (In one launch, a cluster streaming its request's rows, few clusters ran at once: 64 requests of 9 rows, 131072 numbers each: 280 us.)
+// 64 requests of 9 rows, 131072 numbers, bf16, with fp32 probabilities: 82 us, rows_kernel 35 of them (4.3 TB/s), verify_kernel 49, bound by
+// its instructions, the 64-bit ones among them; 200 of up to 6 rows, 50257 numbers, fp32: 63-68; one of 4 rows, 32000 numbers: 14, two launches and
+// a chain of exchanges in a cluster. (In one launch, a cluster streaming its request's rows, few clusters ran at once: 64 requests of 9 rows, 131072 numbers each: 280 us.)
 // A random number beside a border decides between two tokens, so what is compared with it is summed up in 64 bits, with exponentials
 // that are exact to 2^-44: the row of the next token always, a draft's own row where 32 bits leave the verdict open. Sums have one order.
 #include <cuda_bf16.h>
