@@ -39,6 +39,10 @@ __device__ __forceinline__ PackedTile packed_tile(const int32_t* cu, int n, int 
   t.begin = packed_bound(cu, n, total, lo);
   t.end = max(t.begin, packed_bound(cu, n, total, lo + 1));
   t.tile = slot - (t.begin / rows + lo + 1);
+  if (t.tile < 0) {  // boundaries that do not ascend: no rows in front of the sequence
+    t.tile = 0;
+    t.end = t.begin;
+  }
   return t;
 }
 // The rows of the other tensor that a sequence has.

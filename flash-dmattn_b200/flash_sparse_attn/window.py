@@ -105,8 +105,8 @@ def flash_sparse_attn_window_varlen_func(
 ):
     """`flash_sparse_attn_window_func` on packed sequences: arguments and results as of `flash_sparse_attn_varlen_func`, positions,
     window and sinks in each sequence. Up to head dim 128 the sequences run in one launch per direction and nothing synchronises: the boundaries stay
-    on the GPU, where they must ascend from 0 or more; what they leave out, or what lies beyond the tensors, belongs to no sequence, whose
-    rows are 0, gradients too. Other calls go sequence by sequence, their boundaries read on the host."""
+    on the GPU, where they must ascend from 0 or more (otherwise results are undefined, within the tensors); what they leave out, or what lies
+    beyond the tensors, belongs to no sequence, whose rows are 0, gradients too. Other calls go sequence by sequence, their boundaries read on the host."""
     check_window(sliding_window, sink_tokens)
     _check_scale(softmax_scale)
     if not return_attn_probs and not torch.compiler.is_compiling() and _interface._kernel_path == _lib.PATH_AUTO and query.is_cuda:

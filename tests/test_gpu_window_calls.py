@@ -262,6 +262,22 @@ def test_packed_sequences_one_by_one(what):
     check([out, *torch.autograd.grad(out, (q, k, v), dout)], *packed_reference(q, k, v, cu_list, cu_list, window, sinks, dout))
 
 
+def test_boundaries_that_do_not_ascend_stay_within_the_tensors():
+    T = 900
+    q, k, v, dout = (x[0].detach().requires_grad_(i < 3) for i, x in enumerate(tensors(1, T, T, 4, 2, 64, torch.bfloat16)))
+
+    def run(bounds):
+        cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+        out = varlen_func(q, k, v, cu, cu, T, T, 60, 70)
+        return [out, *torch.autograd.grad(out, (q, k, v), dout)]
+
+    want = run([0, 400, 410, T])
+    for bad in ([0, 500, 100, T], [T, 0, 500, 20], [-5, 700, 2 ** 31 - 1, 3], [300, 200, 100, 0], [0, 0, 0, -7]):
+        run(bad)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(run([0, 400, 410, T]), want))
+
+
 def test_refusals():
     q, k, v, dout = (x.detach() for x in tensors(2, 40, 40, 4, 2, 64, torch.bfloat16))
     mask = torch.ones((2, 1, 1, 40), dtype=torch.bool, device="cuda")
