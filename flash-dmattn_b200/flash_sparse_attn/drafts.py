@@ -41,6 +41,8 @@ def verify_drafts(
     follows token i. uniforms (tokens,), float32 in [0, 1). draft_probs (tokens, vocabulary), bf16, fp16 or fp32: row i the probabilities
     that the draft behind token i was drawn from (the last row of a request is not read); None: drafts that were not drawn, such as looked up ones.
     temperature: a number or float32 (requests,).
+    Of the step its cu_seqlens, lengths and granted count. Where others' prompt parts are in the step, gather the rows that matter (the last one
+    of a part, all of a request with drafts) and give their boundaries: step._replace(cu_seqlens=...).
 
     With p = softmax(logits / temperature) and q the drafter's row, the draft x behind token i is accepted if uniforms[i] * q(x) < p(x), and the
     first one that is not ends the request's. The next token is drawn from what that row leaves, max(p - q, 0) (without draft_probs: p

@@ -247,6 +247,16 @@ def test_a_step_with_its_tables(dev):  # noqa: F811
     assert some > 0
 
 
+def test_rows_gathered_from_a_step_with_a_prompt_part(dev):  # noqa: F811
+    new, V = [300, 4, 0, 1], 700
+    step = plan(dev, new)
+    ids, logits, u, q = drafts(dev, new, V, torch.bfloat16, torch.float32, 6)
+    rows = torch.tensor([299, 300, 301, 302, 303, 304], device=dev)
+    part = step._replace(cu_seqlens=ints([0, 1, 5, 5, 6], dev))
+    got = check(dev, part, ids[rows], logits[rows], u[rows], q[rows], 0.9)
+    assert got.lengths[0] == step.lengths[0] and got.lengths[3] == step.lengths[3]
+
+
 def test_refusals(dev):  # noqa: F811
     new, V = [2, 3], 50
     ids, logits, u, q = drafts(dev, new, V, torch.float32, torch.float32, 1)
