@@ -120,6 +120,11 @@ fdma_fwd_params normalise_window(const fdma_fwd_params& in) {
   return p;
 }
 
+// A single query of each head goes to the kernel that splits its keys over CTAs.
+bool decodes_window(const fdma_fwd_params& p, int32_t n) {
+  return n == 0 && p.seqlen_q == 1 && p.path == FDMA_PATH_AUTO && decode_window_supported(p);
+}
+
 }  // namespace
 
 int encode_tmap_4d(void* out_map, const void* base, int elem_bytes, const uint64_t dims[4],
@@ -324,6 +329,12 @@ int fdma_bwd_varlen(const fdma_bwd_params* pp, const int32_t* cu_q, const int32_
   return tc_bwd(p, static_cast<cudaStream_t>(stream_), seqs);
 }
 
+size_t fdma_fwd_window_workspace_bytes(const fdma_fwd_params* pp, int32_t window, int32_t sinks, int32_t n) {
+  if (!pp || window <= 0 || sinks < 0 || n < 0 || validate_fwd(*pp)) return 0;
+  const fdma_fwd_params p = normalise_window(*pp);
+  return decodes_window(p, n) ? decode_window_workspace_bytes(p, window_of(p, window, sinks)) : 0;
+}
+
 int fdma_fwd_window(const fdma_fwd_params* pp, int32_t window, int32_t sinks, const int32_t* cu_q, const int32_t* cu_k, int32_t n, void* stream_) {
   if (!pp) return FDMA_ERR_BAD_ARG;
   int st = validate_fwd(*pp);
@@ -332,6 +343,7 @@ int fdma_fwd_window(const fdma_fwd_params* pp, int32_t window, int32_t sinks, co
   st = check_arch();
   if (st) return st;
   const fdma_fwd_params p = normalise_window(*pp);
+  if (decodes_window(p, n)) return decode_window_fwd(p, window_of(p, window, sinks), static_cast<cudaStream_t>(stream_));
   if (!tc_fwd_supported(p)) return FDMA_ERR_UNSUPPORTED;
   return tc_fwd(p, static_cast<cudaStream_t>(stream_), PackedSeqs{cu_q, cu_k, n}, window_of(p, window, sinks));
 }

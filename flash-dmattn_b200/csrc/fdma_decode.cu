@@ -52,7 +52,7 @@ struct Ring {
 
 struct DecodeParams {
   const uint16_t *q, *k, *v, *bias;
-  const int32_t* pos;    // kept positions, ascending, or null: slot i is key i
+  const int32_t* pos;    // kept positions, ascending, or null: slot i is key i, from gap_at on key i + gap
   const int32_t* count;  // kept keys per list, or null: all `slots`
   uint16_t* out;
   float* lse;
@@ -61,6 +61,9 @@ struct DecodeParams {
   int k_sr, v_sr;        // row strides in elements, below 2^31: one widening multiply per address
   int64_t pos_sb, pos_sh, count_sb, count_sh, bias_sb, bias_sh;
   int h, h_k, h_pos, h_bias, d, seqlen_k, slots, nsplit;
+  int gap_at, gap;       // sliding window: keys between the sinks and the window
+  const uint8_t* mask;   // sliding window: bool mask of the keys of (batch element, kv head), or null. Then there is no bias
+  int64_t mask_sb, mask_sh;
   int row_align;         // kPieces: bytes K and V rows are aligned to
   int heads;             // query heads per CTA
   int head_blocks;       // CTA rows per (batch, split)
@@ -140,11 +143,13 @@ __device__ __forceinline__ float exp2_or_zero(float x) { return x == -CUDART_INF
 
 // kM16: 9 to 16 query heads (both halves of the M rows of the products), else up to 8. Fragments of mma.m16n8k16
 // (g = lane / 4, c = lane % 4): A row g (+ 8), k = 2c, 2c+1 (+ 8); B k = 2c, 2c+1 (+ 8), n = g; C row g (+ 8), n = 2c, 2c+1.
-// kPieces: K / V rows that are aligned to 4 or 8 bytes only.
-template <int NJ, bool kBf16, bool kM16, bool kPieces>
+// kPieces: K / V rows that are aligned to 4 or 8 bytes only. kWindow: 1 with a gap (of 0, too), 2 with a mask as well;
+// instances of their own, since the gap's comparison alone took one request of 4097 keys from 16.5 to 17.6 us.
+template <int NJ, bool kBf16, bool kM16, bool kPieces, int kWindow>
 __global__ void __launch_bounds__(kThreads, NJ <= 4 && !kPieces ? 3 : 1) decode_rows_kernel(const DecodeParams p) {
   using L = Ring<NJ>;
   constexpr int D = NJ * 32;
+  constexpr bool kMask = kWindow == 2;
   constexpr int kHalves = kM16 ? 2 : 1;
   constexpr int kHeads = 8 * kHalves;
   // Head dims above 128, and rows in pieces: the probabilities keep their 32 bits, as sums of three 16-bit values with a product
@@ -196,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, NJ <= 4 && !kPieces ? 3 : 1) decode_
     const int head = h0 + min(g + 8 * t, nh - 1);
     bias_row[t] = p.bias ? p.bias + b * p.bias_sb + (p.h_bias == p.h ? head : (p.h_bias == p.h_k ? hk : 0)) * p.bias_sh : nullptr;
   }
+  const uint8_t* mask_row = kMask ? p.mask + b * p.mask_sb + hk * p.mask_sh : nullptr;
   float o[kHalves][4 * NJ][2];  // O[head g + 8 t][8 nt + 2c + {0, 1}]
   float m[kHalves], l[kHalves];  // running max of the head; this LANE's share of the sum
 #pragma unroll
@@ -218,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, NJ <= 4 && !kPieces ? 3 : 1) decode_
   // stage that needs it: a comparison beside the load made every stage wait for it.
   auto load_pos = [&](int i) {
     const int slot = (first + i) * kChunk + lane;
-    return slot < n_keys && i < n ? (pos_row ? __ldg(pos_row + slot) : slot) : -1;
+    return slot < n_keys && i < n ? (pos_row ? __ldg(pos_row + slot) : !kWindow || slot < p.gap_at ? slot : slot + p.gap) : -1;
   };
   int my_pos = -1, next_pos = load_pos(0);
   const uint64_t policy = evict_first_policy();
@@ -259,7 +265,8 @@ __global__ void __launch_bounds__(kThreads, NJ <= 4 && !kPieces ? 3 : 1) decode_
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     kp = __shfl_sync(0xffffffffu, my_pos, (i & 1) * kChunk + (lane & 15));
-    kb = kp < 0 ? kNegInf : p.bias && !head_bias ? __ldg(bias_row[0] + kp) : static_cast<uint16_t>(0);
+    if (kMask) kb = kp < 0 ? static_cast<uint16_t>(0) : __ldg(mask_row + kp);  // (0: -inf)
+    else kb = kp < 0 ? kNegInf : p.bias && !head_bias ? __ldg(bias_row[0] + kp) : static_cast<uint16_t>(0);
   };
   auto consume = [&](int st, int kp, uint16_t kb) {
     const uint32_t kst = ring + st * L::kStageBytes, vst = kst + kChunk * L::kRowBytes;
@@ -277,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, NJ <= 4 && !kPieces ? 3 : 1) decode_
       for (int u = 0; u < 2; ++u)
         mma_16816<kBf16>(s0[u], kM16 ? s8[u] : zero, q0, q1, q2, q3, f[2 * u], f[2 * u + 1]);
     }
-    const float kbf = raw_to_f<kBf16>(kb) * kLog2e;
+    const float kbf = kMask ? (kb == 0 ? -CUDART_INF_F : 0.f) : raw_to_f<kBf16>(kb) * kLog2e;
     uint32_t pa[kTerms][kHalves][2];
 #pragma unroll
     for (int t = 0; t < kHalves; ++t) {
@@ -492,9 +499,9 @@ DecodePlan plan(const fdma_fwd_params& p, int slots, int h_pos, bool index) {
   return pl;
 }
 
-template <int NJ, bool kBf16, bool kM16, bool kPieces>
+template <int NJ, bool kBf16, bool kM16, bool kPieces, int kWindow>
 int launch(const DecodeParams& dp, const DecodePlan& pl, int batch, cudaStream_t stream) {
-  auto kern = decode_rows_kernel<NJ, kBf16, kM16, kPieces>;
+  auto kern = decode_rows_kernel<NJ, kBf16, kM16, kPieces, kWindow>;
   constexpr int parts = kWarps * (kM16 ? 16 : 8) * NJ * 32 * static_cast<int>(sizeof(float));
   constexpr int smem = std::max(parts, kWarps * Ring<NJ>::kWarpBytes);
   if (smem > 40 * 1024) {
@@ -514,12 +521,17 @@ int launch(const DecodeParams& dp, const DecodePlan& pl, int batch, cudaStream_t
   cfg.numAttrs = 1;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, dp));
 }
-template <int NJ, bool kPieces>
-int launch_nj(const DecodeParams& dp, const DecodePlan& pl, int batch, bool bf16, cudaStream_t stream) {
+template <int NJ, bool kPieces, int kWindow>
+int launch_w(const DecodeParams& dp, const DecodePlan& pl, int batch, bool bf16, cudaStream_t stream) {
   constexpr bool kM16 = NJ <= 4;
   if (kM16 && pl.heads > 8)
-    return bf16 ? launch<NJ, true, kM16, kPieces>(dp, pl, batch, stream) : launch<NJ, false, kM16, kPieces>(dp, pl, batch, stream);
-  return bf16 ? launch<NJ, true, false, kPieces>(dp, pl, batch, stream) : launch<NJ, false, false, kPieces>(dp, pl, batch, stream);
+    return bf16 ? launch<NJ, true, kM16, kPieces, kWindow>(dp, pl, batch, stream) : launch<NJ, false, kM16, kPieces, kWindow>(dp, pl, batch, stream);
+  return bf16 ? launch<NJ, true, false, kPieces, kWindow>(dp, pl, batch, stream) : launch<NJ, false, false, kPieces, kWindow>(dp, pl, batch, stream);
+}
+template <int NJ, bool kPieces>
+int launch_nj(const DecodeParams& dp, const DecodePlan& pl, int batch, bool bf16, cudaStream_t stream) {
+  if (dp.mask) return launch_w<NJ, kPieces, 2>(dp, pl, batch, bf16, stream);
+  return dp.gap ? launch_w<NJ, kPieces, 1>(dp, pl, batch, bf16, stream) : launch_w<NJ, kPieces, 0>(dp, pl, batch, bf16, stream);
 }
 
 // Bytes that every row of K and V is aligned to: 16, 8, 4 or 2.
@@ -532,8 +544,15 @@ int row_align(const fdma_fwd_params& p) {
 }
 
 int run(const fdma_fwd_params& p, const DecodePlan& pl, const int32_t* pos, int64_t pos_sb, int64_t pos_sh, int h_pos,
-        const int32_t* count, int64_t count_sb, int64_t count_sh, int slots, cudaStream_t stream) {
+        const int32_t* count, int64_t count_sb, int64_t count_sh, int slots, cudaStream_t stream, int gap_at = 0, int gap = 0, bool masked = false) {
   DecodeParams dp = {};
+  dp.gap_at = gap ? gap_at : 0x7FFFFFFF;
+  dp.gap = gap;
+  if (masked) {
+    dp.mask = static_cast<const uint8_t*>(p.mask);
+    dp.mask_sb = p.mask_batch_stride;
+    dp.mask_sh = p.h_mask == 1 ? 0 : p.mask_head_stride;
+  }
   dp.q = static_cast<const uint16_t*>(p.q); dp.k = static_cast<const uint16_t*>(p.k);
   dp.v = static_cast<const uint16_t*>(p.v); dp.bias = static_cast<const uint16_t*>(p.bias);
   dp.out = static_cast<uint16_t*>(p.out); dp.lse = p.lse;
@@ -607,6 +626,23 @@ int decode_fwd(const fdma_fwd_params& p, cudaStream_t stream) {
   if (st) return st;
   return run(p, pl, pos, static_cast<int64_t>(p.h_mask) * cap, cap, p.h_mask, count, p.h_mask, p.h_mask == 1 ? 0 : 1,
              p.seqlen_k, stream);
+}
+
+// A sliding window: the last window.keys and the first window.sinks keys, without a list. A mask is read key by key, beside the rows, for
+// the heads that share a pass. 1 / 16 requests of 4096 + 4 of 40000 keys, 32 heads over 8, d = 128: 18 / 64 us, as a tile of the forward
+// kernel 82 / 162.
+bool decode_window_supported(const fdma_fwd_params& p) {
+  return decode_supported(p) && !p.bias && (!p.mask || p.h_mask == 1 || p.h_mask == p.h_k);
+}
+static int window_slots(const fdma_fwd_params& p, const Window& w) {
+  return static_cast<int>(std::min<int64_t>(static_cast<int64_t>(w.keys) + w.sinks, p.seqlen_k));
+}
+size_t decode_window_workspace_bytes(const fdma_fwd_params& p, const Window& w) { return plan(p, window_slots(p, w), 1, false).total; }
+int decode_window_fwd(const fdma_fwd_params& p, const Window& w, cudaStream_t stream) {
+  const int slots = window_slots(p, w);
+  const DecodePlan pl = plan(p, slots, 1, false);
+  if (pl.total && (!p.workspace || p.workspace_bytes < pl.total)) return FDMA_ERR_WORKSPACE;
+  return run(p, pl, nullptr, 0, 0, 1, nullptr, 0, 0, slots, stream, w.sinks, p.seqlen_k - slots, p.mask != nullptr);
 }
 
 // The same for a bool mask in less scratch than the position lists of all rows take: one batch element and as many mask heads

@@ -109,6 +109,9 @@ bool decode_supported(const fdma_fwd_params& p);
 size_t decode_workspace_bytes(const fdma_fwd_params& p);
 int decode_fwd(const fdma_fwd_params& p, cudaStream_t stream);
 int decode_fwd_sliced(const fdma_fwd_params& p, cudaStream_t stream);
+bool decode_window_supported(const fdma_fwd_params& p);
+size_t decode_window_workspace_bytes(const fdma_fwd_params& p, const Window& window);
+int decode_window_fwd(const fdma_fwd_params& p, const Window& window, cudaStream_t stream);
 // fdma_fwd for a single query with a bool mask in whatever workspace there is: position lists a few rows at a time, or where
 // not even one list fits, the kernels that need none. FDMA_ERR_TOO_LARGE for other calls.
 int single_query_fwd_in(const fdma_fwd_params& p, cudaStream_t stream);

@@ -52,6 +52,7 @@ struct Api {
   decltype(&fdma_bwd) bwd;
   decltype(&fdma_fwd_varlen) fwd_varlen;
   decltype(&fdma_bwd_varlen) bwd_varlen;
+  decltype(&fdma_fwd_window_workspace_bytes) fwd_window_workspace_bytes;
   decltype(&fdma_fwd_window) fwd_window;
   decltype(&fdma_bwd_window_workspace_bytes) bwd_window_workspace_bytes;
   decltype(&fdma_bwd_window) bwd_window;
@@ -77,6 +78,7 @@ void init(const std::string& path) {
   get(api.bwd, "fdma_bwd");
   get(api.fwd_varlen, "fdma_fwd_varlen");
   get(api.bwd_varlen, "fdma_bwd_varlen");
+  get(api.fwd_window_workspace_bytes, "fdma_fwd_window_workspace_bytes");
   get(api.fwd_window, "fdma_fwd_window");
   get(api.bwd_window_workspace_bytes, "fdma_bwd_window_workspace_bytes");
   get(api.bwd_window, "fdma_bwd_window");
@@ -640,18 +642,16 @@ std::optional<Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor
       fill_mask_bias(p, mask, bias, activity, c);
     }
     fill_out(p, out, lse);
-    if (c.window) {
-      check(api.fwd_window(&p, static_cast<int32_t>(c.window), static_cast<int32_t>(c.sinks), nullptr, nullptr, 0, stream), "fdma_fwd_window");
-    } else {
-      const size_t bytes = api.fwd_workspace_bytes(&p);
-      Tensor ws;
-      if (bytes) {
-        ws = empty({static_cast<int64_t>(bytes)}, at::kByte, q);
-        p.workspace = ws.data_ptr();
-        p.workspace_bytes = bytes;
-      }
-      check(api.fwd(&p, stream), "fdma_fwd");
+    const int32_t window = static_cast<int32_t>(c.window), sinks = static_cast<int32_t>(c.sinks);
+    const size_t bytes = window ? api.fwd_window_workspace_bytes(&p, window, sinks, 0) : api.fwd_workspace_bytes(&p);
+    Tensor ws;
+    if (bytes) {
+      ws = empty({static_cast<int64_t>(bytes)}, at::kByte, q);
+      p.workspace = ws.data_ptr();
+      p.workspace_bytes = bytes;
     }
+    if (window) check(api.fwd_window(&p, window, sinks, nullptr, nullptr, 0, stream), "fdma_fwd_window");
+    else check(api.fwd(&p, stream), "fdma_fwd");
   }
   if (grad) {
     auto node = std::shared_ptr<AttnBackward>(new AttnBackward(), torch::autograd::deleteNode);

@@ -68,6 +68,7 @@ EXPORTED_SYMBOLS = (
     "fdma_bwd",
     "fdma_fwd_varlen",
     "fdma_bwd_varlen",
+    "fdma_fwd_window_workspace_bytes",
     "fdma_fwd_window",
     "fdma_bwd_window_workspace_bytes",
     "fdma_bwd_window",
@@ -179,6 +180,8 @@ def load():
     lib.fdma_bwd_workspace_bytes.argtypes = [POINTER(BwdParams)]
     lib.fdma_bwd.restype = c_int
     lib.fdma_bwd.argtypes = [POINTER(BwdParams), c_void_p]
+    lib.fdma_fwd_window_workspace_bytes.restype = c_size_t
+    lib.fdma_fwd_window_workspace_bytes.argtypes = [POINTER(FwdParams), c_int32, c_int32, c_int32]
     lib.fdma_fwd_window.restype = c_int
     lib.fdma_fwd_window.argtypes = [POINTER(FwdParams), c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p]
     lib.fdma_bwd_window_workspace_bytes.restype = c_size_t

@@ -160,6 +160,9 @@ def _window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
         lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
         p = _lib.FwdParams()
         _interface._fill_fwd(p, q, k, v, mask, None, out, lse, softmax_scale, True)
+        size = lib.fdma_fwd_window_workspace_bytes(ctypes.byref(p), window, sinks, 0)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), size
         _lib.check(lib.fdma_fwd_window(ctypes.byref(p), window, sinks, None, None, 0, _interface._stream_ptr(q.device)), "fdma_fwd_window")
     return out, lse
 

@@ -195,9 +195,11 @@ int fdma_bwd_varlen(const fdma_bwd_params* p, const int32_t* cu_q, const int32_t
  * the query at position t (query q of seqlen_q: q + seqlen_k - seqlen_q) only if t - k < window or k < sinks; window at least 1, sinks at
  * least 0, is_causal set. Tiles that no query of a tile sees are neither loaded nor multiplied. The mask is NULL or broadcast over the
  * queries, bias and key_pos are NULL. n > 0: packed sequences as above, positions within each, without a mask. Rows that see no key give 0
- * and LSE = +inf. The forward needs no workspace. Backward of packed sequences up to head dim 128; the sums have a fixed order.
+ * and LSE = +inf. The forward needs a workspace only for a single query (seqlen_q 1, dense), whose keys are split over CTAs. Backward of
+ * packed sequences up to head dim 128; the sums have a fixed order.
  * FDMA_ERR_UNSUPPORTED for layouts that the tcgen05 kernels do not take.
  */
+size_t fdma_fwd_window_workspace_bytes(const fdma_fwd_params* p, int32_t window, int32_t sinks, int32_t n);
 int fdma_fwd_window(const fdma_fwd_params* p, int32_t window, int32_t sinks, const int32_t* cu_q, const int32_t* cu_k, int32_t n, void* stream);
 size_t fdma_bwd_window_workspace_bytes(const fdma_bwd_params* p, int32_t window, int32_t sinks, int32_t n);
 int fdma_bwd_window(const fdma_bwd_params* p, int32_t window, int32_t sinks, const int32_t* cu_q, const int32_t* cu_k, int32_t n, void* stream);

@@ -57,6 +57,16 @@ def test_attention_refuses(cls, name, args, change, status):
     assert entry(name, ctypes.c_int)(None, 8, 0, None, None, 0, None) == BAD
 
 
+def test_workspace_of_the_forward_pass():
+    size = entry("fdma_fwd_window_workspace_bytes", ctypes.c_size_t)
+    assert size(None, 8, 0, 0) == 0
+    assert size(ctypes.byref(params(_lib.FwdParams)), 8, 4, 0) == 0  # several queries
+    one = params(_lib.FwdParams, seqlen_q=1, seqlen_k=1 << 20)
+    for window, sinks, n in ((0, 0, 0), (8, -1, 0), (8, 0, -1), (8, 4, 1)):
+        assert size(ctypes.byref(one), window, sinks, n) == 0
+    assert size(ctypes.byref(one), 1 << 20, 0, 0) > 0  # the keys are split over more CTAs than a cluster has
+
+
 def test_workspace_of_the_backward_pass():
     size = entry("fdma_bwd_window_workspace_bytes", ctypes.c_size_t)
     assert size(None, 8, 0, 0) == 0

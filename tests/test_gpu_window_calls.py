@@ -60,6 +60,33 @@ def test_other_head_dims_and_lse(d, masked):
     check([out, *torch.autograd.grad(out, (q, k, v), dout)], *reference(q, k, v, 40, 2, mask, dout=dout))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("heads", [None, "one", "kv", "query"])
+@pytest.mark.parametrize("B,Sk,H,Hk,d,window,sinks", [(1, 1, 2, 1, 64, 1, 0), (2, 700, 4, 2, 128, 1, 0), (3, 700, 4, 2, 128, 300, 4), (1, 9000, 16, 1, 64, 4096, 130),
+                                                     (2, 20000, 2, 2, 96, 15000, 3), (2, 300, 2, 1, 256, 20, 270), (3, 333, 6, 2, 72, 40, 293), (1, 500, 2, 1, 128, 499, 0)])
+def test_single_tokens(B, Sk, H, Hk, d, window, sinks, heads, dtype):
+    """One query of each head, at the last position, from training and while serving."""
+    q, k, v, dout = tensors(B, 1, Sk, H, Hk, d, dtype)
+    mask = None if heads is None else padding(B, Sk, {"one": 1, "kv": Hk, "query": H}[heads])
+    if d > 128 and heads == "query":
+        q, k, v = (x.detach() for x in (q, k, v))
+        want, off = reference(q, k, v, window, sinks, mask)
+        check([window_func(q, k, v, window, sinks, attn_mask=mask)], want, off)
+        return
+    check(step(q, k, v, dout, window, sinks, attn_mask=mask), *reference(q, k, v, window, sinks, mask, dout=dout))
+    with torch.no_grad():
+        out, lse, _ = window_func(q, k, v, window, sinks, attn_mask=mask, return_attn_probs=True)
+        assert torch.equal(out, window_func(q, k, v, window, sinks, attn_mask=mask))
+        j = torch.arange(Sk, device="cuda")
+        seen = ((Sk - 1 - j < window) | (j < sinks))[None, None]
+        if mask is not None:
+            seen = seen & mask[:, :, 0].repeat_interleave(H // mask.shape[1], 1)
+        x = torch.einsum("bhd,bkhd->bhk", q[:, 0].double(), k.double().repeat_interleave(H // Hk, 2)) * d ** -0.5
+        want = x.masked_fill(~seen, -torch.inf).logsumexp(-1)
+        some = seen.any(-1).expand_as(want)
+        assert (lse[:, :, 0].double() - want)[some].abs().max() <= 3e-5 and bool((lse[:, :, 0][~some] == torch.inf).all())
+
+
 @pytest.mark.parametrize("scale", [0.0, 0.3, 3.0])
 def test_scales(scale):
     q, k, v, dout = tensors(1, 200, 200, 2, 1, 64, torch.bfloat16)
