@@ -175,6 +175,7 @@ __device__ __forceinline__ Peak of_lane(const Peak& x, int lane) {
   return Peak{__shfl_sync(0xffffffffu, x.m, lane), __shfl_sync(0xffffffffu, x.z, lane)};
 }
 
+template <bool kWindow>
 __device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
   const fdma_cache& c = a.p.c;
   Request q;
@@ -185,7 +186,8 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int r) {
   q.chunks = max(0, chunk1 - chunk0);
   q.rows = q.chunks ? min(q.n, a.p.max_seqlen_q) * a.group : 0;  // no chunks: refused
   if (a.prompts && q.n >= kPromptTokens && *a.prompts == 0) q.rows = -1;
-  q.chunks = a.list_chunks ? a.list_chunks : min(q.chunks, a.unit_chunks);
+  if (a.list_chunks) q.chunks = a.list_chunks;
+  else if (kWindow) q.chunks = min(q.chunks, a.unit_chunks);
   return q;
 }
 
@@ -224,13 +226,14 @@ struct Held {
 struct Cursor {
   int r, hk, tile;
 };
+template <bool kWindow>
 struct Units {
   const AttnArgs& a;
   const Held* held;  // null: too many requests
   __device__ const int32_t* pre() const { return held ? held->pre : a.pre; }
   __device__ int64_t total() const { return static_cast<int64_t>(pre()[a.p.c.requests]) * a.p.c.h_k; }
   __device__ Request request(int r) const {
-    if (!held) return load_request(a, r);
+    if (!held) return load_request<kWindow>(a, r);
     return Request{held->token0[r], held->n[r], held->length[r], held->rows[r], held->chunks[r]};
   }
   __device__ Unit of(const Cursor& x, const Request& q) const {
@@ -278,13 +281,14 @@ struct Units {
   }
 };
 // All threads of a CTA of at least 128.
-__device__ __forceinline__ Units make_units(const AttnArgs& a, Held& h) {
+template <bool kWindow>
+__device__ __forceinline__ Units<kWindow> make_units(const AttnArgs& a, Held& h) {
   const int R = a.p.c.requests;
-  if (R > kHeld) return Units{a, nullptr};
+  if (R > kHeld) return Units<kWindow>{a, nullptr};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int w = 0;
   if (tid < R) {
-    const Request q = load_request(a, tid);
+    const Request q = load_request<kWindow>(a, tid);
     h.token0[tid] = q.token0; h.n[tid] = q.n; h.length[tid] = q.length; h.rows[tid] = q.rows; h.chunks[tid] = q.chunks;
     w = q.chunks * tiles_of(a, q.rows);
   }
@@ -301,7 +305,7 @@ __device__ __forceinline__ Units make_units(const AttnArgs& a, Held& h) {
     if (tid == 0) h.pre[0] = 0;
   }
   __syncthreads();
-  return Units{a, &h};
+  return Units<kWindow>{a, &h};
 }
 // The same of a CTA that knows its unit.
 struct OneUnit {
@@ -315,13 +319,14 @@ struct OneUnit {
   }
   __device__ void advance(Cursor& at, Request&) const { at.r = a.p.c.requests; }
 };
+template <bool kWindow>
 __device__ __forceinline__ OneUnit make_one_unit(const AttnArgs& a) {
   const int slot = static_cast<int>(blockIdx.x) / a.cluster, per_request = a.p.c.h_k * a.tiles;
   Cursor x;
   x.r = slot / per_request;
   x.hk = (slot - x.r * per_request) / a.tiles;
   x.tile = slot - (x.r * a.p.c.h_k + x.hk) * a.tiles;
-  OneUnit u{a, x, load_request(a, x.r)};
+  OneUnit u{a, x, load_request<kWindow>(a, x.r)};
   if (a.list_chunks && a.p.kept_count) {
     const int kept = a.p.kept_count[x.r * a.p.count_batch_stride + x.hk * a.p.count_head_stride];
     u.q.chunks = (max(0, min(kept, a.p.kept_capacity)) + kChunk - 1) / kChunk;
@@ -410,8 +415,8 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   if (kGather && c.d < D)  // columns beyond the head dim stay zero in every stage
     for (int i = tid; i < L::kStages * L::kStageBytes / 16; i += L::kThreads) reinterpret_cast<uint4*>(smem + L::kRing)[i] = make_uint4(0, 0, 0, 0);
   const auto units = [&] {
-    if constexpr (kCluster) return make_one_unit(a);
-    else return make_units(a, s_held);
+    if constexpr (kCluster) return make_one_unit<kWindow>(a);
+    else return make_units<kWindow>(a, s_held);
   }();
   if (kCluster && tid < ROWS) s_part[tid] = make_float4(kNone, 0.f, 0.f, 0.f);
   __syncthreads();
@@ -799,8 +804,7 @@ cache_attend_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               const float add = bias_log2(raw_to_f<kBf16>(raw_bias[nt][k >> 1][k & 1]));
               v = add == -CUDART_INF_F ? add : v + add;
             }
-            const int pos = pos0 + (k >> 1) * 8 + key;
-            if (!clean && (pos > newest[nt][k & 1] || behind(pos, nt, k) || meta.x == 0.f)) v = -CUDART_INF_F;
+            if (!clean && (pos0 + (k >> 1) * 8 + key > newest[nt][k & 1] || behind(pos0 + (k >> 1) * 8 + key, nt, k) || meta.x == 0.f)) v = -CUDART_INF_F;
           }
           d[nt][k] = ratio(nt, k);
           grows |= d[nt][k] > 0.f;
@@ -1089,7 +1093,7 @@ __global__ void __launch_bounds__(1024) cache_sums_kernel(const __grid_constant_
   for (int base = 0; base < R; base += 1024) {
     int x = 0;
     if (base + tid < R) {
-      const Request q = load_request(a, base + tid);
+      const Request q = load_request<true>(a, base + tid);
       x = q.chunks * tiles_of(a, q.rows);
     }
 #pragma unroll
@@ -1136,7 +1140,7 @@ __global__ void __launch_bounds__(128, D > 128 ? 4 : 8) cache_merge_kernel(const
     __syncthreads();
     r = s_request;
   }
-  const Units units{a, nullptr};
+  const Units<true> units{a, nullptr};
   const int64_t step = (static_cast<int64_t>(D) + 4) << a.row_shift;
   Request q{};
   if (r >= 0) q = units.request(r);
