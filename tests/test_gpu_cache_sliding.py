@@ -166,3 +166,30 @@ def test_refusals(dev):  # noqa: F811
                         (TypeError, dict(sliding_window=True)), (ValueError, dict(sliding_window=4, is_causal=False))):
         with pytest.raises(error):
             fsa.flash_sparse_attn_cache_func(q, cache, tables, step, **args)
+
+
+def test_compiled(dev):  # noqa: F811
+    tables, cache, step, q, _ = case(dev, [300, 70, 0], [4, 1, 40], 4, 2, 64, 16, torch.bfloat16)
+    want = fsa.flash_sparse_attn_cache_func(q, cache, tables, step, sliding_window=90, sink_tokens=20)
+    torch._dynamo.reset()
+    fn = torch.compile(lambda q: fsa.flash_sparse_attn_cache_func(q, cache, tables, step, sliding_window=90, sink_tokens=20), backend="aot_eager",
+                       fullgraph=True)
+    assert torch.equal(fn(q), want)
+
+
+def test_same_bits_every_time_beside_other_launches(dev):  # noqa: F811
+    tables, cache, step, q, _ = case(dev, [3000, 70, 0, 900], [4, 1, 300, 9], 8, 2, 128, 16, torch.bfloat16)
+
+    def run():
+        return fsa.flash_sparse_attn_cache_func(q, cache, tables, step, sliding_window=500, sink_tokens=4)
+
+    want = run()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    runs = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                runs.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in runs)

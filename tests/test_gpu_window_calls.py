@@ -338,3 +338,13 @@ def test_refusals():
             window_func(q, k, v, 8, 1)
     finally:
         set_kernel_path("auto")
+
+
+def test_packed_single_tokens():
+    """A batch of one query each, over keys of its own length."""
+    keys, window, sinks = [500, 1, 90, 3000], 64, 3
+    cu_q, cu_k = list(range(5)), [sum(keys[:i]) for i in range(5)]
+    q, k, v, dout = (x[0].detach().requires_grad_(i < 3) for i, x in enumerate(tensors(1, 4, cu_k[-1], 4, 2, 64, torch.bfloat16)))
+    cu = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (cu_q, cu_k)]
+    out = varlen_func(q, k, v, *cu, 1, max(keys), window, sinks)
+    check([out, *torch.autograd.grad(out, (q, k, v), dout)], *packed_reference(q, k, v, cu_q, cu_k, window, sinks, dout))
