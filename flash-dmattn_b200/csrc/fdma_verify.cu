@@ -371,6 +371,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_consta
   const float temperature = p.temperatures ? p.temperatures[r] : p.temperature;
   const bool lead = rank == 0 && tid == 0;
   if (n == 0 || (p.granted && !p.granted[r])) {  // (the whole cluster agrees)
+    // A call may be made of such requests alone. It does not end before rows_kernel, whose parts lie in scratch that the caller has back then.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (lead) {
       p.accepted[r] = 0;
       p.next_tokens[r] = -1;
@@ -692,7 +694,7 @@ int launch(const VerifyArgs& a, cudaStream_t stream) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its CTAs look up the drafts while the last rows are streamed
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = a.p.tokens > 0 ? 2 : 1;  // (without rows what runs before it is somebody else's)
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, a));
 }
 template <typename T>
