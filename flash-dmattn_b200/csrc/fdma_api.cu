@@ -98,6 +98,12 @@ Window window_of(const fdma_fwd_params& p, int32_t window, int32_t sinks) {
   w.sinks = sinks < p.seqlen_k ? sinks : p.seqlen_k;
   return w;
 }
+// The backward's: none where it hides nothing, so that few queries over many keys are split as without a window. (128 queries over 65536 keys, 8
+// heads over 2, d = 128: 215 us, as a window 934.)
+Window backward_window_of(const fdma_fwd_params& p, int32_t window, int32_t sinks, int32_t n) {
+  const Window w = window_of(p, window, sinks);
+  return n == 0 && !p.mask && static_cast<int64_t>(w.keys) + w.sinks >= p.seqlen_k ? Window{} : w;
+}
 // Normalised copy: absent mask/bias get head count 1 so head-ratio arithmetic never divides by zero, and
 // causal is dropped for single-query calls (flash_api.cpp:441).
 fdma_fwd_params normalise(const fdma_fwd_params& in) {
@@ -352,7 +358,7 @@ size_t fdma_bwd_window_workspace_bytes(const fdma_bwd_params* pp, int32_t window
   if (!pp || window <= 0 || sinks < 0 || n < 0 || validate_bwd(*pp)) return 0;
   fdma_bwd_params p = *pp;
   p.f = normalise_window(pp->f);
-  const Window w = window_of(p.f, window, sinks);
+  const Window w = backward_window_of(p.f, window, sinks, n);
   return tc_bwd_window_supported(p, w, n) ? tc_bwd_window_workspace_bytes(p, w, n) : 0;
 }
 
@@ -365,7 +371,7 @@ int fdma_bwd_window(const fdma_bwd_params* pp, int32_t window, int32_t sinks, co
   if (st) return st;
   fdma_bwd_params p = *pp;
   p.f = normalise_window(pp->f);
-  const Window w = window_of(p.f, window, sinks);
+  const Window w = backward_window_of(p.f, window, sinks, n);
   if (!tc_bwd_window_supported(p, w, n)) return FDMA_ERR_UNSUPPORTED;
   return tc_bwd_window(p, static_cast<cudaStream_t>(stream_), PackedSeqs{cu_q, cu_k, n}, w);
 }
