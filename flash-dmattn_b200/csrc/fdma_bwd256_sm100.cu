@@ -729,7 +729,7 @@ Plan256 plan256(const fdma_bwd_params& bp, const Window& window) {
   Plan256 pl;
   pl.sq_r = static_cast<int>(round_up(p.seqlen_q, kBM));
   pl.nsplit = window.keys ? 1 : pick_nsplit256(p);
-  pl.sink_rows = window.keys ? std::min(window.sinks, p.seqlen_k) : 0;
+  pl.sink_rows = window.keys && p.seqlen_k >= window.keys + kBN ? std::min(window.sinks, p.seqlen_k) : 0;  // (otherwise no query is beyond a tile's)
   pl.sink_tiles = (pl.sink_rows + kBN - 1) / kBN;
   pl.far_rows = kFarRows;
   while (pl.far_rows < p.seqlen_q / 2 && static_cast<int64_t>(pl.sink_tiles) * p.h_k * p.b * (p.seqlen_q / pl.far_rows) > kFarCtas) pl.far_rows *= 2;

@@ -32,6 +32,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fdma_internal.h"
 #include "fdma_packed.cuh"
@@ -56,7 +57,7 @@ constexpr int kMaxBits = 4096;   // 64-key tiles the activity bits of a row-pass
 constexpr int kMaxHeads = 4096;  // query heads of a group whose activity differs from head to head
 // Sliding windows: queries beyond the window that a CTA works on for a tile of sink keys (such a tile is seen by all queries behind it, the
 // others by window + 128 of them), or that times a power of two where the CTAs would be more than kFarCtas: by then every SM has many of
-// them, and each leaves an fp32 row per sink, head and 16-bit row.
+// them, and each leaves an fp32 row per sink and kv head, of dV and of dK.
 constexpr int kFarRows = 2048, kFarCtas = 4096;
 constexpr int kDbHeads = 16;    // query heads of a group whose dBias sums have room in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
@@ -101,11 +102,17 @@ struct BwdRowsParams {
   // items walk the sinks' and the window's key tiles, numbered without the gap between. 10 d products per pair that is seen and head, of which
   // S and dP are formed twice; 32 heads over 8, d = 128, bf16: 32768 queries, 2048 keys + 4 sinks 4400 us (625 TFLOP/s counted once, 875 as
   // issued), 8192 queries: 1024 keys 585 us, 128 + 4 sinks 282, 1 key 199. Bound by the softmax arithmetic, narrow windows by the CTAs' set-up.
-  // Where a sequence has far queries, near and far leave fp32 sums of the sinks' rows, which sinks_kernel adds up in their order:
-  // [2: dV, dK][near of each sequence or batch element, then a place for each part of far_rows queries][h_k][sink_rows][D]
+  // Where a sequence has far queries, near and far leave fp32 sums of the sinks' rows, which sinks_kernel adds up in their order: the near ones
+  // where the tile's moved sums lie, the far ones in far_sums [2: dV, dK][h_k][far_total][D], from far_place on, a tile's rows as move_sums lays
+  // them out.
   Window window;
-  float* sink_sums;
-  int sink_rows, sink_tiles, near_units, far_slots, far_rows, n_far_ctas;
+  float* far_sums;
+  int sink_rows, sink_tiles, far_slots, far_rows, n_far_ctas, far_total;
+  // Packed sequences, first parts: a sequence with far queries has more than far_keys = window + 127 keys, so that its first key's number over
+  // that is its own. sink_rows for each such number, or a row for each key where those are fewer: scratch goes with the tokens, however many
+  // sequences and sinks there are.
+  int far_keys, first_rows;  // first_rows: of all first parts
+  bool first_by_key, sinks_by_key;
   int n_tiles;       // key tiles (packed: places for them)
   int q_tiles;       // row-pass tiles (packed: places for them)
   int nsplit;        // query-range splits per key tile
@@ -246,9 +253,38 @@ __device__ __forceinline__ int near_end(int key0, int coff, const Window& window
 __device__ __forceinline__ bool far_part(int key0, int key_end, int q_lo, int q_hi, int coff, const Window& window) {
   return key0 < key_end && q_lo < q_hi && q_hi > near_end(key0, coff, window);
 }
-// Where the far CTAs' rows begin in dkv_sums, behind the near ones' (half: dV, dK)
-__device__ __forceinline__ int64_t far_rows_at(const BwdRowsParams& p, int half, int key_tiles) {
-  return static_cast<int64_t>(2) * p.b * p.h_k * key_tiles * kBN + static_cast<int64_t>(half) * p.n_far_ctas * kBN;
+// The row from which on a part of far_rows queries has its sinks' sums in far_sums. unit: batch element
+template <bool packed>
+__device__ __forceinline__ int far_place(const BwdRowsParams& p, int unit, int first_key, int first_query, int part) {
+  if (!packed) return (unit * p.far_slots + part) * p.sink_rows;
+  if (part > 0) return p.first_rows + (first_query / p.far_rows + part - 1) * p.sink_rows;  // (no other sequence has part of these)
+  return p.first_by_key ? first_key : first_key / p.far_keys * p.sink_rows;
+}
+// What a far CTA works on: tile n of a sequence's sinks, and a part of its queries.
+struct FarTile {
+  int key0, key_end, q_lo, q_hi, coff, place;
+  bool any;  // whether there are such queries
+};
+template <bool packed>
+__device__ __forceinline__ FarTile far_tile(const BwdRowsParams& p, int item) {
+  FarTile f;
+  const int n = item % p.sink_tiles, slot = item / (p.sink_tiles * p.h_k) % p.far_slots, b = item / (p.sink_tiles * p.h_k * p.far_slots);
+  int2 keys = make_int2(0, p.seqlen_k), queries = make_int2(0, p.seqlen_q);
+  int part = slot;
+  if (packed) {
+    const PackedTile t = packed_tile(p.seqs.cu_q, p.seqs.n, p.seqlen_q, p.far_rows, slot);
+    keys = packed_range(p.seqs.cu_k, p.seqs.n, p.seqlen_k, t.seq);
+    queries = make_int2(t.begin, t.end);
+    part = t.tile;
+  }
+  f.key0 = keys.x + n * kBN;
+  f.key_end = min(keys.y, keys.x + p.window.sinks);
+  f.q_lo = queries.x + part * p.far_rows;
+  f.q_hi = min(queries.y, f.q_lo + p.far_rows);
+  f.coff = keys.y - queries.y;
+  f.any = far_part(f.key0, f.key_end, f.q_lo, f.q_hi, f.coff, p.window);
+  f.place = far_place<packed>(p, b, keys.x, queries.x, part) + n * kBN;
+  return f;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -279,16 +315,14 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
   int hk = blockIdx.x / per % p.h_k, b = blockIdx.x / per / p.h_k;
   // Sliding window: the far CTAs run first (the longest ones where there are several query heads). n: the tile of the sequence
   const bool far = kWindow && static_cast<int>(blockIdx.x) < p.n_far_ctas;
-  int slot = 0, sink_unit = -1;
+  bool has_sinks = far;  // whether rows of the tile are summed up in 32 bits
   if (kWindow) {
     split = 0;
     if (far) {
       item = blockIdx.x;
       n = item % p.sink_tiles;
       hk = item / p.sink_tiles % p.h_k;
-      slot = item / (p.sink_tiles * p.h_k) % p.far_slots;
       b = item / (p.sink_tiles * p.h_k * p.far_slots);
-      sink_unit = p.near_units + b * p.far_slots + slot;
     } else {
       item = blockIdx.x - p.n_far_ctas;
       n = item % p.n_tiles;
@@ -324,28 +358,21 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
     m_start = (causal ? max(q_lo, key0 - coff) : q_lo) / kBM;
     M64 = warp_uniform(q_lo < q_hi ? min(M64, (q_hi + kBM - 1) / kBM) : 0);
     n_in_seq = t.tile;
-    if (kWindow && t.seq >= 0 && t.seq < p.seqs.n && t.tile < p.sink_tiles) sink_unit = t.seq;
-  } else if (kWindow && !far && n < p.sink_tiles) {
-    sink_unit = b;
+    has_sinks = kWindow && t.seq >= 0 && t.seq < p.seqs.n && t.tile < p.sink_tiles;
+  } else if (kWindow && !far) {
+    has_sinks = n < p.sink_tiles;
   }
-  int behind = 0;  // where the near queries end and the far ones begin
+  int behind = 0, place = 0;  // where the near queries end and the far ones begin, row of far_sums
   if (kWindow) {
-    if (!far && sink_unit >= 0 && !far_part(key0, key_end, q_lo, q_hi, coff, p.window)) sink_unit = -1;  // nobody is beyond
+    if (!far && has_sinks) has_sinks = far_part(key0, key_end, q_lo, q_hi, coff, p.window);  // (false: nobody is beyond)
     if (far) {
-      if (packed) {
-        const PackedTile t = packed_tile(p.seqs.cu_q, p.seqs.n, Sq, p.far_rows, slot);
-        const int2 keys = packed_range(p.seqs.cu_k, p.seqs.n, Sk, t.seq);
-        key0 = keys.x + n * kBN;
-        key_end = min(keys.y, keys.x + p.window.sinks);
-        q_lo = t.begin + t.tile * p.far_rows;
-        q_hi = min(t.end, q_lo + p.far_rows);
-        coff = keys.y - t.end;
-      } else {
-        key_end = min(Sk, p.window.sinks);
-        q_lo = slot * p.far_rows;
-        q_hi = min(Sq, q_lo + p.far_rows);
-      }
-      if (!far_part(key0, key_end, q_lo, q_hi, coff, p.window)) return;  // (the whole CTA agrees)
+      const FarTile t = far_tile<packed>(p, blockIdx.x);
+      key0 = t.key0;
+      key_end = t.key_end;
+      q_lo = t.q_lo;
+      q_hi = t.q_hi;
+      coff = t.coff;
+      place = t.place;
       behind = near_end(key0, coff, p.window);
       m_start = max(q_lo, behind) / kBM;
       M64 = (q_hi + kBM - 1) / kBM;
@@ -559,9 +586,9 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
     // dV (team 0) and dK (team 1) out of tensor memory: 128 columns of this thread's key, in pieces that a warp stores in one go
     const uint32_t acc_addr = tmem_base + lane_addr + (half == 0 ? C::kAcc : kAcc2);
     const int rows = min(kBN, key_end - key0);
-    float4* const sums = reinterpret_cast<float4*>(p.dkv_sums) +
-                         (far ? far_rows_at(p, half, NT) + (blockIdx.x * kBN)
-                              : (((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key0) * (D / 4) + krow;
+    const int64_t sums_row = far ? (static_cast<int64_t>(half) * p.h_k + hk) * p.far_total + place
+                                 : (((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key0;
+    float4* const sums = reinterpret_cast<float4*>(far ? p.far_sums : p.dkv_sums) + sums_row * (D / 4) + krow;
     int moved = 0;  // how often
     auto move_sums = [&]() {
 #pragma unroll 1  // (little code: it lies in the loop over the steps)
@@ -707,15 +734,14 @@ __device__ __forceinline__ void key_pass(const BwdRowsParams& p, unsigned char* 
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = 0u;
         }
-        if (kWindow ? sink_unit >= 0 && n_in_seq * kBN + krow < p.window.sinks : p.dkv_part != nullptr) {
-          // fp32 partial: part[dv|dk][split][b][hk][key][d]
+        if (kWindow ? has_sinks && n_in_seq * kBN + krow < p.window.sinks : p.dkv_part != nullptr) {
+          // fp32 partial: part[dv|dk][split][b][hk][key][d]; sinks: as moved sums
           if ((packed || kWindow) && !key_ok) continue;  // (after the warp-wide load)
-          float* part = kWindow ? p.sink_sums + (((static_cast<int64_t>(half) * (p.near_units + p.b * p.far_slots) + sink_unit) * p.h_k + hk) *
-                                                     p.sink_rows + (n_in_seq * kBN + krow)) * D + c * 32
-                                : p.dkv_part + ((((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key) * D + c * 32;
+          float4* part = kWindow ? sums + c * 8 * rows
+                                 : reinterpret_cast<float4*>(p.dkv_part + ((((static_cast<int64_t>(half) * p.nsplit + split) * p.b + b) * p.h_k + hk) * (NT * kBN) + key) * D + c * 32);
 #pragma unroll
           for (int v4 = 0; v4 < 8; ++v4)
-            *reinterpret_cast<float4*>(part + v4 * 4) =
+            part[kWindow ? v4 * rows : v4] =
                 make_float4(__uint_as_float(r[v4 * 4 + 0]) * mul, __uint_as_float(r[v4 * 4 + 1]) * mul,
                             __uint_as_float(r[v4 * 4 + 2]) * mul, __uint_as_float(r[v4 * 4 + 3]) * mul);
         } else if (key_ok) {
@@ -1193,6 +1219,7 @@ __global__ void __launch_bounds__(kThreads, 1) bwd_rows_kernel(const __grid_cons
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const WaitCtl ctl{s_abort, p.status};
+  if (kWindow && static_cast<int>(blockIdx.x) < p.n_far_ctas && !far_tile<packed>(p, blockIdx.x).any) return;  // (the whole CTA agrees)
   if (tid == 0) {
     *s_abort = 0;
     mbar_init(bar.x_full, 1);
@@ -1245,29 +1272,43 @@ __global__ void __launch_bounds__(kThreads, 1) bwd_rows_kernel(const __grid_cons
 // have left, in the order of the queries. A warp per key row.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) sinks_kernel(const __grid_constant__ BwdRowsParams p) {
-  const int lane = threadIdx.x & 31, rows = p.sink_rows;
+  const int lane = threadIdx.x & 31;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int unit = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * rows)), hk = static_cast<int>(w / rows % p.h_k), row = static_cast<int>(w % rows);
-  if (unit >= p.near_units) return;
   const bool packed = p.seqs.cu_q != nullptr;
+  int unit, hk, row;  // sequence or batch element, kv head, key of it
   int2 keys = make_int2(0, p.seqlen_k), queries = make_int2(0, p.seqlen_q);
-  int first = p.near_units + unit * p.far_slots;
+  if (p.sinks_by_key) {
+    const int slots = packed_slots(p.seqlen_k, p.seqs.n, 1);
+    const PackedTile t = packed_tile(p.seqs.cu_k, p.seqs.n, p.seqlen_k, 1, static_cast<int>(w % slots));
+    unit = t.seq;
+    hk = static_cast<int>(w / slots);
+    row = t.tile;
+  } else {
+    row = static_cast<int>(w % p.sink_rows);
+    hk = static_cast<int>(w / p.sink_rows % p.h_k);
+    unit = static_cast<int>(w / (static_cast<int64_t>(p.h_k) * p.sink_rows));
+  }
+  if (unit < 0 || unit >= (packed ? p.seqs.n : p.b) || hk >= p.h_k || row >= p.sink_rows) return;
   if (packed) {
     keys = packed_range(p.seqs.cu_k, p.seqs.n, p.seqlen_k, unit);
     queries = packed_range(p.seqs.cu_q, p.seqs.n, p.seqlen_q, unit);
-    first = p.near_units + queries.x / p.far_rows + unit + 1;  // the sequence's first place
   }
   if (keys.x + row >= keys.y) return;
   const int key0 = keys.x + row / kBN * kBN, coff = keys.y - queries.y;
   if (!far_part(key0, key0 + 1, queries.x, queries.y, coff, p.window)) return;  // written by the CTA of the tile
-  const int64_t units = p.near_units + static_cast<int64_t>(p.b) * p.far_slots;
-  const int b = packed ? 0 : unit;
+  const int b = packed ? 0 : unit, NT = (p.seqlen_k + kBN - 1) / kBN;
+  const int near_rows = min(kBN, keys.y - key0), far_rows = min(kBN, min(keys.y, keys.x + p.window.sinks) - key0);
 #pragma unroll
   for (int x = 0; x < 2; ++x) {  // dV, dK
+    // numbers [lane * D / 32, + D / 32) of the row, in a tile's sums that begin at `tile`
+    using Vec = std::conditional_t<D == 128, float4, float2>;
+    auto load = [&](const float* tile, int rows, float (&y)[D / 32]) {
+      const Vec v = *reinterpret_cast<const Vec*>(tile + (static_cast<int64_t>(lane * (D / 32) / 4) * rows + row % kBN) * 4 + lane * (D / 32) % 4);
+      memcpy(y, &v, sizeof(v));
+    };
     float acc[D / 32];
-    auto at = [&](int64_t u) { return p.sink_sums + (((x * units + u) * p.h_k + hk) * rows + row) * D + lane * (D / 32); };
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = at(unit)[i];
+    load(p.dkv_sums + (((static_cast<int64_t>(x) * p.b + b) * p.h_k + hk) * (NT * kBN) + key0) * D, near_rows, acc);
+    const float* far = p.far_sums + ((static_cast<int64_t>(x) * p.h_k + hk) * p.far_total + row / kBN * kBN) * D;
     // parts that reach beyond the window: those from this one on. Eight are asked for at a time.
     const int parts = (queries.y - queries.x + p.far_rows - 1) / p.far_rows;
     int c0 = 0;
@@ -1275,13 +1316,15 @@ __global__ void __launch_bounds__(256) sinks_kernel(const __grid_constant__ BwdR
     for (; c0 < parts; c0 += 8) {
       float y[8][D / 32];
 #pragma unroll
+      for (int j = 0; j < 8; ++j) {  // (without a branch: the loads do not wait for one another)
+        const int c = min(c0 + j, parts - 1);
+        const int place = packed ? far_place<true>(p, b, keys.x, queries.x, c) : far_place<false>(p, b, 0, 0, c);
+        load(far + static_cast<int64_t>(place) * D, far_rows, y[j]);
+      }
+#pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) y[j][i] = c0 + j < parts ? at(first + c0 + j)[i] : 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] += y[j][i];
+        for (int i = 0; i < D / 32; ++i) acc[i] += c0 + j < parts ? y[j][i] : 0.f;
     }
     uint16_t* dst = x == 0 ? reinterpret_cast<uint16_t*>(p.dv) + b * p.dv_batch_stride + hk * p.dv_head_stride + static_cast<int64_t>(keys.x + row) * p.dv_row_stride
                            : reinterpret_cast<uint16_t*>(p.dk) + b * p.dk_batch_stride + hk * p.dk_head_stride + static_cast<int64_t>(keys.x + row) * p.dk_row_stride;
@@ -1299,7 +1342,8 @@ struct RowsPlan {
   int ranges;  // key ranges per row-pass tile
   bool part;  // dK, dV (and column sums) leave the kernel as fp32 partials
   size_t lse2_off, dsum_off, dq_off, dbias_off, sums_off, part_off, dbpart_off, sinks_off, total;
-  int sink_rows, sink_tiles, near_units, far_slots, far_rows;  // sliding window
+  int sink_rows, sink_tiles, far_slots, far_rows, far_keys, first_rows;  // sliding window
+  int64_t far_total;
 };
 
 // Query-range splits per key tile: one CTA per SM, as long as a split keeps 32 steps, and on to two per SM while it keeps 160. The row pass,
@@ -1357,22 +1401,29 @@ RowsPlan plan(const fdma_bwd_params& bp, const Window& window, int sequences) {
   pl.dbias_off = o;
   if (pl.dbias_mode == kDbAtomic) o += align256(static_cast<size_t>(bp.dbias_b) * bp.dbias_h * atomic_keys(bp) * 4);
   pl.nsplit = window.keys ? 1 : pick_nsplit(p);
-  pl.sink_rows = pl.sink_tiles = pl.near_units = pl.far_slots = 0;
+  pl.sink_rows = pl.sink_tiles = pl.far_slots = pl.first_rows = 0;
+  pl.far_total = 0;
   pl.far_rows = kFarRows;
-  if (window.keys && window.sinks) {
+  pl.far_keys = window.keys + kBN - 1;
+  if (window.keys && window.sinks && p.seqlen_k > pl.far_keys) {  // (otherwise nobody is beyond)
     pl.sink_rows = std::min(window.sinks, p.seqlen_k);
     pl.sink_tiles = (pl.sink_rows + kBN - 1) / kBN;
     while (pl.far_rows < p.seqlen_q / 2 && static_cast<int64_t>(pl.sink_tiles) * p.h_k * p.b * (p.seqlen_q / pl.far_rows) > kFarCtas) pl.far_rows *= 2;
-    pl.near_units = sequences ? sequences : p.b;
-    pl.far_slots = sequences ? packed_slots(p.seqlen_q, sequences, pl.far_rows) : (p.seqlen_q + pl.far_rows - 1) / pl.far_rows;
+    const int parts = (p.seqlen_q + pl.far_rows - 1) / pl.far_rows;
+    pl.far_slots = sequences ? packed_slots(p.seqlen_q, sequences, pl.far_rows) : parts;
+    if (sequences) {
+      pl.first_rows = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.seqlen_k / pl.far_keys) * pl.sink_rows, p.seqlen_k));
+      pl.far_total = pl.first_rows + static_cast<int64_t>(std::max(parts - 1, 0)) * pl.sink_rows;
+    } else {
+      pl.far_total = static_cast<int64_t>(p.b) * parts * pl.sink_rows;
+    }
   }
   pl.sums_off = o;
   const int64_t m_tiles = (p.seqlen_q + kBM - 1) / kBM;
-  if ((m_tiles + pl.nsplit - 1) / pl.nsplit * (p.h / p.h_k) > kKeyFlush)
-    o += align256((static_cast<size_t>(2) * pl.nsplit * p.b * p.h_k * round_up(p.seqlen_k, kBN) +
-                   static_cast<size_t>(2) * p.b * pl.far_slots * p.h_k * pl.sink_tiles * kBN) * pl.D * 4);
+  if (pl.sink_rows || (m_tiles + pl.nsplit - 1) / pl.nsplit * (p.h / p.h_k) > kKeyFlush)
+    o += align256(static_cast<size_t>(2) * pl.nsplit * p.b * p.h_k * round_up(p.seqlen_k, kBN) * pl.D * 4);
   pl.sinks_off = o;
-  o += align256(static_cast<size_t>(2) * (pl.near_units + p.b * pl.far_slots) * p.h_k * pl.sink_rows * pl.D * 4);
+  o += align256(static_cast<size_t>(2) * pl.far_total * p.h_k * pl.D * 4);
   pl.part = pl.nsplit > 1 || bp.scatter_pos != nullptr;
   pl.part_off = pl.dbpart_off = o;
   if (pl.part) {
@@ -1465,8 +1516,14 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   kp.n_tiles = seqs.cu_q ? packed_slots(p.seqlen_k, seqs.n, kBN) : (p.seqlen_k + kBN - 1) / kBN;
   kp.q_tiles = seqs.cu_q ? packed_slots(p.seqlen_q, seqs.n, kBN) : (p.seqlen_q + kBN - 1) / kBN;
   kp.window = window;
-  kp.sink_sums = reinterpret_cast<float*>(ws + pl.sinks_off);
-  kp.sink_rows = pl.sink_rows; kp.sink_tiles = pl.sink_tiles; kp.far_rows = pl.far_rows; kp.near_units = pl.near_units; kp.far_slots = pl.far_slots;
+  if (pl.far_total > 0x7FFFFFFF) return FDMA_ERR_TOO_LARGE;
+  kp.far_sums = reinterpret_cast<float*>(ws + pl.sinks_off);
+  kp.sink_rows = pl.sink_rows; kp.sink_tiles = pl.sink_tiles; kp.far_rows = pl.far_rows; kp.far_slots = pl.far_slots;
+  kp.far_keys = pl.far_keys; kp.first_rows = pl.first_rows; kp.far_total = static_cast<int>(pl.far_total);
+  kp.first_by_key = pl.first_rows == p.seqlen_k;
+  // rows that sinks_kernel looks at: every sequence's, or all keys where those are fewer
+  const int64_t all_sinks = static_cast<int64_t>(seqs.cu_q ? seqs.n : p.b) * pl.sink_rows;
+  kp.sinks_by_key = seqs.cu_q && all_sinks > packed_slots(p.seqlen_k, seqs.n, 1);
   kp.n_far_ctas = pl.sink_tiles * p.h_k * pl.far_slots * p.b;
   kp.nsplit = pl.nsplit;
   kp.ranges = seqs.cu_q ? 1 : pl.ranges;
@@ -1492,7 +1549,7 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   if (e != cudaSuccess) return static_cast<int>(e);
   if (window.keys) {
     if (!pl.sink_tiles) return 0;
-    const int64_t rows = static_cast<int64_t>(pl.near_units) * p.h_k * pl.sink_rows;
+    const int64_t rows = (kp.sinks_by_key ? packed_slots(p.seqlen_k, seqs.n, 1) : all_sinks) * p.h_k;
     sinks_kernel<D, kBf16><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(kp);
     return static_cast<int>(cudaGetLastError());
   }
