@@ -35,7 +35,8 @@ def flash_sparse_attention_forward(
     **kwargs,
 ):
     """kv_cache (keyword, not in the reference): the layer's `CachedLayer`; query, key and value are then the step's new tokens
-    (1, H, tokens, d) of all requests, attention_bias is ({1|requests}, {1|Hk|H}, 1, keys), and attention runs over the 8-bit cache."""
+    (1, H, tokens, d) of all requests, attention_bias is ({1|requests}, {1|Hk|H}, 1, keys), and attention runs over the 8-bit cache.
+    sliding_window (keyword, as models hand it over): a query sees the last so many keys, its own among them."""
     query_len, key_len = query.shape[2], key.shape[2]
     if any(dim == 0 for dim in query.shape):
         raise ValueError("FlashSparseAttention does not support inputs with a zero dimension; check the input "
@@ -52,7 +53,8 @@ def flash_sparse_attention_forward(
         if softcap:
             raise NotImplementedError("softcap > 0 is not built into the B200 kernels")
         return _cached_attention_forward(query, key, value, attention_mask, attention_bias, kv_cache, softmax_scale=scaling,
-                                         window_size=window_size, is_causal=is_causal, target_dtype=target_dtype), None
+                                         window_size=window_size, is_causal=is_causal, target_dtype=target_dtype,
+                                         sliding_window=kwargs.get("sliding_window")), None
     out = _flash_sparse_attention_forward(
         query, key, value, attention_mask, attention_bias,
         query_length=query_len, key_length=key_len, is_causal=is_causal, softmax_scale=scaling, softcap=softcap,

@@ -15,6 +15,9 @@ reference's varlen kernel as well. Here small packs (Tq x Tk up to `_PACKED_MASK
 sequence under a per-query visibility mask (same example, and causal inside the example with the bottom-right
 alignment of its own lengths), which the full-range kernels skip tile by tile -- one launch however many examples
 there are; larger packs go through `flash_sparse_attn_varlen_func`, which runs every example as a zero-copy slice.
+
+`sliding_window`, which models hand over for their windowed layers (the reference drops it): a query sees the last so many keys, its own among
+them. Dense, padded and packed calls go to the window's operators; with a bias, or a mask per query, the window becomes part of the mask.
 """
 import math
 import os
@@ -26,6 +29,7 @@ from ..cache import BlockTables, CacheStep, QuantizedCache, cache_append, flash_
 from ..flash_sparse_attn_interface import flash_sparse_attn_func, flash_sparse_attn_varlen_func
 from ..rotary import RotaryFrequencies
 from ..utils.mask import create_kept_keys, create_mask
+from ..window import check_window, flash_sparse_attn_window_func, flash_sparse_attn_window_varlen_func
 
 
 def fsa_peft_integration_check(q, k, v, bias, target_dtype: Optional[torch.dtype] = None):
@@ -70,6 +74,20 @@ def _packed_visibility(cu_q: torch.Tensor, cu_k: torch.Tensor, total_q: int, tot
     return visible
 
 
+def _window_that_hides(sliding_window: Optional[int], keys: int, is_causal: bool, softcap: Optional[float]) -> Optional[int]:
+    """The window, or None where `keys` keys are all in it."""
+    if sliding_window is None:
+        return None
+    check_window(sliding_window, 0)
+    if sliding_window >= keys:
+        return None
+    if not is_causal:
+        raise NotImplementedError("sliding_window is built for causal attention only")
+    if softcap:
+        raise NotImplementedError("softcap > 0 is not built into the B200 kernels")
+    return sliding_window
+
+
 def _flash_sparse_attention_forward(
     query_states: torch.Tensor,
     key_states: torch.Tensor,
@@ -90,9 +108,12 @@ def _flash_sparse_attention_forward(
     max_length_k: Optional[int] = None,
     target_dtype: Optional[torch.dtype] = None,
     implementation: Optional[str] = None,
+    sliding_window: Optional[int] = None,
     **kwargs,
 ):
-    """query/key/value (B, S, H, d). Returns (B, Sq, H, d). Same argument list as the reference function."""
+    """query/key/value (B, S, H, d). Returns (B, Sq, H, d). Same argument list as the reference function, and `sliding_window`: of the keys
+    that a call without it sees, a query sees the last so many (with `window_size`: those of the kept keys). A single query, which sees all keys,
+    is at the last of them."""
     if attention_mask is not None and attention_mask.dim() == 2 and attention_bias is not None:
         raise ValueError("If shape of attention_mask is (batch_size, seq_len), attention_bias has to be None.")
     padded = attention_mask is not None and attention_mask.dim() == 2
@@ -114,10 +135,16 @@ def _flash_sparse_attention_forward(
         q1 = query_states.reshape(1, -1, query_states.size(-2), query_states.size(-1))
         k1 = key_states.reshape(1, -1, key_states.size(-2), key_states.size(-1))
         v1 = value_states.reshape(1, -1, value_states.size(-2), value_states.size(-1))
-        if q1.size(1) * k1.size(1) > _PACKED_MASK_LIMIT:
+        window = _window_that_hides(sliding_window, k1.size(1), is_causal, softcap)
+        if window is not None or q1.size(1) * k1.size(1) > _PACKED_MASK_LIMIT:
             if max_length_q is None or max_length_k is None:
                 max_length_q = int((cu_seq_lens_q[1:] - cu_seq_lens_q[:-1]).max())
                 max_length_k = int((cu_seq_lens_k[1:] - cu_seq_lens_k[:-1]).max())
+            if window is not None:
+                cu = [x.to(device=q1.device, dtype=torch.int32) for x in (cu_seq_lens_q, cu_seq_lens_k)]
+                out = flash_sparse_attn_window_varlen_func(q1[0], k1[0], v1[0], *cu, max_length_q, max_length_k, window,
+                                                           softmax_scale=softmax_scale, deterministic=deterministic)
+                return out.view(B, -1, out.size(-2), out.size(-1))
             out = flash_sparse_attn_varlen_func(q1[0], k1[0], v1[0], cu_seq_lens_q, cu_seq_lens_k, max_length_q,
                                                 max_length_k, softmax_scale=softmax_scale, is_causal=is_causal,
                                                 softcap=softcap, deterministic=deterministic)
@@ -140,10 +167,18 @@ def _flash_sparse_attention_forward(
             query_valid = None
         else:
             query_valid = key_valid[:, -query_length:]  # left padding, as the reference assumes
-        out = flash_sparse_attn_func(
-            query_states, key_states, value_states, key_valid[:, None, None, :], None,
-            softmax_scale=softmax_scale, is_causal=is_causal and query_length != 1,
-            softcap=softcap, deterministic=deterministic)
+        window = _window_that_hides(sliding_window, key_states.shape[1], is_causal or query_length == 1, softcap)
+        if window is not None and query_length == 1:  # the last keys that are there, wherever the padding is
+            key_valid = key_valid & (key_valid.flip(-1).cumsum(-1).flip(-1) <= window)
+            window = None
+        if window is not None:
+            out = flash_sparse_attn_window_func(query_states, key_states, value_states, window, attn_mask=key_valid[:, None, None, :],
+                                                softmax_scale=softmax_scale, deterministic=deterministic)
+        else:
+            out = flash_sparse_attn_func(
+                query_states, key_states, value_states, key_valid[:, None, None, :], None,
+                softmax_scale=softmax_scale, is_causal=is_causal and query_length != 1,
+                softcap=softcap, deterministic=deterministic)
         out = out[0] if isinstance(out, tuple) else out
         if query_valid is not None:
             out = torch.where(query_valid[:, :, None, None], out, torch.zeros((), dtype=out.dtype, device=out.device))
@@ -153,6 +188,17 @@ def _flash_sparse_attention_forward(
         attention_mask = create_mask(
             attention_bias, attention_mask, batch_size=query_states.size(0), query_len=query_length,
             key_len=key_length, window_size=window_size, min_dtype=torch.finfo(attention_bias.dtype).min)
+    window = _window_that_hides(sliding_window, key_states.shape[1], is_causal or query_length == 1, softcap)
+    if window is not None:
+        Sq, Sk, mask = query_states.shape[1], key_states.shape[1], attention_mask
+        # (gradients at head dims above 128 take no mask of its own for each query head beside a window)
+        if attention_bias is None and (mask is None or (mask.dim() == 4 and mask.shape[2] == 1 and mask.shape[1] in (1, key_states.shape[2]))):
+            return flash_sparse_attn_window_func(query_states, key_states, value_states, window, attn_mask=mask, softmax_scale=softmax_scale,
+                                                 deterministic=deterministic)
+        if mask is not None and mask.dtype != torch.bool:
+            raise RuntimeError("attention_mask must be a bool tensor")
+        inside = torch.arange(Sk, device=query_states.device) > torch.arange(Sk - Sq, Sk, device=query_states.device)[:, None] - window
+        attention_mask = inside[None, None] if mask is None else mask[..., :Sk] & inside
     out = flash_sparse_attn_func(
         query_states, key_states, value_states, attention_mask, attention_bias,
         softmax_scale=softmax_scale, is_causal=is_causal and query_length != 1,
@@ -173,10 +219,10 @@ class CachedLayer(NamedTuple):
 
 def _cached_attention_forward(query_states, key_states, value_states, attention_mask, attention_bias, kv_cache: CachedLayer,
                               softmax_scale: Optional[float] = None, window_size: Optional[int] = None, is_causal: bool = True,
-                              target_dtype: Optional[torch.dtype] = None):
+                              target_dtype: Optional[torch.dtype] = None, sliding_window: Optional[int] = None):
     """The step's keys and values (1, tokens, Hk, d) go into the cache, and its queries (1, tokens, H, d) attend over it: everything, or
     with a bias of more than `window_size` keys the `window_size` keys of each request that each row of the bias ranks highest: one
-    row for all heads, or one per kv head or query head. Returns (1, tokens, H, d). What the attention would refuse is refused here,
+    row for all heads, or one per kv head or query head; of these those in the `sliding_window`. Returns (1, tokens, H, d). What the attention would refuse is refused here,
     before anything is written."""
     if attention_mask is not None:
         raise ValueError("attention over a cache takes no attention_mask: the requests' lengths are in the step.")
@@ -187,6 +233,7 @@ def _cached_attention_forward(query_states, key_states, value_states, attention_
     R, H, Hk = step.lengths.shape[0], q.shape[1], k.shape[1]
     if Hk == 0 or H % Hk:
         raise ValueError("attention over a cache takes as many query heads for each kv head.")
+    window = _window_that_hides(sliding_window, tables.table.shape[-1] * tables.block_size, is_causal, None)
     if any(bound is not None and bound < 0 for bound in (max_q, max_k)):
         raise ValueError("max_seqlen_q and max_seqlen_k must not be negative.")
     if bias is not None:
@@ -210,5 +257,5 @@ def _cached_attention_forward(query_states, key_states, value_states, attention_
     turned = cache_append(cache, tables, step, k, v, query=q if frequencies is not None else None, frequencies=frequencies)
     q = q if turned is None else turned
     out = flash_sparse_attn_cache_func(q, cache, tables, step, attn_mask=kept, attn_bias=bias, softmax_scale=softmax_scale,
-                                       is_causal=is_causal, max_seqlen_q=max_q, max_seqlen_k=max_k)
+                                       is_causal=is_causal, max_seqlen_q=max_q, max_seqlen_k=max_k, sliding_window=window)
     return out[None]
