@@ -359,7 +359,7 @@ size_t fdma_bwd_window_workspace_bytes(const fdma_bwd_params* pp, int32_t window
   fdma_bwd_params p = *pp;
   p.f = normalise_window(pp->f);
   const Window w = backward_window_of(p.f, window, sinks, n);
-  return tc_bwd_window_supported(p, w, n) ? tc_bwd_window_workspace_bytes(p, w, n) : 0;
+  return tc_bwd_window_supported(p, n) ? tc_bwd_window_workspace_bytes(p, w, n) : 0;
 }
 
 int fdma_bwd_window(const fdma_bwd_params* pp, int32_t window, int32_t sinks, const int32_t* cu_q, const int32_t* cu_k, int32_t n, void* stream_) {
@@ -372,7 +372,7 @@ int fdma_bwd_window(const fdma_bwd_params* pp, int32_t window, int32_t sinks, co
   fdma_bwd_params p = *pp;
   p.f = normalise_window(pp->f);
   const Window w = backward_window_of(p.f, window, sinks, n);
-  if (!tc_bwd_window_supported(p, w, n)) return FDMA_ERR_UNSUPPORTED;
+  if (!tc_bwd_window_supported(p, n)) return FDMA_ERR_UNSUPPORTED;
   return tc_bwd_window(p, static_cast<cudaStream_t>(stream_), PackedSeqs{cu_q, cu_k, n}, w);
 }
 

@@ -113,6 +113,7 @@ struct BwdRowsParams {
   // sequences and sinks there are.
   int far_keys, first_rows;  // first_rows: of all first parts
   bool first_by_key, sinks_by_key;
+  bool mask_bits;  // a mask, whose tiles with a kept key the row pass has room for; beyond, it works on every tile that a query tile sees
   int n_tiles;       // key tiles (packed: places for them)
   int q_tiles;       // row-pass tiles (packed: places for them)
   int nsplit;        // query-range splits per key tile
@@ -805,7 +806,7 @@ __device__ __forceinline__ void row_pass(const BwdRowsParams& p, unsigned char* 
   auto mask_of = [&](int h) {
     return p.mask ? p.mask + b * p.mask_batch_stride + (p.h_mask == p.h ? h : (p.h_mask == p.h_k ? h / G : 0)) * p.mask_head_stride : nullptr;
   };
-  const bool use_bits = p.mask != nullptr;
+  const bool use_bits = kWindow ? p.mask_bits : p.mask != nullptr;
   // Sliding window: the tiles of the sinks and those of the window, numbered without the gap between
   const int sink_subs = kWindow ? (min(p.window.sinks, sk) + kBM - 1) / kBM : 0;
   auto tile_of = [&](int m, int gap) { return kWindow && m >= sink_subs ? m + gap : m; };
@@ -1525,6 +1526,9 @@ int launch(const fdma_bwd_params& bp, const RowsPlan& pl, const PackedSeqs& seqs
   const int64_t all_sinks = static_cast<int64_t>(seqs.cu_q ? seqs.n : p.b) * pl.sink_rows;
   kp.sinks_by_key = seqs.cu_q && all_sinks > packed_slots(p.seqlen_k, seqs.n, 1);
   kp.n_far_ctas = pl.sink_tiles * p.h_k * pl.far_slots * p.b;
+  // the 64-key tiles that a query tile sees
+  const int64_t seen = (std::min(window.sinks, p.seqlen_k) + kBM - 1) / kBM + (std::min(window.keys, p.seqlen_k) + kBN) / kBM + 2;
+  kp.mask_bits = p.mask && std::min<int64_t>(seen, (p.seqlen_k + kBM - 1) / kBM) <= kMaxBits;
   kp.nsplit = pl.nsplit;
   kp.ranges = seqs.cu_q ? 1 : pl.ranges;
   kp.heads_per_cta = pick_heads_per_cta(static_cast<int64_t>(kp.q_tiles) * p.b * kp.ranges, p.h, window.keys > 0);
@@ -1620,13 +1624,10 @@ bool bwd_rows_taken_packed(const fdma_bwd_params& bp) { return bp.f.seqlen_k < 4
 
 size_t bwd_rows_workspace_bytes(const fdma_bwd_params& bp, const Window& window, int sequences) { return plan(bp, window, sequences).total; }
 
-bool tc_bwd_window_supported(const fdma_bwd_params& bp, const Window& window, int sequences) {
+bool tc_bwd_window_supported(const fdma_bwd_params& bp, int sequences) {
   const fdma_fwd_params& p = bp.f;
   if (bp.dbias || bp.scatter_pos || !tc_bwd_supported(bp)) return false;
-  if (tile_head_dim(p.d) == 256) return !sequences;
-  // the 64-key tiles that a query tile sees have to find room in the table of those with a kept key
-  const int64_t seen = (std::min(window.sinks, p.seqlen_k) + kBM - 1) / kBM + (std::min(window.keys, p.seqlen_k) + kBN) / kBM + 2;
-  return !p.mask || std::min<int64_t>(seen, (p.seqlen_k + kBM - 1) / kBM) <= kMaxBits;
+  return tile_head_dim(p.d) <= 128 || !sequences;
 }
 size_t tc_bwd_window_workspace_bytes(const fdma_bwd_params& bp, const Window& window, int sequences) {
   return tile_head_dim(bp.f.d) == 256 ? tc_bwd256_workspace_bytes(bp, window) : bwd_rows_workspace_bytes(bp, window, sequences);

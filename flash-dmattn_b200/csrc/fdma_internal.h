@@ -52,7 +52,7 @@ bool tc_bwd_supported(const fdma_bwd_params& p);
 size_t tc_bwd_workspace_bytes(const fdma_bwd_params& p);
 int tc_bwd(const fdma_bwd_params& p, cudaStream_t stream, const PackedSeqs& seqs = {});  // seqs: head dims up to 128
 // The same with a sliding window; sequences: 0, or the number of packed ones
-bool tc_bwd_window_supported(const fdma_bwd_params& p, const Window& window, int sequences);
+bool tc_bwd_window_supported(const fdma_bwd_params& p, int sequences);
 size_t tc_bwd_window_workspace_bytes(const fdma_bwd_params& p, const Window& window, int sequences);
 int tc_bwd_window(const fdma_bwd_params& p, cudaStream_t stream, const PackedSeqs& seqs, const Window& window);
 

@@ -39,7 +39,9 @@ def _sums_without_order(query, key, value) -> bool:
     Sq, Sk = query.shape[1], key.shape[1]
     if query.shape[-1] > 128 or not torch.is_grad_enabled() or not any(t.requires_grad for t in (query, key, value)):
         return False
-    return Sk >= 2048 and Sk >= (4 if Sk >= 4096 else 8) * Sq and Sk <= 2 ** 20
+    if _interface._kernel_path not in (_lib.PATH_AUTO, _lib.PATH_TCGEN05) or Sk > 2 ** 20:  # not the window's
+        return False
+    return Sk >= 2048 and Sk >= (4 if Sk >= 4096 else 8) * Sq
 
 
 def flash_sparse_attn_window_func(
@@ -59,7 +61,7 @@ def flash_sparse_attn_window_func(
     i + Sk - Sq, as under `flash_sparse_attn_func(is_causal=True)`, which this equals where the window is as long as the keys.
     attn_mask: bool ({B|1}, {H|Hk|1}, 1, {Sk|1}), False = masked out, such as padding; masks per query are not built. Rows that see no key
     return 0. Keys and values are expected to be finite, also where the mask hides them. softmax_scale, 0 or above, defaults to d ** -0.5.
-    B, Sq and Sk are at least 1 (packed sequences may be empty).
+    B, Sq and Sk are at least 1 (packed sequences may be empty), Sk at most 2^20 where the window leaves keys out.
     return_attn_probs=True returns (out, softmax_lse (B, H, Sq) fp32, empty tensor).
 
     Time and traffic go with the window, not with Sk. Returns out (B, Sq, H, d); gradients flow to query, key and value, each a sum in
