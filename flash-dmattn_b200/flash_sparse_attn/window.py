@@ -129,8 +129,21 @@ def flash_sparse_attn_window_varlen_func(
                                               sink_tokens)
         if res is not None:
             return res[0]
+    if torch.compiler.is_compiling() and not return_attn_probs and _traces_packed(query, key, value, cu_seqlens_q, cu_seqlens_k):
+        d = query.shape[-1]
+        softmax_scale = d ** -0.5 if softmax_scale is None else softmax_scale
+        if d % 8:  # 16-bit rows are kept 16-byte aligned
+            query, key, value = (torch.nn.functional.pad(t, [0, 8 - d % 8]) for t in (query, key, value))
+        return _PackedWindowAttnFunc.apply(query, key, value, cu_seqlens_q, cu_seqlens_k, softmax_scale, sliding_window, sink_tokens)[0][..., :d]
     return _interface._varlen(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, True, None,
                               deterministic, return_attn_probs, sliding_window, sink_tokens)
+
+
+def _traces_packed(q, k, v, cu_q, cu_k) -> bool:
+    """Whether a call that is traced is one operator, as it is one launch without tracing; others read the boundaries."""
+    return (_interface._kernel_path == _lib.PATH_AUTO and q.is_cuda and q.dim() == k.dim() == v.dim() == 3 and q.shape[-1] <= 128
+            and 0 < q.shape[0] <= 2 ** 19 and 0 < k.shape[0] <= 2 ** 20 and cu_q.dim() == cu_k.dim() == 1
+            and cu_q.shape[0] == cu_k.shape[0] >= 2 and cu_q.dtype == cu_k.dtype == torch.int32)
 
 
 class _WindowAttnFunc(torch.autograd.Function):
@@ -148,6 +161,22 @@ class _WindowAttnFunc(torch.autograd.Function):
         return (*torch.ops.flash_sparse_attn._window_backward(dout, q, k, v, mask, out, lse, *ctx.args), None, None, None, None)
 
 
+class _PackedWindowAttnFunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, scale, window, sinks):
+        # (cu: the backward's own boundaries, since the caller may fill its buffers for the next call before)
+        out, lse, cu = torch.ops.flash_sparse_attn._window_varlen_forward(q, k, v, cu_q, cu_k, scale, window, sinks)
+        ctx.save_for_backward(q, k, v, cu, out, lse)
+        ctx.args = (scale, window, sinks)
+        ctx.mark_non_differentiable(lse, cu)
+        return out, lse, cu
+
+    @staticmethod
+    def backward(ctx, dout, *_):
+        q, k, v, cu, out, lse = ctx.saved_tensors
+        return (*torch.ops.flash_sparse_attn._window_varlen_backward(dout, q, k, v, cu, out, lse, *ctx.args), None, None, None, None, None)
+
+
 def _aligned(t: Optional[torch.Tensor], unit: int) -> Optional[torch.Tensor]:
     """The tensor as the kernels load it: 16-byte aligned base and strides, innermost dimension dense."""
     if t is None:
@@ -163,10 +192,7 @@ def _prepare(q, k, v, mask):
     return q, k, v, mask
 
 
-@torch.library.custom_op("flash_sparse_attn::_window_forward", mutates_args=(), device_types="cuda")
-def _window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor], softmax_scale: float, window: int,
-                    sinks: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    q, k, v, mask = _prepare(q, k, v, mask)
+def _launch_forward(q, k, v, mask, softmax_scale, window, sinks, cu=None):
     lib = _lib.load()
     with torch.cuda.device(q.device):
         _interface._raise_if_kernel_timed_out(lib)
@@ -174,11 +200,38 @@ def _window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
         lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
         p = _lib.FwdParams()
         _interface._fill_fwd(p, q, k, v, mask, None, out, lse, softmax_scale, True)
-        size = lib.fdma_fwd_window_workspace_bytes(ctypes.byref(p), window, sinks, 0)
+        cu_q, cu_k, n = (None, None, 0) if cu is None else (cu[0].data_ptr(), cu[1].data_ptr(), cu.shape[1] - 1)
+        size = lib.fdma_fwd_window_workspace_bytes(ctypes.byref(p), window, sinks, n)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device)
         p.workspace, p.workspace_bytes = ws.data_ptr(), size
-        _lib.check(lib.fdma_fwd_window(ctypes.byref(p), window, sinks, None, None, 0, _interface._stream_ptr(q.device)), "fdma_fwd_window")
+        _lib.check(lib.fdma_fwd_window(ctypes.byref(p), window, sinks, cu_q, cu_k, n, _interface._stream_ptr(q.device)), "fdma_fwd_window")
     return out, lse
+
+
+def _launch_backward(dout, q, k, v, mask, out, lse, softmax_scale, window, sinks, cu=None):
+    dout, out, lse = _aligned(dout, 8), _aligned(out, 8), lse.contiguous()
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        _interface._raise_if_kernel_timed_out(lib)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        bp = _lib.BwdParams()
+        _interface._fill_fwd(bp.f, q, k, v, mask, None, out, lse, softmax_scale, True)
+        for name, t in (("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+            setattr(bp, "dout" if name == "do" else name, t.data_ptr())
+            for x, stride in zip(("batch", "row", "head"), _interface._bsh(t)):
+                setattr(bp, f"{name}_{x}_stride", stride)
+        cu_q, cu_k, n = (None, None, 0) if cu is None else (cu[0].data_ptr(), cu[1].data_ptr(), cu.shape[1] - 1)
+        size = lib.fdma_bwd_window_workspace_bytes(ctypes.byref(bp), window, sinks, n)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        bp.f.workspace, bp.f.workspace_bytes = ws.data_ptr(), size
+        _lib.check(lib.fdma_bwd_window(ctypes.byref(bp), window, sinks, cu_q, cu_k, n, _interface._stream_ptr(q.device)), "fdma_bwd_window")
+    return dq, dk, dv
+
+
+@torch.library.custom_op("flash_sparse_attn::_window_forward", mutates_args=(), device_types="cuda")
+def _window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor], softmax_scale: float, window: int,
+                    sinks: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _launch_forward(*_prepare(q, k, v, mask), softmax_scale, window, sinks)
 
 
 @torch.library.register_fake("flash_sparse_attn::_window_forward")
@@ -190,25 +243,44 @@ def _window_forward_fake(q, k, v, mask, softmax_scale, window, sinks):
 @torch.library.custom_op("flash_sparse_attn::_window_backward", mutates_args=(), device_types="cuda")
 def _window_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor], out: torch.Tensor,
                      softmax_lse: torch.Tensor, softmax_scale: float, window: int, sinks: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    q, k, v, mask = _prepare(q, k, v, mask)
-    dout, out, lse = _aligned(dout, 8), _aligned(out, 8), softmax_lse.contiguous()
-    lib = _lib.load()
-    with torch.cuda.device(q.device):
-        _interface._raise_if_kernel_timed_out(lib)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        bp = _lib.BwdParams()
-        _interface._fill_fwd(bp.f, q, k, v, mask, None, out, lse, softmax_scale, True)
-        for name, t in (("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
-            setattr(bp, "dout" if name == "do" else name, t.data_ptr())
-            for s, x in zip(("batch", "row", "head"), _interface._bsh(t)):
-                setattr(bp, f"{name}_{s}_stride", x)
-        size = lib.fdma_bwd_window_workspace_bytes(ctypes.byref(bp), window, sinks, 0)
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-        bp.f.workspace, bp.f.workspace_bytes = ws.data_ptr(), size
-        _lib.check(lib.fdma_bwd_window(ctypes.byref(bp), window, sinks, None, None, 0, _interface._stream_ptr(q.device)), "fdma_bwd_window")
-    return dq, dk, dv
+    return _launch_backward(dout, *_prepare(q, k, v, mask), out, softmax_lse, softmax_scale, window, sinks)
 
 
 @torch.library.register_fake("flash_sparse_attn::_window_backward")
 def _window_backward_fake(dout, q, k, v, mask, out, softmax_lse, softmax_scale, window, sinks):
+    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+
+
+# Packed sequences: (tokens, heads, d), lse (heads, tokens), cu (2, sequences + 1): the boundaries of the queries and of the keys
+def _prepare_packed(q, k, v):
+    return _prepare(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), None)
+
+
+@torch.library.custom_op("flash_sparse_attn::_window_varlen_forward", mutates_args=(), device_types="cuda")
+def _window_varlen_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor, softmax_scale: float,
+                           window: int, sinks: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    for cu in (cu_q, cu_k):
+        if cu.dtype != torch.int32 or cu.dim() != 1 or cu.device != q.device or cu.shape != cu_q.shape or cu.shape[0] < 2:
+            raise RuntimeError("cu_seqlens_q and cu_seqlens_k must be int32 tensors (sequences + 1) on the query's device")
+    cu = torch.stack((cu_q, cu_k))
+    out, lse = _launch_forward(*_prepare_packed(q, k, v), softmax_scale, window, sinks, cu)
+    return out[0], lse[0], cu
+
+
+@torch.library.register_fake("flash_sparse_attn::_window_varlen_forward")
+def _window_varlen_forward_fake(q, k, v, cu_q, cu_k, softmax_scale, window, sinks):
+    return (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device),
+            torch.empty((2, cu_q.shape[0]), dtype=torch.int32, device=q.device))
+
+
+@torch.library.custom_op("flash_sparse_attn::_window_varlen_backward", mutates_args=(), device_types="cuda")
+def _window_varlen_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, out: torch.Tensor,
+                            softmax_lse: torch.Tensor, softmax_scale: float, window: int,
+                            sinks: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    res = _launch_backward(dout.unsqueeze(0), *_prepare_packed(q, k, v), out.unsqueeze(0), softmax_lse, softmax_scale, window, sinks, cu)
+    return tuple(x[0] for x in res)
+
+
+@torch.library.register_fake("flash_sparse_attn::_window_varlen_backward")
+def _window_varlen_backward_fake(dout, q, k, v, cu, out, softmax_lse, softmax_scale, window, sinks):
     return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
