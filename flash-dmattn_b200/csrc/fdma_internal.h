@@ -120,6 +120,11 @@ int single_query_fwd_in(const fdma_fwd_params& p, cudaStream_t stream);
 int create_mask(const fdma_mask_params& p, cudaStream_t stream);
 
 // ---- attention over the 8-bit cache ---------------------------------------------------------------
+// Sliding window: the keys that count, of all; a block of 256 queries goes over so many of them.
+__host__ __device__ inline int64_t window_keys(int64_t keys, int64_t window, int64_t sinks) {
+  const int64_t seen = window + sinks + 256;
+  return seen < keys ? seen : keys;
+}
 // Requests with kPromptTokens or more new tokens have their keys converted to 16 bits once, for the tensor-core forward kernel
 // (fdma_cache_prompt.cu), if there is enough work for it; otherwise keys are read for 16 rows of queries at a time
 // (fdma_cache_attn.cu). The former takes about 37 us and 17 us per 1000 keys, however few its CTAs are; the latter 14 us and 3.1 us for a
@@ -128,11 +133,6 @@ int create_mask(const fdma_mask_params& p, cudaStream_t stream);
 // 8 heads over 2, 8 x up to 244 tokens over 43 41, 56; d = 256, 16 heads over 1, 32000 keys, 4 x 64 tokens 715, 750.
 constexpr int kPromptTokens = 32, kTileKeys = 800;
 // work: sum of tokens x heads x (keys + kTileKeys)
-// Sliding window: the keys that count, of all; a block of 256 queries goes over so many of them.
-__host__ __device__ inline int64_t window_keys(int64_t keys, int64_t window, int64_t sinks) {
-  const int64_t seen = window + sinks + 256;
-  return seen < keys ? seen : keys;
-}
 __host__ __device__ inline bool prompt_pays(int64_t work, int64_t longest, int d) { return work >= 2600000 + (d > 128 ? 3700 : 5500) * longest; }
 int check_cache(const fdma_cache& c);
 // Whether the call may have such requests, and scratch and layouts for them. Then cache_prompt writes all rows, those of other
