@@ -80,7 +80,8 @@ struct Bwd256Params {
   int64_t pos_batch_stride, pos_head_stride;
   int h_pos, causal_shift;
   // Sliding window (kWindow): as in fdma_bwd_rows_sm100.cu, near and far CTAs of the tiles that hold sinks leave fp32 sums,
-  // [2: dV, dK][near of each batch element, then its parts of far_rows queries][h_k][sink_rows][256]
+  // [2: dV, dK][near of each batch element, then its parts of far_rows queries][h_k][sink_rows][256]. 8192 queries, 16 heads over 4, d = 256, 1024
+  // keys: 695 us with the kernels around it (463 TFLOP/s; 8 products instead of the 5 counted); floor 193.
   Window window;
   float* sink_sums;
   int sink_rows, sink_tiles, far_slots, far_rows, n_far_ctas;  // far CTAs of a pass

@@ -57,7 +57,9 @@ constexpr int kMaxBits = 4096;   // 64-key tiles the activity bits of a row-pass
 constexpr int kMaxHeads = 4096;  // query heads of a group whose activity differs from head to head
 // Sliding windows: queries beyond the window that a CTA works on for a tile of sink keys (such a tile is seen by all queries behind it, the
 // others by window + 128 of them), or that times a power of two where the CTAs would be more than kFarCtas: by then every SM has many of
-// them, and each leaves an fp32 row per sink and kv head, of dV and of dK.
+// them, and each leaves an fp32 row per sink and kv head, of dV and of dK. Backward in us with 512 / 1024 / 2048 / 4096 / 8192 queries: 8192, 8 heads
+// over 2, d = 128, 512 keys + 4 sinks 147 / 142 / 149 / 263 / 441; 32 over 8, 128 + 4 318 / 316 / 312 / 310 / 517; 32768, 128 + 1024 sinks 2680 / 2540 / 2500 /
+// 2520 / 2490. With up to 16384 CTAs the last one 2440, for twice the rows.
 constexpr int kFarRows = 2048, kFarCtas = 4096;
 constexpr int kDbHeads = 16;    // query heads of a group whose dBias sums have room in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
@@ -100,7 +102,7 @@ struct BwdRowsParams {
   // Sliding window (kWindow). A key tile's CTA takes the query tiles whose windows reach it (near); those beyond, which see the sinks alone,
   // come from CTAs of their own (far), far_rows queries each: one CTA for a sink tile and all queries would be the whole launch's tail. Row-pass
   // items walk the sinks' and the window's key tiles, numbered without the gap between. 10 d products per pair that is seen and head, of which
-  // S and dP are formed twice; 32 heads over 8, d = 128, bf16: 32768 queries, 2048 keys + 4 sinks 4400 us (625 TFLOP/s counted once, 875 as
+  // S and dP are formed twice; 32 heads over 8, d = 128, bf16: 32768 queries, 2048 keys + 4 sinks 4400 us (606 TFLOP/s counted once, 849 as
   // issued), 8192 queries: 1024 keys 585 us, 128 + 4 sinks 282, 1 key 199. Bound by the softmax arithmetic, narrow windows by the CTAs' set-up.
   // Where a sequence has far queries, near and far leave fp32 sums of the sinks' rows, which sinks_kernel adds up in their order: the near ones
   // where the tile's moved sums lie, the far ones in far_sums [2: dV, dK][h_k][far_total][D], from far_place on, a tile's rows as move_sums lays

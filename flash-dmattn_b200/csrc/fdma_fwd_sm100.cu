@@ -195,7 +195,7 @@ __device__ __forceinline__ FwdItem fwd_item(const FwdKernelParams& p, int item, 
 // of the sinks and, from the first one that its first row sees, those up to the causal limit, numbered without the gap between (gap_of), so
 // that producer, mask, MMA and softmax warps walk one row of tiles; per element only the tiles on the window's two ends are masked. What it
 // cannot do without is 4 d products per pair that is seen and head. 32 heads over 8, d = 128, bf16: 32768 queries, 2048 keys + 4 sinks 1180 us
-// (930 TFLOP/s; causal over all keys 8990), 8192 queries: 1024 keys 175 us (750 TFLOP/s; causal 527), 128 + 4 sinks 92, 1 key 63. Bound by the
+// (904 TFLOP/s; causal over all keys 8990), 8192 queries: 1024 keys 175 us (736 TFLOP/s; causal 527), 128 + 4 sinks 92, 1 key 63. Bound by the
 // softmax chain as without a window, and below some 1000 keys by what an item costs beside its tiles: about 8000 cycles for its queries' way
 // in, the first product and the results' way out (stalls for instructions, twice those of a window of 1024 keys at 128, are part of it).
 template <int D, bool kBf16, bool kBcast, bool kVariant = false, bool kWindow = false>

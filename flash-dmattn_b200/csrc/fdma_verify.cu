@@ -192,7 +192,8 @@ struct Raw {
 };
 
 // Every CTA has an equal share of all rows' units: for each row of them the largest number and, relative to that, the sum of the exponentials.
-// What it does for a number beside the load are seven instructions, one of them an exponential: 3/4 of the time that memory takes.
+// What it does for a number beside the load are seven instructions, one of them an exponential: 3/4 of the time that memory takes. 4.3 TB/s; at the 64
+// registers that leave four CTAs on an SM the 16-bit instances spill 112 and 136 bytes (bf16, fp16) of the two sets of vectors.
 // kAhead vectors, of the next row too, are on their way while as many are worked on. (Two sets of registers in turn: when one was copied to the
 // other the compiler put the loads behind the work, to save registers, and load and work took turns.)
 template <typename T>

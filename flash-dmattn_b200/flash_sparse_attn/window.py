@@ -5,7 +5,7 @@ number of keys that a dynamic mask keeps. Over the paged 8-bit cache: `flash_spa
 
 Key tiles that no query of a tile sees are neither loaded nor multiplied (csrc/fdma_fwd_sm100.cu, fdma_bwd_rows_sm100.cu,
 fdma_bwd256_sm100.cu; a single query: fdma_decode.cu); the mask is one of the keys, for all queries. Probabilities and dS are rounded to the
-inputs' type before they enter a product, as in the calls without a window.
+inputs' type before they enter a product, as in the calls without a window, and the backward's rowsum(dout * out) is formed from the rounded out.
 """
 import ctypes
 import math
